@@ -21,7 +21,7 @@ def _host_path() -> str | None:
             return path
     return None if _ELSEWHERE else path
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 GDN_OK = 0
 GDN_ERR_INVALID = -1
@@ -49,7 +49,7 @@ FLAG_SCAN_PAIR = 1 << 21
 FLAG_SCAN_NO_WARM = 1 << 22
 FLAG_RECORD_P = 1 << 23
 
-ACT_NONE, ACT_SILU, ACT_SIGMOID = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_SIGMOID, ACT_GELU_TANH = 0, 1, 2, 3
 
 # name -> (restype, argtypes); one entry per declaration in include/gdn_hip.h
 SIGNATURES = {
@@ -173,6 +173,8 @@ SIGNATURES['gdn_norm_gated_bwd'] = (c_int, [
     c_void_p, c_void_p, c_void_p, c_void_p,            # dx dg dw_part db_part
     c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p])   # T D ld parts ...
 SIGNATURES['gdn_step_linear'] = (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_void_p])     # x N hidden segments nseg dtype
+SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 8 + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y g u h, M D F, activation dtype
+SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 14 + [c_int64] * 3 + [c_int, c_int, c_void_p])     # dy x wg wu wd g u h dg du dx dwg dwu dwd
 SIGNATURES['gdn_calib_rmw'] = (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p])
 CHUNK_STATIC_WORKSPACE_BYTES = 64 << 20
 CONV_BWD_TILES_PER_PART = 8

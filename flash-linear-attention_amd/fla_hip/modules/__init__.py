@@ -19,9 +19,11 @@ from fla_hip.modules.fused_norm_gate import (
     layer_norm_gated_fwd,
     rms_norm_gated,
 )
+from fla_hip.modules.mlp import GatedMLP, gated_mlp
 
 __all__ = [
     'ShortConvolution', 'causal_conv1d', 'causal_conv1d_fwd', 'causal_conv1d_bwd', 'causal_conv1d_update', 'causal_conv1d_update_states',
     'FusedLayerNormGated', 'FusedLayerNormSwishGate', 'FusedRMSNormGated', 'FusedRMSNormSwishGate',
+    'GatedMLP', 'gated_mlp',
     'layer_norm_gated', 'layer_norm_gated_fwd', 'layer_norm_gated_bwd', 'rms_norm_gated',
 ]

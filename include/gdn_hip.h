@@ -61,7 +61,8 @@ extern "C" {
 /* activation codes of the convolution and normalisation entry points */
 #define GDN_ACT_NONE    0
 #define GDN_ACT_SILU    1   /* swish / silu: x * sigmoid(x)                                  */
-#define GDN_ACT_SIGMOID 2   /* gate of the normalisation only                                */
+#define GDN_ACT_SIGMOID 2   /* gates: of the normalisation, of the feed-forward block        */
+#define GDN_ACT_GELU_TANH 3 /* gate of the feed-forward block only                           */
 
 /* Library ABI version (bumped on any signature change). */
 int gdn_hip_abi_version(void);
@@ -641,6 +642,29 @@ int gdn_norm_gated_bwd(
     void* dx, void* dg, float* dw_part, float* db_part,
     int64_t T, int64_t D, int64_t ld, int64_t parts,
     int x_dtype, int w_dtype, int activation, int is_rms_norm, void* stream);
+
+/*
+ * The gated feed-forward block: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T.  Replaces the projections and swiglu_linear of GatedMLP
+ * (fla/modules/mlp.py).
+ *   x, y [M,D]; wg, wu [F,D]; wd [D,F]; h [M,F], all dtype (GDN_DTYPE_BF16 or GDN_DTYPE_F16), contiguous and 16-byte aligned, D and F multiples of 8 up to
+ *   GDN_MLP_MAX_FEATURES; activation GDN_ACT_SILU, GDN_ACT_SIGMOID or GDN_ACT_GELU_TANH
+ *   g, u [M,F] or NULL (both): kept for the backward.  h is written in any case (the down projection reads it)
+ *   Accumulators, activation and product in fp32; h is rounded once to dtype, from the accumulators of g and u.
+ */
+#define GDN_MLP_MAX_FEATURES 1048576
+int gdn_gated_mlp_fwd(
+    const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
+    int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
+
+/*
+ * Its gradients: dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h.
+ *   g, u, h as the forward left them; dg, du [M,F]: room for the inner gradients (dh itself is not stored)
+ *   dx, dwg, dwu, dwd in dtype, each may be NULL: not asked for (then what only it needs may be NULL, too).  M == 0 clears the weights' gradients.
+ */
+int gdn_gated_mlp_bwd(
+    const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
+    void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
+    int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference (bench.py --workload calib_rmw): the memory traffic and the
