@@ -123,7 +123,7 @@ struct Gemm {
             {
                 const uint64_t base = (uint64_t)p.A[seg] + 2 * (A_DOWN ? (int64_t)k0 * p.lda + m0 : (int64_t)m0 * p.lda + k0);
                 const int64_t rest = 2 * ((int64_t)left * p.lda - m0);
-                const uint32_t extent = left <= 0 ? 0 : A_DOWN ? (uint32_t)min(rest, GM_EXTENT) : (uint32_t)GM_EXTENT;
+                const uint32_t extent = left <= 0 ? 0 : A_DOWN && rest < GM_EXTENT ? (uint32_t)rest : (uint32_t)GM_EXTENT;
 #pragma unroll
                 for (int i = 0; i < PA; ++i)
                     buffer_1k_to_lds(base, extent, !A_DOWN && chunk8 >= left ? GM_NOWHERE : va[i], to + 1024 * (w * PA + i));
@@ -133,7 +133,7 @@ struct Gemm {
                 const void* b = DUAL ? p.B[w * PB + i >= SideB::PIECES / 2] : p.B[seg];
                 const uint64_t base = (uint64_t)b + 2 * (B_DOWN ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0);
                 const int64_t rest = 2 * ((int64_t)left * p.ldb - n0);
-                const uint32_t extent = left <= 0 ? 0 : B_DOWN ? (uint32_t)min(rest, GM_EXTENT) : (uint32_t)GM_EXTENT;
+                const uint32_t extent = left <= 0 ? 0 : B_DOWN && rest < GM_EXTENT ? (uint32_t)rest : (uint32_t)GM_EXTENT;
                 buffer_1k_to_lds(base, extent, !B_DOWN && chunk8 >= left ? GM_NOWHERE : vb[i], to + SideA::BYTES + 1024 * (w * PB + i));
             }
         };

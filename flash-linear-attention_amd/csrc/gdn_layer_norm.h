@@ -1,0 +1,131 @@
+// Layer / RMS normalisation of rows of D features with the residual stream added first (fla/modules/layernorm.py): what the forward and the
+// backward kernels share.
+//
+//   r = x (+ residual), rounded to the stream's type RT;  mean = sum r / D (rms norm: 0);  rstd = 1 / sqrt(sum (r - mean)^2 / D + eps)
+//   xh = (r - mean) rstd;  y = xh w + b
+//   dr = rstd (dy w - xh mean(dy w xh) - [layer norm: mean(dy w)]) + dstream;  dw = sum over rows of dy xh;  db = sum over rows of dy
+//
+// The stream is a tensor of its own type, and that tensor is normalised: forward and backward see the same numbers, and the gradients of the
+// parameters are as exact as their sums.
+//
+// A few operations an element: bound by memory, every element read and written once.  A row belongs to LANES lanes - part of a wave, a wave, a
+// workgroup - each of which holds PIECES pieces of 16 bytes (of x) in registers.
+#pragma once
+#include "gdn_common.h"
+#include <algorithm>
+#include <type_traits>
+
+namespace gdn {
+
+template <typename T, int LANES, bool ALIGNED>
+struct NormRow {
+    static constexpr int VEC = 16 / sizeof(T), THREADS = LANES < 256 ? 256 : LANES, GROUPS = THREADS / LANES;
+    // the column of element e of lane l's piece i: pieces of 16 bytes, or, where rows do not begin on 16-byte boundaries, single elements side by side
+    static __device__ __forceinline__ int column(int l, int i, int e) { return ALIGNED ? (l + LANES * i) * VEC + e : (i * VEC + e) * LANES + l; }
+
+    template <typename S> using Piece = S __attribute__((ext_vector_type(VEC)));
+
+    template <typename S>
+    static __device__ __forceinline__ Piece<S> load(const S* row, int l, int i, int D) {
+        Piece<S> v;
+        if constexpr (ALIGNED) {
+            const int c = column(l, i, 0);
+            if (c < D) v = *(const Piece<S>*)(row + c);
+            else v = Piece<S>{};
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { const int c = column(l, i, e); v[e] = c < D ? row[c] : (S)0.f; }
+        }
+        return v;
+    }
+    template <typename S>
+    static __device__ __forceinline__ void store(S* row, int l, int i, int D, Piece<S> v) {
+        if constexpr (ALIGNED) {
+            const int c = column(l, i, 0);
+            if (c < D) *(Piece<S>*)(row + c) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { const int c = column(l, i, e); if (c < D) row[c] = v[e]; }
+        }
+    }
+    // weight or bias, of T's type or fp32; `fill` where there is none and past the end
+    static __device__ __forceinline__ void params(const void* w, int dtype, float fill, int l, int i, int D, float (&out)[VEC]) {
+        if (!w) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = fill;
+        } else if (dtype == GDN_DTYPE_F32) {
+            const Piece<float> v = load((const float*)w, l, i, D);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = v[e];
+        } else {
+            const Piece<T> v = load((const T*)w, l, i, D);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = (float)v[e];
+        }
+    }
+    // The same registers as values that the compiler knows nothing about: what follows is worked out from the pieces again and not kept, widened to fp32, from
+    // before a reduction until after it.
+    template <typename P> static __device__ __forceinline__ void forget(P& v) {
+        if constexpr (sizeof(P) == 16) { u32x4 t = __builtin_bit_cast(u32x4, v); asm("" : "+v"(t)); v = __builtin_bit_cast(P, t); }
+        else {
+            struct Two { u32x4 a, b; } t = __builtin_bit_cast(Two, v);
+            asm("" : "+v"(t.a)); asm("" : "+v"(t.b));
+            v = __builtin_bit_cast(P, t);
+        }
+    }
+    // sums over the lanes of a row.  `red`: a place for this sum that the last sum of the same workgroup did not use (LANES > 64)
+    static __device__ __forceinline__ void sum2(float& a, float& b, float (*red)[2]) {
+#pragma unroll
+        for (int m = (LANES < 64 ? LANES : 64) / 2; m >= 1; m >>= 1) { a += __shfl_xor(a, m, 64); b += __shfl_xor(b, m, 64); }
+        if constexpr (LANES > 64) {
+            if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6][0] = a; red[threadIdx.x >> 6][1] = b; }
+            __syncthreads();
+            a = 0.f; b = 0.f;
+#pragma unroll
+            for (int w = 0; w < LANES / 64; ++w) { a += red[w][0]; b += red[w][1]; }
+        }
+    }
+};
+
+// The forms of a row that there are kernels for, by the pieces of 16 bytes in it: f(LANES, PIECES, ALIGNED) as integral constants.
+template <int LANES, int PIECES, bool ALIGNED, typename F>
+static int norm_form_is(F&& f) {
+    return f(std::integral_constant<int, LANES>{}, std::integral_constant<int, PIECES>{}, std::integral_constant<bool, ALIGNED>{});
+}
+template <typename F>
+static int norm_form(int64_t pieces, bool aligned, F&& f) {
+    if (!aligned) {
+        if (pieces <= 128) return norm_form_is<64, 2, false>(f);
+        if (pieces <= 512) return norm_form_is<256, 2, false>(f);
+        return norm_form_is<1024, 4, false>(f);
+    }
+    if (pieces <= 16) return norm_form_is<16, 1, true>(f);
+    if (pieces <= 64) return norm_form_is<64, 1, true>(f);
+    if (pieces <= 128) return norm_form_is<64, 2, true>(f);
+    if (pieces <= 256) return norm_form_is<256, 1, true>(f);
+    if (pieces <= 512) return norm_form_is<256, 2, true>(f);
+    if (pieces <= 1024) return norm_form_is<512, 2, true>(f);
+    return norm_form_is<1024, 4, true>(f);
+}
+
+// f(T, RT) as values of the row's and the stream's types
+template <typename F>
+static int norm_types(const char* who, int dtype, int stream_dtype, F&& f) {
+    if (dtype == GDN_DTYPE_BF16 && stream_dtype == GDN_DTYPE_BF16) return f(bf16_t{}, bf16_t{});
+    if (dtype == GDN_DTYPE_BF16 && stream_dtype == GDN_DTYPE_F32) return f(bf16_t{}, float{});
+    if (dtype == GDN_DTYPE_F16 && stream_dtype == GDN_DTYPE_F16) return f(f16_t{}, f16_t{});
+    if (dtype == GDN_DTYPE_F16 && stream_dtype == GDN_DTYPE_F32) return f(f16_t{}, float{});
+    if (dtype == GDN_DTYPE_F32 && stream_dtype == GDN_DTYPE_F32) return f(float{}, float{});
+    set_error("%s: rows in bf16, f16 or f32, the residual stream in the rows' type or f32", who);
+    return GDN_ERR_UNSUPPORTED;
+}
+
+inline int check_norm(const char* who, int64_t rows, int64_t D, int dtype, int w_dtype) {
+    GDN_CHECK_ARG(rows >= 0 && rows < (1ll << 31) && D >= 1, GDN_ERR_INVALID, "%s: bad sizes rows=%lld D=%lld", who, (long long)rows, (long long)D);
+    GDN_CHECK_ARG(D <= GDN_NORM_MAX_ROW_BYTES / (dtype == GDN_DTYPE_F32 ? 4 : 2), GDN_ERR_UNSUPPORTED, "%s: rows of more than 64 KB are not supported (D=%lld)",
+                  who, (long long)D);
+    GDN_CHECK_ARG(w_dtype == GDN_DTYPE_F32 || w_dtype == dtype, GDN_ERR_UNSUPPORTED, "%s: weight and bias in the rows' type or f32", who);
+    return GDN_OK;
+}
+
+}  // namespace gdn

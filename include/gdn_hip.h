@@ -644,6 +644,32 @@ int gdn_norm_gated_bwd(
     int x_dtype, int w_dtype, int activation, int is_rms_norm, void* stream);
 
 /*
+ * Layer / RMS normalisation of rows of D features, the residual stream added first.  Replaces layer_norm_fwd (fla/modules/layernorm.py).
+ *   r = x (+ residual), rounded to stream_dtype; y = (r - mean) * rstd * weight + bias, rstd = 1/sqrt(var + eps), of r as it is handed on
+ *   (is_rms_norm != 0: mean = 0 and var = mean(r^2))
+ *   x, y [rows,D] dtype; residual, stream_out [rows,D] stream_dtype (dtype itself or fp32; stream_out may be NULL without a residual);
+ *   weight, bias [D] w_dtype (dtype or fp32) or NULL; mean, rstd [rows] fp32 or NULL (not stored).  All contiguous, of any alignment.
+ *   Requires D * sizeof(element of x) <= GDN_NORM_MAX_ROW_BYTES.
+ */
+int gdn_layer_norm_fwd(
+    const void* x, const void* residual, const void* weight, const void* bias,
+    void* y, void* stream_out, float* mean, float* rstd, int64_t rows, int64_t D, float eps,
+    int dtype, int stream_dtype, int w_dtype, int is_rms_norm, void* stream);
+
+/*
+ * Its backward.  Replaces layer_norm_bwd (fla/modules/layernorm.py).
+ *   r [rows,D] stream_dtype: what was normalised (stream_out, or x); dstream [rows,D] stream_dtype or NULL: gradient of stream_out, added to dx
+ *   dx [rows,D] dtype, dresidual [rows,D] stream_dtype: the same gradient in two types, either may be NULL
+ *   part [parts][dweight, then dbias, whichever is asked for][D] fp32: one row of partial sums per workgroup, for gdn_sum_rows;
+ *   gdn_layer_norm_bwd_parts says how many workgroups pay
+ */
+int64_t gdn_layer_norm_bwd_parts(int64_t rows, int64_t D, int dtype);
+int gdn_layer_norm_bwd(
+    const void* dy, const void* r, const void* weight, const float* mean, const float* rstd, const void* dstream,
+    void* dx, void* dresidual, float* part, int64_t rows, int64_t D, int64_t parts, int with_dweight, int with_dbias,
+    int dtype, int stream_dtype, int w_dtype, int is_rms_norm, void* stream);
+
+/*
  * The gated feed-forward block: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T.  Replaces the projections and swiglu_linear of GatedMLP
  * (fla/modules/mlp.py).
  *   x, y [M,D]; wg, wu [F,D]; wd [D,F]; h [M,F], all dtype (GDN_DTYPE_BF16 or GDN_DTYPE_F16), contiguous and 16-byte aligned, D and F multiples of 8 up to
