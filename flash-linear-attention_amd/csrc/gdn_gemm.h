@@ -26,6 +26,7 @@ struct GemmOperands {
     int M, N, K, segments;
     int tiles_m, tiles_n;
     int first;                           // the launch's tile where this product begins
+    int splits;                          // parts of the contraction, a workgroup each
 };
 
 typedef uint32_t gm_rsrc __attribute__((ext_vector_type(4)));
@@ -103,7 +104,8 @@ struct Gemm {
         return DUAL ? (j < NT / 2 ? wn * (NT / 2) + j : BN / 32 + wn * (NT / 2) + j - NT / 2) : wn * NT + j;
     }
 
-    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, char* smem, f32x4 (&acc)[NT][MT]) {
+    // `part` of p.splits: that share of the contraction's steps
+    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, int part, char* smem, f32x4 (&acc)[NT][MT]) {
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w % WM, wn = w / WM;
         const int m0 = tm * BM, n0 = tn * COLUMNS;
         uint32_t va[PA], vb[PB];
@@ -115,57 +117,76 @@ struct Gemm {
             vb[i] = SideB::source(DUAL ? piece % (SideB::PIECES / 2) : piece, lane, p.ldb, p.N - n0);
         }
         const int chunk8 = 8 * ((lane & 3) ^ (-(lane >> 4) & 3));    // where this lane's piece of a row along k begins
-        const int steps = (p.K + GM_K - 1) / GM_K, total = steps * p.segments;
+        const int steps = max(1, (p.K + GM_K - 1) / GM_K), all = steps * p.segments;      // (no contraction at all: one step on zeros)
+        const int begin = (int)((int64_t)all * part / p.splits), total = (int)((int64_t)all * (part + 1) / p.splits) - begin;
 
-        auto request = [&](int t) {
-            const int seg = t >= steps && p.segments == 2, k0 = (t - seg * steps) * GM_K, left = t < total ? p.K - k0 : 0;
-            const uint32_t to = (uint32_t)(t % GM_STAGES) * STAGE;
-            {
-                const uint64_t base = (uint64_t)p.A[seg] + 2 * (A_DOWN ? (int64_t)k0 * p.lda + m0 : (int64_t)m0 * p.lda + k0);
-                const int64_t rest = 2 * ((int64_t)left * p.lda - m0);
-                const uint32_t extent = left <= 0 ? 0 : A_DOWN && rest < GM_EXTENT ? (uint32_t)rest : (uint32_t)GM_EXTENT;
-#pragma unroll
-                for (int i = 0; i < PA; ++i)
-                    buffer_1k_to_lds(base, extent, !A_DOWN && chunk8 >= left ? GM_NOWHERE : va[i], to + 1024 * (w * PA + i));
-            }
-#pragma unroll
-            for (int i = 0; i < PB; ++i) {
-                const void* b = DUAL ? p.B[w * PB + i >= SideB::PIECES / 2] : p.B[seg];
-                const uint64_t base = (uint64_t)b + 2 * (B_DOWN ? (int64_t)k0 * p.ldb + n0 : (int64_t)n0 * p.ldb + k0);
-                const int64_t rest = 2 * ((int64_t)left * p.ldb - n0);
-                const uint32_t extent = left <= 0 ? 0 : B_DOWN && rest < GM_EXTENT ? (uint32_t)rest : (uint32_t)GM_EXTENT;
-                buffer_1k_to_lds(base, extent, !B_DOWN && chunk8 >= left ? GM_NOWHERE : vb[i], to + SideA::BYTES + 1024 * (w * PB + i));
-            }
+        // where the next step's tiles begin, kept in scalar registers: a load of a parameter inside the loop would be waited for with the LDS reads
+        struct Walk { uint64_t at, second; uint32_t stride; };
+        auto walk = [&](const void* first, const void* second, bool down, int64_t ld, int corner) {
+            const int64_t offset = 2 * (down ? (int64_t)corner : corner * ld), stride = 2 * (down ? GM_K * ld : GM_K);
+            const bool in_second = begin >= steps;
+            return Walk{(uint64_t)(in_second ? second : first) + offset + (uint64_t)stride * (begin - (in_second ? steps : 0)), (uint64_t)second + offset, (uint32_t)stride};
+        };
+        Walk wa = walk(p.A[0], p.A[1], A_DOWN, p.lda, m0);
+        const void* b0 = DUAL ? p.B[w * PB >= SideB::PIECES / 2] : p.B[0];          // (all pieces of a wave are of one product)
+        Walk wb = walk(b0, p.B[1], B_DOWN, p.ldb, n0);
+        const int K = p.K, lda2 = 2 * (int)p.lda, ldb2 = 2 * (int)p.ldb;
+        int asked = 0, left = K - GM_K * (begin % steps), until_second = p.segments == 2 && begin < steps ? steps - begin : -1;
+        uint32_t to = 0;
+        auto extent = [&](bool down, int ld2, int corner) {
+            const uint32_t whole = (uint32_t)GM_EXTENT, rest = (uint32_t)(left * ld2 - 2 * corner);
+            return asked >= total || left <= 0 ? 0u : down && left < GM_K ? rest : whole;
+        };
+        // the copies of one more step: this wave's piece i of PA + PB, and then on to the next step
+        uint32_t ea = 0, eb = 0;
+        auto request = [&](int i) {
+            if (i == 0) { ea = extent(A_DOWN, lda2, m0); eb = extent(B_DOWN, ldb2, n0); }
+            if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && chunk8 >= left ? GM_NOWHERE : va[i < PA ? i : 0], to + 1024 * (w * PA + i));
+            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && chunk8 >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], to + SideA::BYTES + 1024 * (w * PB + i - PA));
+            if (i < PA + PB - 1) return;
+            ++asked;
+            const bool second = asked == until_second;
+            wa.at = second ? wa.second : wa.at + wa.stride;
+            wb.at = second ? wb.second : wb.at + wb.stride;
+            left = second ? K : left - GM_K;
+            to = to + STAGE == LDS ? 0 : to + STAGE;
         };
         const uint32_t sa = SideA::share(lane), sb = SideB::share(lane);
         V8 fa[2][MT], fb[2][NT];
-        auto fetch = [&](int t, V8 (&a)[MT], V8 (&b)[NT]) {
+        // fragment i of NT + MT of step t
+        auto fetch = [&](int t, int i, V8 (&a)[MT], V8 (&b)[NT]) {
             const char* stage = smem + (t % GM_STAGES) * STAGE;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = SideB::fragment(stage + SideA::BYTES, sb, column_tile(wn, j));
-#pragma unroll
-            for (int i = 0; i < MT; ++i) a[i] = SideA::fragment(stage, sa, wm * MT + i);
+            if (i < NT) b[i < NT ? i : 0] = SideB::fragment(stage + SideA::BYTES, sb, column_tile(wn, i));
+            else a[i < NT ? 0 : i - NT] = SideA::fragment(stage, sa, wm * MT + i - NT);
         };
+        // A step's products in MT rounds, each with its share of the fragments of the next step and of the copies in front of its NT products: whatever they take
+        // to issue hides behind the products, which one after the other keep the matrix core busy.
         auto step = [&](int t, V8 (&a)[MT], V8 (&b)[NT], V8 (&a1)[MT], V8 (&b1)[NT]) {
             wait_vm_at_most<(GM_STAGES - 2) * (PA + PB)>();          // this wave's share of stage t + 1 is there
             lds_barrier();                                           // ... everyone's is, and everyone has read stage t
-            request(t + GM_STAGES);
-            fetch(t + 1, a1, b1);
-            __builtin_amdgcn_sched_barrier(0);                       // (requested before the products, to be there after them)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int f = i * (NT + MT) / MT; f < (i + 1) * (NT + MT) / MT; ++f) fetch(t + 1, f, a1, b1);
+#pragma unroll
+                for (int r = i * (PA + PB) / MT; r < (i + 1) * (PA + PB) / MT; ++r) request(r);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][i] = Mma<T>::run(b[j], a[i], acc[j][i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < GM_STAGES; ++t) request(t);
+        for (int t = 0; t < GM_STAGES; ++t)
+#pragma unroll
+            for (int r = 0; r < PA + PB; ++r) request(r);
         wait_vm_at_most<(GM_STAGES - 1) * (PA + PB)>();
         lds_barrier();
-        fetch(0, fa[0], fb[0]);
+#pragma unroll
+        for (int f = 0; f < NT + MT; ++f) fetch(0, f, fa[0], fb[0]);
         // (an odd number of steps: one more on zeros)
         for (int t = 0; t < total; t += 2) {
             step(t, fa[0], fb[0], fa[1], fb[1]);

@@ -29,73 +29,128 @@ struct MlpGemm {
     int ops, tiles;
     void* C[3];                          // results (of a DUAL product's epilogue: h, g, u; of dh's: dg, du)
     const void* G; const void* U;
+    float* part;                         // splits > 1: [splits][1 or 2 (both products of a DUAL)][M][N]
     int act;
 };
 
 enum MlpEpilogue { MLP_PLAIN, MLP_GATE, MLP_GRAD };
 
+// What becomes of four neighbours of a result (of both products where there are two), at offset `at` of the outputs.
+template <typename T, int EPI>
+__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x4 x, f32x4 u) {
+    typedef typename Mma<T>::V4 V4;
+    if constexpr (EPI == MLP_PLAIN) {
+        *(V4*)((T*)p.C[which] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+    } else if constexpr (EPI == MLP_GATE) {
+        V4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a, da;
+            mlp_act(p.act, x[e], a, da);
+            h[e] = (T)(a * u[e]);
+        }
+        *(V4*)((T*)p.C[0] + at) = h;
+        if (p.C[1]) {
+            *(V4*)((T*)p.C[1] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+            *(V4*)((T*)p.C[2] + at) = V4{(T)u[0], (T)u[1], (T)u[2], (T)u[3]};
+        }
+    } else {
+        const V4 gv = *(const V4*)((const T*)p.G + at), uv = *(const V4*)((const T*)p.U + at);
+        V4 dg, du;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a, da;
+            mlp_act(p.act, (float)gv[e], a, da);
+            dg[e] = (T)(x[e] * (float)uv[e] * da);
+            du[e] = (T)(x[e] * a);
+        }
+        *(V4*)((T*)p.C[0] + at) = dg;
+        *(V4*)((T*)p.C[1] + at) = du;
+    }
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     typedef Gemm<T, BM, BN, WM, WN, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
-    typedef typename Mma<T>::V4 V4;
     extern __shared__ __align__(16) char smem[];
     int tile = gemm_tile_of((int)blockIdx.x, p.tiles), which = 0;
     while (which + 1 < p.ops && tile >= p.op[which + 1].first) ++which;
     const GemmOperands& o = p.op[which];
+    tile -= o.first;
+    // (the parts of a tile one after the other: they share nothing, their neighbours in the band share rows and columns)
+    const int area = o.tiles_m * o.tiles_n, part = tile / area;
     int tm, tn;
-    gemm_place(tile - o.first, o.tiles_m, o.tiles_n, tm, tn);
+    gemm_place(tile - part * area, o.tiles_m, o.tiles_n, tm, tn);
     f32x4 acc[G::NT][G::MT];
-    G::run(o, tm, tn, smem, acc);
+    G::run(o, tm, tn, part, smem, acc);
 
     const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % WM, wn = w / WM, c16 = lane & 15, g4 = 4 * (lane >> 4);
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
         const int m = tm * BM + 16 * (wm * G::MT + i) + c16;
         if (m >= o.M) continue;
 #pragma unroll
-        for (int j = 0; j < (EPI == MLP_GATE ? G::NT / 2 : G::NT); ++j) {
+        for (int j = 0; j < COLS; ++j) {
             const int n = tn * G::COLUMNS + 16 * G::column_tile(wn, j) + g4;
             if (n >= o.N) continue;
             const int64_t at = (int64_t)m * o.N + n;
-            const f32x4 x = acc[j][i];
-            if constexpr (EPI == MLP_PLAIN) {
-                *(V4*)((T*)p.C[which] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-            } else if constexpr (EPI == MLP_GATE) {
-                const f32x4 u = acc[j + G::NT / 2][i];
-                V4 h;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float a, da;
-                    mlp_act(p.act, x[e], a, da);
-                    h[e] = (T)(a * u[e]);
-                }
-                *(V4*)((T*)p.C[0] + at) = h;
-                if (p.C[1]) {
-                    *(V4*)((T*)p.C[1] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-                    *(V4*)((T*)p.C[2] + at) = V4{(T)u[0], (T)u[1], (T)u[2], (T)u[3]};
-                }
-            } else {
-                const V4 gv = *(const V4*)((const T*)p.G + at), uv = *(const V4*)((const T*)p.U + at);
-                V4 dg, du;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float a, da;
-                    mlp_act(p.act, (float)gv[e], a, da);
-                    dg[e] = (T)(x[e] * (float)uv[e] * da);
-                    du[e] = (T)(x[e] * a);
-                }
-                *(V4*)((T*)p.C[0] + at) = dg;
-                *(V4*)((T*)p.C[1] + at) = du;
-            }
+            const f32x4 x = acc[j][i], u = acc[j + (KINDS - 1) * COLS][i];
+            if (o.splits > 1) {
+                float* to = p.part + (int64_t)part * KINDS * o.M * o.N + at;
+                *(f32x4*)to = x;
+                if (KINDS == 2) *(f32x4*)(to + (int64_t)o.M * o.N) = u;
+            } else
+                mlp_result<T, EPI>(p, which, at, x, u);
         }
     }
 }
 
+// The parts of a contraction added up, in order, and what becomes of the sums.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void mlp_join_kernel(MlpGemm p) {
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1;
+    const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= size) return;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, u = x;
+    for (int s = 0; s < p.op[0].splits; ++s) {
+        x += *(const f32x4*)(p.part + s * KINDS * size + at);
+        if (KINDS == 2) u += *(const f32x4*)(p.part + (s * KINDS + 1) * size + at);
+    }
+    mlp_result<T, EPI>(p, 0, at, x, u);
+}
+
 static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t ldb, int64_t M, int64_t N, int64_t K) {
     GemmOperands o{};
-    o.A[0] = A; o.B[0] = B; o.lda = lda; o.ldb = ldb; o.M = (int)M; o.N = (int)N; o.K = (int)K; o.segments = 1;
+    o.A[0] = A; o.B[0] = B; o.lda = lda; o.ldb = ldb; o.M = (int)M; o.N = (int)N; o.K = (int)K; o.segments = 1; o.splits = 1;
     return o;
 }
+
+// How a product (or several in a launch) is cut: the tile, and into how many parts the contraction.
+struct MlpPlan { bool large; int splits; };
+static MlpPlan plan_gemm(const MlpGemm& p, int kinds) {
+    int64_t large = 0, small = 0;
+    for (int i = 0; i < p.ops; ++i) {
+        const int64_t M = p.op[i].M, N = (int64_t)p.op[i].N * kinds;
+        large += ((M + 255) / 256) * ((N + 255) / 256);
+        small += ((M + 127) / 128) * ((N + 127) / 128);
+    }
+    MlpPlan plan{large >= 160, 1};
+    if (getenv("MLP_LARGE")) plan.large = atoi(getenv("MLP_LARGE"));
+    if (!plan.large && p.ops == 1) {
+        const int64_t steps = (int64_t)((p.op[0].K + GM_K - 1) / GM_K) * p.op[0].segments;
+        plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / std::max<int64_t>(small, 1), steps / 8), 16));
+        if (getenv("MLP_SPLIT")) plan.splits = atoi(getenv("MLP_SPLIT"));
+    }
+    return plan;
+}
+static size_t plan_bytes(const MlpGemm& p, int kinds) {
+    const MlpPlan plan = plan_gemm(p, kinds);
+    return plan.splits > 1 ? (size_t)plan.splits * kinds * p.op[0].M * p.op[0].N * 4 : 0;
+}
+
+struct Workspace { void* at; size_t bytes; };
 
 template <typename T, int BM, int BN, int WM, int WN, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, hipStream_t stream) {
@@ -105,7 +160,7 @@ static int launch_tiles(MlpGemm& p, hipStream_t stream) {
         GemmOperands& o = p.op[i];
         o.first = (int)tiles;
         o.tiles_m = (o.M + BM - 1) / BM; o.tiles_n = (o.N + G::COLUMNS - 1) / G::COLUMNS;
-        tiles += (int64_t)o.tiles_m * o.tiles_n;
+        tiles += (int64_t)o.tiles_m * o.tiles_n * o.splits;
         GDN_CHECK_ARG(tiles < (1ll << 32) / G::THREADS, GDN_ERR_UNSUPPORTED, "the gated feed-forward block: %lld x %lld results are too many for one launch",
                       (long long)o.M, (long long)o.N);
     }
@@ -119,46 +174,76 @@ static int launch_tiles(MlpGemm& p, hipStream_t stream) {
 }
 
 template <typename T, bool A_DOWN, bool B_DOWN, int EPI>
-static int launch_gemm(MlpGemm& p, hipStream_t stream) {
-    return launch_tiles<T, 256, 256, 2, 4, A_DOWN, B_DOWN, EPI>(p, stream);
+static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1;
+    const MlpPlan plan = plan_gemm(p, KINDS);
+    p.op[0].splits = plan.splits;
+    if (plan.splits > 1) {
+        GDN_CHECK_ARG(ws.at && ws.bytes >= plan_bytes(p, KINDS), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes,
+                      plan_bytes(p, KINDS));
+        p.part = (float*)ws.at;
+    }
+    int rc = plan.large ? launch_tiles<T, 256, 256, 2, 4, A_DOWN, B_DOWN, EPI>(p, stream) : launch_tiles<T, 128, 128, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream);
+    if (rc != GDN_OK || plan.splits <= 1) return rc;
+    const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
+    hipLaunchKernelGGL((mlp_join_kernel<T, EPI>), dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, stream, p);
+    return check_launch("mlp_join_kernel");
+}
+
+// The products of a forward and a backward pass.
+static MlpGemm gate_up(const void* x, const void* wg, const void* wu, int64_t M, int64_t D, int64_t F) {
+    MlpGemm p{};
+    p.ops = 1;
+    p.op[0] = operands(x, wg, D, D, M, F, D);
+    p.op[0].B[1] = wu;
+    return p;
+}
+static MlpGemm down(const void* h, const void* wd, int64_t M, int64_t D, int64_t F) {
+    MlpGemm p{};
+    p.ops = 1;
+    p.op[0] = operands(h, wd, F, F, M, D, F);
+    return p;
+}
+static MlpGemm grad_inner(const void* dy, const void* wd, int64_t M, int64_t D, int64_t F) {
+    MlpGemm p{};
+    p.ops = 1;
+    p.op[0] = operands(dy, wd, D, F, M, F, D);
+    return p;
+}
+static MlpGemm grad_x(const void* dg, const void* du, const void* wg, const void* wu, int64_t M, int64_t D, int64_t F) {
+    MlpGemm p{};
+    p.ops = 1;
+    p.op[0] = operands(dg, wg, F, D, M, D, F);
+    p.op[0].A[1] = du; p.op[0].B[1] = wu; p.op[0].segments = 2;
+    return p;
 }
 
 template <typename T>
-static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h, int64_t M, int64_t D, int64_t F,
+static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h, Workspace ws, int64_t M, int64_t D, int64_t F,
                    int act, hipStream_t stream) {
-    MlpGemm p{};
-    p.ops = 1; p.act = act;
-    p.op[0] = operands(x, wg, D, D, M, F, D);
-    p.op[0].B[1] = wu;
-    p.C[0] = h; p.C[1] = g; p.C[2] = u;
-    int rc = launch_gemm<T, false, false, MLP_GATE>(p, stream);
+    MlpGemm p = gate_up(x, wg, wu, M, D, F);
+    p.act = act; p.C[0] = h; p.C[1] = g; p.C[2] = u;
+    const int rc = launch_gemm<T, false, false, MLP_GATE>(p, ws, stream);
     if (rc != GDN_OK) return rc;
-    MlpGemm q{};
-    q.ops = 1;
-    q.op[0] = operands(h, wd, F, F, M, D, F);
+    MlpGemm q = down(h, wd, M, D, F);
     q.C[0] = y;
-    return launch_gemm<T, false, false, MLP_PLAIN>(q, stream);
+    return launch_gemm<T, false, false, MLP_PLAIN>(q, ws, stream);
 }
 
 template <typename T>
 static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
-                   void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd, int64_t M, int64_t D, int64_t F, int act, hipStream_t stream) {
+                   void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd, Workspace ws, int64_t M, int64_t D, int64_t F, int act, hipStream_t stream) {
     int rc = GDN_OK;
-    if (dx || dwg || dwu) {
-        MlpGemm p{};
-        p.ops = 1; p.act = act; p.G = g; p.U = u;
-        p.op[0] = operands(dy, wd, D, F, M, F, D);
-        p.C[0] = dg; p.C[1] = du;
-        rc = launch_gemm<T, false, true, MLP_GRAD>(p, stream);
+    if (M > 0 && (dx || dwg || dwu)) {
+        MlpGemm p = grad_inner(dy, wd, M, D, F);
+        p.act = act; p.G = g; p.U = u; p.C[0] = dg; p.C[1] = du;
+        rc = launch_gemm<T, false, true, MLP_GRAD>(p, ws, stream);
         if (rc != GDN_OK) return rc;
     }
-    if (dx) {
-        MlpGemm p{};
-        p.ops = 1;
-        p.op[0] = operands(dg, wg, F, D, M, D, F);
-        p.op[0].A[1] = du; p.op[0].B[1] = wu; p.op[0].segments = 2;
+    if (M > 0 && dx) {
+        MlpGemm p = grad_x(dg, du, wg, wu, M, D, F);
         p.C[0] = dx;
-        rc = launch_gemm<T, false, true, MLP_PLAIN>(p, stream);
+        rc = launch_gemm<T, false, true, MLP_PLAIN>(p, ws, stream);
         if (rc != GDN_OK) return rc;
     }
     MlpGemm p{};
@@ -170,7 +255,7 @@ static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu
     add(dg, x, F, D, dwg);
     add(du, x, F, D, dwu);
     add(dy, h, D, F, dwd);
-    return p.ops ? launch_gemm<T, true, true, MLP_PLAIN>(p, stream) : GDN_OK;
+    return p.ops ? launch_gemm<T, true, true, MLP_PLAIN>(p, ws, stream) : GDN_OK;
 }
 
 }  // namespace gdn
@@ -187,8 +272,14 @@ static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, 
     return GDN_OK;
 }
 
+extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward) {
+    if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16) != GDN_OK || M == 0) return 0;
+    if (!backward) return std::max(plan_bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2), plan_bytes(down(nullptr, nullptr, M, D, F), 1));
+    return std::max(plan_bytes(grad_inner(nullptr, nullptr, M, D, F), 1), plan_bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1));
+}
+
 extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
-                                 int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
+                                 void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
     const char* who = "gdn_gated_mlp_fwd";
     const int rc = check_mlp(who, M, D, F, activation, dtype);
     if (rc != GDN_OK) return rc;
@@ -197,13 +288,14 @@ extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, 
     GDN_CHECK_ARG((((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)g | (uintptr_t)u | (uintptr_t)h) & 15) == 0,
                   GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
     hipStream_t s = (hipStream_t)stream;
-    return dtype == GDN_DTYPE_BF16 ? mlp_fwd<bf16_t>(x, wg, wu, wd, y, g, u, h, M, D, F, activation, s)
-                                   : mlp_fwd<f16_t>(x, wg, wu, wd, y, g, u, h, M, D, F, activation, s);
+    const Workspace ws{workspace, workspace_bytes};
+    return dtype == GDN_DTYPE_BF16 ? mlp_fwd<bf16_t>(x, wg, wu, wd, y, g, u, h, ws, M, D, F, activation, s)
+                                   : mlp_fwd<f16_t>(x, wg, wu, wd, y, g, u, h, ws, M, D, F, activation, s);
 }
 
 extern "C" int gdn_gated_mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
                                  void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
-                                 int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
+                                 void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
     const char* who = "gdn_gated_mlp_bwd";
     const int rc = check_mlp(who, M, D, F, activation, dtype);
     if (rc != GDN_OK) return rc;
@@ -214,6 +306,7 @@ extern "C" int gdn_gated_mlp_bwd(const void* dy, const void* x, const void* wg, 
                     (uintptr_t)du | (uintptr_t)dx | (uintptr_t)dwg | (uintptr_t)dwu | (uintptr_t)dwd) & 15) == 0,
                   GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
     hipStream_t s = (hipStream_t)stream;
-    return dtype == GDN_DTYPE_BF16 ? mlp_bwd<bf16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, M, D, F, activation, s)
-                                   : mlp_bwd<f16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, M, D, F, activation, s);
+    const Workspace ws{workspace, workspace_bytes};
+    return dtype == GDN_DTYPE_BF16 ? mlp_bwd<bf16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, activation, s)
+                                   : mlp_bwd<f16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, activation, s);
 }

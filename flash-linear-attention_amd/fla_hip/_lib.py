@@ -176,8 +176,9 @@ SIGNATURES['gdn_step_linear'] = (c_int, [c_void_p, c_int64, c_int64, c_void_p, c
 SIGNATURES['gdn_layer_norm_fwd'] = (c_int, [c_void_p] * 8 + [c_int64, c_int64, c_float] + [c_int] * 4 + [c_void_p])    # x residual weight bias y stream_out mean rstd ...
 SIGNATURES['gdn_layer_norm_bwd_parts'] = (c_int64, [c_int64, c_int64, c_int])
 SIGNATURES['gdn_layer_norm_bwd'] = (c_int, [c_void_p] * 9 + [c_int64] * 3 + [c_int] * 6 + [c_void_p])    # dy r weight mean rstd dstream dx dresidual part, rows D parts ...
-SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 8 + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y g u h, M D F, activation dtype
-SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 14 + [c_int64] * 3 + [c_int, c_int, c_void_p])     # dy x wg wu wd g u h dg du dx dwg dwu dwd
+SIGNATURES['gdn_gated_mlp_workspace_bytes'] = (c_size_t, [c_int64, c_int64, c_int64, c_int])
+SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 9 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y g u h workspace bytes, M D F, activation dtype
+SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 15 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])     # dy x wg wu wd g u h dg du dx dwg dwu dwd
 SIGNATURES['gdn_calib_rmw'] = (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p])
 CHUNK_STATIC_WORKSPACE_BYTES = 64 << 20
 CONV_BWD_TILES_PER_PART = 8

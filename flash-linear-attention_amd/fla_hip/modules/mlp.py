@@ -27,6 +27,11 @@ def _operands(x, gate_weight, up_weight, down_weight):
     return _pad(x, M, D8), _pad(gate_weight, F8, D8), _pad(up_weight, F8, D8), _pad(down_weight, D8, F8)
 
 
+def _workspace(M, D, inner, backward, dev):
+    n = _lib.load().gdn_gated_mlp_workspace_bytes(M, D, inner, backward)
+    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
+
+
 def _forward(x, wg, wu, wd, activation, keep):
     M, D = x.shape
     inner = wg.shape[0]
@@ -34,7 +39,8 @@ def _forward(x, wg, wu, wd, activation, keep):
     y = torch.empty_like(x)
     h = torch.empty(M, inner, dtype=x.dtype, device=dev)
     g, u = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
-    launch(_lib.load().gdn_gated_mlp_fwd, dev, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(y), ptr(g), ptr(u), ptr(h), M, D, inner,
+    ws, n = _workspace(M, D, inner, 0, dev)
+    launch(_lib.load().gdn_gated_mlp_fwd, dev, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(y), ptr(g), ptr(u), ptr(h), ptr(ws), n, M, D, inner,
            activation, dtype_code(x.dtype))
     return y, g, u, h
 
@@ -68,8 +74,9 @@ class GatedMLPFunction(torch.autograd.Function):
             return torch.empty(shape, dtype=dt, device=dev) if need else None
 
         dx, dwg, dwu, dwd = empty(need_x, M, D8), empty(need_g, F8, D8), empty(need_u, F8, D8), empty(need_d, D8, F8)
+        ws, n = _workspace(M, D8, F8, 1, dev)
         launch(_lib.load().gdn_gated_mlp_bwd, dev, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dg), ptr(du),
-               ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), M, D8, F8, ctx.activation, dtype_code(dt))
+               ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ptr(ws), n, M, D8, F8, ctx.activation, dtype_code(dt))
 
         def cut(t, rows, cols):
             return t if t is None or t.shape == (rows, cols) else t[:rows, :cols].contiguous()

@@ -676,11 +676,14 @@ int gdn_layer_norm_bwd(
  *   GDN_MLP_MAX_FEATURES; activation GDN_ACT_SILU, GDN_ACT_SIGMOID or GDN_ACT_GELU_TANH
  *   g, u [M,F] or NULL (both): kept for the backward.  h is written in any case (the down projection reads it)
  *   Accumulators, activation and product in fp32; h is rounded once to dtype, from the accumulators of g and u.
+ *   workspace: gdn_gated_mlp_workspace_bytes(M, D, F, backward) bytes, 16-byte aligned (NULL where that is 0): partial sums of contractions that are
+ *   shared out over workgroups because there are few rows
  */
 #define GDN_MLP_MAX_FEATURES 1048576
+size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward);
 int gdn_gated_mlp_fwd(
     const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
-    int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
+    void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
 
 /*
  * Its gradients: dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h.
@@ -690,7 +693,7 @@ int gdn_gated_mlp_fwd(
 int gdn_gated_mlp_bwd(
     const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
     void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
-    int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
+    void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference (bench.py --workload calib_rmw): the memory traffic and the
