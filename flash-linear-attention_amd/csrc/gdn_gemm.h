@@ -1,23 +1,30 @@
 // Matrix products of 16-bit operands for large row counts: C[m][n] = sum_k A(m, k) B(n, k), fp32 accumulators, with either operand stored with the
 // contraction along its rows (A[m][k]) or down its columns (A[k][m]).  What becomes of an accumulator is an epilogue's business.
 //
-// A workgroup takes a BM x BN tile of C and walks over k in steps of 32.  A step's operands are (BM + BN) * 64 bytes of LDS; GM_STAGES of them are in
-// flight or in use: at step t the wave's matrix instructions work on fragments of t in registers, the fragments of t + 1 leave LDS for the other set of
-// registers, and the stage that t has just been read from is filled with t + GM_STAGES straight from memory (buffer_load ... lds).  One barrier a step.
-// Places past the end of a row, a column or the contraction are requested beyond the buffer's extent and arrive as zeros, so every size
-// that is a multiple of 8 along rows runs the same code.
+// A workgroup takes a BM x BN tile of C and walks over k in stages of 64: (BM + BN) * 128 bytes of LDS each, STAGES of them in flight or in use, filled straight
+// from memory (buffer_load ... lds).  Stages are 64 wide because a row's share is then a whole 128-byte line: with stages of 32 every line was asked for twice, in
+// halves, and the L2's requests, not its bytes, were the limit (8192 x 4096 x 11008, both projections: 1214 us then).  The matrix cores work through a stage
+// in two halves, each on fragments in registers while those of the next half leave LDS for another set of registers: a barrier a stage, after which the stage
+// before is filled again.  Places past the end of a row, a column or the contraction are requested beyond the buffer's extent and arrive as zeros, so every
+// size that is a multiple of 8 along rows runs the same code.
 //
 // LDS layout (a CU serves 256 bytes a cycle; of a 16-byte read the lanes {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31} of each half wave together, of
 // an 8-byte transposing read a half wave):
-//   contraction along rows   a row of the tile is 64 bytes, piece c (16 bytes) of row r in slot c ^ (-(r >> 2) & 3)
-//   down columns             row k of the stage is 2 BM (BN) bytes, its 32-byte pieces (16 columns) XORed with 3 bits of k
+//   contraction along rows   a row of the tile is 128 bytes, piece c (16 bytes) of row r in slot c ^ ((r >> 1) & 7)
+//   down columns             row k of the stage is 2 BM (BN) bytes, its 64-byte pieces (32 columns) XORed with k & 3
 // Neither meets a bank conflict, and both are whole 1 KB runs for the copies.
 #pragma once
 #include "gdn_chunk_common.h"
 
 namespace gdn {
 
-constexpr int GM_STAGES = 4, GM_K = 32;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+// 32 x 32 results, 16 deep: lane l holds index l % 32 and the contraction indices 8 (l / 32) .. + 7 of either operand; of the result column l % 32 (b's
+// index) and, in element 4 q + e, row 8 q + 4 (l / 32) + e (a's index).  Half the operand registers per product of the 16 x 16 form.
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+constexpr int GM_K = 64;
 
 // One product of a launch.  A second pair of operands (A1, B1) continues the contraction of the first (segments == 2, K columns each).
 struct GemmOperands {
@@ -47,65 +54,68 @@ constexpr int64_t GM_EXTENT = 1ll << 31;
 
 // One operand's share in a step: how its tile of ROWS rows (or columns) comes from memory and how its fragments are read.
 // DOWN: the contraction runs down the columns of the stored matrix.
-template <typename T, int ROWS, bool DOWN>
+// SPREAD (the operand whose index becomes the rows of a result): row i of a fragment is row 16 ((i >> 2) & 1) + 4 (i >> 3) + (i & 3) of its 32, so that a
+// lane's sixteen results are neighbours.
+template <typename T, int ROWS, bool DOWN, bool SPREAD>
 struct GemmSide {
-    static constexpr int BYTES = ROWS * 64, PIECES = BYTES / 1024;
+    static constexpr int BYTES = ROWS * 2 * GM_K, PIECES = BYTES / 1024;
     static constexpr int SLOTS = ROWS / 16;                          // DOWN: 32-byte pieces of a stage's row
-    static_assert(!DOWN || SLOTS >= 4, "at least four pieces to a row");
-    static __device__ __forceinline__ int flip(int k) {              // DOWN: the XOR of row k's pieces
-        return SLOTS >= 8 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
-    }
+    static_assert(!DOWN || SLOTS >= 8, "256 bytes to a row at least");
+    // !DOWN: where along k this lane's 16 bytes of piece p begin
+    static __device__ __forceinline__ int first_k(int p, int lane) { return 8 * ((lane & 7) ^ (4 * (p & 1) + (lane >> 4))); }
     // byte offset of this lane's 16 bytes of piece p from the tile's corner, GM_NOWHERE where the matrix ends before
     static __device__ __forceinline__ uint32_t source(int p, int lane, int64_t ld, int left) {
         if constexpr (!DOWN) {
-            const int row = 16 * p + (lane >> 2), c = (lane & 3) ^ (-(lane >> 4) & 3);
-            return row < left ? (uint32_t)(row * (int)ld * 2 + 16 * c) : GM_NOWHERE;
+            const int row = 8 * p + (lane >> 3);
+            return row < left ? (uint32_t)(row * (int)ld * 2 + 2 * first_k(p, lane)) : GM_NOWHERE;
         } else {
             constexpr int LANES = 2 * SLOTS;                         // 16-byte pieces of a row
-            const int k = (64 / LANES) * p + lane / LANES, s = lane % LANES, c = 2 * ((s >> 1) ^ flip(k)) + (s & 1);
+            const int k = (64 / LANES) * p + lane / LANES, s = lane % LANES, c = s ^ (4 * (k & 3));
             return 8 * c < left ? (uint32_t)(k * (int)ld * 2 + 16 * c) : GM_NOWHERE;
         }
     }
-    // this lane's share of the place of a fragment, and the fragment of the 16 rows (columns) 16 i ..
+    // this lane's share of the place of a fragment, and the fragment of the 32 rows (columns) 32 i .., contraction indices 16 kk ..
     static __device__ __forceinline__ uint32_t share(int lane) {
-        const int c16 = lane & 15, g = lane >> 4;
-        if constexpr (!DOWN) return (uint32_t)(c16 * 64 + 16 * (g ^ (-(c16 >> 2) & 3)));
-        else {
-            const int k = 8 * g + (c16 >> 2);                        // (and k + 4: the same XOR)
-            return (uint32_t)(k * 2 * ROWS + 32 * flip(k) + 8 * (c16 & 3));
+        if constexpr (!DOWN) {
+            const int l = lane & 31, r = SPREAD ? 16 * ((l >> 2) & 1) + 4 * (l >> 3) + (l & 3) : l;
+            return (uint32_t)(r * 128 + 16 * ((lane >> 5) ^ ((r >> 1) & 7)));
+        } else {
+            // sixteen lanes read four rows of k, four runs of four columns each; run t of a fragment's eight
+            const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), t = 4 * ((lane >> 4) & 1) + (lane & 3), run = SPREAD ? 4 * (t & 1) + (t >> 1) : t;
+            return (uint32_t)(k * 2 * ROWS + 64 * (k & 3) + 8 * run);
         }
     }
-    static __device__ __forceinline__ typename Mma<T>::V8 fragment(const char* stage, uint32_t share, int i) {
+    static __device__ __forceinline__ typename Mma<T>::V8 fragment(const char* stage, uint32_t share, int i, int kk) {
         typedef typename Mma<T>::V8 V8;
-        if constexpr (!DOWN) return *(const V8*)(stage + share + 1024 * i);
+        if constexpr (!DOWN) return *(const V8*)(stage + (share ^ (uint32_t)(32 * kk)) + 4096 * i);
         else {
-            const char* at = stage + (share ^ (uint32_t)(32 * i));
-            return join<V8>(Mma<T>::tr_read((const T*)at), Mma<T>::tr_read((const T*)(at + 8 * ROWS)));
+            const char* at = stage + (share ^ (uint32_t)(64 * i)) + 32 * ROWS * kk;
+            return join<V8>(Mma<T>::tr_read((const T*)at), Mma<T>::tr_read((const T*)(at + 8 * ROWS)));      // (k and k + 4: the same XOR)
         }
     }
 };
 
 // The workgroup's tile of C.  DUAL: the tile's first BN / 2 columns come from B[0], the others from B[1] at the same columns (two products of the same A,
 // side by side in every wave); else B[1] is the second segment's.
-template <typename T, int BM, int BN, int WM, int WN, bool A_DOWN, bool B_DOWN, bool DUAL>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, bool DUAL>
 struct Gemm {
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MT = BM / WM / 16, NT = BN / WN / 16;
-    static constexpr int STAGE = (BM + BN) * 64, LDS = GM_STAGES * STAGE;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MT = BM / WM / 32, NT = BN / WN / 32;
+    static constexpr int STAGE = (BM + BN) * 2 * GM_K, LDS = STAGES * STAGE;
     static constexpr int COLUMNS = DUAL ? BN / 2 : BN;               // columns of C (of each product)
-    typedef GemmSide<T, BM, A_DOWN> SideA;
-    typedef GemmSide<T, BN, B_DOWN> SideB;
+    typedef GemmSide<T, BM, A_DOWN, false> SideA;
+    typedef GemmSide<T, BN, B_DOWN, true> SideB;
     static constexpr int PA = SideA::PIECES / WAVES, PB = SideB::PIECES / WAVES;
     static_assert(SideA::PIECES % WAVES == 0 && SideB::PIECES % WAVES == 0 && !(DUAL && B_DOWN), "whole pieces to every wave");
     static_assert(!DUAL || NT % 2 == 0, "both products in every wave");
     typedef typename Mma<T>::V8 V8;
 
-    // the column (of C, in the tile) of a wave's fragment j, in tiles of 16; DUAL: j and j + NT / 2 are the same column of the two products
+    // the column (of C, in the tile) of a wave's fragment j, in tiles of 32; DUAL: j and j + NT / 2 are the same column of the two products
     static __device__ __forceinline__ int column_tile(int wn, int j) {
-        return DUAL ? (j < NT / 2 ? wn * (NT / 2) + j : BN / 32 + wn * (NT / 2) + j - NT / 2) : wn * NT + j;
+        return DUAL ? (j < NT / 2 ? wn * (NT / 2) + j : BN / 64 + wn * (NT / 2) + j - NT / 2) : wn * NT + j;
     }
 
     // `part` of p.splits: that share of the contraction's steps
-    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, int part, char* smem, f32x4 (&acc)[NT][MT]) {
+    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, int part, char* smem, f32x16 (&acc)[NT][MT]) {
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w % WM, wn = w / WM;
         const int m0 = tm * BM, n0 = tn * COLUMNS;
         uint32_t va[PA], vb[PB];
@@ -116,7 +126,6 @@ struct Gemm {
             const int piece = w * PB + i;
             vb[i] = SideB::source(DUAL ? piece % (SideB::PIECES / 2) : piece, lane, p.ldb, p.N - n0);
         }
-        const int chunk8 = 8 * ((lane & 3) ^ (-(lane >> 4) & 3));    // where this lane's piece of a row along k begins
         const int steps = max(1, (p.K + GM_K - 1) / GM_K), all = steps * p.segments;      // (no contraction at all: one step on zeros)
         const int begin = (int)((int64_t)all * part / p.splits), total = (int)((int64_t)all * (part + 1) / p.splits) - begin;
 
@@ -141,8 +150,8 @@ struct Gemm {
         uint32_t ea = 0, eb = 0;
         auto request = [&](int i) {
             if (i == 0) { ea = extent(A_DOWN, lda2, m0); eb = extent(B_DOWN, ldb2, n0); }
-            if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && chunk8 >= left ? GM_NOWHERE : va[i < PA ? i : 0], to + 1024 * (w * PA + i));
-            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && chunk8 >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], to + SideA::BYTES + 1024 * (w * PB + i - PA));
+            if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && SideA::first_k(w * PA + i, lane) >= left ? GM_NOWHERE : va[i < PA ? i : 0], to + 1024 * (w * PA + i));
+            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && SideB::first_k(w * PB + i - PA, lane) >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], to + SideA::BYTES + 1024 * (w * PB + i - PA));
             if (i < PA + PB - 1) return;
             ++asked;
             const bool second = asked == until_second;
@@ -152,45 +161,51 @@ struct Gemm {
             to = to + STAGE == LDS ? 0 : to + STAGE;
         };
         const uint32_t sa = SideA::share(lane), sb = SideB::share(lane);
-        V8 fa[2][MT], fb[2][NT];
-        // fragment i of NT + MT of step t
-        auto fetch = [&](int t, int i, V8 (&a)[MT], V8 (&b)[NT]) {
-            const char* stage = smem + (t % GM_STAGES) * STAGE;
-            if (i < NT) b[i < NT ? i : 0] = SideB::fragment(stage + SideA::BYTES, sb, column_tile(wn, i));
-            else a[i < NT ? 0 : i - NT] = SideA::fragment(stage, sa, wm * MT + i - NT);
+        struct Fragments { V8 a[2][MT], b[2][NT]; } f0, f1;              // of the two halves of a stage
+        constexpr int FRAGMENTS = 2 * (NT + MT), ROUNDS = 2 * MT, COPIES = PA + PB;
+        // fragment i of a half of the stage at `from`: in the order in which the products ask for them
+        auto fetch = [&](const char* from, int half, int i, Fragments& f) {
+            const int kk = i / (NT + MT), x = i % (NT + MT);
+            if (x < NT) f.b[kk][x < NT ? x : 0] = SideB::fragment(from + SideA::BYTES, sb, column_tile(wn, x), 2 * half + kk);
+            else f.a[kk][x < NT ? 0 : x - NT] = SideA::fragment(from, sa, wm * MT + x - NT, 2 * half + kk);
         };
-        // A step's products in MT rounds, each with its share of the fragments of the next step and of the copies in front of its NT products: whatever they take
-        // to issue hides behind the products, which one after the other keep the matrix core busy.
-        auto step = [&](int t, V8 (&a)[MT], V8 (&b)[NT], V8 (&a1)[MT], V8 (&b1)[NT]) {
-            wait_vm_at_most<(GM_STAGES - 2) * (PA + PB)>();          // this wave's share of stage t + 1 is there
-            lds_barrier();                                           // ... everyone's is, and everyone has read stage t
+        // The products of half a stage in rounds of NT, each with its share of the next half's fragments in front (and, early on, of the copies): whatever
+        // they take to issue hides behind the products, which one after the other keep the matrix core busy.
+        auto half = [&](Fragments& now, const char* from, int which, Fragments& next, bool copies) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
+            for (int i = 0; i < ROUNDS; ++i) {
 #pragma unroll
-                for (int f = i * (NT + MT) / MT; f < (i + 1) * (NT + MT) / MT; ++f) fetch(t + 1, f, a1, b1);
+                for (int f = i * FRAGMENTS / ROUNDS; f < (i + 1) * FRAGMENTS / ROUNDS; ++f) fetch(from, which, f, next);
+                if (copies && i < ROUNDS / 2) {
 #pragma unroll
-                for (int r = i * (PA + PB) / MT; r < (i + 1) * (PA + PB) / MT; ++r) request(r);
+                    for (int r = i * COPIES * 2 / ROUNDS; r < (i + 1) * COPIES * 2 / ROUNDS; ++r) request(r);
+                }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j][i] = Mma<T>::run(b[j], a[i], acc[j][i]);
+                for (int j = 0; j < NT; ++j) acc[j][i % MT] = mma32(now.b[i / MT][j], now.a[i / MT][i % MT], acc[j][i % MT]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int t = 0; t < GM_STAGES; ++t)
+                for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
 #pragma unroll
-            for (int r = 0; r < PA + PB; ++r) request(r);
-        wait_vm_at_most<(GM_STAGES - 1) * (PA + PB)>();
+        for (int t = 0; t < STAGES; ++t)
+#pragma unroll
+            for (int r = 0; r < COPIES; ++r) request(r);
+        wait_vm_at_most<(STAGES - 1) * COPIES>();
         lds_barrier();
 #pragma unroll
-        for (int f = 0; f < NT + MT; ++f) fetch(0, f, fa[0], fb[0]);
-        // (an odd number of steps: one more on zeros)
-        for (int t = 0; t < total; t += 2) {
-            step(t, fa[0], fb[0], fa[1], fb[1]);
-            step(t + 1, fa[1], fb[1], fa[0], fb[0]);
+        for (int f = 0; f < FRAGMENTS; ++f) fetch(smem, 0, f, f0);
+        uint32_t from = 0;
+        for (int s = 0; s < total; ++s) {
+            half(f0, smem + from, 1, f1, false);
+            wait_vm_at_most<(STAGES - 2) * COPIES>();                // this wave's share of the next stage is there
+            lds_barrier();                                           // ... everyone's is, and everyone has read this stage
+            from = from + STAGE == LDS ? 0 : from + STAGE;
+            half(f1, smem + from, 0, f0, true);
         }
         wait_vm_at_most<0>();                                        // no copy into LDS outlives the workgroup, or meets the epilogue's use of it
         lds_barrier();

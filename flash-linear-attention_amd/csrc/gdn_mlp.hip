@@ -35,43 +35,46 @@ struct MlpGemm {
 
 enum MlpEpilogue { MLP_PLAIN, MLP_GATE, MLP_GRAD };
 
-// What becomes of four neighbours of a result (of both products where there are two), at offset `at` of the outputs.
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs.
 template <typename T, int EPI>
-__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x4 x, f32x4 u) {
-    typedef typename Mma<T>::V4 V4;
+__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x8 x, f32x8 u) {
+    typedef typename Mma<T>::V8 V8;
+    auto rounded = [](f32x8 v) { return V8{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]}; };
     if constexpr (EPI == MLP_PLAIN) {
-        *(V4*)((T*)p.C[which] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+        *(V8*)((T*)p.C[which] + at) = rounded(x);
     } else if constexpr (EPI == MLP_GATE) {
-        V4 h;
+        V8 h;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
             float a, da;
             mlp_act(p.act, x[e], a, da);
             h[e] = (T)(a * u[e]);
         }
-        *(V4*)((T*)p.C[0] + at) = h;
+        *(V8*)((T*)p.C[0] + at) = h;
         if (p.C[1]) {
-            *(V4*)((T*)p.C[1] + at) = V4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-            *(V4*)((T*)p.C[2] + at) = V4{(T)u[0], (T)u[1], (T)u[2], (T)u[3]};
+            *(V8*)((T*)p.C[1] + at) = rounded(x);
+            *(V8*)((T*)p.C[2] + at) = rounded(u);
         }
     } else {
-        const V4 gv = *(const V4*)((const T*)p.G + at), uv = *(const V4*)((const T*)p.U + at);
-        V4 dg, du;
+        const V8 gv = *(const V8*)((const T*)p.G + at), uv = *(const V8*)((const T*)p.U + at);
+        V8 dg, du;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
             float a, da;
             mlp_act(p.act, (float)gv[e], a, da);
             dg[e] = (T)(x[e] * (float)uv[e] * da);
             du[e] = (T)(x[e] * a);
         }
-        *(V4*)((T*)p.C[0] + at) = dg;
-        *(V4*)((T*)p.C[1] + at) = du;
+        *(V8*)((T*)p.C[0] + at) = dg;
+        *(V8*)((T*)p.C[1] + at) = du;
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool A_DOWN, bool B_DOWN, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    typedef Gemm<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
     extern __shared__ __align__(16) char smem[];
     int tile = gemm_tile_of((int)blockIdx.x, p.tiles), which = 0;
     while (which + 1 < p.ops && tile >= p.op[which + 1].first) ++which;
@@ -81,27 +84,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     const int area = o.tiles_m * o.tiles_n, part = tile / area;
     int tm, tn;
     gemm_place(tile - part * area, o.tiles_m, o.tiles_n, tm, tn);
-    f32x4 acc[G::NT][G::MT];
+    f32x16 acc[G::NT][G::MT];
     G::run(o, tm, tn, part, smem, acc);
 
-    const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % WM, wn = w / WM, c16 = lane & 15, g4 = 4 * (lane >> 4);
+    const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % WM, wn = w / WM;
     constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
-        const int m = tm * BM + 16 * (wm * G::MT + i) + c16;
+        const int m = tm * BM + 32 * (wm * G::MT + i) + (lane & 31);
         if (m >= o.M) continue;
 #pragma unroll
         for (int j = 0; j < COLS; ++j) {
-            const int n = tn * G::COLUMNS + 16 * G::column_tile(wn, j) + g4;
-            if (n >= o.N) continue;
-            const int64_t at = (int64_t)m * o.N + n;
-            const f32x4 x = acc[j][i], u = acc[j + (KINDS - 1) * COLS][i];
-            if (o.splits > 1) {
-                float* to = p.part + (int64_t)part * KINDS * o.M * o.N + at;
-                *(f32x4*)to = x;
-                if (KINDS == 2) *(f32x4*)(to + (int64_t)o.M * o.N) = u;
-            } else
-                mlp_result<T, EPI>(p, which, at, x, u);
+#pragma unroll
+            for (int q = 0; q < 16; q += 8) {
+                const int n = tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * (lane >> 5) + q;
+                if (n >= o.N) continue;
+                const int64_t at = (int64_t)m * o.N + n;
+                f32x8 x, u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { x[e] = acc[j][i][q + e]; u[e] = acc[j + (KINDS - 1) * COLS][i][q + e]; }
+                if (o.splits > 1) {
+                    float* to = p.part + (int64_t)part * KINDS * o.M * o.N + at;
+                    *(f32x8*)to = x;
+                    if (KINDS == 2) *(f32x8*)(to + (int64_t)o.M * o.N) = u;
+                } else
+                    mlp_result<T, EPI>(p, which, at, x, u);
+            }
         }
     }
 }
@@ -111,12 +119,12 @@ template <typename T, int EPI>
 __global__ __launch_bounds__(256) void mlp_join_kernel(MlpGemm p) {
     constexpr int KINDS = EPI == MLP_GATE ? 2 : 1;
     const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (at >= size) return;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f}, u = x;
+    f32x8 x = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, u = x;
     for (int s = 0; s < p.op[0].splits; ++s) {
-        x += *(const f32x4*)(p.part + s * KINDS * size + at);
-        if (KINDS == 2) u += *(const f32x4*)(p.part + (s * KINDS + 1) * size + at);
+        x += *(const f32x8*)(p.part + s * KINDS * size + at);
+        if (KINDS == 2) u += *(const f32x8*)(p.part + (s * KINDS + 1) * size + at);
     }
     mlp_result<T, EPI>(p, 0, at, x, u);
 }
@@ -128,7 +136,7 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 }
 
 // How a product (or several in a launch) is cut: the tile, and into how many parts the contraction.
-struct MlpPlan { bool large; int splits; };
+struct MlpPlan { int large; int splits; };
 static MlpPlan plan_gemm(const MlpGemm& p, int kinds) {
     int64_t large = 0, small = 0;
     for (int i = 0; i < p.ops; ++i) {
@@ -152,9 +160,9 @@ static size_t plan_bytes(const MlpGemm& p, int kinds) {
 
 struct Workspace { void* at; size_t bytes; };
 
-template <typename T, int BM, int BN, int WM, int WN, bool A_DOWN, bool B_DOWN, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, hipStream_t stream) {
-    typedef Gemm<T, BM, BN, WM, WN, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    typedef Gemm<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
         GemmOperands& o = p.op[i];
@@ -166,7 +174,7 @@ static int launch_tiles(MlpGemm& p, hipStream_t stream) {
     }
     if (tiles == 0) return GDN_OK;
     p.tiles = (int)tiles;
-    auto kernel = mlp_gemm_kernel<T, BM, BN, WM, WN, A_DOWN, B_DOWN, EPI>;
+    auto kernel = mlp_gemm_kernel<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI>;
     const int rc = ensure_dynamic_smem_for((const void*)kernel, G::LDS, "mlp_gemm_kernel");
     if (rc != GDN_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)p.tiles), dim3(G::THREADS), G::LDS, stream, p);
@@ -183,10 +191,11 @@ static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
                       plan_bytes(p, KINDS));
         p.part = (float*)ws.at;
     }
-    int rc = plan.large ? launch_tiles<T, 256, 256, 2, 4, A_DOWN, B_DOWN, EPI>(p, stream) : launch_tiles<T, 128, 128, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream);
+    int rc = plan.large == 1 ? launch_tiles<T, 256, 256, 2, 4, 2, A_DOWN, B_DOWN, EPI>(p, stream) : plan.large == 2 ? launch_tiles<T, 256, 128, 2, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream) :
+                                                                                                                    launch_tiles<T, 128, 128, 2, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream);
     if (rc != GDN_OK || plan.splits <= 1) return rc;
     const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
-    hipLaunchKernelGGL((mlp_join_kernel<T, EPI>), dim3((unsigned)((size / 4 + 255) / 256)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((mlp_join_kernel<T, EPI>), dim3((unsigned)((size / 8 + 255) / 256)), dim3(256), 0, stream, p);
     return check_launch("mlp_join_kernel");
 }
 
