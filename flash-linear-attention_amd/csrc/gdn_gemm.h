@@ -1,10 +1,11 @@
 // Matrix products of 16-bit operands for large row counts: C[m][n] = sum_k A(m, k) B(n, k), fp32 accumulators, with either operand stored with the
 // contraction along its rows (A[m][k]) or down its columns (A[k][m]).  What becomes of an accumulator is an epilogue's business.
 //
-// A workgroup takes a BM x BN tile of C and walks over k in stages of 64: (BM + BN) * 128 bytes of LDS each, STAGES of them in flight or in use, filled straight
+// A workgroup takes a BM x BN tile of C and walks over k in stages of KS = 64: (BM + BN) * 128 bytes of LDS each, STAGES of them in flight or in use, filled straight
 // from memory (buffer_load ... lds).  Stages are 64 wide because a row's share is then a whole 128-byte line: with stages of 32 every line was asked for twice, in
-// halves, and the L2's requests, not its bytes, were the limit (8192 x 4096 x 11008, both projections: 1214 us then).  The matrix cores work through a stage
-// in two halves, each on fragments in registers while those of the next half leave LDS for another set of registers: a barrier a stage, after which the stage
+// halves, and the L2's requests, not its bytes, were the limit (8192 x 4096 x 11008, both projections: 1214 -> 1178 us).  Where both operands have the
+// contraction down their columns a stage of 32 asks for whole lines as well, and four of those keep requests in flight longer.  The matrix cores work through a stage
+// in halves of 32, each on fragments in registers while those of the next half leave LDS for another set of registers: a barrier a stage, after which the stage
 // before is filled again.  Places past the end of a row, a column or the contraction are requested beyond the buffer's extent and arrive as zeros, so every
 // size that is a multiple of 8 along rows runs the same code.
 //
@@ -24,7 +25,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-constexpr int GM_K = 64;
+
 
 // One product of a launch.  A second pair of operands (A1, B1) continues the contraction of the first (segments == 2, K columns each).
 struct GemmOperands {
@@ -33,7 +34,6 @@ struct GemmOperands {
     int M, N, K, segments;
     int tiles_m, tiles_n;
     int first;                           // the launch's tile where this product begins
-    int splits;                          // parts of the contraction, a workgroup each
 };
 
 typedef uint32_t gm_rsrc __attribute__((ext_vector_type(4)));
@@ -56,11 +56,11 @@ constexpr int64_t GM_EXTENT = 1ll << 31;
 // DOWN: the contraction runs down the columns of the stored matrix.
 // SPREAD (the operand whose index becomes the rows of a result): row i of a fragment is row 16 ((i >> 2) & 1) + 4 (i >> 3) + (i & 3) of its 32, so that a
 // lane's sixteen results are neighbours.
-template <typename T, int ROWS, bool DOWN, bool SPREAD>
+template <typename T, int ROWS, int KS, bool DOWN, bool SPREAD>
 struct GemmSide {
-    static constexpr int BYTES = ROWS * 2 * GM_K, PIECES = BYTES / 1024;
+    static constexpr int BYTES = ROWS * 2 * KS, PIECES = BYTES / 1024;
     static constexpr int SLOTS = ROWS / 16;                          // DOWN: 32-byte pieces of a stage's row
-    static_assert(!DOWN || SLOTS >= 8, "256 bytes to a row at least");
+    static_assert(DOWN ? SLOTS >= 8 : KS == 64, "256 bytes to a row of k at least, whole lines of a row along k");
     // !DOWN: where along k this lane's 16 bytes of piece p begin
     static __device__ __forceinline__ int first_k(int p, int lane) { return 8 * ((lane & 7) ^ (4 * (p & 1) + (lane >> 4))); }
     // byte offset of this lane's 16 bytes of piece p from the tile's corner, GM_NOWHERE where the matrix ends before
@@ -97,13 +97,13 @@ struct GemmSide {
 
 // The workgroup's tile of C.  DUAL: the tile's first BN / 2 columns come from B[0], the others from B[1] at the same columns (two products of the same A,
 // side by side in every wave); else B[1] is the second segment's.
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, bool DUAL>
+template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, bool DUAL>
 struct Gemm {
-    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MT = BM / WM / 32, NT = BN / WN / 32;
-    static constexpr int STAGE = (BM + BN) * 2 * GM_K, LDS = STAGES * STAGE;
+    static constexpr int ROWS = BM, WAVES_M = WM, WAVES = WM * WN, THREADS = 64 * WAVES, MT = BM / WM / 32, NT = BN / WN / 32;
+    static constexpr int STAGE = (BM + BN) * 2 * KS, LDS = STAGES * STAGE;
     static constexpr int COLUMNS = DUAL ? BN / 2 : BN;               // columns of C (of each product)
-    typedef GemmSide<T, BM, A_DOWN, false> SideA;
-    typedef GemmSide<T, BN, B_DOWN, true> SideB;
+    typedef GemmSide<T, BM, KS, A_DOWN, false> SideA;
+    typedef GemmSide<T, BN, KS, B_DOWN, true> SideB;
     static constexpr int PA = SideA::PIECES / WAVES, PB = SideB::PIECES / WAVES;
     static_assert(SideA::PIECES % WAVES == 0 && SideB::PIECES % WAVES == 0 && !(DUAL && B_DOWN), "whole pieces to every wave");
     static_assert(!DUAL || NT % 2 == 0, "both products in every wave");
@@ -114,8 +114,8 @@ struct Gemm {
         return DUAL ? (j < NT / 2 ? wn * (NT / 2) + j : BN / 64 + wn * (NT / 2) + j - NT / 2) : wn * NT + j;
     }
 
-    // `part` of p.splits: that share of the contraction's steps
-    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, int part, char* smem, f32x16 (&acc)[NT][MT]) {
+    // `part` of `parts`: that share of the contraction's stages
+    static __device__ __forceinline__ void run(const GemmOperands& p, int tm, int tn, int part, int parts, char* smem, f32x16 (&acc)[NT][MT]) {
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w % WM, wn = w / WM;
         const int m0 = tm * BM, n0 = tn * COLUMNS;
         uint32_t va[PA], vb[PB];
@@ -126,13 +126,13 @@ struct Gemm {
             const int piece = w * PB + i;
             vb[i] = SideB::source(DUAL ? piece % (SideB::PIECES / 2) : piece, lane, p.ldb, p.N - n0);
         }
-        const int steps = max(1, (p.K + GM_K - 1) / GM_K), all = steps * p.segments;      // (no contraction at all: one step on zeros)
-        const int begin = (int)((int64_t)all * part / p.splits), total = (int)((int64_t)all * (part + 1) / p.splits) - begin;
+        const int steps = max(1, (p.K + KS - 1) / KS), all = steps * p.segments;      // (no contraction at all: one step on zeros)
+        const int begin = (int)((int64_t)all * part / parts), total = (int)((int64_t)all * (part + 1) / parts) - begin;
 
         // where the next step's tiles begin, kept in scalar registers: a load of a parameter inside the loop would be waited for with the LDS reads
         struct Walk { uint64_t at, second; uint32_t stride; };
         auto walk = [&](const void* first, const void* second, bool down, int64_t ld, int corner) {
-            const int64_t offset = 2 * (down ? (int64_t)corner : corner * ld), stride = 2 * (down ? GM_K * ld : GM_K);
+            const int64_t offset = 2 * (down ? (int64_t)corner : corner * ld), stride = 2 * (down ? KS * ld : KS);
             const bool in_second = begin >= steps;
             return Walk{(uint64_t)(in_second ? second : first) + offset + (uint64_t)stride * (begin - (in_second ? steps : 0)), (uint64_t)second + offset, (uint32_t)stride};
         };
@@ -140,11 +140,11 @@ struct Gemm {
         const void* b0 = DUAL ? p.B[w * PB >= SideB::PIECES / 2] : p.B[0];          // (all pieces of a wave are of one product)
         Walk wb = walk(b0, p.B[1], B_DOWN, p.ldb, n0);
         const int K = p.K, lda2 = 2 * (int)p.lda, ldb2 = 2 * (int)p.ldb;
-        int asked = 0, left = K - GM_K * (begin % steps), until_second = p.segments == 2 && begin < steps ? steps - begin : -1;
+        int asked = 0, left = K - KS * (begin % steps), until_second = p.segments == 2 && begin < steps ? steps - begin : -1;
         uint32_t to = 0;
         auto extent = [&](bool down, int ld2, int corner) {
             const uint32_t whole = (uint32_t)GM_EXTENT, rest = (uint32_t)(left * ld2 - 2 * corner);
-            return asked >= total || left <= 0 ? 0u : down && left < GM_K ? rest : whole;
+            return asked >= total || left <= 0 ? 0u : down && left < KS ? rest : whole;
         };
         // the copies of one more step: this wave's piece i of PA + PB, and then on to the next step
         uint32_t ea = 0, eb = 0;
@@ -157,7 +157,7 @@ struct Gemm {
             const bool second = asked == until_second;
             wa.at = second ? wa.second : wa.at + wa.stride;
             wb.at = second ? wb.second : wb.at + wb.stride;
-            left = second ? K : left - GM_K;
+            left = second ? K : left - KS;
             to = to + STAGE == LDS ? 0 : to + STAGE;
         };
         const uint32_t sa = SideA::share(lane), sb = SideB::share(lane);
@@ -200,12 +200,25 @@ struct Gemm {
 #pragma unroll
         for (int f = 0; f < FRAGMENTS; ++f) fetch(smem, 0, f, f0);
         uint32_t from = 0;
-        for (int s = 0; s < total; ++s) {
-            half(f0, smem + from, 1, f1, false);
+        auto next_stage = [&]() {
             wait_vm_at_most<(STAGES - 2) * COPIES>();                // this wave's share of the next stage is there
             lds_barrier();                                           // ... everyone's is, and everyone has read this stage
             from = from + STAGE == LDS ? 0 : from + STAGE;
-            half(f1, smem + from, 0, f0, true);
+        };
+        if constexpr (KS == 64) {
+            for (int s = 0; s < total; ++s) {
+                half(f0, smem + from, 1, f1, false);
+                next_stage();
+                half(f1, smem + from, 0, f0, true);
+            }
+        } else {
+            // (an odd number of stages: one more, on zeros)
+            for (int s = 0; s < total; s += 2) {
+                next_stage();
+                half(f0, smem + from, 0, f1, true);
+                next_stage();
+                half(f1, smem + from, 0, f0, true);
+            }
         }
         wait_vm_at_most<0>();                                        // no copy into LDS outlives the workgroup, or meets the epilogue's use of it
         lds_barrier();

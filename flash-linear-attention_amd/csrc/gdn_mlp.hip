@@ -26,10 +26,11 @@ __device__ __forceinline__ void mlp_act(int act, float g, float& a, float& da) {
 
 struct MlpGemm {
     GemmOperands op[3];
-    int ops, tiles;
+    int ops;
+    int full, rest, parts;               // tiles with a workgroup each, and tiles after them whose contraction is shared out over `parts` workgroups
     void* C[3];                          // results (of a DUAL product's epilogue: h, g, u; of dh's: dg, du)
     const void* G; const void* U;
-    float* part;                         // splits > 1: [splits][1 or 2 (both products of a DUAL)][M][N]
+    float* sums;                         // [rest][parts][a tile's accumulators, as the lanes hold them]
     int act;
 };
 
@@ -72,131 +73,150 @@ __device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t 
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
-    extern __shared__ __align__(16) char smem[];
-    int tile = gemm_tile_of((int)blockIdx.x, p.tiles), which = 0;
-    while (which + 1 < p.ops && tile >= p.op[which + 1].first) ++which;
-    const GemmOperands& o = p.op[which];
-    tile -= o.first;
-    // (the parts of a tile one after the other: they share nothing, their neighbours in the band share rows and columns)
-    const int area = o.tiles_m * o.tiles_n, part = tile / area;
-    int tm, tn;
-    gemm_place(tile - part * area, o.tiles_m, o.tiles_n, tm, tn);
-    f32x16 acc[G::NT][G::MT];
-    G::run(o, tm, tn, part, smem, acc);
-
-    const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % WM, wn = w / WM;
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS;
-#pragma unroll
-    for (int i = 0; i < G::MT; ++i) {
-        const int m = tm * BM + 32 * (wm * G::MT + i) + (lane & 31);
-        if (m >= o.M) continue;
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) {
-#pragma unroll
-            for (int q = 0; q < 16; q += 8) {
-                const int n = tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * (lane >> 5) + q;
-                if (n >= o.N) continue;
-                const int64_t at = (int64_t)m * o.N + n;
-                f32x8 x, u;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { x[e] = acc[j][i][q + e]; u[e] = acc[j + (KINDS - 1) * COLS][i][q + e]; }
-                if (o.splits > 1) {
-                    float* to = p.part + (int64_t)part * KINDS * o.M * o.N + at;
-                    *(f32x8*)to = x;
-                    if (KINDS == 2) *(f32x8*)(to + (int64_t)o.M * o.N) = u;
-                } else
-                    mlp_result<T, EPI>(p, which, at, x, u);
-            }
-        }
-    }
+struct MlpTile { int which, tm, tn; };
+__device__ __forceinline__ MlpTile mlp_tile(const MlpGemm& p, int tile) {
+    MlpTile t{0, 0, 0};
+    while (t.which + 1 < p.ops && tile >= p.op[t.which + 1].first) ++t.which;
+    const GemmOperands& o = p.op[t.which];
+    gemm_place(tile - o.first, o.tiles_m, o.tiles_n, t.tm, t.tn);
+    return t;
 }
 
-// The parts of a contraction added up, in order, and what becomes of the sums.
-template <typename T, int EPI>
-__global__ __launch_bounds__(256) void mlp_join_kernel(MlpGemm p) {
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1;
-    const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (at >= size) return;
-    f32x8 x = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, u = x;
-    for (int s = 0; s < p.op[0].splits; ++s) {
-        x += *(const f32x8*)(p.part + s * KINDS * size + at);
-        if (KINDS == 2) u += *(const f32x8*)(p.part + (s * KINDS + 1) * size + at);
+// Eight neighbours of this lane's results of a tile: fragment (i, j), its q-th half
+template <typename T, typename G, int EPI>
+__device__ __forceinline__ void mlp_chunk(const MlpGemm& p, MlpTile t, int i, int j, int q, f32x8 x, f32x8 u) {
+    const GemmOperands& o = p.op[t.which];
+    const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % G::WAVES_M, wn = w / G::WAVES_M;
+    const int m = t.tm * G::ROWS + 32 * (wm * G::MT + i) + (lane & 31), n = t.tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * (lane >> 5) + 8 * q;
+    if (m < o.M && n < o.N) mlp_result<T, EPI>(p, t.which, (int64_t)m * o.N + n, x, u);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
+    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    extern __shared__ __align__(16) char smem[];
+    const int id = (int)blockIdx.x, shared = id - p.full;
+    int tile, part = 0;
+    if (shared < 0) tile = gemm_tile_of(id, p.full);
+    else {
+        // (part by part: neighbours share rows and columns, the parts of a tile share nothing)
+        const int at = gemm_tile_of(shared, p.rest * p.parts);
+        part = at / p.rest; tile = p.full + at % p.rest;
     }
-    mlp_result<T, EPI>(p, 0, at, x, u);
+    f32x16 acc[G::NT][G::MT];
+    const MlpTile at = mlp_tile(p, tile);
+    G::run(p.op[at.which], at.tm, at.tn, part, shared < 0 ? 1 : p.parts, smem, acc);
+
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS;
+    float* sums = shared < 0 || p.parts == 1 ? nullptr : p.sums + ((int64_t)(tile - p.full) * p.parts + part) * (BM * BN);
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < COLS; ++j)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                f32x8 x, u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { x[e] = acc[j][i][8 * q + e]; u[e] = acc[j + (KINDS - 1) * COLS][i][8 * q + e]; }
+                if (sums) {
+                    const int chunk = (i * COLS + j) * 2 + q;
+                    *(f32x8*)(sums + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8) = x;
+                    if (KINDS == 2) *(f32x8*)(sums + ((int64_t)(chunk * KINDS + 1) * G::THREADS + threadIdx.x) * 8) = u;
+                } else
+                    mlp_chunk<T, G, EPI>(p, at, i, j, q, x, u);
+            }
+}
+
+// The parts of a shared tile added up, in order, and what becomes of the sums: a workgroup for eight results of every lane.
+template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+__global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
+    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS, CHUNKS = G::MT * COLS * 2;
+    const int tile = (int)blockIdx.x / CHUNKS, chunk = (int)blockIdx.x % CHUNKS;
+    const float* sums = p.sums + (int64_t)tile * p.parts * (BM * BN) + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8;
+    f32x8 x = *(const f32x8*)sums, u = x;
+    if (KINDS == 2) u = *(const f32x8*)(sums + G::THREADS * 8);
+    for (int s = 1; s < p.parts; ++s) {
+        x += *(const f32x8*)(sums + (int64_t)s * (BM * BN));
+        if (KINDS == 2) u += *(const f32x8*)(sums + (int64_t)s * (BM * BN) + G::THREADS * 8);
+    }
+    mlp_chunk<T, G, EPI>(p, mlp_tile(p, p.full + tile), chunk / 2 / COLS, chunk / 2 % COLS, chunk % 2, x, u);
 }
 
 static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t ldb, int64_t M, int64_t N, int64_t K) {
     GemmOperands o{};
-    o.A[0] = A; o.B[0] = B; o.lda = lda; o.ldb = ldb; o.M = (int)M; o.N = (int)N; o.K = (int)K; o.segments = 1; o.splits = 1;
+    o.A[0] = A; o.B[0] = B; o.lda = lda; o.ldb = ldb; o.M = (int)M; o.N = (int)N; o.K = (int)K; o.segments = 1;
     return o;
 }
 
-// How a product (or several in a launch) is cut: the tile, and into how many parts the contraction.
-struct MlpPlan { int large; int splits; };
+// How the products of a launch are cut: 256 x 256 tiles, a workgroup of eight waves a CU, or 128 x 128, two of four waves; and over how many workgroups the
+// contraction of each tile is shared out that does not fill a round of the chip.  The least of the times that the launch would take by these figures:
+//   a stage of 64 of a full round     1.7 us (256 x 256), 1.03 us (128 x 128: 512 tiles, half the area; 0.65 us where no two share a CU)
+//   a round's begin and end           4 us; joining parts 5 us and their bytes, written and read, at 4 TB/s
+// 8192 x 2048 x 5632, the weights' gradients (528 tiles of 256 x 256, two rounds and 16 tiles): the third round shared out over 16 workgroups a tile.
+struct MlpPlan { bool large; int full, rest, parts; double us; };
 static MlpPlan plan_gemm(const MlpGemm& p, int kinds) {
-    int64_t large = 0, small = 0;
-    for (int i = 0; i < p.ops; ++i) {
-        const int64_t M = p.op[i].M, N = (int64_t)p.op[i].N * kinds;
-        large += ((M + 255) / 256) * ((N + 255) / 256);
-        small += ((M + 127) / 128) * ((N + 127) / 128);
+    MlpPlan best{true, 0, 0, 1, 1e30};
+    for (int large = 0; large < 2; ++large) {
+        const int64_t side = large ? 256 : 128, slots = large ? 256 : 512;
+        int64_t tiles = 0, stages = 1;
+        for (int i = 0; i < p.ops; ++i) {
+            tiles += ((p.op[i].M + side - 1) / side) * (((int64_t)p.op[i].N * kinds + side - 1) / side);
+            stages = std::max<int64_t>(stages, (int64_t)((p.op[i].K + 63) / 64) * p.op[i].segments);
+        }
+        if (tiles >= (1ll << 31)) continue;
+        const int64_t rest = tiles % slots, rounds = tiles / slots;
+        const double stage = large ? 1.7 : 1.03;
+        const double before = rounds * (stages * stage + 4);
+        auto tail = [&](int64_t workgroups) { return large || workgroups > 256 ? stage : 0.65; };
+        for (int64_t parts = 1; parts <= 16 && (parts == 1 || (rest * parts <= slots && stages / parts >= 2)); ++parts) {
+            double us = before + (rest ? ((stages + parts - 1) / parts) * tail(rest * parts) + 4 : 0);
+            if (parts > 1) us += 5 + rest * parts * side * side * 8 / 4e6;
+            if (us < best.us) best = MlpPlan{large != 0, parts > 1 ? (int)(tiles - rest) : (int)tiles, parts > 1 ? (int)rest : 0, (int)parts, us};
+        }
     }
-    MlpPlan plan{large >= 160, 1};
-    if (getenv("MLP_LARGE")) plan.large = atoi(getenv("MLP_LARGE"));
-    if (!plan.large && p.ops == 1) {
-        const int64_t steps = (int64_t)((p.op[0].K + GM_K - 1) / GM_K) * p.op[0].segments;
-        plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / std::max<int64_t>(small, 1), steps / 8), 16));
-        if (getenv("MLP_SPLIT")) plan.splits = atoi(getenv("MLP_SPLIT"));
-    }
-    return plan;
+    return best;
 }
-static size_t plan_bytes(const MlpGemm& p, int kinds) {
-    const MlpPlan plan = plan_gemm(p, kinds);
-    return plan.splits > 1 ? (size_t)plan.splits * kinds * p.op[0].M * p.op[0].N * 4 : 0;
-}
+static size_t plan_bytes(const MlpPlan& plan) { return (size_t)plan.rest * plan.parts * (plan.large ? 65536 : 16384) * 4; }
+static size_t plan_bytes(const MlpGemm& p, int kinds) { return plan_bytes(plan_gemm(p, kinds)); }
 
 struct Workspace { void* at; size_t bytes; };
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
-static int launch_tiles(MlpGemm& p, hipStream_t stream) {
-    typedef Gemm<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+template <typename T, int SIDE, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
+    typedef Gemm<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
         GemmOperands& o = p.op[i];
         o.first = (int)tiles;
-        o.tiles_m = (o.M + BM - 1) / BM; o.tiles_n = (o.N + G::COLUMNS - 1) / G::COLUMNS;
-        tiles += (int64_t)o.tiles_m * o.tiles_n * o.splits;
+        o.tiles_m = (o.M + SIDE - 1) / SIDE; o.tiles_n = (o.N + G::COLUMNS - 1) / G::COLUMNS;
+        tiles += (int64_t)o.tiles_m * o.tiles_n;
         GDN_CHECK_ARG(tiles < (1ll << 32) / G::THREADS, GDN_ERR_UNSUPPORTED, "the gated feed-forward block: %lld x %lld results are too many for one launch",
                       (long long)o.M, (long long)o.N);
     }
     if (tiles == 0) return GDN_OK;
-    p.tiles = (int)tiles;
-    auto kernel = mlp_gemm_kernel<T, BM, BN, WM, WN, STAGES, A_DOWN, B_DOWN, EPI>;
+    p.full = plan.full; p.rest = plan.rest; p.parts = plan.parts;
+    GDN_CHECK_ARG(tiles == (int64_t)p.full + p.rest, GDN_ERR_INVALID, "the gated feed-forward block: a plan for %d tiles, not %lld", p.full + p.rest, (long long)tiles);
+    auto kernel = mlp_gemm_kernel<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>;
     const int rc = ensure_dynamic_smem_for((const void*)kernel, G::LDS, "mlp_gemm_kernel");
     if (rc != GDN_OK) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)p.tiles), dim3(G::THREADS), G::LDS, stream, p);
-    return check_launch("mlp_gemm_kernel");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.full + p.rest * p.parts)), dim3(G::THREADS), G::LDS, stream, p);
+    if (p.rest == 0) return check_launch("mlp_gemm_kernel");
+    const int rc2 = check_launch("mlp_gemm_kernel");
+    if (rc2 != GDN_OK) return rc2;
+    hipLaunchKernelGGL((mlp_join_kernel<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>), dim3((unsigned)(p.rest * G::MT * G::NT * 2 / (EPI == MLP_GATE ? 2 : 1))),
+                       dim3(G::THREADS), 0, stream, p);
+    return check_launch("mlp_join_kernel");
 }
 
 template <typename T, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1;
-    const MlpPlan plan = plan_gemm(p, KINDS);
-    p.op[0].splits = plan.splits;
-    if (plan.splits > 1) {
-        GDN_CHECK_ARG(ws.at && ws.bytes >= plan_bytes(p, KINDS), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes,
-                      plan_bytes(p, KINDS));
-        p.part = (float*)ws.at;
-    }
-    int rc = plan.large == 1 ? launch_tiles<T, 256, 256, 2, 4, 2, A_DOWN, B_DOWN, EPI>(p, stream) : plan.large == 2 ? launch_tiles<T, 256, 128, 2, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream) :
-                                                                                                                    launch_tiles<T, 128, 128, 2, 2, 2, A_DOWN, B_DOWN, EPI>(p, stream);
-    if (rc != GDN_OK || plan.splits <= 1) return rc;
-    const int64_t size = (int64_t)p.op[0].M * p.op[0].N;
-    hipLaunchKernelGGL((mlp_join_kernel<T, EPI>), dim3((unsigned)((size / 8 + 255) / 256)), dim3(256), 0, stream, p);
-    return check_launch("mlp_join_kernel");
+    const MlpPlan plan = plan_gemm(p, EPI == MLP_GATE ? 2 : 1);
+    const size_t need = plan_bytes(plan);
+    GDN_CHECK_ARG(need == 0 || (ws.at && ws.bytes >= need), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes, need);
+    p.sums = (float*)ws.at;
+    constexpr int KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = 128 / KS;
+    return plan.large ? launch_tiles<T, 256, 4, KS, STAGES, A_DOWN, B_DOWN, EPI>(p, plan, stream) : launch_tiles<T, 128, 2, KS, STAGES, A_DOWN, B_DOWN, EPI>(p, plan, stream);
 }
 
 // The products of a forward and a backward pass.
@@ -224,6 +244,19 @@ static MlpGemm grad_x(const void* dg, const void* du, const void* wg, const void
     p.ops = 1;
     p.op[0] = operands(dg, wg, F, D, M, D, F);
     p.op[0].A[1] = du; p.op[0].B[1] = wu; p.op[0].segments = 2;
+    return p;
+}
+
+static MlpGemm grad_weights(const void* dy, const void* x, const void* h, const void* dg, const void* du, void* dwg, void* dwu, void* dwd, int64_t M, int64_t D, int64_t F) {
+    MlpGemm p{};
+    auto add = [&](const void* A, const void* B, int64_t rows, int64_t cols, void* C) {
+        if (!C) return;
+        p.op[p.ops] = operands(A, B, rows, cols, rows, cols, M);
+        p.C[p.ops++] = C;
+    };
+    add(dg, x, F, D, dwg);
+    add(du, x, F, D, dwu);
+    add(dy, h, D, F, dwd);
     return p;
 }
 
@@ -255,15 +288,7 @@ static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu
         rc = launch_gemm<T, false, true, MLP_PLAIN>(p, ws, stream);
         if (rc != GDN_OK) return rc;
     }
-    MlpGemm p{};
-    auto add = [&](const void* A, const void* B, int64_t rows, int64_t cols, void* C) {
-        if (!C) return;
-        p.op[p.ops] = operands(A, B, rows, cols, rows, cols, M);
-        p.C[p.ops++] = C;
-    };
-    add(dg, x, F, D, dwg);
-    add(du, x, F, D, dwu);
-    add(dy, h, D, F, dwd);
+    MlpGemm p = grad_weights(dy, x, h, dg, du, dwg, dwu, dwd, M, D, F);
     return p.ops ? launch_gemm<T, true, true, MLP_PLAIN>(p, ws, stream) : GDN_OK;
 }
 
@@ -284,7 +309,14 @@ static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, 
 extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward) {
     if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16) != GDN_OK || M == 0) return 0;
     if (!backward) return std::max(plan_bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2), plan_bytes(down(nullptr, nullptr, M, D, F), 1));
-    return std::max(plan_bytes(grad_inner(nullptr, nullptr, M, D, F), 1), plan_bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1));
+    size_t most = std::max(plan_bytes(grad_inner(nullptr, nullptr, M, D, F), 1), plan_bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1));
+    // (which of the weights' gradients will be asked for is not known here: those of Wg and Wu are alike)
+    char some;
+    for (int asked = 1; asked < 6; ++asked) {
+        const int alike = asked % 3;
+        most = std::max(most, plan_bytes(grad_weights(nullptr, nullptr, nullptr, nullptr, nullptr, alike ? &some : nullptr, alike > 1 ? &some : nullptr, asked > 2 ? &some : nullptr, M, D, F), 1));
+    }
+    return most;
 }
 
 extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
