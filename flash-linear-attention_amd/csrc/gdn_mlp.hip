@@ -149,41 +149,54 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
     return o;
 }
 
-// How the products of a launch are cut: 256 x 256 tiles, a workgroup of eight waves a CU, or 128 x 128, two of four waves; and over how many workgroups the
-// contraction of each tile is shared out that does not fill a round of the chip.  The least of the times that the launch would take by these figures:
-//   a stage of 64 of a full round     1.7 us (256 x 256), 1.03 us (128 x 128: 512 tiles, half the area; 0.65 us where no two share a CU)
-//   a round's begin and end           4 us; joining parts 5 us and their bytes, written and read, at 4 TB/s
-// 8192 x 2048 x 5632, the weights' gradients (528 tiles of 256 x 256, two rounds and 16 tiles): the third round shared out over 16 workgroups a tile.
-struct MlpPlan { bool large; int full, rest, parts; double us; };
-static MlpPlan plan_gemm(const MlpGemm& p, int kinds) {
-    MlpPlan best{true, 0, 0, 1, 1e30};
-    for (int large = 0; large < 2; ++large) {
-        const int64_t side = large ? 256 : 128, slots = large ? 256 : 512;
+// How the products of a launch are cut: the tiles, and over how many workgroups the contraction of each tile is shared out that does not fill a round of the
+// chip (`rest` tiles of `parts` workgroups after `full` of one): the least of the times that the launch would take by these figures.
+//   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)
+//   256 x 256   8      1 a CU       1.7                                   1.12
+//   128 x 128   4      2 a CU       1.0                                   0.65      two stages of LDS: half the CU's
+//   128 x 128   4      1 a CU       0.58                                  0.46      four stages: more in flight, for few workgroups
+//   64 x 64     2      2 a CU       0.45                                  0.29      the same, where no operand has the contraction down its columns
+// In between the time grows with the workgroups: a full chip is held back by its power, not by the stages.  A round begins and ends in 2.5 us; joining parts
+// takes 5.5 us and their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
+// forward): 48 rows 61 us in 128 x 128 tiles, 26 us; 333 rows 85 -> 51 us; 2000 rows 213 us in 256 x 256 tiles, 154 us.  The weights' gradients of 8192 x 2048 x
+// 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 16 parts each, the backward 1186 -> 1026 us.
+struct MlpTiles { int side, waves_n, stages, per_cu; double full, least; };
+constexpr MlpTiles MLP_TILES[] = {{256, 4, 2, 1, 1.7, 1.12}, {128, 2, 2, 2, 1.0, 0.65}, {128, 2, 4, 1, 0.58, 0.46}, {64, 1, 4, 2, 0.45, 0.29}};
+struct MlpPlan { int tiles, full, rest, parts; };
+static MlpPlan plan_gemm(const MlpGemm& p, int kinds, bool rows) {
+    MlpPlan best{0, 0, 0, 1};
+    double best_us = 1e30;
+    for (int t = 0; t < (rows ? 4 : 3); ++t) {
+        const MlpTiles& k = MLP_TILES[t];
+        const int64_t slots = 256 * k.per_cu;
         int64_t tiles = 0, stages = 1;
         for (int i = 0; i < p.ops; ++i) {
-            tiles += ((p.op[i].M + side - 1) / side) * (((int64_t)p.op[i].N * kinds + side - 1) / side);
-            stages = std::max<int64_t>(stages, (int64_t)((p.op[i].K + 63) / 64) * p.op[i].segments);
+            tiles += ((p.op[i].M + k.side - 1ll) / k.side) * (((int64_t)p.op[i].N * kinds + k.side - 1) / k.side);
+            stages = std::max<int64_t>(stages, (p.op[i].K + 63ll) / 64 * p.op[i].segments);
         }
         if (tiles >= (1ll << 31)) continue;
-        const int64_t rest = tiles % slots, rounds = tiles / slots;
-        const double stage = large ? 1.7 : 1.03;
-        const double before = rounds * (stages * stage + 4);
-        auto tail = [&](int64_t workgroups) { return large || workgroups > 256 ? stage : 0.65; };
-        for (int64_t parts = 1; parts <= 16 && (parts == 1 || (rest * parts <= slots && stages / parts >= 2)); ++parts) {
-            double us = before + (rest ? ((stages + parts - 1) / parts) * tail(rest * parts) + 4 : 0);
-            if (parts > 1) us += 5 + rest * parts * side * side * 8 / 4e6;
-            if (us < best.us) best = MlpPlan{large != 0, parts > 1 ? (int)(tiles - rest) : (int)tiles, parts > 1 ? (int)rest : 0, (int)parts, us};
+        const int64_t rest = tiles % slots;
+        const double before = (double)(tiles / slots) * (stages * k.full + 2.5);
+        for (int64_t parts = 1; parts <= 16 && (parts == 1 || (rest > 0 && rest * parts <= slots && stages / parts >= 2)); ++parts) {
+            double us = before;
+            if (rest) us += (stages + parts - 1) / parts * std::max(k.least, k.full * (rest * parts) / slots) + 2.5;
+            if (parts > 1) us += 5.5 + (double)(rest * parts) * k.side * k.side * 8 / 4e6;
+            if (us < best_us) {
+                best_us = us;
+                best = MlpPlan{t, (int)(parts > 1 ? tiles - rest : tiles), (int)(parts > 1 ? rest : 0), (int)parts};
+            }
         }
     }
     return best;
 }
-static size_t plan_bytes(const MlpPlan& plan) { return (size_t)plan.rest * plan.parts * (plan.large ? 65536 : 16384) * 4; }
-static size_t plan_bytes(const MlpGemm& p, int kinds) { return plan_bytes(plan_gemm(p, kinds)); }
+static size_t plan_bytes(const MlpPlan& plan) { return (size_t)plan.rest * plan.parts * MLP_TILES[plan.tiles].side * MLP_TILES[plan.tiles].side * 4; }
 
 struct Workspace { void* at; size_t bytes; };
 
-template <typename T, int SIDE, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+template <typename T, int TILES, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
+    // (both operands down their columns: stages of half the width, twice as many)
+    constexpr int SIDE = MLP_TILES[TILES].side, WN = MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
     typedef Gemm<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
@@ -211,12 +224,17 @@ static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
 
 template <typename T, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
-    const MlpPlan plan = plan_gemm(p, EPI == MLP_GATE ? 2 : 1);
+    constexpr bool ROWS = !A_DOWN && !B_DOWN;
+    const MlpPlan plan = plan_gemm(p, EPI == MLP_GATE ? 2 : 1, ROWS);
     const size_t need = plan_bytes(plan);
     GDN_CHECK_ARG(need == 0 || (ws.at && ws.bytes >= need), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes, need);
     p.sums = (float*)ws.at;
-    constexpr int KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = 128 / KS;
-    return plan.large ? launch_tiles<T, 256, 4, KS, STAGES, A_DOWN, B_DOWN, EPI>(p, plan, stream) : launch_tiles<T, 128, 2, KS, STAGES, A_DOWN, B_DOWN, EPI>(p, plan, stream);
+    if (plan.tiles == 0) return launch_tiles<T, 0, A_DOWN, B_DOWN, EPI>(p, plan, stream);
+    if (plan.tiles == 1) return launch_tiles<T, 1, A_DOWN, B_DOWN, EPI>(p, plan, stream);
+    if constexpr (ROWS) {
+        if (plan.tiles == 3) return launch_tiles<T, 3, A_DOWN, B_DOWN, EPI>(p, plan, stream);
+    }
+    return launch_tiles<T, 2, A_DOWN, B_DOWN, EPI>(p, plan, stream);
 }
 
 // The products of a forward and a backward pass.
@@ -260,9 +278,103 @@ static MlpGemm grad_weights(const void* dy, const void* x, const void* h, const 
     return p;
 }
 
+// ---------------------------------------------------------------------------------------------
+// A few rows (a decode step): every weight is read once and little else, so what counts is how much of the weights is in flight.  A workgroup takes CT tiles of 16
+// weight rows - eight of Wg and the eight of Wu at the same columns, or 16 rows of Wd - and its waves a share of
+// the contraction each, operands straight from memory to registers, partial sums through LDS.
+// ---------------------------------------------------------------------------------------------
+struct MlpFew {
+    const void* x; const void* w[2];
+    void* C[3];
+    int M, N, K, act;
+};
+
+template <typename T, int CT, int WAVES, int EPI, int COLS>
+__global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
+    typedef typename Mma<T>::V8 V8;
+    constexpr int U = 8, PITCH = 16 * CT + 1;                      // U: steps of 32 requested together
+    __shared__ float sums[WAVES][16][PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
+    const int n0 = (int)blockIdx.x * COLS * CT, K = p.K;
+    const int steps = (K + 31) / 32, s0 = w * steps / WAVES, s1 = (w + 1) * steps / WAVES;
+    // (columns and rows past the end repeat the last ones, their results are dropped)
+    const T* wr[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+        wr[c] = (const T*)(EPI == MLP_GATE && c16 >= 8 ? p.w[1] : p.w[0]) + (int64_t)min(n0 + COLS * c + c16 % COLS, p.N - 1) * K;
+    const T* xr = (const T*)p.x + (int64_t)min(c16, p.M - 1) * K;
+    f32x4 acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = s0; s < s1; s += U) {
+        V8 fw[CT][U], fx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s + u < s1) {                                      // (the same for the wave)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) fw[c][u] = *(const V8*)(wr[c] + min(32 * (s + u) + 8 * g, K - 8));
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) if (s + u < s1) fx[u] = *(const V8*)(xr + min(32 * (s + u) + 8 * g, K - 8));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s + u < s1) {
+                const bool past = 32 * (s + u) + 8 * g >= K;       // (in the last step of a contraction that is no multiple of 32)
+                if (past) fx[u] = V8{};
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    if (past) fw[c][u] = V8{};
+                    acc[c] = Mma<T>::run(fw[c][u], fx[u], acc[c]);
+                }
+            }
+    }
+    // lane (c16, g): row c16, columns 4g .. 4g + 3 of each tile
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[w][c16][16 * c + 4 * g + e] = acc[c][e];
+    __syncthreads();
+    for (int i = tid; i < COLS * CT * p.M; i += 64 * WAVES) {
+        const int m = i / (COLS * CT), j = i % (COLS * CT), n = n0 + j, at16 = 16 * (j / COLS) + j % COLS;
+        if (n >= p.N) continue;
+        float x = 0.f, u = 0.f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            x += sums[v][m][at16];
+            if (EPI == MLP_GATE) u += sums[v][m][at16 + 8];
+        }
+        const int64_t at = (int64_t)m * p.N + n;
+        if constexpr (EPI == MLP_GATE) {
+            float a, da;
+            mlp_act(p.act, x, a, da);
+            ((T*)p.C[0])[at] = (T)(a * u);
+            if (p.C[1]) { ((T*)p.C[1])[at] = (T)x; ((T*)p.C[2])[at] = (T)u; }
+        } else
+            ((T*)p.C[0])[at] = (T)x;
+    }
+}
+
+// Up to 16 rows (one matrix tile of them): 16 rows of 2048 x 5632 24.3 us, in 64 x 64 tiles 25.7; one row 19.5 us against 25.3.  Rows of x cost a workgroup as much
+// as a tile of weights, so from five rows on it takes three tiles of Wg and Wu: 16 rows 26.7 -> 24.3 us; one row of 4096 x 11008 50.6 us with one tile
+// (270 MB: 5.3 TB/s), 54.5 with three.
+constexpr int64_t MLP_FEW_ROWS = 16;
+
+template <typename T, int CT, int EPI>
+static int launch_few(const MlpFew& p, hipStream_t stream) {
+    constexpr int WAVES = 8, COLS = EPI == MLP_GATE ? 8 : 16;
+    hipLaunchKernelGGL((mlp_few_kernel<T, CT, WAVES, EPI, COLS>), dim3((unsigned)((p.N + COLS * CT - 1) / (COLS * CT))), dim3(64 * WAVES), 0, stream, p);
+    return check_launch("mlp_few_kernel");
+}
+
 template <typename T>
 static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h, Workspace ws, int64_t M, int64_t D, int64_t F,
                    int act, hipStream_t stream) {
+    if (M <= MLP_FEW_ROWS) {
+        const MlpFew first{x, {wg, wu}, {h, g, u}, (int)M, (int)F, (int)D, act};
+        const int rc = M <= 4 ? launch_few<T, 1, MLP_GATE>(first, stream) : launch_few<T, 3, MLP_GATE>(first, stream);
+        return rc != GDN_OK ? rc : launch_few<T, 1, MLP_PLAIN>(MlpFew{h, {wd, wd}, {y, nullptr, nullptr}, (int)M, (int)D, (int)F, act}, stream);
+    }
     MlpGemm p = gate_up(x, wg, wu, M, D, F);
     p.act = act; p.C[0] = h; p.C[1] = g; p.C[2] = u;
     const int rc = launch_gemm<T, false, false, MLP_GATE>(p, ws, stream);
@@ -308,14 +420,15 @@ static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, 
 
 extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward) {
     if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16) != GDN_OK || M == 0) return 0;
-    if (!backward) return std::max(plan_bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2), plan_bytes(down(nullptr, nullptr, M, D, F), 1));
-    size_t most = std::max(plan_bytes(grad_inner(nullptr, nullptr, M, D, F), 1), plan_bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1));
-    // (which of the weights' gradients will be asked for is not known here: those of Wg and Wu are alike)
+    auto bytes = [](const MlpGemm& p, int kinds, bool rows) { return plan_bytes(plan_gemm(p, kinds, rows)); };
+    if (!backward) return M <= MLP_FEW_ROWS ? 0 : std::max(bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2, true), bytes(down(nullptr, nullptr, M, D, F), 1, true));
+    size_t most = std::max(bytes(grad_inner(nullptr, nullptr, M, D, F), 1, false), bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1, false));
+    // (which of the weights' gradients will be asked for is not known here: none, one or both of Wg's and Wu's, which are alike, with Wd's or without)
     char some;
-    for (int asked = 1; asked < 6; ++asked) {
-        const int alike = asked % 3;
-        most = std::max(most, plan_bytes(grad_weights(nullptr, nullptr, nullptr, nullptr, nullptr, alike ? &some : nullptr, alike > 1 ? &some : nullptr, asked > 2 ? &some : nullptr, M, D, F), 1));
-    }
+    for (int inner = 0; inner < 3; ++inner)
+        for (int with_down = inner == 0; with_down < 2; ++with_down)
+            most = std::max(most, bytes(grad_weights(nullptr, nullptr, nullptr, nullptr, nullptr, inner > 0 ? &some : nullptr, inner > 1 ? &some : nullptr,
+                                                     with_down ? &some : nullptr, M, D, F), 1, false));
     return most;
 }
 
