@@ -38,9 +38,10 @@ enum MlpEpilogue { MLP_PLAIN, MLP_GATE, MLP_GRAD };
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs.
+// What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs; MLP_GRAD: gv, uv are the forward's
+// g and u there.
 template <typename T, int EPI>
-__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x8 x, f32x8 u) {
+__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x8 x, f32x8 u, typename Mma<T>::V8 gv, typename Mma<T>::V8 uv) {
     typedef typename Mma<T>::V8 V8;
     auto rounded = [](f32x8 v) { return V8{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]}; };
     if constexpr (EPI == MLP_PLAIN) {
@@ -59,7 +60,6 @@ __device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t 
             *(V8*)((T*)p.C[2] + at) = rounded(u);
         }
     } else {
-        const V8 gv = *(const V8*)((const T*)p.G + at), uv = *(const V8*)((const T*)p.U + at);
         V8 dg, du;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -82,13 +82,13 @@ __device__ __forceinline__ MlpTile mlp_tile(const MlpGemm& p, int tile) {
     return t;
 }
 
-// Eight neighbours of this lane's results of a tile: fragment (i, j), its q-th half
-template <typename T, typename G, int EPI>
-__device__ __forceinline__ void mlp_chunk(const MlpGemm& p, MlpTile t, int i, int j, int q, f32x8 x, f32x8 u) {
+// Where eight neighbours of this lane's results of a tile go - fragment (i, j), its q-th half - or -1: past the end of C.
+template <typename G>
+__device__ __forceinline__ int64_t mlp_place(const MlpGemm& p, MlpTile t, int i, int j, int q) {
     const GemmOperands& o = p.op[t.which];
     const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % G::WAVES_M, wn = w / G::WAVES_M;
     const int m = t.tm * G::ROWS + 32 * (wm * G::MT + i) + (lane & 31), n = t.tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * (lane >> 5) + 8 * q;
-    if (m < o.M && n < o.N) mlp_result<T, EPI>(p, t.which, (int64_t)m * o.N + n, x, u);
+    return m < o.M && n < o.N ? (int64_t)m * o.N + n : -1;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
@@ -107,24 +107,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     const MlpTile at = mlp_tile(p, tile);
     G::run(p.op[at.which], at.tm, at.tn, part, shared < 0 ? 1 : p.parts, smem, acc);
 
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS;
-    float* sums = shared < 0 || p.parts == 1 ? nullptr : p.sums + ((int64_t)(tile - p.full) * p.parts + part) * (BM * BN);
+    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS, ROUND = 2 * COLS;
+    auto result = [&](int i, int jq) {
+        f32x8 x;
 #pragma unroll
-    for (int i = 0; i < G::MT; ++i)
+        for (int e = 0; e < 8; ++e) x[e] = acc[jq / 2][i][8 * (jq % 2) + e];
+        return x;
+    };
+    if (shared >= 0 && p.parts > 1) {
+        float* sums = p.sums + ((int64_t)(tile - p.full) * p.parts + part) * (BM * BN) + threadIdx.x * 8;
 #pragma unroll
-        for (int j = 0; j < COLS; ++j)
+        for (int i = 0; i < G::MT; ++i)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                f32x8 x, u;
+            for (int c = 0; c < ROUND; ++c)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { x[e] = acc[j][i][8 * q + e]; u[e] = acc[j + (KINDS - 1) * COLS][i][8 * q + e]; }
-                if (sums) {
-                    const int chunk = (i * COLS + j) * 2 + q;
-                    *(f32x8*)(sums + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8) = x;
-                    if (KINDS == 2) *(f32x8*)(sums + ((int64_t)(chunk * KINDS + 1) * G::THREADS + threadIdx.x) * 8) = u;
-                } else
-                    mlp_chunk<T, G, EPI>(p, at, i, j, q, x, u);
+                for (int kind = 0; kind < KINDS; ++kind) *(f32x8*)(sums + (int64_t)((i * ROUND + c) * KINDS + kind) * G::THREADS * 8) = result(i, kind * ROUND + c);
+        return;
+    }
+    // (g and u are asked for a round of MT before they are needed: dh's product of 8192 x 4096 x 11008 930 -> 830 us)
+    typedef typename Mma<T>::V8 V8;
+    V8 gv[2][ROUND], uv[2][ROUND];
+    auto inner = [&](int i) {
+        if constexpr (EPI == MLP_GRAD) {
+#pragma unroll
+            for (int c = 0; c < ROUND; ++c) {
+                const int64_t to = max(mlp_place<G>(p, at, i, c / 2, c % 2), (int64_t)0);
+                gv[i % 2][c] = *(const V8*)((const T*)p.G + to); uv[i % 2][c] = *(const V8*)((const T*)p.U + to);
             }
+        }
+    };
+    inner(0);
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i) {
+        if (i + 1 < G::MT) inner(i + 1);
+#pragma unroll
+        for (int c = 0; c < ROUND; ++c) {
+            const int64_t to = mlp_place<G>(p, at, i, c / 2, c % 2);
+            if (to >= 0) mlp_result<T, EPI>(p, at.which, to, result(i, c), result(i, (KINDS - 1) * ROUND + c), gv[i % 2][c], uv[i % 2][c]);
+        }
+    }
 }
 
 // The parts of a shared tile added up, in order, and what becomes of the sums: a workgroup for eight results of every lane.
@@ -140,7 +161,12 @@ __global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
         x += *(const f32x8*)(sums + (int64_t)s * (BM * BN));
         if (KINDS == 2) u += *(const f32x8*)(sums + (int64_t)s * (BM * BN) + G::THREADS * 8);
     }
-    mlp_chunk<T, G, EPI>(p, mlp_tile(p, p.full + tile), chunk / 2 / COLS, chunk / 2 % COLS, chunk % 2, x, u);
+    const MlpTile at = mlp_tile(p, p.full + tile);
+    const int64_t to = mlp_place<G>(p, at, chunk / 2 / COLS, chunk / 2 % COLS, chunk % 2);
+    if (to < 0) return;
+    typename Mma<T>::V8 gv{}, uv{};
+    if constexpr (EPI == MLP_GRAD) { gv = *(const decltype(gv)*)((const T*)p.G + to); uv = *(const decltype(uv)*)((const T*)p.U + to); }
+    mlp_result<T, EPI>(p, at.which, to, x, u, gv, uv);
 }
 
 static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t ldb, int64_t M, int64_t N, int64_t K) {
