@@ -1,7 +1,12 @@
 // The gated feed-forward block (fla/modules/mlp.py: GatedMLP) and its gradients:
 //
 //   g = x Wg^T, u = x Wu^T;  h = act(g) u;  y = h Wd^T             x [M][D]; Wg, Wu [F][D]; Wd [D][F]
-//   dh = dy Wd;  dg = dh u act'(g), du = dh act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//   dh = dy Wd;  dg = dh s, du = dh a  with  s = act'(g) u, a = act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// For the backward the forward keeps s and a, each rounded once from the accumulators, where g and u would do: of those, two roundings (and a slope's
+// steepness) would go into dg, and the backward would work the activation out again.  With the one rounding of s or a, that of dg and du and that of the result the
+// gradients come out 1.7 times as far from the exact ones as their own rounding (bf16: 2.9e-3 against 1.7e-3, 2-norms).  More bits of s and a would be
+// more memory held from the forward to the backward, which is what training runs out of.
 //
 // Forward two launches (both projections with the activation and the product on top; the down projection), backward three (dh with dg and du on top; dx;
 // the weights' gradients together).  Many rows are bound by the matrix cores: gdn_gemm.h.
@@ -28,8 +33,8 @@ struct MlpGemm {
     GemmOperands op[3];
     int ops;
     int full, rest, parts;               // tiles with a workgroup each, and tiles after them whose contraction is shared out over `parts` workgroups
-    void* C[3];                          // results (of a DUAL product's epilogue: h, g, u; of dh's: dg, du)
-    const void* G; const void* U;
+    void* C[3];                          // results (of a DUAL product's epilogue: h, s, a; of dh's: dg, du)
+    const void* S; const void* A;        // dh's epilogue: s and a of the forward
     float* sums;                         // [rest][parts][a tile's accumulators, as the lanes hold them]
     int act;
 };
@@ -38,36 +43,31 @@ enum MlpEpilogue { MLP_PLAIN, MLP_GATE, MLP_GRAD };
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs; MLP_GRAD: gv, uv are the forward's
-// g and u there.
+// What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs; MLP_GRAD: sv, av are the
+// forward's s and a there.
 template <typename T, int EPI>
-__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x8 x, f32x8 u, typename Mma<T>::V8 gv, typename Mma<T>::V8 uv) {
+__device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t at, f32x8 x, f32x8 u, typename Mma<T>::V8 sv, typename Mma<T>::V8 av) {
     typedef typename Mma<T>::V8 V8;
     auto rounded = [](f32x8 v) { return V8{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]}; };
     if constexpr (EPI == MLP_PLAIN) {
         *(V8*)((T*)p.C[which] + at) = rounded(x);
     } else if constexpr (EPI == MLP_GATE) {
-        V8 h;
+        V8 h, s, a;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float a, da;
-            mlp_act(p.act, x[e], a, da);
-            h[e] = (T)(a * u[e]);
+            float act, slope;
+            mlp_act(p.act, x[e], act, slope);
+            h[e] = (T)(act * u[e]); s[e] = (T)(slope * u[e]); a[e] = (T)act;
         }
         *(V8*)((T*)p.C[0] + at) = h;
         if (p.C[1]) {
-            *(V8*)((T*)p.C[1] + at) = rounded(x);
-            *(V8*)((T*)p.C[2] + at) = rounded(u);
+            *(V8*)((T*)p.C[1] + at) = s;
+            *(V8*)((T*)p.C[2] + at) = a;
         }
     } else {
         V8 dg, du;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float a, da;
-            mlp_act(p.act, (float)gv[e], a, da);
-            dg[e] = (T)(x[e] * (float)uv[e] * da);
-            du[e] = (T)(x[e] * a);
-        }
+        for (int e = 0; e < 8; ++e) { dg[e] = (T)(x[e] * (float)sv[e]); du[e] = (T)(x[e] * (float)av[e]); }
         *(V8*)((T*)p.C[0] + at) = dg;
         *(V8*)((T*)p.C[1] + at) = du;
     }
@@ -124,15 +124,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
                 for (int kind = 0; kind < KINDS; ++kind) *(f32x8*)(sums + (int64_t)((i * ROUND + c) * KINDS + kind) * G::THREADS * 8) = result(i, kind * ROUND + c);
         return;
     }
-    // (g and u are asked for a round of MT before they are needed: dh's product of 8192 x 4096 x 11008 930 -> 830 us)
+    // (s and a are asked for a round of MT before they are needed: dh's product of 8192 x 4096 x 11008 930 -> 830 us)
     typedef typename Mma<T>::V8 V8;
-    V8 gv[2][ROUND], uv[2][ROUND];
+    V8 sv[2][ROUND], av[2][ROUND];
     auto inner = [&](int i) {
         if constexpr (EPI == MLP_GRAD) {
 #pragma unroll
             for (int c = 0; c < ROUND; ++c) {
                 const int64_t to = max(mlp_place<G>(p, at, i, c / 2, c % 2), (int64_t)0);
-                gv[i % 2][c] = *(const V8*)((const T*)p.G + to); uv[i % 2][c] = *(const V8*)((const T*)p.U + to);
+                sv[i % 2][c] = *(const V8*)((const T*)p.S + to); av[i % 2][c] = *(const V8*)((const T*)p.A + to);
             }
         }
     };
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
 #pragma unroll
         for (int c = 0; c < ROUND; ++c) {
             const int64_t to = mlp_place<G>(p, at, i, c / 2, c % 2);
-            if (to >= 0) mlp_result<T, EPI>(p, at.which, to, result(i, c), result(i, (KINDS - 1) * ROUND + c), gv[i % 2][c], uv[i % 2][c]);
+            if (to >= 0) mlp_result<T, EPI>(p, at.which, to, result(i, c), result(i, (KINDS - 1) * ROUND + c), sv[i % 2][c], av[i % 2][c]);
         }
     }
 }
@@ -164,9 +164,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
     const MlpTile at = mlp_tile(p, p.full + tile);
     const int64_t to = mlp_place<G>(p, at, chunk / 2 / COLS, chunk / 2 % COLS, chunk % 2);
     if (to < 0) return;
-    typename Mma<T>::V8 gv{}, uv{};
-    if constexpr (EPI == MLP_GRAD) { gv = *(const decltype(gv)*)((const T*)p.G + to); uv = *(const decltype(uv)*)((const T*)p.U + to); }
-    mlp_result<T, EPI>(p, at.which, to, x, u, gv, uv);
+    typename Mma<T>::V8 sv{}, av{};
+    if constexpr (EPI == MLP_GRAD) { sv = *(const decltype(sv)*)((const T*)p.S + to); av = *(const decltype(av)*)((const T*)p.A + to); }
+    mlp_result<T, EPI>(p, at.which, to, x, u, sv, av);
 }
 
 static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t ldb, int64_t M, int64_t N, int64_t K) {
@@ -372,10 +372,10 @@ __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
         }
         const int64_t at = (int64_t)m * p.N + n;
         if constexpr (EPI == MLP_GATE) {
-            float a, da;
-            mlp_act(p.act, x, a, da);
-            ((T*)p.C[0])[at] = (T)(a * u);
-            if (p.C[1]) { ((T*)p.C[1])[at] = (T)x; ((T*)p.C[2])[at] = (T)u; }
+            float act, slope;
+            mlp_act(p.act, x, act, slope);
+            ((T*)p.C[0])[at] = (T)(act * u);
+            if (p.C[1]) { ((T*)p.C[1])[at] = (T)(slope * u); ((T*)p.C[2])[at] = (T)act; }
         } else
             ((T*)p.C[0])[at] = (T)x;
     }
@@ -394,15 +394,15 @@ static int launch_few(const MlpFew& p, hipStream_t stream) {
 }
 
 template <typename T>
-static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h, Workspace ws, int64_t M, int64_t D, int64_t F,
+static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* s, void* a, void* h, Workspace ws, int64_t M, int64_t D, int64_t F,
                    int act, hipStream_t stream) {
     if (M <= MLP_FEW_ROWS) {
-        const MlpFew first{x, {wg, wu}, {h, g, u}, (int)M, (int)F, (int)D, act};
+        const MlpFew first{x, {wg, wu}, {h, s, a}, (int)M, (int)F, (int)D, act};
         const int rc = M <= 4 ? launch_few<T, 1, MLP_GATE>(first, stream) : launch_few<T, 3, MLP_GATE>(first, stream);
         return rc != GDN_OK ? rc : launch_few<T, 1, MLP_PLAIN>(MlpFew{h, {wd, wd}, {y, nullptr, nullptr}, (int)M, (int)D, (int)F, act}, stream);
     }
     MlpGemm p = gate_up(x, wg, wu, M, D, F);
-    p.act = act; p.C[0] = h; p.C[1] = g; p.C[2] = u;
+    p.act = act; p.C[0] = h; p.C[1] = s; p.C[2] = a;
     const int rc = launch_gemm<T, false, false, MLP_GATE>(p, ws, stream);
     if (rc != GDN_OK) return rc;
     MlpGemm q = down(h, wd, M, D, F);
@@ -411,12 +411,12 @@ static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd
 }
 
 template <typename T>
-static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
-                   void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd, Workspace ws, int64_t M, int64_t D, int64_t F, int act, hipStream_t stream) {
+static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* s, const void* a, const void* h,
+                   void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd, Workspace ws, int64_t M, int64_t D, int64_t F, hipStream_t stream) {
     int rc = GDN_OK;
     if (M > 0 && (dx || dwg || dwu)) {
         MlpGemm p = grad_inner(dy, wd, M, D, F);
-        p.act = act; p.G = g; p.U = u; p.C[0] = dg; p.C[1] = du;
+        p.S = s; p.A = a; p.C[0] = dg; p.C[1] = du;
         rc = launch_gemm<T, false, true, MLP_GRAD>(p, ws, stream);
         if (rc != GDN_OK) return rc;
     }
@@ -458,35 +458,35 @@ extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F,
     return most;
 }
 
-extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
+extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* s, void* a, void* h,
                                  void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
     const char* who = "gdn_gated_mlp_fwd";
     const int rc = check_mlp(who, M, D, F, activation, dtype);
     if (rc != GDN_OK) return rc;
     if (M == 0) return GDN_OK;
-    GDN_CHECK_ARG(x && wg && wu && wd && y && h && !g == !u, GDN_ERR_INVALID, "%s: x, the weights, y and h are required, g goes with u", who);
-    GDN_CHECK_ARG((((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)g | (uintptr_t)u | (uintptr_t)h) & 15) == 0,
+    GDN_CHECK_ARG(x && wg && wu && wd && y && h && !s == !a, GDN_ERR_INVALID, "%s: x, the weights, y and h are required, s goes with a", who);
+    GDN_CHECK_ARG((((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h) & 15) == 0,
                   GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
-    hipStream_t s = (hipStream_t)stream;
+    hipStream_t q = (hipStream_t)stream;
     const Workspace ws{workspace, workspace_bytes};
-    return dtype == GDN_DTYPE_BF16 ? mlp_fwd<bf16_t>(x, wg, wu, wd, y, g, u, h, ws, M, D, F, activation, s)
-                                   : mlp_fwd<f16_t>(x, wg, wu, wd, y, g, u, h, ws, M, D, F, activation, s);
+    return dtype == GDN_DTYPE_BF16 ? mlp_fwd<bf16_t>(x, wg, wu, wd, y, s, a, h, ws, M, D, F, activation, q)
+                                   : mlp_fwd<f16_t>(x, wg, wu, wd, y, s, a, h, ws, M, D, F, activation, q);
 }
 
-extern "C" int gdn_gated_mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
+extern "C" int gdn_gated_mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* s, const void* a, const void* h,
                                  void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
-                                 void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
+                                 void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int dtype, void* stream) {
     const char* who = "gdn_gated_mlp_bwd";
-    const int rc = check_mlp(who, M, D, F, activation, dtype);
+    const int rc = check_mlp(who, M, D, F, GDN_ACT_SILU, dtype);
     if (rc != GDN_OK) return rc;
     const bool inner = dx || dwg || dwu;
-    GDN_CHECK_ARG(M == 0 || (dy && (!inner || (wd && g && u && dg && du)) && (!dx || (wg && wu)) && ((!dwg && !dwu) || x) && (!dwd || h)), GDN_ERR_INVALID,
+    GDN_CHECK_ARG(M == 0 || (dy && (!inner || (wd && s && a && dg && du)) && (!dx || (wg && wu)) && ((!dwg && !dwu) || x) && (!dwd || h)), GDN_ERR_INVALID,
                   "%s: a tensor that the asked gradients need is missing", who);
-    GDN_CHECK_ARG((((uintptr_t)dy | (uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)g | (uintptr_t)u | (uintptr_t)h | (uintptr_t)dg |
+    GDN_CHECK_ARG((((uintptr_t)dy | (uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h | (uintptr_t)dg |
                     (uintptr_t)du | (uintptr_t)dx | (uintptr_t)dwg | (uintptr_t)dwu | (uintptr_t)dwd) & 15) == 0,
                   GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
-    hipStream_t s = (hipStream_t)stream;
+    hipStream_t q = (hipStream_t)stream;
     const Workspace ws{workspace, workspace_bytes};
-    return dtype == GDN_DTYPE_BF16 ? mlp_bwd<bf16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, activation, s)
-                                   : mlp_bwd<f16_t>(dy, x, wg, wu, wd, g, u, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, activation, s);
+    return dtype == GDN_DTYPE_BF16 ? mlp_bwd<bf16_t>(dy, x, wg, wu, wd, s, a, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, q)
+                                   : mlp_bwd<f16_t>(dy, x, wg, wu, wd, s, a, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, q);
 }

@@ -12,6 +12,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -36,6 +37,12 @@ decltype(&gdn_causal_conv1d_fwd) p_conv_fwd;
 decltype(&gdn_causal_conv1d_bwd_runs) p_conv_bwd_runs;
 decltype(&gdn_gate_bwd) p_gate_bwd;
 decltype(&gdn_sum_rows) p_sum_rows;
+decltype(&gdn_layer_norm_fwd) p_layer_norm_fwd;
+decltype(&gdn_layer_norm_bwd) p_layer_norm_bwd;
+decltype(&gdn_layer_norm_bwd_parts) p_layer_norm_bwd_parts;
+decltype(&gdn_gated_mlp_fwd) p_gated_mlp_fwd;
+decltype(&gdn_gated_mlp_bwd) p_gated_mlp_bwd;
+decltype(&gdn_gated_mlp_workspace_bytes) p_gated_mlp_workspace_bytes;
 decltype(&gdn_last_error) p_last_error;
 
 PyObject* bind(PyObject*, PyObject* table) {
@@ -51,6 +58,8 @@ PyObject* bind(PyObject*, PyObject* table) {
         !take("gdn_step_linear", p_step_linear) || !take("gdn_norm_gated_fwd", p_norm_gated_fwd) || !take("gdn_norm_gated_bwd", p_norm_gated_bwd) ||
         !take("gdn_chunk_bwd_heads", p_chunk_bwd_heads) || !take("gdn_chunk_bwd_heads_workspace_bytes", p_chunk_bwd_heads_workspace_bytes) ||
         !take("gdn_causal_conv1d_fwd", p_conv_fwd) || !take("gdn_causal_conv1d_bwd_runs", p_conv_bwd_runs) || !take("gdn_gate_bwd", p_gate_bwd) ||
+        !take("gdn_layer_norm_fwd", p_layer_norm_fwd) || !take("gdn_layer_norm_bwd", p_layer_norm_bwd) || !take("gdn_layer_norm_bwd_parts", p_layer_norm_bwd_parts) ||
+        !take("gdn_gated_mlp_fwd", p_gated_mlp_fwd) || !take("gdn_gated_mlp_bwd", p_gated_mlp_bwd) || !take("gdn_gated_mlp_workspace_bytes", p_gated_mlp_workspace_bytes) ||
         !take("gdn_sum_rows", p_sum_rows) || !take("gdn_last_error", p_last_error))
         return nullptr;
     Py_RETURN_NONE;
@@ -388,11 +397,14 @@ PyObject* layer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #include "gdn_host_train.h"
+#include "gdn_host_block.h"
 
 PyMethodDef methods[] = {
     {"chunk_train", (PyCFunction)(void*)chunk_train, METH_FASTCALL, "chunked operator with gradients; None: not a call for the native path"},
     {"layer_train", (PyCFunction)(void*)layer_train, METH_FASTCALL, "the layer's forward with gradients; None: not a call for the native path"},
     {"layer_step", (PyCFunction)(void*)layer_step, METH_FASTCALL, "one decode step of the layer; None: not a call for the native path"},
+    {"layer_norm", (PyCFunction)(void*)layer_norm, METH_FASTCALL, "normalisation with the residual stream; None: not a call for the native path"},
+    {"gated_mlp", (PyCFunction)(void*)gated_mlp, METH_FASTCALL, "the gated feed-forward block; None: not a call for the native path"},
     {"bind", bind, METH_O, "bind({name: address}) - entry points of libgdn_hip.so"},
     {"fused_recurrent", (PyCFunction)(void*)fused_recurrent, METH_FASTCALL, "token recurrence; None: not a call for the native path"},
     {"chunk_fwd", (PyCFunction)(void*)chunk_fwd, METH_FASTCALL, "chunked forward; None: not a call for the native path"},

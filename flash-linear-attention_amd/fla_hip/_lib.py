@@ -177,8 +177,8 @@ SIGNATURES['gdn_layer_norm_fwd'] = (c_int, [c_void_p] * 8 + [c_int64, c_int64, c
 SIGNATURES['gdn_layer_norm_bwd_parts'] = (c_int64, [c_int64, c_int64, c_int])
 SIGNATURES['gdn_layer_norm_bwd'] = (c_int, [c_void_p] * 9 + [c_int64] * 3 + [c_int] * 6 + [c_void_p])    # dy r weight mean rstd dstream dx dresidual part, rows D parts ...
 SIGNATURES['gdn_gated_mlp_workspace_bytes'] = (c_size_t, [c_int64, c_int64, c_int64, c_int])
-SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 9 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y g u h workspace bytes, M D F, activation dtype
-SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 15 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])     # dy x wg wu wd g u h dg du dx dwg dwu dwd
+SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 9 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y s a h workspace bytes, M D F, activation dtype
+SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 15 + [c_size_t] + [c_int64] * 3 + [c_int, c_void_p])     # dy x wg wu wd s a h dg du dx dwg dwu dwd
 SIGNATURES['gdn_calib_rmw'] = (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p])
 CHUNK_STATIC_WORKSPACE_BYTES = 64 << 20
 CONV_BWD_TILES_PER_PART = 8
@@ -224,7 +224,7 @@ class _PythonHost:
     def _leave(*args):
         return None
 
-    fused_recurrent = chunk_fwd = chunk_train = layer_step = layer_train = _leave
+    fused_recurrent = chunk_fwd = chunk_train = layer_step = layer_train = layer_norm = gated_mlp = _leave
 
 
 _host = None

@@ -182,6 +182,9 @@ def layer_norm(
 ):
     """Layer norm of ``x (+ residual)`` over the last dimension.  ``prenorm``: returns ``(y, stream)`` with ``stream = x + residual`` in the residual's type
     (without one: x's, or fp32 with ``residual_in_fp32``).  ``x`` bf16, fp16 or fp32; the stream in x's type or fp32."""
+    out = _lib.host().layer_norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, is_rms_norm)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LayerNormFunction.apply(x, weight, bias, residual, eps, prenorm, residual_in_fp32, is_rms_norm)
     y, _, _, stream = _run(x, weight, bias, residual, eps, residual_in_fp32, is_rms_norm)

@@ -38,11 +38,11 @@ def _forward(x, wg, wu, wd, activation, keep):
     dev = x.device
     y = torch.empty_like(x)
     h = torch.empty(M, inner, dtype=x.dtype, device=dev)
-    g, u = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
+    s, a = (torch.empty_like(h), torch.empty_like(h)) if keep else (None, None)
     ws, n = _workspace(M, D, inner, 0, dev)
-    launch(_lib.load().gdn_gated_mlp_fwd, dev, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(y), ptr(g), ptr(u), ptr(h), ptr(ws), n, M, D, inner,
+    launch(_lib.load().gdn_gated_mlp_fwd, dev, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(y), ptr(s), ptr(a), ptr(h), ptr(ws), n, M, D, inner,
            activation, dtype_code(x.dtype))
-    return y, g, u, h
+    return y, s, a, h
 
 
 class GatedMLPFunction(torch.autograd.Function):
@@ -52,31 +52,31 @@ class GatedMLPFunction(torch.autograd.Function):
         ops = _operands(x, gate_weight, up_weight, down_weight)
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
         inner = need_x or need_g or need_u
-        y, g, u, h = _forward(*ops, activation, inner)
+        y, s, a, h = _forward(*ops, activation, inner)
         x_k, wg, wu, wd = ops
         ctx.save_for_backward(x_k if need_g or need_u else None, wg if need_x else None, wu if need_x else None, wd if inner else None,
-                              g, u, h if need_d else None)
-        ctx.activation, ctx.sizes = activation, (*x.shape, gate_weight.shape[0])
+                              s, a, h if need_d else None)
+        ctx.sizes = (*x.shape, gate_weight.shape[0])
         return y if y.shape == x.shape else y[:, :x.shape[1]].contiguous()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, g, u, h = ctx.saved_tensors
+        x, wg, wu, wd, s, a, h = ctx.saved_tensors
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
         M, D, inner = ctx.sizes
         D8, F8 = (D + 7) // 8 * 8, (inner + 7) // 8 * 8
         dev, dt = dy.device, dy.dtype
         dy = _pad(dy, M, D8)
-        dg, du = (torch.empty_like(g), torch.empty_like(g)) if g is not None else (None, None)
+        dg, du = (torch.empty_like(s), torch.empty_like(s)) if s is not None else (None, None)
 
         def empty(need, *shape):
             return torch.empty(shape, dtype=dt, device=dev) if need else None
 
         dx, dwg, dwu, dwd = empty(need_x, M, D8), empty(need_g, F8, D8), empty(need_u, F8, D8), empty(need_d, D8, F8)
         ws, n = _workspace(M, D8, F8, 1, dev)
-        launch(_lib.load().gdn_gated_mlp_bwd, dev, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dg), ptr(du),
-               ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ptr(ws), n, M, D8, F8, ctx.activation, dtype_code(dt))
+        launch(_lib.load().gdn_gated_mlp_bwd, dev, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(s), ptr(a), ptr(h), ptr(dg), ptr(du),
+               ptr(dx), ptr(dwg), ptr(dwu), ptr(dwd), ptr(ws), n, M, D8, F8, dtype_code(dt))
 
         def cut(t, rows, cols):
             return t if t is None or t.shape == (rows, cols) else t[:rows, :cols].contiguous()
@@ -96,6 +96,10 @@ def gated_mlp(
     Under autocast the operands are cast to its type first.  D and F that are no multiples of 8 are zero-padded (copies of the weights per call)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f'Unsupported activation: {activation}')
+    if not torch.is_autocast_enabled():
+        y = _lib.host().gated_mlp(x, gate_weight, up_weight, down_weight, _ACTIVATIONS[activation])
+        if y is not None:
+            return y
     if gate_weight.dim() != 2 or x.dim() < 1 or gate_weight.shape[1] != x.shape[-1]:
         raise ValueError(f'gate_weight must be [F, {x.shape[-1] if x.dim() else 1}] as x is {tuple(x.shape)}, got {tuple(gate_weight.shape)}')
     if up_weight.shape != gate_weight.shape or down_weight.shape != gate_weight.shape[::-1]:

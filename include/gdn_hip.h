@@ -674,7 +674,7 @@ int gdn_layer_norm_bwd(
  * (fla/modules/mlp.py).
  *   x, y [M,D]; wg, wu [F,D]; wd [D,F]; h [M,F], all dtype (GDN_DTYPE_BF16 or GDN_DTYPE_F16), contiguous and 16-byte aligned, D and F multiples of 8 up to
  *   GDN_MLP_MAX_FEATURES; activation GDN_ACT_SILU, GDN_ACT_SIGMOID or GDN_ACT_GELU_TANH
- *   g, u [M,F] or NULL (both): kept for the backward.  h is written in any case (the down projection reads it)
+ *   s, a [M,F] dtype or NULL (both): act'(g) u and act(g), kept for the backward.  h is written in any case (the down projection reads it)
  *   Accumulators, activation and product in fp32; h is rounded once to dtype, from the accumulators of g and u.
  *   workspace: gdn_gated_mlp_workspace_bytes(M, D, F, backward) bytes, 16-byte aligned (NULL where that is 0): partial sums of contractions that are
  *   shared out over workgroups because there are few rows
@@ -682,18 +682,18 @@ int gdn_layer_norm_bwd(
 #define GDN_MLP_MAX_FEATURES 1048576
 size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward);
 int gdn_gated_mlp_fwd(
-    const void* x, const void* wg, const void* wu, const void* wd, void* y, void* g, void* u, void* h,
+    const void* x, const void* wg, const void* wu, const void* wd, void* y, void* s, void* a, void* h,
     void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
 
 /*
- * Its gradients: dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h.
- *   g, u, h as the forward left them; dg, du [M,F]: room for the inner gradients (dh itself is not stored)
+ * Its gradients: dh = dy Wd, dg = dh s, du = dh a, dx = dg Wg + du Wu, dwg = dg^T x, dwu = du^T x, dwd = dy^T h.
+ *   s, a, h as the forward left them; dg, du [M,F]: room for the inner gradients (dh itself is not stored)
  *   dx, dwg, dwu, dwd in dtype, each may be NULL: not asked for (then what only it needs may be NULL, too).  M == 0 clears the weights' gradients.
  */
 int gdn_gated_mlp_bwd(
-    const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
+    const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* s, const void* a, const void* h,
     void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
-    void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream);
+    void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int dtype, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference (bench.py --workload calib_rmw): the memory traffic and the
