@@ -8,10 +8,9 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import dtype_code, launch, ptr, require_gpu, sum_rows
+from fla_hip.ops.gated_delta_rule._common import differentiable_once, dtype_code, launch, ptr, require_gpu, sum_rows
 
 
 def _stream_dtype(x: torch.Tensor, residual: torch.Tensor | None, residual_dtype: torch.dtype | None) -> torch.dtype:
@@ -146,7 +145,7 @@ class LayerNormFunction(torch.autograd.Function):
         return y.view(shape), stream.view(shape)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy, dstream=None):
         stream, weight, bias, mean, rstd = ctx.saved_tensors
         need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]

@@ -6,10 +6,9 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import aligned16, dtype_code, launch, ptr, require_gpu
+from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, ptr, require_gpu
 
 _ACTIVATIONS = {'swish': _lib.ACT_SILU, 'silu': _lib.ACT_SILU, 'sigmoid': _lib.ACT_SIGMOID, 'gelu_tanh': _lib.ACT_GELU_TANH}
 
@@ -60,7 +59,7 @@ class GatedMLPFunction(torch.autograd.Function):
         return y if y.shape == x.shape else y[:, :x.shape[1]].contiguous()
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         x, wg, wu, wd, s, a, h = ctx.saved_tensors
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]

@@ -2,6 +2,8 @@
 argument normalisation.  Nothing here computes on tensors beyond casts/copies."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from fla_hip import _lib
@@ -137,3 +139,24 @@ def sum_rows(part: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty(part.shape[1:], dtype=dtype if dtype in _DTYPE_CODE else torch.float32, device=part.device)
     launch(_lib.load().gdn_sum_rows, part.device, ptr(part), ptr(out), part.shape[0], out.numel(), dtype_code(out.dtype))
     return out.to(dtype)
+
+
+def differentiable_once(backward):
+    """A ``backward`` whose gradients raise when a second derivative is taken of them: there are kernels for the first one only.  (torch's own
+    ``once_differentiable`` lets the gradients through where the incoming ones carry no graph, and they count as constants then.)"""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            outs = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return outs
+        at = [i for i, x in enumerate(outs) if x is not None]
+        raising = torch._C._functions.DelayedError(b'trying to differentiate twice a function that was marked with @once_differentiable', len(at))
+        present = raising(*(outs[i].detach().requires_grad_(True) for i in at))
+        outs = list(outs)
+        for i, x in zip(at, (present,) if isinstance(present, torch.Tensor) else present):
+            outs[i] = x
+        return tuple(outs)
+
+    return wrapper

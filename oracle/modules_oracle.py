@@ -140,3 +140,56 @@ def norm_gated_grads(x, g, weight, bias, residual, dy, dres_out=None, eps=1e-5, 
         loss = loss + (r * dres_out.to(dtype)).sum()
     loss.backward()
     return {('d' + k): (None if v is None else v.grad) for k, v in leaves.items()}
+
+
+def layer_norm(r, weight=None, bias=None, eps=1e-5, is_rms_norm=False, dtype=torch.float64):
+    """Rows r [T,D] (what is normalised) -> (y, xh, rstd): y = xh * weight + bias, xh = (r - mean) * rstd."""
+    r = r.to(dtype)
+    c = r if is_rms_norm else r - r.mean(-1, keepdim=True)
+    rstd = (c.square().mean(-1, keepdim=True) + eps).rsqrt()
+    xh = c * rstd
+    y = xh if weight is None else xh * weight.to(dtype)
+    return (y if bias is None else y + bias.to(dtype)), xh, rstd
+
+
+def layer_norm_grads(r, weight, dy, dstream=None, eps=1e-5, is_rms_norm=False, dtype=torch.float64):
+    """By the formula: (dr, dweight, dbias) of layer_norm for the gradients of y and of the rows handed on."""
+    _, xh, rstd = layer_norm(r, None, None, eps, is_rms_norm, dtype)
+    dy = dy.to(dtype)
+    g = dy if weight is None else dy * weight.to(dtype)
+    dr = g - xh * (g * xh).mean(-1, keepdim=True)
+    if not is_rms_norm:
+        dr = dr - g.mean(-1, keepdim=True)
+    dr = dr * rstd
+    if dstream is not None:
+        dr = dr + dstream.to(dtype)
+    return dr, (dy * xh).sum(0), dy.sum(0)
+
+
+def gate_activation(x, activation):
+    """(act(x), act'(x)) of the gated feed-forward block."""
+    s = torch.sigmoid(x)
+    if activation == 'sigmoid':
+        return s, s * (1 - s)
+    if activation == 'gelu_tanh':
+        c = (2 / torch.pi) ** 0.5
+        s = torch.sigmoid(2 * c * (x + 0.044715 * x ** 3))               # (1 + tanh z) / 2
+        return x * s, s + x * 2 * s * (1 - s) * c * (1 + 0.134145 * x ** 2)
+    assert activation in ('swish', 'silu')
+    return x * s, s * (1 + x * (1 - s))
+
+
+def gated_mlp(x, wg, wu, wd, activation='swish', dtype=torch.float64):
+    """x [M,D]; wg, wu [F,D]; wd [D,F] -> y [M,D]."""
+    x, wg, wu, wd = (t.to(dtype) for t in (x, wg, wu, wd))
+    return (gate_activation(x @ wg.t(), activation)[0] * (x @ wu.t())) @ wd.t()
+
+
+def gated_mlp_grads(x, wg, wu, wd, dy, activation='swish', dtype=torch.float64):
+    """By the formula: (dx, dwg, dwu, dwd)."""
+    x, wg, wu, wd, dy = (t.to(dtype) for t in (x, wg, wu, wd, dy))
+    g, u = x @ wg.t(), x @ wu.t()
+    a, da = gate_activation(g, activation)
+    dh = dy @ wd
+    dg, du = dh * u * da, dh * a
+    return dg @ wg + du @ wu, dg.t() @ x, du.t() @ x, dy.t() @ (a * u)
