@@ -20,7 +20,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_kernel(L
     const int l = threadIdx.x % LANES, D = p.D;
     const int64_t step = (int64_t)gridDim.x * R::GROUPS;
     const float inv = 1.f / (float)D;
-    constexpr bool KEEP = PIECES <= 2;                                       // longer rows read the parameters (from the caches) for every row
+    constexpr bool KEEP = PIECES <= 3;                                       // longer rows read the parameters (from the caches) for every row
     float w[PIECES][VEC], b[PIECES][VEC];
     auto parameters = [&](int i) {
         R::params(p.weight, p.w_dtype, 1.f, l, i, D, w[i]);

@@ -307,7 +307,7 @@ static MlpGemm grad_weights(const void* dy, const void* x, const void* h, const 
 // ---------------------------------------------------------------------------------------------
 // A few rows (a decode step): every weight is read once and little else, so what counts is how much of the weights is in flight.  A workgroup takes CT tiles of 16
 // weight rows - eight of Wg and the eight of Wu at the same columns, or 16 rows of Wd - and its waves a share of
-// the contraction each, operands straight from memory to registers, partial sums through LDS.
+// the contraction each, operands straight from memory to registers, partial sums through LDS.  Rows may begin at any address and end anywhere.
 // ---------------------------------------------------------------------------------------------
 struct MlpFew {
     const void* x; const void* w[2];
@@ -318,42 +318,54 @@ struct MlpFew {
 template <typename T, int CT, int WAVES, int EPI, int COLS>
 __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
     typedef typename Mma<T>::V8 V8;
+    typedef T AnyV8 __attribute__((ext_vector_type(8), aligned(2)));
     constexpr int U = 8, PITCH = 16 * CT + 1;                      // U: steps of 32 requested together
     __shared__ float sums[WAVES][16][PITCH];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
     const int n0 = (int)blockIdx.x * COLS * CT, K = p.K;
-    const int steps = (K + 31) / 32, s0 = w * steps / WAVES, s1 = (w + 1) * steps / WAVES;
+    const int steps = (K + 31) / 32, whole = K / 32, s0 = w * steps / WAVES, s1 = (w + 1) * steps / WAVES;
     // (columns and rows past the end repeat the last ones, their results are dropped)
     const T* wr[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
-        wr[c] = (const T*)(EPI == MLP_GATE && c16 >= 8 ? p.w[1] : p.w[0]) + (int64_t)min(n0 + COLS * c + c16 % COLS, p.N - 1) * K;
-    const T* xr = (const T*)p.x + (int64_t)min(c16, p.M - 1) * K;
+        wr[c] = (const T*)(EPI == MLP_GATE && c16 >= 8 ? p.w[1] : p.w[0]) + (int64_t)min(n0 + COLS * c + c16 % COLS, p.N - 1) * K + 8 * g;
+    const T* xr = (const T*)p.x + (int64_t)min(c16, p.M - 1) * K + 8 * g;
     f32x4 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; s += U) {
+    const int end = min(s1, whole);
+    for (int s = s0; s < end; s += U) {
         V8 fw[CT][U], fx[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (s + u < s1) {                                      // (the same for the wave)
+            if (s + u < end) {                                     // (the same for the wave)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) fw[c][u] = *(const V8*)(wr[c] + min(32 * (s + u) + 8 * g, K - 8));
+                for (int c = 0; c < CT; ++c) fw[c][u] = *(const AnyV8*)(wr[c] + 32 * (s + u));
             }
 #pragma unroll
-        for (int u = 0; u < U; ++u) if (s + u < s1) fx[u] = *(const V8*)(xr + min(32 * (s + u) + 8 * g, K - 8));
+        for (int u = 0; u < U; ++u) if (s + u < end) fx[u] = *(const AnyV8*)(xr + 32 * (s + u));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (s + u < s1) {
-                const bool past = 32 * (s + u) + 8 * g >= K;       // (in the last step of a contraction that is no multiple of 32)
-                if (past) fx[u] = V8{};
+            if (s + u < end) {
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    if (past) fw[c][u] = V8{};
-                    acc[c] = Mma<T>::run(fw[c][u], fx[u], acc[c]);
-                }
+                for (int c = 0; c < CT; ++c) acc[c] = Mma<T>::run(fw[c][u], fx[u], acc[c]);
             }
+    }
+    if (s1 > whole) {                                              // the last step of a contraction that is no multiple of 32: zeros from K on
+        auto rest = [&](const T* at) {
+            const int left = K - 32 * whole - 8 * g;
+            V8 v{};
+            if (left >= 8) v = *(const AnyV8*)(at + 32 * whole);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) if (e < left) v[e] = at[32 * whole + e];
+            }
+            return v;
+        };
+        const V8 fx = rest(xr);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[c] = Mma<T>::run(rest(wr[c]), fx, acc[c]);
     }
     // lane (c16, g): row c16, columns 4g .. 4g + 3 of each tile
 #pragma unroll
@@ -384,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
 // Up to 16 rows (one matrix tile of them): 16 rows of 2048 x 5632 24.3 us, in 64 x 64 tiles 25.7; one row 19.5 us against 25.3.  Rows of x cost a workgroup as much
 // as a tile of weights, so from five rows on it takes three tiles of Wg and Wu: 16 rows 26.7 -> 24.3 us; one row of 4096 x 11008 50.6 us with one tile
 // (270 MB: 5.3 TB/s), 54.5 with three.
-constexpr int64_t MLP_FEW_ROWS = 16;
+constexpr int64_t MLP_FEW_ROWS = GDN_MLP_FEW_ROWS;
 
 template <typename T, int CT, int EPI>
 static int launch_few(const MlpFew& p, hipStream_t stream) {
@@ -430,22 +442,69 @@ static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu
     return p.ops ? launch_gemm<T, true, true, MLP_PLAIN>(p, ws, stream) : GDN_OK;
 }
 
+// Matrices of 16-bit elements with other row lengths and counts: zeros where the source has nothing, cut where the destination has less.  A thread for eight
+// elements of a row of a destination, at any address.
+struct PadSegments { gdn_pad_segment s[GDN_PAD_SEGMENTS]; int64_t first[GDN_PAD_SEGMENTS + 1]; int n; };
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadSegments p) {
+    typedef uint16_t Any8 __attribute__((ext_vector_type(8), aligned(2)));
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int i = 0;
+    while (i + 1 < p.n && at >= p.first[i + 1]) ++i;
+    const gdn_pad_segment& s = p.s[i];
+    const int64_t pieces = (s.dst_cols + 7) / 8, row = (at - p.first[i]) / pieces, c = (at - p.first[i] - row * pieces) * 8;
+    if (row >= s.dst_rows) return;
+    const int64_t have = row < s.src_rows ? s.src_cols - c : 0;
+    const uint16_t* from = (const uint16_t*)s.src + row * s.src_cols + c;
+    uint16_t* to = (uint16_t*)s.dst + row * s.dst_cols + c;
+    Any8 v{};
+    if (have >= 8) v = *(const Any8*)from;
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (e < have) v[e] = from[e];
+    }
+    if (c + 8 <= s.dst_cols) *(Any8*)to = v;
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (c + e < s.dst_cols) to[e] = v[e];
+    }
+}
+
 }  // namespace gdn
 
 using namespace gdn;
 
-static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, int dtype) {
+extern "C" int gdn_pad_rows(const gdn_pad_segment* segments, int count, void* stream) {
+    const char* who = "gdn_pad_rows";
+    GDN_CHECK_ARG(segments && count >= 1 && count <= GDN_PAD_SEGMENTS, GDN_ERR_INVALID, "%s: 1 to %d segments are required", who, GDN_PAD_SEGMENTS);
+    PadSegments p{};
+    p.n = count;
+    for (int i = 0; i < count; ++i) {
+        const gdn_pad_segment& s = segments[i];
+        const bool reads = s.src_rows > 0 && s.src_cols > 0, writes = s.dst_rows > 0 && s.dst_cols > 0;
+        GDN_CHECK_ARG(s.src_rows >= 0 && s.src_cols >= 0 && s.dst_rows >= 0 && s.dst_cols >= 0 && (!writes || s.dst) && (!writes || !reads || s.src), GDN_ERR_INVALID,
+                      "%s: segment %d has no tensor or a negative size", who, i);
+        p.s[i] = s;
+        p.first[i + 1] = p.first[i] + (writes ? s.dst_rows * ((s.dst_cols + 7) / 8) : 0);
+    }
+    const int64_t pieces = p.first[count];
+    if (pieces == 0) return GDN_OK;
+    GDN_CHECK_ARG(pieces < (1ll << 32) - 256, GDN_ERR_UNSUPPORTED, "%s: too many elements for one launch", who);
+    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p);
+    return check_launch("pad_rows_kernel");
+}
+
+static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, int dtype, bool any_width = false) {
     GDN_CHECK_ARG(M >= 0 && D >= 1 && F >= 1, GDN_ERR_INVALID, "%s: bad sizes M=%lld D=%lld F=%lld", who, (long long)M, (long long)D, (long long)F);
     GDN_CHECK_ARG(dtype == GDN_DTYPE_BF16 || dtype == GDN_DTYPE_F16, GDN_ERR_UNSUPPORTED, "%s: bf16 or f16 only", who);
     GDN_CHECK_ARG(act == GDN_ACT_SILU || act == GDN_ACT_SIGMOID || act == GDN_ACT_GELU_TANH, GDN_ERR_UNSUPPORTED, "%s: unknown activation", who);
-    GDN_CHECK_ARG(D % 8 == 0 && F % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: D and F must be multiples of 8 (got %lld, %lld)", who, (long long)D, (long long)F);
+    GDN_CHECK_ARG(any_width || (D % 8 == 0 && F % 8 == 0), GDN_ERR_UNSUPPORTED, "%s: D and F must be multiples of 8 (got %lld, %lld)", who, (long long)D, (long long)F);
     GDN_CHECK_ARG(D <= GDN_MLP_MAX_FEATURES && F <= GDN_MLP_MAX_FEATURES && M < (1ll << 30), GDN_ERR_UNSUPPORTED,
                   "%s: D and F up to %d and fewer than 2^30 rows (got M=%lld D=%lld F=%lld)", who, GDN_MLP_MAX_FEATURES, (long long)M, (long long)D, (long long)F);
     return GDN_OK;
 }
 
 extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward) {
-    if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16) != GDN_OK || M == 0) return 0;
+    if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16, !backward && M <= MLP_FEW_ROWS) != GDN_OK || M == 0) return 0;
     auto bytes = [](const MlpGemm& p, int kinds, bool rows) { return plan_bytes(plan_gemm(p, kinds, rows)); };
     if (!backward) return M <= MLP_FEW_ROWS ? 0 : std::max(bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2, true), bytes(down(nullptr, nullptr, M, D, F), 1, true));
     size_t most = std::max(bytes(grad_inner(nullptr, nullptr, M, D, F), 1, false), bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1, false));
@@ -461,11 +520,12 @@ extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F,
 extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd, void* y, void* s, void* a, void* h,
                                  void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int activation, int dtype, void* stream) {
     const char* who = "gdn_gated_mlp_fwd";
-    const int rc = check_mlp(who, M, D, F, activation, dtype);
+    const bool few = M <= MLP_FEW_ROWS;
+    const int rc = check_mlp(who, M, D, F, activation, dtype, few);
     if (rc != GDN_OK) return rc;
     if (M == 0) return GDN_OK;
     GDN_CHECK_ARG(x && wg && wu && wd && y && h && !s == !a, GDN_ERR_INVALID, "%s: x, the weights, y and h are required, s goes with a", who);
-    GDN_CHECK_ARG((((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h) & 15) == 0,
+    GDN_CHECK_ARG(few || (((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h) & 15) == 0,
                   GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
     hipStream_t q = (hipStream_t)stream;
     const Workspace ws{workspace, workspace_bytes};

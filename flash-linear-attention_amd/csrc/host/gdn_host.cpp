@@ -43,6 +43,7 @@ decltype(&gdn_layer_norm_bwd_parts) p_layer_norm_bwd_parts;
 decltype(&gdn_gated_mlp_fwd) p_gated_mlp_fwd;
 decltype(&gdn_gated_mlp_bwd) p_gated_mlp_bwd;
 decltype(&gdn_gated_mlp_workspace_bytes) p_gated_mlp_workspace_bytes;
+decltype(&gdn_pad_rows) p_pad_rows;
 decltype(&gdn_last_error) p_last_error;
 
 PyObject* bind(PyObject*, PyObject* table) {
@@ -60,6 +61,7 @@ PyObject* bind(PyObject*, PyObject* table) {
         !take("gdn_causal_conv1d_fwd", p_conv_fwd) || !take("gdn_causal_conv1d_bwd_runs", p_conv_bwd_runs) || !take("gdn_gate_bwd", p_gate_bwd) ||
         !take("gdn_layer_norm_fwd", p_layer_norm_fwd) || !take("gdn_layer_norm_bwd", p_layer_norm_bwd) || !take("gdn_layer_norm_bwd_parts", p_layer_norm_bwd_parts) ||
         !take("gdn_gated_mlp_fwd", p_gated_mlp_fwd) || !take("gdn_gated_mlp_bwd", p_gated_mlp_bwd) || !take("gdn_gated_mlp_workspace_bytes", p_gated_mlp_workspace_bytes) ||
+        !take("gdn_pad_rows", p_pad_rows) ||
         !take("gdn_sum_rows", p_sum_rows) || !take("gdn_last_error", p_last_error))
         return nullptr;
     Py_RETURN_NONE;

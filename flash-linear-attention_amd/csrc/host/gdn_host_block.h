@@ -146,15 +146,24 @@ struct MlpDims { int64_t M, D, F; int act, code; };
 at::Tensor mlp_workspace(const MlpDims& d, int backward, c10::Device dev) {
     return empty_on(dev, at::kByte, {(int64_t)p_gated_mlp_workspace_bytes(d.M, d.D, d.F, backward)});
 }
-// The kernels take rows of a multiple of 8 elements: zeros up to there, and off again.
+// The kernels take rows of a multiple of 8 elements: copies with zeros up to there, and cut off again, several matrices in a launch.
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
-at::Tensor padded(const at::Tensor& t, int64_t rows, int64_t cols) {
-    const int64_t r = rows - t.size(0), c = cols - t.size(1);
-    return r || c ? at::constant_pad_nd(t, {0, c, 0, r}) : t;
-}
-at::Tensor cut(const at::Tensor& t, int64_t rows, int64_t cols) {
-    return !t.defined() || (t.size(0) == rows && t.size(1) == cols) ? t : t.slice(0, 0, rows).slice(1, 0, cols).contiguous();
-}
+struct Resize {
+    gdn_pad_segment seg[GDN_PAD_SEGMENTS];
+    int n = 0;
+    c10::Device dev;
+    explicit Resize(c10::Device d) : dev(d) {}
+    // t [..][cols] as [rows_to][cols_to]: itself where it is that already
+    at::Tensor operator()(const at::Tensor& t, int64_t rows, int64_t cols, int64_t rows_to, int64_t cols_to) {
+        if (!t.defined() || (rows == rows_to && cols == cols_to)) return t;
+        const at::Tensor out = empty_on(dev, t.scalar_type(), {rows_to, cols_to});
+        seg[n++] = {t.data_ptr(), out.data_ptr(), rows, cols, rows_to, cols_to};
+        return out;
+    }
+    void run() {
+        if (n) check_rc(p_pad_rows(seg, n, stream_of(dev)), "gdn_pad_rows");
+    }
+};
 // s, a: undefined where no backward follows that needs them; x [M][D]
 at::Tensor mlp_forward(const MlpDims& d, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, bool keep, at::Tensor& s, at::Tensor& a, at::Tensor& h) {
     const c10::Device dev = x.device();
@@ -172,9 +181,12 @@ struct MlpTrain : torch::autograd::Function<MlpTrain> {
     static variable_list forward(AutogradContext* ctx, const Variable& x, const Variable& wg, const Variable& wu, const Variable& wd, const MlpDims& d) {
         const bool need_x = x.requires_grad(), weights = wg.requires_grad() || wu.requires_grad(), inner = need_x || weights;
         const int64_t D = wg.size(1), F = wg.size(0);
-        const at::Tensor xk = padded(x.reshape({d.M, D}), d.M, d.D), gk = padded(wg, d.F, d.D), uk = padded(wu, d.F, d.D), dk = padded(wd, d.D, d.F), none;
+        Resize pad(x.device()), cut(x.device());
+        const at::Tensor xk = pad(x, d.M, D, d.M, d.D), gk = pad(wg, F, D, d.F, d.D), uk = pad(wu, F, D, d.F, d.D), dk = pad(wd, D, F, d.D, d.F), none;
+        pad.run();
         at::Tensor s, a, h;
-        const at::Tensor y = cut(mlp_forward(d, xk, gk, uk, dk, inner, s, a, h), d.M, D).view(x.sizes());
+        const at::Tensor yk = mlp_forward(d, xk, gk, uk, dk, inner, s, a, h), y = cut(yk, d.M, d.D, d.M, D).view(x.sizes());
+        cut.run();
         ctx->save_for_backward({weights ? xk : none, need_x ? gk : none, need_x ? uk : none, inner ? dk : none, s, a, wd.requires_grad() ? h : none});
         ctx->saved_data["dims"] = std::vector<int64_t>{d.M, d.D, d.F, d.code, D, F};
         ctx->saved_data["shape"] = x.sizes().vec();
@@ -193,15 +205,18 @@ struct MlpTrain : torch::autograd::Function<MlpTrain> {
         auto s = ctx->get_saved_variables();
         for (auto& t : s) t = saved(t, type, dev);
         const int64_t D = n[4], F = n[5];
-        const at::Tensor dy = saved(padded(grads[0].reshape({d.M, D}), d.M, d.D), type, dev);
+        Resize pad(dev), cut(dev);
+        const at::Tensor whole = saved(grads[0], type, dev), dy = pad(whole, d.M, D, d.M, d.D);
+        pad.run();
         auto room = [&](bool need, at::IntArrayRef sizes) { return need ? empty_on(dev, type, sizes) : at::Tensor(); };
         const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2), inner = need_x || need_g || need_u;
         const at::Tensor dx = room(need_x, {d.M, d.D}), dwg = room(need_g, {d.F, d.D}), dwu = room(need_u, {d.F, d.D}), dwd = room(ctx->needs_input_grad(3), {d.D, d.F});
         const at::Tensor dg = room(inner, {d.M, d.F}), du = room(inner, {d.M, d.F}), ws = mlp_workspace(d, 1, dev);
         check_rc(p_gated_mlp_bwd(dy.data_ptr(), ptr_of(s[0]), ptr_of(s[1]), ptr_of(s[2]), ptr_of(s[3]), ptr_of(s[4]), ptr_of(s[5]), ptr_of(s[6]), ptr_of(dg), ptr_of(du),
                                  ptr_of(dx), ptr_of(dwg), ptr_of(dwu), ptr_of(dwd), ws.data_ptr(), (size_t)ws.numel(), d.M, d.D, d.F, d.code, stream_of(dev)), "gdn_gated_mlp_bwd");
-        const at::Tensor dx_cut = cut(dx, d.M, D);
-        return differentiable_once({need_x ? dx_cut.view(shape) : none, cut(dwg, F, D), cut(dwu, F, D), cut(dwd, D, F), none});
+        const at::Tensor dx1 = cut(dx, d.M, d.D, d.M, D), dwg1 = cut(dwg, d.F, d.D, F, D), dwu1 = cut(dwu, d.F, d.D, F, D), dwd1 = cut(dwd, d.D, d.F, D, F);
+        cut.run();
+        return differentiable_once({need_x ? dx1.view(shape) : none, dwg1, dwu1, dwd1, none});
     }
 };
 
@@ -215,21 +230,32 @@ PyObject* gated_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::ScalarType type = x->scalar_type();
     if (dev.index() != c10::hip::current_device() || (type != at::kBFloat16 && type != at::kHalf)) Py_RETURN_NONE;
     for (const Arg* t : {&x, &wg, &wu, &wd})
-        if (!plain(*t, dev) || (*t)->scalar_type() != type || !aligned16(t->ptr())) Py_RETURN_NONE;
-    MlpDims d{};
+        if (!plain(*t, dev) || (*t)->scalar_type() != type) Py_RETURN_NONE;
     const int64_t D = x->size(-1), F = wg->size(0);
-    d.D = up8(D); d.M = x->numel() / D; d.F = up8(F); d.code = code_of(type);
+    if (wg->size(1) != D || wu->sizes() != wg->sizes() || wd->size(0) != D || wd->size(1) != F || F == 0) Py_RETURN_NONE;
+    const bool train = needs_grad({&x, &wg, &wu, &wd});
+    MlpDims d{};
+    d.M = x->numel() / D;
+    const bool few = !train && d.M <= GDN_MLP_FEW_ROWS;             // (a step of a few rows: of any width, at any address)
+    d.D = few ? D : up8(D); d.F = few ? F : up8(F); d.code = code_of(type);
     d.act = (int)PyLong_AsLong(a[4]);
     if (PyErr_Occurred()) return nullptr;
-    if (wg->size(1) != D || wu->sizes() != wg->sizes() || wd->size(0) != D || wd->size(1) != F || F == 0) Py_RETURN_NONE;
+    if (!few)
+        for (const Arg* t : {&x, &wg, &wu, &wd})
+            if (!aligned16(t->ptr())) Py_RETURN_NONE;
     at::Tensor y;
-    if (needs_grad({&x, &wg, &wu, &wd})) {
+    if (train) {
         const NoGil free;
         y = MlpTrain::apply(*x.t, *wg.t, *wu.t, *wd.t, d)[0];
     } else {
         at::Tensor s, act, h;
         const NoGil free;
-        y = cut(mlp_forward(d, padded(x->reshape({d.M, D}), d.M, d.D), padded(*wg.t, d.F, d.D), padded(*wu.t, d.F, d.D), padded(*wd.t, d.D, d.F), false, s, act, h), d.M, D).view(x->sizes());
+        Resize pad(dev), cut(dev);
+        const at::Tensor xk = pad(*x.t, d.M, D, d.M, d.D), gk = pad(*wg.t, F, D, d.F, d.D), uk = pad(*wu.t, F, D, d.F, d.D), dk = pad(*wd.t, D, F, d.D, d.F);
+        pad.run();
+        const at::Tensor yk = mlp_forward(d, xk, gk, uk, dk, false, s, act, h);
+        y = cut(yk, d.M, d.D, d.M, D).view(x->sizes());
+        cut.run();
     }
     return THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS

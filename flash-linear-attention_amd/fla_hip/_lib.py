@@ -179,9 +179,11 @@ SIGNATURES['gdn_layer_norm_bwd'] = (c_int, [c_void_p] * 9 + [c_int64] * 3 + [c_i
 SIGNATURES['gdn_gated_mlp_workspace_bytes'] = (c_size_t, [c_int64, c_int64, c_int64, c_int])
 SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 9 + [c_size_t] + [c_int64] * 3 + [c_int, c_int, c_void_p])      # x wg wu wd y s a h workspace bytes, M D F, activation dtype
 SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 15 + [c_size_t] + [c_int64] * 3 + [c_int, c_void_p])     # dy x wg wu wd s a h dg du dx dwg dwu dwd
+SIGNATURES['gdn_pad_rows'] = (c_int, [c_void_p, c_int, c_void_p])     # segments count
 SIGNATURES['gdn_calib_rmw'] = (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p])
 CHUNK_STATIC_WORKSPACE_BYTES = 64 << 20
 CONV_BWD_TILES_PER_PART = 8
+MLP_FEW_ROWS = 16
 
 _lib = None
 _lock = threading.Lock()

@@ -19,9 +19,11 @@ def _pad(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     return aligned16(F.pad(t, (0, c, 0, r)) if r or c else t.contiguous())
 
 
-def _operands(x, gate_weight, up_weight, down_weight):
+def _operands(x, gate_weight, up_weight, down_weight, keep):
     """The operands as the kernels read them: rows of a multiple of 8 elements."""
     M, D = x.shape
+    if M <= _lib.MLP_FEW_ROWS and not keep:                                     # (a step of a few rows: of any width, at any address)
+        return x.contiguous(), gate_weight.contiguous(), up_weight.contiguous(), down_weight.contiguous()
     D8, F8 = (D + 7) // 8 * 8, (gate_weight.shape[0] + 7) // 8 * 8
     return _pad(x, M, D8), _pad(gate_weight, F8, D8), _pad(up_weight, F8, D8), _pad(down_weight, D8, F8)
 
@@ -48,7 +50,7 @@ class GatedMLPFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, down_weight, activation):
-        ops = _operands(x, gate_weight, up_weight, down_weight)
+        ops = _operands(x, gate_weight, up_weight, down_weight, True)
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
         inner = need_x or need_g or need_u
         y, s, a, h = _forward(*ops, activation, inner)
@@ -118,7 +120,7 @@ def gated_mlp(
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_weight, up_weight, down_weight)):
         y = GatedMLPFunction.apply(x2, gate_weight, up_weight, down_weight, code)
     else:
-        y = _forward(*_operands(x2, gate_weight, up_weight, down_weight), code, False)[0]
+        y = _forward(*_operands(x2, gate_weight, up_weight, down_weight, False), code, False)[0]
         if y.shape != x2.shape:
             y = y[:, :x2.shape[1]].contiguous()
     return y.reshape(x.shape)

@@ -675,11 +675,13 @@ int gdn_layer_norm_bwd(
  *   x, y [M,D]; wg, wu [F,D]; wd [D,F]; h [M,F], all dtype (GDN_DTYPE_BF16 or GDN_DTYPE_F16), contiguous and 16-byte aligned, D and F multiples of 8 up to
  *   GDN_MLP_MAX_FEATURES; activation GDN_ACT_SILU, GDN_ACT_SIGMOID or GDN_ACT_GELU_TANH
  *   s, a [M,F] dtype or NULL (both): act'(g) u and act(g), kept for the backward.  h is written in any case (the down projection reads it)
+ *   Up to GDN_MLP_FEW_ROWS rows D and F are of any size and the tensors of any alignment.
  *   Accumulators, activation and product in fp32; h is rounded once to dtype, from the accumulators of g and u.
  *   workspace: gdn_gated_mlp_workspace_bytes(M, D, F, backward) bytes, 16-byte aligned (NULL where that is 0): partial sums of contractions that are
  *   shared out over workgroups because there are few rows
  */
 #define GDN_MLP_MAX_FEATURES 1048576
+#define GDN_MLP_FEW_ROWS 16
 size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward);
 int gdn_gated_mlp_fwd(
     const void* x, const void* wg, const void* wu, const void* wd, void* y, void* s, void* a, void* h,
@@ -694,6 +696,17 @@ int gdn_gated_mlp_bwd(
     const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* s, const void* a, const void* h,
     void* dg, void* du, void* dx, void* dwg, void* dwu, void* dwd,
     void* workspace, size_t workspace_bytes, int64_t M, int64_t D, int64_t F, int dtype, void* stream);
+
+/*
+ * Up to GDN_PAD_SEGMENTS matrices of 16-bit elements copied to other row lengths and counts in one launch: dst [dst_rows,dst_cols] = src
+ * [src_rows,src_cols] where both are, zero elsewhere (the feed-forward block's operands of widths that are no multiples of 8, and its results back).
+ */
+#define GDN_PAD_SEGMENTS 4
+typedef struct gdn_pad_segment {
+    const void* src; void* dst;
+    int64_t src_rows, src_cols, dst_rows, dst_cols;
+} gdn_pad_segment;
+int gdn_pad_rows(const gdn_pad_segment* segments, int count, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference (bench.py --workload calib_rmw): the memory traffic and the

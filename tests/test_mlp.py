@@ -433,3 +433,53 @@ def test_the_entry_points_refuse():
     assert bwd(F=12) == bwd(dt=2) == _lib.GDN_ERR_UNSUPPORTED
     assert bwd(48, 2048, 64, ws=None) == _lib.GDN_ERR_WORKSPACE
     assert lib.gdn_gated_mlp_workspace_bytes(-1, 8, 8, 0) == lib.gdn_gated_mlp_workspace_bytes(8, 12, 8, 1) == 0
+
+
+@gpu
+def test_matrices_of_other_sizes():
+    """gdn_pad_rows: zeros where there is no source, several matrices in a launch, nothing beside them."""
+    import ctypes
+
+    from fla_hip import _lib
+    from fla_hip.ops.gated_delta_rule._common import launch, ptr
+
+    class Segment(ctypes.Structure):
+        _fields_ = [('src', ctypes.c_void_p), ('dst', ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ('src_rows', 'src_cols', 'dst_rows', 'dst_cols')]
+
+    lib, dev = _lib.load(), torch.device('cuda', torch.cuda.current_device())
+    sizes = [((5, 7), (8, 8)), ((300, 1001), (300, 1008)), ((16, 24), (13, 19)), ((1, 1), (3, 2))]
+    src = [torch.randn(*a, device=DEV).to(BF) for a, _ in sizes]
+    dst = [torch.full((b[0] * b[1] + 33,), 7.0, dtype=BF, device=DEV) for _, b in sizes]
+    segs = (Segment * 4)(*(Segment(ptr(s), d.data_ptr() + 2, *a, *b) for s, d, (a, b) in zip(src, dst, sizes)))      # (destinations at odd places)
+    launch(lib.gdn_pad_rows, dev, ctypes.addressof(segs), 4)
+    torch.cuda.synchronize()
+    for s, d, (a, b) in zip(src, dst, sizes):
+        want = torch.zeros(*b, dtype=BF, device=DEV)
+        r, c = min(a[0], b[0]), min(a[1], b[1])
+        want[:r, :c] = s[:r, :c]
+        n = b[0] * b[1]
+        assert torch.equal(d[1:1 + n].view(b), want) and (d[:1] == 7).all() and (d[1 + n:] == 7).all()
+
+
+def test_the_resizing_entry_point_refuses():
+    from fla_hip import _lib
+    try:
+        lib = _lib.load()
+    except _lib.GDNLibraryError:
+        pytest.skip('not built in this checkout')
+    assert lib.gdn_pad_rows(None, 1, None) == lib.gdn_pad_rows(1 << 20, 0, None) == lib.gdn_pad_rows(1 << 20, 5, None) == _lib.GDN_ERR_INVALID
+
+
+@gpu
+@pytest.mark.parametrize('rows', [1, 3, 16])
+@pytest.mark.parametrize(('D', 'F'), [(1, 1), (7, 9), (31, 33), (250, 1001), (1003, 517), (2049, 40)])
+def test_few_rows_of_any_width_at_any_address(rows, D, F):
+    """Inference of up to 16 rows reads everything where it is."""
+    t = _inputs(rows, D, F, BF)
+    ref = _reference(t, 'swish')['y']
+
+    def off(x):
+        return torch.cat([x.new_full((1,), float('nan')), x.flatten(), x.new_full((9,), float('nan'))])[1:1 + x.numel()].view(x.shape)
+
+    with torch.no_grad():
+        _near('y', _mods().gated_mlp(off(t['x']), off(t['wg']), off(t['wu']), off(t['wd'])), *ref)
