@@ -14,16 +14,17 @@
 
 namespace gdn {
 
-// act(g) and act'(g)
+// act(g) and act'(g).  (The hardware's reciprocal and base-2 exponential, 1 ulp each: what follows is rounded to 16 bits, and a tile's 32768 activations are 3 us
+// of its eight waves' time this way, 10 with full division.)
 __device__ __forceinline__ void mlp_act(int act, float g, float& a, float& da) {
     if (act == GDN_ACT_GELU_TANH) {
         // (tanh has reached 1 long before 16; beyond, g^2 times its vanishing slope could be infinity times zero)
         const float c = g > 16.f ? 16.f : g < -16.f ? -16.f : g, z = 0.7978845608028654f * (c + 0.044715f * c * c * c);
-        const float s = sigmoid_f(2.f * z);                          // (1 + tanh z) / 2
+        const float s = sigmoid_stream(2.f * z);                     // (1 + tanh z) / 2
         a = g * s;
         da = s + c * 2.f * s * (1.f - s) * 0.7978845608028654f * (1.f + 0.134145f * c * c);
     } else {
-        const float s = sigmoid_f(g);
+        const float s = sigmoid_stream(g);
         if (act == GDN_ACT_SIGMOID) { a = s; da = s * (1.f - s); }
         else { a = g * s; da = s * (1.f + g * (1.f - s)); }
     }
@@ -36,10 +37,11 @@ struct MlpGemm {
     void* C[3];                          // results (of a DUAL product's epilogue: h, s, a; of dh's: dg, du)
     const void* S; const void* A;        // dh's epilogue: s and a of the forward
     float* sums;                         // [rest][parts][a tile's accumulators, as the lanes hold them]
-    int act;
 };
 
-enum MlpEpilogue { MLP_PLAIN, MLP_GATE, MLP_GRAD };
+// MLP_GATE + an activation's code: the epilogue of both projections (the activation is the kernel's, or its choice would be made for every result)
+enum MlpEpilogue { MLP_PLAIN, MLP_GRAD, MLP_GATE };
+constexpr bool is_gate(int epilogue) { return epilogue >= MLP_GATE; }
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
@@ -51,12 +53,12 @@ __device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t 
     auto rounded = [](f32x8 v) { return V8{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]}; };
     if constexpr (EPI == MLP_PLAIN) {
         *(V8*)((T*)p.C[which] + at) = rounded(x);
-    } else if constexpr (EPI == MLP_GATE) {
+    } else if constexpr (is_gate(EPI)) {
         V8 h, s, a;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float act, slope;
-            mlp_act(p.act, x[e], act, slope);
+            mlp_act(EPI - MLP_GATE, x[e], act, slope);
             h[e] = (T)(act * u[e]); s[e] = (T)(slope * u[e]); a[e] = (T)act;
         }
         *(V8*)((T*)p.C[0] + at) = h;
@@ -93,7 +95,7 @@ __device__ __forceinline__ int64_t mlp_place(const MlpGemm& p, MlpTile t, int i,
 
 template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
     extern __shared__ __align__(16) char smem[];
     const int id = (int)blockIdx.x, shared = id - p.full;
     int tile, part = 0;
@@ -107,7 +109,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     const MlpTile at = mlp_tile(p, tile);
     G::run(p.op[at.which], at.tm, at.tn, part, shared < 0 ? 1 : p.parts, smem, acc);
 
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS, ROUND = 2 * COLS;
+    constexpr int KINDS = is_gate(EPI) ? 2 : 1, COLS = G::NT / KINDS, ROUND = 2 * COLS;
     auto result = [&](int i, int jq) {
         f32x8 x;
 #pragma unroll
@@ -151,8 +153,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
 // The parts of a shared tile added up, in order, and what becomes of the sums: a workgroup for eight results of every lane.
 template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
-    constexpr int KINDS = EPI == MLP_GATE ? 2 : 1, COLS = G::NT / KINDS, CHUNKS = G::MT * COLS * 2;
+    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
+    constexpr int KINDS = is_gate(EPI) ? 2 : 1, COLS = G::NT / KINDS, CHUNKS = G::MT * COLS * 2;
     const int tile = (int)blockIdx.x / CHUNKS, chunk = (int)blockIdx.x % CHUNKS;
     const float* sums = p.sums + (int64_t)tile * p.parts * (BM * BN) + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8;
     f32x8 x = *(const f32x8*)sums, u = x;
@@ -186,8 +188,8 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 // takes 5.5 us and their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
 // forward): 48 rows 61 us in 128 x 128 tiles, 26 us; 333 rows 85 -> 51 us; 2000 rows 213 us in 256 x 256 tiles, 154 us.  The weights' gradients of 8192 x 2048 x
 // 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 16 parts each, the backward 1186 -> 1026 us.
-struct MlpTiles { int side, waves_n, stages, per_cu; double full, least; };
-constexpr MlpTiles MLP_TILES[] = {{256, 4, 2, 1, 1.7, 1.12}, {128, 2, 2, 2, 1.0, 0.65}, {128, 2, 4, 1, 0.58, 0.46}, {64, 1, 4, 2, 0.45, 0.29}};
+struct MlpTiles { int side, waves_m, waves_n, stages, per_cu; double full, least; };
+constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 2, 1, 1.7, 1.12}, {128, 2, 2, 2, 2, 1.0, 0.65}, {128, 4, 2, 4, 1, 0.58, 0.46}, {64, 2, 1, 4, 2, 0.45, 0.29}};
 struct MlpPlan { int tiles, full, rest, parts; };
 static MlpPlan plan_gemm(const MlpGemm& p, int kinds, bool rows) {
     MlpPlan best{0, 0, 0, 1};
@@ -222,8 +224,8 @@ struct Workspace { void* at; size_t bytes; };
 template <typename T, int TILES, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
     // (both operands down their columns: stages of half the width, twice as many)
-    constexpr int SIDE = MLP_TILES[TILES].side, WN = MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
-    typedef Gemm<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI == MLP_GATE> G;
+    constexpr int SIDE = MLP_TILES[TILES].side, WM = MLP_TILES[TILES].waves_m, WN = MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
+    typedef Gemm<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
         GemmOperands& o = p.op[i];
@@ -236,14 +238,14 @@ static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
     if (tiles == 0) return GDN_OK;
     p.full = plan.full; p.rest = plan.rest; p.parts = plan.parts;
     GDN_CHECK_ARG(tiles == (int64_t)p.full + p.rest, GDN_ERR_INVALID, "the gated feed-forward block: a plan for %d tiles, not %lld", p.full + p.rest, (long long)tiles);
-    auto kernel = mlp_gemm_kernel<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>;
+    auto kernel = mlp_gemm_kernel<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>;
     const int rc = ensure_dynamic_smem_for((const void*)kernel, G::LDS, "mlp_gemm_kernel");
     if (rc != GDN_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(p.full + p.rest * p.parts)), dim3(G::THREADS), G::LDS, stream, p);
     if (p.rest == 0) return check_launch("mlp_gemm_kernel");
     const int rc2 = check_launch("mlp_gemm_kernel");
     if (rc2 != GDN_OK) return rc2;
-    hipLaunchKernelGGL((mlp_join_kernel<T, SIDE, SIDE, 2, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>), dim3((unsigned)(p.rest * G::MT * G::NT * 2 / (EPI == MLP_GATE ? 2 : 1))),
+    hipLaunchKernelGGL((mlp_join_kernel<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>), dim3((unsigned)(p.rest * G::MT * G::NT * 2 / (is_gate(EPI) ? 2 : 1))),
                        dim3(G::THREADS), 0, stream, p);
     return check_launch("mlp_join_kernel");
 }
@@ -251,7 +253,7 @@ static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
 template <typename T, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
     constexpr bool ROWS = !A_DOWN && !B_DOWN;
-    const MlpPlan plan = plan_gemm(p, EPI == MLP_GATE ? 2 : 1, ROWS);
+    const MlpPlan plan = plan_gemm(p, is_gate(EPI) ? 2 : 1, ROWS);
     const size_t need = plan_bytes(plan);
     GDN_CHECK_ARG(need == 0 || (ws.at && ws.bytes >= need), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes, need);
     p.sums = (float*)ws.at;
@@ -328,7 +330,7 @@ __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
     const T* wr[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c)
-        wr[c] = (const T*)(EPI == MLP_GATE && c16 >= 8 ? p.w[1] : p.w[0]) + (int64_t)min(n0 + COLS * c + c16 % COLS, p.N - 1) * K + 8 * g;
+        wr[c] = (const T*)(is_gate(EPI) && c16 >= 8 ? p.w[1] : p.w[0]) + (int64_t)min(n0 + COLS * c + c16 % COLS, p.N - 1) * K + 8 * g;
     const T* xr = (const T*)p.x + (int64_t)min(c16, p.M - 1) * K + 8 * g;
     f32x4 acc[CT];
 #pragma unroll
@@ -380,10 +382,10 @@ __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
             x += sums[v][m][at16];
-            if (EPI == MLP_GATE) u += sums[v][m][at16 + 8];
+            if (is_gate(EPI)) u += sums[v][m][at16 + 8];
         }
         const int64_t at = (int64_t)m * p.N + n;
-        if constexpr (EPI == MLP_GATE) {
+        if constexpr (is_gate(EPI)) {
             float act, slope;
             mlp_act(p.act, x, act, slope);
             ((T*)p.C[0])[at] = (T)(act * u);
@@ -400,7 +402,7 @@ constexpr int64_t MLP_FEW_ROWS = GDN_MLP_FEW_ROWS;
 
 template <typename T, int CT, int EPI>
 static int launch_few(const MlpFew& p, hipStream_t stream) {
-    constexpr int WAVES = 8, COLS = EPI == MLP_GATE ? 8 : 16;
+    constexpr int WAVES = 8, COLS = is_gate(EPI) ? 8 : 16;
     hipLaunchKernelGGL((mlp_few_kernel<T, CT, WAVES, EPI, COLS>), dim3((unsigned)((p.N + COLS * CT - 1) / (COLS * CT))), dim3(64 * WAVES), 0, stream, p);
     return check_launch("mlp_few_kernel");
 }
@@ -414,8 +416,10 @@ static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd
         return rc != GDN_OK ? rc : launch_few<T, 1, MLP_PLAIN>(MlpFew{h, {wd, wd}, {y, nullptr, nullptr}, (int)M, (int)D, (int)F, act}, stream);
     }
     MlpGemm p = gate_up(x, wg, wu, M, D, F);
-    p.act = act; p.C[0] = h; p.C[1] = s; p.C[2] = a;
-    const int rc = launch_gemm<T, false, false, MLP_GATE>(p, ws, stream);
+    p.C[0] = h; p.C[1] = s; p.C[2] = a;
+    const int rc = act == GDN_ACT_SILU ? launch_gemm<T, false, false, MLP_GATE + GDN_ACT_SILU>(p, ws, stream) :
+                   act == GDN_ACT_SIGMOID ? launch_gemm<T, false, false, MLP_GATE + GDN_ACT_SIGMOID>(p, ws, stream) :
+                                            launch_gemm<T, false, false, MLP_GATE + GDN_ACT_GELU_TANH>(p, ws, stream);
     if (rc != GDN_OK) return rc;
     MlpGemm q = down(h, wd, M, D, F);
     q.C[0] = y;
