@@ -179,19 +179,20 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 
 // How the products of a launch are cut: the tiles, and over how many workgroups the contraction of each tile is shared out that does not fill a round of the
 // chip (`rest` tiles of `parts` workgroups after `full` of one): the least of the times that the launch would take by these figures.
-//   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)
-//   256 x 256   8      1 a CU       1.7                                   1.12
-//   128 x 128   4      2 a CU       1.0                                   0.65      two stages of LDS: half the CU's
-//   128 x 128   4      1 a CU       0.58                                  0.46      four stages: more in flight, for few workgroups
-//   64 x 64     2      2 a CU       0.45                                  0.29      the same, where no operand has the contraction down its columns
-// In between the time grows with the workgroups: a full chip is held back by its power, not by the stages.  A round begins and ends in 2.5 us; joining parts
-// takes 5.5 us and their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
-// forward): 48 rows 61 us in 128 x 128 tiles, 26 us; 333 rows 85 -> 51 us; 2000 rows 213 us in 256 x 256 tiles, 154 us.  The weights' gradients of 8192 x 2048 x
-// 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 16 parts each, the backward 1186 -> 1026 us.
-struct MlpTiles { int side, waves_m, waves_n, stages, per_cu; double full, least; };
-constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 2, 1, 1.7, 1.12}, {128, 2, 2, 2, 2, 1.0, 0.65}, {128, 4, 2, 4, 1, 0.58, 0.46}, {64, 2, 1, 4, 2, 0.45, 0.29}};
+//   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)   a round's begin and end, more with an activation or
+//   256 x 256   8      1 a CU       1.65                                  1.05                            8, 4                          the inner gradients
+//   128 x 128   4      2 a CU       1.0                                   0.6                             4, 3      two stages of LDS: half the CU's
+//   128 x 128   8      1 a CU       0.58                                  0.4                             4.5, 2.5  four stages: more in flight, for few workgroups
+//   64 x 64     2      2 a CU       0.45                                  0.28                            4, 2.5    the same, where no operand is read down its columns
+// In between a stage's time grows with the workgroups: a full chip is held back by its power and its caches, not by the stages.  Joining parts takes 5.5 us and
+// their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
+// forward): 48 rows 61 us in 128 x 128 tiles, 28 us; 333 rows 85 -> 49 us; 2000 rows 213 us in 256 x 256 tiles, 155 us.  The weights' gradients of 8192 x 2048 x
+// 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 8 parts each, the backward 1186 -> 1026 us.
+struct MlpTiles { int side, waves_m, waves_n, stages, per_cu; double full, least, round, more; };
+constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 2, 1, 1.65, 1.05, 8, 4}, {128, 2, 2, 2, 2, 1.0, 0.6, 4, 3}, {128, 4, 2, 4, 1, 0.58, 0.4, 4.5, 2.5}, {64, 2, 1, 4, 2, 0.45, 0.28, 4, 2.5}};
 struct MlpPlan { int tiles, full, rest, parts; };
-static MlpPlan plan_gemm(const MlpGemm& p, int kinds, bool rows) {
+static MlpPlan plan_gemm(const MlpGemm& p, int epilogue, bool rows) {
+    const int kinds = is_gate(epilogue) ? 2 : 1;
     MlpPlan best{0, 0, 0, 1};
     double best_us = 1e30;
     for (int t = 0; t < (rows ? 4 : 3); ++t) {
@@ -204,10 +205,10 @@ static MlpPlan plan_gemm(const MlpGemm& p, int kinds, bool rows) {
         }
         if (tiles >= (1ll << 31)) continue;
         const int64_t rest = tiles % slots;
-        const double before = (double)(tiles / slots) * (stages * k.full + 2.5);
+        const double round = k.round + (epilogue == MLP_PLAIN ? 0 : k.more), before = (double)(tiles / slots) * (stages * k.full + round);
         for (int64_t parts = 1; parts <= 16 && (parts == 1 || (rest > 0 && rest * parts <= slots && stages / parts >= 2)); ++parts) {
             double us = before;
-            if (rest) us += (stages + parts - 1) / parts * std::max(k.least, k.full * (rest * parts) / slots) + 2.5;
+            if (rest) us += (stages + parts - 1) / parts * std::max(k.least, k.full * (rest * parts) / slots) + round;
             if (parts > 1) us += 5.5 + (double)(rest * parts) * k.side * k.side * 8 / 4e6;
             if (us < best_us) {
                 best_us = us;
@@ -253,7 +254,7 @@ static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
 template <typename T, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_gemm(MlpGemm& p, Workspace ws, hipStream_t stream) {
     constexpr bool ROWS = !A_DOWN && !B_DOWN;
-    const MlpPlan plan = plan_gemm(p, is_gate(EPI) ? 2 : 1, ROWS);
+    const MlpPlan plan = plan_gemm(p, EPI, ROWS);
     const size_t need = plan_bytes(plan);
     GDN_CHECK_ARG(need == 0 || (ws.at && ws.bytes >= need), GDN_ERR_WORKSPACE, "the gated feed-forward block: workspace too small (%zu bytes, %zu needed)", ws.bytes, need);
     p.sums = (float*)ws.at;
@@ -509,15 +510,15 @@ static int check_mlp(const char* who, int64_t M, int64_t D, int64_t F, int act, 
 
 extern "C" size_t gdn_gated_mlp_workspace_bytes(int64_t M, int64_t D, int64_t F, int backward) {
     if (check_mlp("gdn_gated_mlp_workspace_bytes", M, D, F, GDN_ACT_SILU, GDN_DTYPE_BF16, !backward && M <= MLP_FEW_ROWS) != GDN_OK || M == 0) return 0;
-    auto bytes = [](const MlpGemm& p, int kinds, bool rows) { return plan_bytes(plan_gemm(p, kinds, rows)); };
-    if (!backward) return M <= MLP_FEW_ROWS ? 0 : std::max(bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), 2, true), bytes(down(nullptr, nullptr, M, D, F), 1, true));
-    size_t most = std::max(bytes(grad_inner(nullptr, nullptr, M, D, F), 1, false), bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), 1, false));
+    auto bytes = [](const MlpGemm& p, int epilogue, bool rows) { return plan_bytes(plan_gemm(p, epilogue, rows)); };
+    if (!backward) return M <= MLP_FEW_ROWS ? 0 : std::max(bytes(gate_up(nullptr, nullptr, nullptr, M, D, F), MLP_GATE, true), bytes(down(nullptr, nullptr, M, D, F), MLP_PLAIN, true));
+    size_t most = std::max(bytes(grad_inner(nullptr, nullptr, M, D, F), MLP_GRAD, false), bytes(grad_x(nullptr, nullptr, nullptr, nullptr, M, D, F), MLP_PLAIN, false));
     // (which of the weights' gradients will be asked for is not known here: none, one or both of Wg's and Wu's, which are alike, with Wd's or without)
     char some;
     for (int inner = 0; inner < 3; ++inner)
         for (int with_down = inner == 0; with_down < 2; ++with_down)
             most = std::max(most, bytes(grad_weights(nullptr, nullptr, nullptr, nullptr, nullptr, inner > 0 ? &some : nullptr, inner > 1 ? &some : nullptr,
-                                                     with_down ? &some : nullptr, M, D, F), 1, false));
+                                                     with_down ? &some : nullptr, M, D, F), MLP_PLAIN, false));
     return most;
 }
 
