@@ -318,6 +318,17 @@ struct MlpFew {
     int M, N, K, act;
 };
 
+template <typename T, int EPI>
+__device__ __forceinline__ void few_result(const MlpFew& p, int64_t at, float x, float u) {
+    if constexpr (is_gate(EPI)) {
+        float act, slope;
+        mlp_act(p.act, x, act, slope);
+        ((T*)p.C[0])[at] = (T)(act * u);
+        if (p.C[1]) { ((T*)p.C[1])[at] = (T)(slope * u); ((T*)p.C[2])[at] = (T)act; }
+    } else
+        ((T*)p.C[0])[at] = (T)x;
+}
+
 template <typename T, int CT, int WAVES, int EPI, int COLS>
 __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
     typedef typename Mma<T>::V8 V8;
@@ -385,25 +396,93 @@ __global__ __launch_bounds__(64 * WAVES) void mlp_few_kernel(MlpFew p) {
             x += sums[v][m][at16];
             if (is_gate(EPI)) u += sums[v][m][at16 + 8];
         }
-        const int64_t at = (int64_t)m * p.N + n;
-        if constexpr (is_gate(EPI)) {
-            float act, slope;
-            mlp_act(p.act, x, act, slope);
-            ((T*)p.C[0])[at] = (T)(act * u);
-            if (p.C[1]) { ((T*)p.C[1])[at] = (T)(slope * u); ((T*)p.C[2])[at] = (T)act; }
-        } else
-            ((T*)p.C[0])[at] = (T)x;
+        few_result<T, EPI>(p, (int64_t)m * p.N + n, x, u);
     }
 }
 
-// Up to 16 rows (one matrix tile of them): 16 rows of 2048 x 5632 24.3 us, in 64 x 64 tiles 25.7; one row 19.5 us against 25.3.  Rows of x cost a workgroup as much
-// as a tile of weights, so from five rows on it takes three tiles of Wg and Wu: 16 rows 26.7 -> 24.3 us; one row of 4096 x 11008 50.6 us with one tile
-// (270 MB: 5.3 TB/s), 54.5 with three.
+// Four rows and fewer: a wave reads whole kilobytes of weight rows (the tiles above take sixteen rows 64 bytes at a time), two columns' - of both projections or
+// of the down projection -, and multiplies them with x two elements at a time, sums over its lanes at the end.
+template <typename T> struct Dot;
+template <> struct Dot<bf16_t> {
+    static __device__ __forceinline__ float add(bf16x2 a, bf16x2 b, float c) { return __builtin_amdgcn_fdot2_f32_bf16(a, b, c, false); }
+};
+template <> struct Dot<f16_t> {
+    typedef f16_t V2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ float add(V2 a, V2 b, float c) { return __builtin_amdgcn_fdot2(a, b, c, false); }
+};
+
+template <typename T, int ROWS, int EPI>
+__global__ __launch_bounds__(256) void mlp_vec_kernel(MlpFew p) {
+    typedef typename Mma<T>::V8 V8;
+    typedef T AnyV8 __attribute__((ext_vector_type(8), aligned(2)));
+    constexpr int COLS = 2, KINDS = is_gate(EPI) ? 2 : 1, W = COLS * KINDS, U = 16 / W;      // W weight rows of a wave, U kilobytes of each requested together
+    const int lane = threadIdx.x & 63, K = p.K, n0 = ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)) * COLS;
+    if (n0 >= p.N) return;
+    const T* wr[W];                                                // (a column past the end repeats the last one, its result is dropped)
+#pragma unroll
+    for (int r = 0; r < W; ++r) wr[r] = (const T*)p.w[r / COLS] + (int64_t)min(n0 + r % COLS, p.N - 1) * K;
+    float acc[W][ROWS] = {};
+    auto load = [&](const T* row, int k) {
+        V8 v{};
+        if (k + 8 <= K) v = *(const AnyV8*)(row + k);
+        else if (k < K) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (k + e < K) v[e] = row[k + e];
+        }
+        return v;
+    };
+    for (int k0 = 0; k0 < K; k0 += 512 * U) {
+        V8 fw[W][U], fx[ROWS][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + 512 * u < K) {                                // (the same for the workgroup)
+#pragma unroll
+                for (int r = 0; r < W; ++r) fw[r][u] = load(wr[r], k0 + 512 * u + 8 * lane);
+#pragma unroll
+                for (int m = 0; m < ROWS; ++m) fx[m][u] = load((const T*)p.x + (int64_t)min(m, p.M - 1) * K, k0 + 512 * u + 8 * lane);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + 512 * u < K) {
+#pragma unroll
+                for (int r = 0; r < W; ++r)
+#pragma unroll
+                    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) acc[r][m] = Dot<T>::add({fw[r][u][e], fw[r][u][e + 1]}, {fx[m][u][e], fx[m][u][e + 1]}, acc[r][m]);
+            }
+    }
+    // every lane gets every sum; lane COLS m + c keeps those of row m, column c
+    float x = 0.f, u = 0.f;
+#pragma unroll
+    for (int r = 0; r < W; ++r)
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m) {
+            float v = acc[r][m];
+#pragma unroll
+            for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+            if (lane == COLS * m + r % COLS) (r < COLS ? x : u) = v;
+        }
+    const int m = lane / COLS, n = n0 + lane % COLS;
+    if (m < p.M && m < ROWS && n < p.N) few_result<T, EPI>(p, (int64_t)m * p.N + n, x, u);
+}
+
+// Up to 16 rows (one matrix tile of them): 16 rows of 2048 x 5632 22.5 us, in 64 x 64 tiles 25.7.  Rows of x cost a workgroup as much as a tile of weights, so it
+// takes three tiles of Wg and Wu.  Up to four rows by whole kilobytes of a row: one row 18.0 -> 14.5 us (69 MB in two launches: 4.8 TB/s), four 19.9 -> 17.7;
+// one of 4096 x 11008 56.4 -> 53.3 us, of 1024 x 2816 10.2 -> 7.9.
 constexpr int64_t MLP_FEW_ROWS = GDN_MLP_FEW_ROWS;
 
-template <typename T, int CT, int EPI>
+template <typename T, int EPI>
 static int launch_few(const MlpFew& p, hipStream_t stream) {
-    constexpr int WAVES = 8, COLS = is_gate(EPI) ? 8 : 16;
+    if (p.M <= 4) {
+        const dim3 grid((unsigned)((p.N + 7) / 8));
+        if (p.M == 1) hipLaunchKernelGGL((mlp_vec_kernel<T, 1, EPI>), grid, dim3(256), 0, stream, p);
+        else if (p.M == 2) hipLaunchKernelGGL((mlp_vec_kernel<T, 2, EPI>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((mlp_vec_kernel<T, 4, EPI>), grid, dim3(256), 0, stream, p);
+        return check_launch("mlp_vec_kernel");
+    }
+    constexpr int WAVES = 8, COLS = is_gate(EPI) ? 8 : 16, CT = is_gate(EPI) ? 3 : 1;
     hipLaunchKernelGGL((mlp_few_kernel<T, CT, WAVES, EPI, COLS>), dim3((unsigned)((p.N + COLS * CT - 1) / (COLS * CT))), dim3(64 * WAVES), 0, stream, p);
     return check_launch("mlp_few_kernel");
 }
@@ -413,8 +492,8 @@ static int mlp_fwd(const void* x, const void* wg, const void* wu, const void* wd
                    int act, hipStream_t stream) {
     if (M <= MLP_FEW_ROWS) {
         const MlpFew first{x, {wg, wu}, {h, s, a}, (int)M, (int)F, (int)D, act};
-        const int rc = M <= 4 ? launch_few<T, 1, MLP_GATE>(first, stream) : launch_few<T, 3, MLP_GATE>(first, stream);
-        return rc != GDN_OK ? rc : launch_few<T, 1, MLP_PLAIN>(MlpFew{h, {wd, wd}, {y, nullptr, nullptr}, (int)M, (int)D, (int)F, act}, stream);
+        const int rc = launch_few<T, MLP_GATE>(first, stream);
+        return rc != GDN_OK ? rc : launch_few<T, MLP_PLAIN>(MlpFew{h, {wd, wd}, {y, nullptr, nullptr}, (int)M, (int)D, (int)F, act}, stream);
     }
     MlpGemm p = gate_up(x, wg, wu, M, D, F);
     p.C[0] = h; p.C[1] = s; p.C[2] = a;
