@@ -54,8 +54,8 @@ constexpr int64_t GM_EXTENT = 1ll << 31;
 
 // One operand's share in a step: how its tile of ROWS rows (or columns) comes from memory and how its fragments are read.
 // DOWN: the contraction runs down the columns of the stored matrix.
-// SPREAD (the operand whose index becomes the rows of a result): row i of a fragment is row 16 ((i >> 2) & 1) + 4 (i >> 3) + (i & 3) of its 32, so that a
-// lane's sixteen results are neighbours.
+// SPREAD (the operand whose index becomes the rows of a result): row i of a fragment is row 16 (i >> 4) + 8 ((i >> 2) & 1) + 4 ((i >> 3) & 1) + (i & 3) of its
+// 32, so that results 8q .. 8q + 7 of lane l are neighbours, and those of lane l + 32 are the next eight.
 template <typename T, int ROWS, int KS, bool DOWN, bool SPREAD>
 struct GemmSide {
     static constexpr int BYTES = ROWS * 2 * KS, PIECES = BYTES / 1024;
@@ -77,11 +77,11 @@ struct GemmSide {
     // this lane's share of the place of a fragment, and the fragment of the 32 rows (columns) 32 i .., contraction indices 16 kk ..
     static __device__ __forceinline__ uint32_t share(int lane) {
         if constexpr (!DOWN) {
-            const int l = lane & 31, r = SPREAD ? 16 * ((l >> 2) & 1) + 4 * (l >> 3) + (l & 3) : l;
+            const int l = lane & 31, r = SPREAD ? 16 * (l >> 4) + 8 * ((l >> 2) & 1) + 4 * ((l >> 3) & 1) + (l & 3) : l;
             return (uint32_t)(r * 128 + 16 * ((lane >> 5) ^ ((r >> 1) & 7)));
         } else {
             // sixteen lanes read four rows of k, four runs of four columns each; run t of a fragment's eight
-            const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), t = 4 * ((lane >> 4) & 1) + (lane & 3), run = SPREAD ? 4 * (t & 1) + (t >> 1) : t;
+            const int k = 8 * (lane >> 5) + ((lane & 15) >> 2), t = 4 * ((lane >> 4) & 1) + (lane & 3), run = SPREAD ? (t & 4) + 2 * (t & 1) + ((t >> 1) & 1) : t;
             return (uint32_t)(k * 2 * ROWS + 64 * (k & 3) + 8 * run);
         }
     }

@@ -63,8 +63,9 @@ __device__ __forceinline__ void mlp_result(const MlpGemm& p, int which, int64_t 
         }
         *(V8*)((T*)p.C[0] + at) = h;
         if (p.C[1]) {
-            *(V8*)((T*)p.C[1] + at) = s;
-            *(V8*)((T*)p.C[2] + at) = a;
+            // (not read again before the backward: past the caches, 2 - 3 % of the launch at 8192 x 2048 x 5632)
+            __builtin_nontemporal_store(s, (V8*)((T*)p.C[1] + at));
+            __builtin_nontemporal_store(a, (V8*)((T*)p.C[2] + at));
         }
     } else {
         V8 dg, du;
@@ -89,7 +90,7 @@ template <typename G>
 __device__ __forceinline__ int64_t mlp_place(const MlpGemm& p, MlpTile t, int i, int j, int q) {
     const GemmOperands& o = p.op[t.which];
     const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6, wm = w % G::WAVES_M, wn = w / G::WAVES_M;
-    const int m = t.tm * G::ROWS + 32 * (wm * G::MT + i) + (lane & 31), n = t.tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * (lane >> 5) + 8 * q;
+    const int m = t.tm * G::ROWS + 32 * (wm * G::MT + i) + (lane & 31), n = t.tn * G::COLUMNS + 32 * G::column_tile(wn, j) + 16 * q + 8 * (lane >> 5);
     return m < o.M && n < o.N ? (int64_t)m * o.N + n : -1;
 }
 
@@ -126,15 +127,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
                 for (int kind = 0; kind < KINDS; ++kind) *(f32x8*)(sums + (int64_t)((i * ROUND + c) * KINDS + kind) * G::THREADS * 8) = result(i, kind * ROUND + c);
         return;
     }
-    // (s and a are asked for a round of MT before they are needed: dh's product of 8192 x 4096 x 11008 930 -> 830 us)
+    // 32 rows at a time through this wave's share of the LDS, from the lanes' order into rows, so that the rows of 64 (32) columns leave in whole lines.  A row's
+    // 16-byte slots are XORed with the row: neither side meets a bank conflict.  s and a are asked for 32 rows before they are needed.  Straight from the lanes, 32 bytes
+    // of a row at a time, 8192 x 2048 x 5632 took 988 us backward (956 now), 32768 rows 3790 (3670).
     typedef typename Mma<T>::V8 V8;
-    V8 sv[2][ROUND], av[2][ROUND];
+    constexpr int CW = 32 * COLS, SLOTS = CW / 4, PER_ROW = CW / 8, ROWS = 64 / PER_ROW, PASSES = 32 / ROWS;
+    static_assert(KINDS * 32 * CW * 4 * G::WAVES <= G::LDS, "32 rows of every wave fit in the LDS of the main loop");
+    const GemmOperands& o = p.op[at.which];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w % WM, wn = w / WM;
+    float* area = (float*)smem + w * (KINDS * 32 * CW);
+    const int row0 = at.tm * BM + 32 * (wm * G::MT) + lane / PER_ROW, n = at.tn * G::COLUMNS + 32 * G::column_tile(wn, 0) + 8 * (lane % PER_ROW);
+    V8 sv[2][PASSES], av[2][PASSES];
     auto inner = [&](int i) {
         if constexpr (EPI == MLP_GRAD) {
 #pragma unroll
-            for (int c = 0; c < ROUND; ++c) {
-                const int64_t to = max(mlp_place<G>(p, at, i, c / 2, c % 2), (int64_t)0);
-                sv[i % 2][c] = *(const V8*)((const T*)p.S + to); av[i % 2][c] = *(const V8*)((const T*)p.A + to);
+            for (int r = 0; r < PASSES; ++r) {
+                const int64_t to = (int64_t)min(row0 + 32 * i + ROWS * r, o.M - 1) * o.N + min(n, o.N - 8);
+                sv[i % 2][r] = __builtin_nontemporal_load((const V8*)((const T*)p.S + to));
+                av[i % 2][r] = __builtin_nontemporal_load((const V8*)((const T*)p.A + to));
             }
         }
     };
@@ -143,9 +153,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     for (int i = 0; i < G::MT; ++i) {
         if (i + 1 < G::MT) inner(i + 1);
 #pragma unroll
-        for (int c = 0; c < ROUND; ++c) {
-            const int64_t to = mlp_place<G>(p, at, i, c / 2, c % 2);
-            if (to >= 0) mlp_result<T, EPI>(p, at.which, to, result(i, c), result(i, (KINDS - 1) * ROUND + c), sv[i % 2][c], av[i % 2][c]);
+        for (int kind = 0; kind < KINDS; ++kind)
+#pragma unroll
+            for (int c = 0; c < ROUND; ++c) {
+                const int m = lane & 31, slot = 4 * c + 2 * (lane >> 5);
+                const f32x8 x = result(i, kind * ROUND + c);
+                float* to = area + kind * 32 * CW + m * CW;
+                *(f32x4*)(to + 4 * (slot ^ (m & (SLOTS - 1)))) = f32x4{x[0], x[1], x[2], x[3]};
+                *(f32x4*)(to + 4 * ((slot + 1) ^ (m & (SLOTS - 1)))) = f32x4{x[4], x[5], x[6], x[7]};
+            }
+#pragma unroll
+        for (int r = 0; r < PASSES; ++r) {
+            const int m = ROWS * r + lane / PER_ROW, slot = 2 * (lane % PER_ROW);
+            f32x8 x[KINDS];
+#pragma unroll
+            for (int kind = 0; kind < KINDS; ++kind) {
+                const float* from = area + kind * 32 * CW + m * CW;
+                const f32x4 lo = *(const f32x4*)(from + 4 * (slot ^ (m & (SLOTS - 1)))), hi = *(const f32x4*)(from + 4 * ((slot + 1) ^ (m & (SLOTS - 1))));
+                x[kind] = f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            }
+            if (row0 + 32 * i + ROWS * r < o.M && n < o.N)
+                mlp_result<T, EPI>(p, at.which, (int64_t)(row0 + 32 * i + ROWS * r) * o.N + n, x[0], x[KINDS - 1], sv[i % 2][r], av[i % 2][r]);
         }
     }
 }
@@ -225,7 +253,9 @@ struct Workspace { void* at; size_t bytes; };
 template <typename T, int TILES, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
     // (both operands down their columns: stages of half the width, twice as many)
-    constexpr int SIDE = MLP_TILES[TILES].side, WM = MLP_TILES[TILES].waves_m, WN = MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
+    // (both projections in a 256 x 256 tile: 64 columns of each to a wave, a whole line of every result's row)
+    constexpr bool WIDE = is_gate(EPI) && MLP_TILES[TILES].side == 256;
+    constexpr int SIDE = MLP_TILES[TILES].side, WM = WIDE ? 4 : MLP_TILES[TILES].waves_m, WN = WIDE ? 2 : MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
     typedef Gemm<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
