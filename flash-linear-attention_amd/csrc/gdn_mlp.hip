@@ -558,15 +558,17 @@ static int mlp_bwd(const void* dy, const void* x, const void* wg, const void* wu
 
 // Matrices of 16-bit elements with other row lengths and counts: zeros where the source has nothing, cut where the destination has less.  A thread for eight
 // elements of a row of a destination, at any address.
-struct PadSegments { gdn_pad_segment s[GDN_PAD_SEGMENTS]; int64_t first[GDN_PAD_SEGMENTS + 1]; int n; };
+struct PadSegments { gdn_pad_segment s[GDN_PAD_SEGMENTS]; uint32_t first[GDN_PAD_SEGMENTS + 1]; int n; };
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadSegments p) {
     typedef uint16_t Any8 __attribute__((ext_vector_type(8), aligned(2)));
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= p.first[p.n]) return;
     int i = 0;
     while (i + 1 < p.n && at >= p.first[i + 1]) ++i;
     const gdn_pad_segment& s = p.s[i];
-    const int64_t pieces = (s.dst_cols + 7) / 8, row = (at - p.first[i]) / pieces, c = (at - p.first[i] - row * pieces) * 8;
-    if (row >= s.dst_rows) return;
+    // (fewer than 2^32 pieces in all, so places count in 32 bits: their division takes a fifth of that in 64)
+    const uint32_t pieces = (uint32_t)((s.dst_cols + 7) / 8), r = (at - p.first[i]) / pieces;
+    const int64_t row = r, c = (int64_t)(at - p.first[i] - r * pieces) * 8;
     const int64_t have = row < s.src_rows ? s.src_cols - c : 0;
     const uint16_t* from = (const uint16_t*)s.src + row * s.src_cols + c;
     uint16_t* to = (uint16_t*)s.dst + row * s.dst_cols + c;
@@ -592,17 +594,18 @@ extern "C" int gdn_pad_rows(const gdn_pad_segment* segments, int count, void* st
     GDN_CHECK_ARG(segments && count >= 1 && count <= GDN_PAD_SEGMENTS, GDN_ERR_INVALID, "%s: 1 to %d segments are required", who, GDN_PAD_SEGMENTS);
     PadSegments p{};
     p.n = count;
+    int64_t pieces = 0;
     for (int i = 0; i < count; ++i) {
         const gdn_pad_segment& s = segments[i];
         const bool reads = s.src_rows > 0 && s.src_cols > 0, writes = s.dst_rows > 0 && s.dst_cols > 0;
         GDN_CHECK_ARG(s.src_rows >= 0 && s.src_cols >= 0 && s.dst_rows >= 0 && s.dst_cols >= 0 && (!writes || s.dst) && (!writes || !reads || s.src), GDN_ERR_INVALID,
                       "%s: segment %d has no tensor or a negative size", who, i);
         p.s[i] = s;
-        p.first[i + 1] = p.first[i] + (writes ? s.dst_rows * ((s.dst_cols + 7) / 8) : 0);
+        pieces += writes ? s.dst_rows * ((s.dst_cols + 7) / 8) : 0;
+        GDN_CHECK_ARG(s.dst_rows < (1ll << 32) && s.dst_cols < (1ll << 32) && pieces < (1ll << 32) - 256, GDN_ERR_UNSUPPORTED, "%s: too many elements for one launch", who);
+        p.first[i + 1] = (uint32_t)pieces;
     }
-    const int64_t pieces = p.first[count];
     if (pieces == 0) return GDN_OK;
-    GDN_CHECK_ARG(pieces < (1ll << 32) - 256, GDN_ERR_UNSUPPORTED, "%s: too many elements for one launch", who);
     hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p);
     return check_launch("pad_rows_kernel");
 }
