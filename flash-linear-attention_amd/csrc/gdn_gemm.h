@@ -1,7 +1,7 @@
 // Matrix products of 16-bit operands for large row counts: C[m][n] = sum_k A(m, k) B(n, k), fp32 accumulators, with either operand stored with the
 // contraction along its rows (A[m][k]) or down its columns (A[k][m]).  What becomes of an accumulator is an epilogue's business.
 //
-// A workgroup takes a BM x BN tile of C and walks over k in stages of KS = 64: (BM + BN) * 128 bytes of LDS each, STAGES of them in flight or in use, filled straight
+// A workgroup takes a BM x BN tile of C and walks over k in stages of KS (64; 32 where both operands are read down their columns): (BM + BN) * 2 KS bytes of LDS each, STAGES of them in flight or in use, filled straight
 // from memory (buffer_load ... lds).  Stages are 64 wide because a row's share is then a whole 128-byte line: with stages of 32 every line was asked for twice, in
 // halves, and the L2's requests, not its bytes, were the limit (8192 x 4096 x 11008, both projections: 1214 -> 1178 us).  Where both operands have the
 // contraction down their columns a stage of 32 asks for whole lines as well, and four of those keep requests in flight longer.  The matrix cores work through a stage
@@ -24,8 +24,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // index) and, in element 4 q + e, row 8 q + 4 (l / 32) + e (a's index).  Half the operand registers per product of the 16 x 16 form.
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
-
 
 // One product of a launch.  A second pair of operands (A1, B1) continues the contraction of the first (segments == 2, K columns each).
 struct GemmOperands {
@@ -143,7 +141,8 @@ struct Gemm {
         int asked = 0, left = K - KS * (begin % steps), until_second = p.segments == 2 && begin < steps ? steps - begin : -1;
         uint32_t to = 0;
         auto extent = [&](bool down, int ld2, int corner) {
-            const uint32_t whole = (uint32_t)GM_EXTENT, rest = (uint32_t)(left * ld2 - 2 * corner);
+            // (unsigned: `rest` is formed, and not used, where more rows are left than 32 bits of bytes hold)
+            const uint32_t whole = (uint32_t)GM_EXTENT, rest = (uint32_t)left * (uint32_t)ld2 - 2u * (uint32_t)corner;
             return asked >= total || left <= 0 ? 0u : down && left < KS ? rest : whole;
         };
         // the copies of one more step: this wave's piece i of PA + PB, and then on to the next step
