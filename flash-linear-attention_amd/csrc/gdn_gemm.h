@@ -1,19 +1,25 @@
 // Matrix products of 16-bit operands for large row counts: C[m][n] = sum_k A(m, k) B(n, k), fp32 accumulators, with either operand stored with the
 // contraction along its rows (A[m][k]) or down its columns (A[k][m]).  What becomes of an accumulator is an epilogue's business.
 //
-// A workgroup takes a BM x BN tile of C and walks over k in stages of KS (64; 32 where both operands are read down their columns): (BM + BN) * 2 KS bytes of LDS each, STAGES of them in flight or in use, filled straight
-// from memory (buffer_load ... lds).  Stages are 64 wide because a row's share is then a whole 128-byte line: with stages of 32 every line was asked for twice, in
-// halves, and the L2's requests, not its bytes, were the limit (8192 x 4096 x 11008, both projections: 1214 -> 1178 us).  Where both operands have the
-// contraction down their columns a stage of 32 asks for whole lines as well, and four of those keep requests in flight longer.  The matrix cores work through a stage
-// in halves of 32, each on fragments in registers while those of the next half leave LDS for another set of registers: a barrier a stage, after which the stage
-// before is filled again.  Places past the end of a row, a column or the contraction are requested beyond the buffer's extent and arrive as zeros, so every
-// size that is a multiple of 8 along rows runs the same code.
+// A workgroup takes a BM x BN tile of C and walks over k in stages of KS (64; 32 where both operands are read down their columns): (BM + BN) * 2 KS
+// bytes of LDS each, filled straight from memory (buffer_load ... lds) into a ring of SLOTS operand shares, A's and B's in turn.  Stages are 64 wide because a
+// row's share is then a whole 128-byte line: with stages of 32 every line was asked for twice, in halves, and both projections of 8192 x 4096 x 11008 took 1214 us
+// where whole lines took 1178.  Where both operands have the contraction down their columns a stage of 32 asks for whole lines as well, and four of those
+// keep requests in flight longer.  The matrix cores work through a stage in halves of 32, each on fragments in registers while those of the next half leave LDS
+// for another set of registers: a barrier a stage, after which the stage before is filled again.  Places past the end of a row, a column or the
+// contraction are requested beyond the buffer's extent and arrive as zeros, so every size that is a multiple of 8 along rows runs the same code.
+//
+// With an odd number of slots (five of 32 KB fill the LDS) A's copies go out in one half of a stage, A a half stage earlier, and B's in the other, spread
+// over three quarters of it; with four slots both operands' went out together in a quarter of a stage.  8192 x 4096 x 11008, four slots and five: both projections
+// 1243 -> 1174 us, down 588 -> 539, dh 694 -> 665, dx 1109 -> 1044 (the down projection's matrix cores busy 66 and 81 % of the cycles).  With four slots and no copies at
+// all after the first ones the down projection took 481 us, with all copies from lines that stay in the caches 567 of 606: the copies cost more than the way
+// to memory.  Four waves of 128 x 128 results, with a third fewer LDS reads, take the same time, and so do ten slots of 32 for operands down their columns.
 //
 // LDS layout (a CU serves 256 bytes a cycle; of a 16-byte read the lanes {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31} of each half wave together, of
 // an 8-byte transposing read a half wave):
 //   contraction along rows   a row of the tile is 128 bytes, piece c (16 bytes) of row r in slot c ^ ((r >> 1) & 7)
 //   down columns             row k of the stage is 2 BM (BN) bytes, its 64-byte pieces (32 columns) XORed with k & 3
-// Neither meets a bank conflict, and both are whole 1 KB runs for the copies.
+// Neither meets a bank conflict (counted: none in tiles of 256 x 256), and both are whole 1 KB runs for the copies.
 #pragma once
 #include "gdn_chunk_common.h"
 
@@ -95,10 +101,12 @@ struct GemmSide {
 
 // The workgroup's tile of C.  DUAL: the tile's first BN / 2 columns come from B[0], the others from B[1] at the same columns (two products of the same A,
 // side by side in every wave); else B[1] is the second segment's.
-template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, bool DUAL>
+template <typename T, int BM, int BN, int WM, int WN, int KS, int SLOTS, bool A_DOWN, bool B_DOWN, bool DUAL>
 struct Gemm {
     static constexpr int ROWS = BM, WAVES_M = WM, WAVES = WM * WN, THREADS = 64 * WAVES, MT = BM / WM / 32, NT = BN / WN / 32;
-    static constexpr int STAGE = (BM + BN) * 2 * KS, LDS = STAGES * STAGE;
+    static constexpr int SLOT = BM * 2 * KS, LDS = SLOTS * SLOT;
+    static constexpr bool TURNS = SLOTS % 2 == 1;                    // A's copies in one half of a stage, B's in the other
+    static_assert(BM == BN && SLOTS >= 4 && !(TURNS && KS != 64), "a slot holds either operand's share of a stage");
     static constexpr int COLUMNS = DUAL ? BN / 2 : BN;               // columns of C (of each product)
     typedef GemmSide<T, BM, KS, A_DOWN, false> SideA;
     typedef GemmSide<T, BN, KS, B_DOWN, true> SideB;
@@ -145,40 +153,41 @@ struct Gemm {
             const uint32_t whole = (uint32_t)GM_EXTENT, rest = (uint32_t)left * (uint32_t)ld2 - 2u * (uint32_t)corner;
             return asked >= total || left <= 0 ? 0u : down && left < KS ? rest : whole;
         };
+        auto next_slot = [](uint32_t at) { return at + SLOT == LDS ? 0u : at + SLOT; };
+        auto slot_of_b = [&](uint32_t at) { return TURNS ? next_slot(at) : at + SLOT; };      // (of a stage whose A is at `at`)
+        auto next_step = [&](uint32_t at) { return TURNS ? next_slot(next_slot(at)) : at + 2 * SLOT == LDS ? 0u : at + 2 * SLOT; };
         // the copies of one more step: this wave's piece i of PA + PB, and then on to the next step
         uint32_t ea = 0, eb = 0;
         auto request = [&](int i) {
             if (i == 0) { ea = extent(A_DOWN, lda2, m0); eb = extent(B_DOWN, ldb2, n0); }
             if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && SideA::first_k(w * PA + i, lane) >= left ? GM_NOWHERE : va[i < PA ? i : 0], to + 1024 * (w * PA + i));
-            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && SideB::first_k(w * PB + i - PA, lane) >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], to + SideA::BYTES + 1024 * (w * PB + i - PA));
+            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && SideB::first_k(w * PB + i - PA, lane) >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], slot_of_b(to) + 1024 * (w * PB + i - PA));
             if (i < PA + PB - 1) return;
             ++asked;
             const bool second = asked == until_second;
             wa.at = second ? wa.second : wa.at + wa.stride;
             wb.at = second ? wb.second : wb.at + wb.stride;
             left = second ? K : left - KS;
-            to = to + STAGE == LDS ? 0 : to + STAGE;
+            to = next_step(to);
         };
         const uint32_t sa = SideA::share(lane), sb = SideB::share(lane);
         struct Fragments { V8 a[2][MT], b[2][NT]; } f0, f1;              // of the two halves of a stage
-        constexpr int FRAGMENTS = 2 * (NT + MT), ROUNDS = 2 * MT, COPIES = PA + PB;
+        constexpr int FRAGMENTS = 2 * (NT + MT), ROUNDS = 2 * MT, COPIES = PA + PB, SPREAD = (ROUNDS * 6 + 7) / 8;      // SPREAD: rounds that the copies of a half are spread over
         // fragment i of a half of the stage at `from`: in the order in which the products ask for them
-        auto fetch = [&](const char* from, int half, int i, Fragments& f) {
+        auto fetch = [&](uint32_t from, int half, int i, Fragments& f) {
             const int kk = i / (NT + MT), x = i % (NT + MT);
-            if (x < NT) f.b[kk][x < NT ? x : 0] = SideB::fragment(from + SideA::BYTES, sb, column_tile(wn, x), 2 * half + kk);
-            else f.a[kk][x < NT ? 0 : x - NT] = SideA::fragment(from, sa, wm * MT + x - NT, 2 * half + kk);
+            if (x < NT) f.b[kk][x < NT ? x : 0] = SideB::fragment(smem + slot_of_b(from), sb, column_tile(wn, x), 2 * half + kk);
+            else f.a[kk][x < NT ? 0 : x - NT] = SideA::fragment(smem + from, sa, wm * MT + x - NT, 2 * half + kk);
         };
         // The products of half a stage in rounds of NT, each with its share of the next half's fragments in front (and, early on, of the copies): whatever
         // they take to issue hides behind the products, which one after the other keep the matrix core busy.
-        auto half = [&](Fragments& now, const char* from, int which, Fragments& next, bool copies) {
+        auto half = [&](Fragments& now, uint32_t from, int which, Fragments& next, int first, int count) {
 #pragma unroll
             for (int i = 0; i < ROUNDS; ++i) {
 #pragma unroll
                 for (int f = i * FRAGMENTS / ROUNDS; f < (i + 1) * FRAGMENTS / ROUNDS; ++f) fetch(from, which, f, next);
-                if (copies && i < ROUNDS / 2) {
 #pragma unroll
-                    for (int r = i * COPIES * 2 / ROUNDS; r < (i + 1) * COPIES * 2 / ROUNDS; ++r) request(r);
-                }
+                for (int r = min(count, i * count / SPREAD); r < min(count, (i + 1) * count / SPREAD); ++r) request(first + r);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[j][i % MT] = mma32(now.b[i / MT][j], now.a[i / MT][i % MT], acc[j][i % MT]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -191,32 +200,32 @@ struct Gemm {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
 #pragma unroll
-        for (int t = 0; t < STAGES; ++t)
+        for (int t = 0; t < SLOTS / 2; ++t)
 #pragma unroll
             for (int r = 0; r < COPIES; ++r) request(r);
-        wait_vm_at_most<(STAGES - 1) * COPIES>();
+        wait_vm_at_most<(SLOTS / 2 - 1) * COPIES>();
         lds_barrier();
 #pragma unroll
-        for (int f = 0; f < FRAGMENTS; ++f) fetch(smem, 0, f, f0);
+        for (int f = 0; f < FRAGMENTS; ++f) fetch(0, 0, f, f0);
         uint32_t from = 0;
         auto next_stage = [&]() {
-            wait_vm_at_most<(STAGES - 2) * COPIES>();                // this wave's share of the next stage is there
+            wait_vm_at_most<(SLOTS / 2 - 2) * COPIES + (TURNS ? PA : 0)>();                // this wave's share of the next stage is there
             lds_barrier();                                           // ... everyone's is, and everyone has read this stage
-            from = from + STAGE == LDS ? 0 : from + STAGE;
+            from = next_step(from);
         };
         if constexpr (KS == 64) {
             for (int s = 0; s < total; ++s) {
-                half(f0, smem + from, 1, f1, false);
+                half(f0, from, 1, f1, 0, TURNS ? PA : 0);
                 next_stage();
-                half(f1, smem + from, 0, f0, true);
+                half(f1, from, 0, f0, TURNS ? PA : 0, TURNS ? PB : COPIES);
             }
         } else {
             // (an odd number of stages: one more, on zeros)
             for (int s = 0; s < total; s += 2) {
                 next_stage();
-                half(f0, smem + from, 0, f1, true);
+                half(f0, from, 0, f1, 0, COPIES);
                 next_stage();
-                half(f1, smem + from, 0, f0, true);
+                half(f1, from, 0, f0, 0, COPIES);
             }
         }
         wait_vm_at_most<0>();                                        // no copy into LDS outlives the workgroup, or meets the epilogue's use of it

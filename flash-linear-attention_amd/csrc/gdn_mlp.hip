@@ -94,9 +94,9 @@ __device__ __forceinline__ int64_t mlp_place(const MlpGemm& p, MlpTile t, int i,
     return m < o.M && n < o.N ? (int64_t)m * o.N + n : -1;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int KS, int SLOTS, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
+    typedef Gemm<T, BM, BN, WM, WN, KS, SLOTS, A_DOWN, B_DOWN, is_gate(EPI)> G;
     extern __shared__ __align__(16) char smem[];
     const int id = (int)blockIdx.x, shared = id - p.full;
     int tile, part = 0;
@@ -128,10 +128,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
         return;
     }
     // 32 rows at a time through this wave's share of the LDS, from the lanes' order into rows, so that the rows of 64 (32) columns leave in whole lines.  A row's
-    // 16-byte slots are XORed with the row: neither side meets a bank conflict.  s and a are asked for 32 rows before they are needed.  Straight from the lanes, 32 bytes
+    // 16-byte slots are XORed with the row: no bank conflicts in tiles of 256 x 256, in the smaller ones of both projections 2 % of the LDS cycles.  s and a are asked for 32 rows before they are needed.  Straight from the lanes, 32 bytes
     // of a row at a time, 8192 x 2048 x 5632 took 988 us backward (956 now), 32768 rows 3790 (3670).
     typedef typename Mma<T>::V8 V8;
-    constexpr int CW = 32 * COLS, SLOTS = CW / 4, PER_ROW = CW / 8, ROWS = 64 / PER_ROW, PASSES = 32 / ROWS;
+    constexpr int CW = 32 * COLS, QUADS = CW / 4, PER_ROW = CW / 8, ROWS = 64 / PER_ROW, PASSES = 32 / ROWS;
     static_assert(KINDS * 32 * CW * 4 * G::WAVES <= G::LDS, "32 rows of every wave fit in the LDS of the main loop");
     const GemmOperands& o = p.op[at.which];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = w % WM, wn = w / WM;
@@ -159,8 +159,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
                 const int m = lane & 31, slot = 4 * c + 2 * (lane >> 5);
                 const f32x8 x = result(i, kind * ROUND + c);
                 float* to = area + kind * 32 * CW + m * CW;
-                *(f32x4*)(to + 4 * (slot ^ (m & (SLOTS - 1)))) = f32x4{x[0], x[1], x[2], x[3]};
-                *(f32x4*)(to + 4 * ((slot + 1) ^ (m & (SLOTS - 1)))) = f32x4{x[4], x[5], x[6], x[7]};
+                *(f32x4*)(to + 4 * (slot ^ (m & (QUADS - 1)))) = f32x4{x[0], x[1], x[2], x[3]};
+                *(f32x4*)(to + 4 * ((slot + 1) ^ (m & (QUADS - 1)))) = f32x4{x[4], x[5], x[6], x[7]};
             }
 #pragma unroll
         for (int r = 0; r < PASSES; ++r) {
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
 #pragma unroll
             for (int kind = 0; kind < KINDS; ++kind) {
                 const float* from = area + kind * 32 * CW + m * CW;
-                const f32x4 lo = *(const f32x4*)(from + 4 * (slot ^ (m & (SLOTS - 1)))), hi = *(const f32x4*)(from + 4 * ((slot + 1) ^ (m & (SLOTS - 1))));
+                const f32x4 lo = *(const f32x4*)(from + 4 * (slot ^ (m & (QUADS - 1)))), hi = *(const f32x4*)(from + 4 * ((slot + 1) ^ (m & (QUADS - 1))));
                 x[kind] = f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
             if (row0 + 32 * i + ROWS * r < o.M && n < o.N)
@@ -179,9 +179,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
 }
 
 // The parts of a shared tile added up, in order, and what becomes of the sums: a workgroup for eight results of every lane.
-template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool A_DOWN, bool B_DOWN, int EPI>
+template <typename T, int BM, int BN, int WM, int WN, int KS, int SLOTS, bool A_DOWN, bool B_DOWN, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
-    typedef Gemm<T, BM, BN, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
+    typedef Gemm<T, BM, BN, WM, WN, KS, SLOTS, A_DOWN, B_DOWN, is_gate(EPI)> G;
     constexpr int KINDS = is_gate(EPI) ? 2 : 1, COLS = G::NT / KINDS, CHUNKS = G::MT * COLS * 2;
     const int tile = (int)blockIdx.x / CHUNKS, chunk = (int)blockIdx.x % CHUNKS;
     const float* sums = p.sums + (int64_t)tile * p.parts * (BM * BN) + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8;
@@ -208,16 +208,16 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 // How the products of a launch are cut: the tiles, and over how many workgroups the contraction of each tile is shared out that does not fill a round of the
 // chip (`rest` tiles of `parts` workgroups after `full` of one): the least of the times that the launch would take by these figures.
 //   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)   a round's begin and end, more with an activation or
-//   256 x 256   8      1 a CU       1.65                                  1.05                            8, 4                          the inner gradients
-//   128 x 128   4      2 a CU       1.0                                   0.6                             4, 3      two stages of LDS: half the CU's
-//   128 x 128   8      1 a CU       0.58                                  0.4                             4.5, 2.5  four stages: more in flight, for few workgroups
+//   256 x 256   8      1 a CU       1.55                                  1.05                            8, 4                          the inner gradients
+//   128 x 128   4      2 a CU       1.0                                   0.6                             4, 3      five slots of LDS: half the CU's
+//   128 x 128   8      1 a CU       0.58                                  0.4                             4.5, 2.5  eight: more in flight, for few workgroups
 //   64 x 64     2      2 a CU       0.45                                  0.28                            4, 2.5    the same, where no operand is read down its columns
-// In between a stage's time grows with the workgroups: a full chip is held back by its power and its caches, not by the stages.  Joining parts takes 5.5 us and
+// In between a stage's time grows with the workgroups: a full chip is held back by its caches and its clock, too.  Joining parts takes 5.5 us and
 // their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
 // forward): 48 rows 61 us in 128 x 128 tiles, 28 us; 333 rows 85 -> 49 us; 2000 rows 213 us in 256 x 256 tiles, 155 us.  The weights' gradients of 8192 x 2048 x
 // 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 8 parts each, the backward 1186 -> 1026 us.
-struct MlpTiles { int side, waves_m, waves_n, stages, per_cu; double full, least, round, more; };
-constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 2, 1, 1.65, 1.05, 8, 4}, {128, 2, 2, 2, 2, 1.0, 0.6, 4, 3}, {128, 4, 2, 4, 1, 0.58, 0.4, 4.5, 2.5}, {64, 2, 1, 4, 2, 0.45, 0.28, 4, 2.5}};
+struct MlpTiles { int side, waves_m, waves_n, slots, per_cu; double full, least, round, more; };
+constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 5, 1, 1.55, 1.05, 8, 4}, {128, 2, 2, 5, 2, 1.0, 0.6, 4, 3}, {128, 4, 2, 8, 1, 0.58, 0.4, 4.5, 2.5}, {64, 2, 1, 8, 2, 0.45, 0.28, 4, 2.5}};
 struct MlpPlan { int tiles, full, rest, parts; };
 static MlpPlan plan_gemm(const MlpGemm& p, int epilogue, bool rows) {
     const int kinds = is_gate(epilogue) ? 2 : 1;
@@ -252,11 +252,11 @@ struct Workspace { void* at; size_t bytes; };
 
 template <typename T, int TILES, bool A_DOWN, bool B_DOWN, int EPI>
 static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
-    // (both operands down their columns: stages of half the width, twice as many)
+    // (both operands down their columns: stages of half the width, twice as many, an even number of slots)
     // (both projections in a 256 x 256 tile: 64 columns of each to a wave, a whole line of every result's row)
     constexpr bool WIDE = is_gate(EPI) && MLP_TILES[TILES].side == 256;
-    constexpr int SIDE = MLP_TILES[TILES].side, WM = WIDE ? 4 : MLP_TILES[TILES].waves_m, WN = WIDE ? 2 : MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, STAGES = MLP_TILES[TILES].stages * 64 / KS;
-    typedef Gemm<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, is_gate(EPI)> G;
+    constexpr int SIDE = MLP_TILES[TILES].side, WM = WIDE ? 4 : MLP_TILES[TILES].waves_m, WN = WIDE ? 2 : MLP_TILES[TILES].waves_n, KS = A_DOWN && B_DOWN ? 32 : 64, SLOTS = KS == 64 ? MLP_TILES[TILES].slots : 4 * (MLP_TILES[TILES].slots / 2);
+    typedef Gemm<T, SIDE, SIDE, WM, WN, KS, SLOTS, A_DOWN, B_DOWN, is_gate(EPI)> G;
     int64_t tiles = 0;
     for (int i = 0; i < p.ops; ++i) {
         GemmOperands& o = p.op[i];
@@ -269,14 +269,14 @@ static int launch_tiles(MlpGemm& p, const MlpPlan& plan, hipStream_t stream) {
     if (tiles == 0) return GDN_OK;
     p.full = plan.full; p.rest = plan.rest; p.parts = plan.parts;
     GDN_CHECK_ARG(tiles == (int64_t)p.full + p.rest, GDN_ERR_INVALID, "the gated feed-forward block: a plan for %d tiles, not %lld", p.full + p.rest, (long long)tiles);
-    auto kernel = mlp_gemm_kernel<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>;
+    auto kernel = mlp_gemm_kernel<T, SIDE, SIDE, WM, WN, KS, SLOTS, A_DOWN, B_DOWN, EPI>;
     const int rc = ensure_dynamic_smem_for((const void*)kernel, G::LDS, "mlp_gemm_kernel");
     if (rc != GDN_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(p.full + p.rest * p.parts)), dim3(G::THREADS), G::LDS, stream, p);
     if (p.rest == 0) return check_launch("mlp_gemm_kernel");
     const int rc2 = check_launch("mlp_gemm_kernel");
     if (rc2 != GDN_OK) return rc2;
-    hipLaunchKernelGGL((mlp_join_kernel<T, SIDE, SIDE, WM, WN, KS, STAGES, A_DOWN, B_DOWN, EPI>), dim3((unsigned)(p.rest * G::MT * G::NT * 2 / (is_gate(EPI) ? 2 : 1))),
+    hipLaunchKernelGGL((mlp_join_kernel<T, SIDE, SIDE, WM, WN, KS, SLOTS, A_DOWN, B_DOWN, EPI>), dim3((unsigned)(p.rest * G::MT * G::NT * 2 / (is_gate(EPI) ? 2 : 1))),
                        dim3(G::THREADS), 0, stream, p);
     return check_launch("mlp_join_kernel");
 }
