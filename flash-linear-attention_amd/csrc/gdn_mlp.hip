@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
     }
     // 32 rows at a time through this wave's share of the LDS, from the lanes' order into rows, so that the rows of 64 (32) columns leave in whole lines.  A row's
     // 16-byte slots are XORed with the row: no bank conflicts in tiles of 256 x 256, in the smaller ones of both projections 2 % of the LDS cycles.  s and a are asked for 32 rows before they are needed.  Straight from the lanes, 32 bytes
-    // of a row at a time, 8192 x 2048 x 5632 took 988 us backward (956 now), 32768 rows 3790 (3670).
+    // of a row at a time, 8192 x 2048 x 5632 took 988 us backward (this way 956), 32768 rows 3790 (3670), with four operand slots.
     typedef typename Mma<T>::V8 V8;
     constexpr int CW = 32 * COLS, QUADS = CW / 4, PER_ROW = CW / 8, ROWS = 64 / PER_ROW, PASSES = 32 / ROWS;
     static_assert(KINDS * 32 * CW * 4 * G::WAVES <= G::LDS, "32 rows of every wave fit in the LDS of the main loop");
