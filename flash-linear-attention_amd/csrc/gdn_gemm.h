@@ -42,7 +42,8 @@ struct GemmOperands {
 
 typedef uint32_t gm_rsrc __attribute__((ext_vector_type(4)));
 
-// 64 x 16 bytes from a buffer into LDS at lds_off + 16 lane; places at or past `extent` arrive as zeros
+// 64 x 16 bytes from a buffer into LDS at lds_off + 16 lane; places at or past `extent` arrive as zeros.  (s_nop: a load into LDS needs one wait state after the
+// scalar write of M0, which the compiler does not see to inside assembly.  M0 is a reserved register: the compiler writes it itself before every use.)
 __device__ __forceinline__ void buffer_1k_to_lds(uint64_t base, uint32_t extent, uint32_t voff, uint32_t lds_off) {
     gm_rsrc r;
     r[0] = __builtin_amdgcn_readfirstlane((uint32_t)base);
@@ -50,7 +51,7 @@ __device__ __forceinline__ void buffer_1k_to_lds(uint64_t base, uint32_t extent,
     r[2] = __builtin_amdgcn_readfirstlane(extent);
     r[3] = 0x00020000;
     lds_off = __builtin_amdgcn_readfirstlane(lds_off);
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_off), "v"(voff), "s"(r));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_off), "v"(voff), "s"(r));
 }
 
 constexpr uint32_t GM_NOWHERE = 0xffff0000u;
