@@ -118,14 +118,19 @@ __device__ __forceinline__ float sigmoid_stream(float x) {
 // 16 bytes at gbase + voff (gbase wave-uniform, voff per lane) and they land at the
 // wave-uniform LDS byte offset `lds_off` + 16 l.  Issued from inline assembly on purpose: the
 // compiler then keeps no account of it, and completion is awaited explicitly with s_waitcnt
-// vmcnt before the barrier that publishes the data.  The compiler does not see to wait states inside assembly either: a load into LDS
-// needs one after the scalar write of M0 (s_nop here, the mask's instruction in the masked form).
+// vmcnt before the barrier that publishes the data.  The compiler does not see to wait states inside assembly either.  A load into LDS
+// needs one after the scalar write of M0, and a vector memory instruction five after a vector instruction (readfirstlane) has written a
+// scalar register that it reads.  So a scalar instruction copies the address onto itself in between, which is both: it waits for
+// the vector instruction by itself, and what it writes may be read at once.
 __device__ __forceinline__ void gather_1k_to_lds(const char* gbase, uint32_t voff, uint32_t lds_off) {
     lds_off = __builtin_amdgcn_readfirstlane(lds_off);          // wave-uniform by construction; make them scalars
     const uint64_t g = (uint64_t)gbase;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)g), hi = __builtin_amdgcn_readfirstlane((uint32_t)(g >> 32));
     const uint64_t gs = ((uint64_t)hi << 32) | lo;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_off), "v"(voff), "s"(gs));
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_mov_b64 %2, %2\n\t"
+                 "global_load_lds_dwordx4 %1, %2"
+                 : : "s"(lds_off), "v"(voff), "s"(gs));
 }
 
 // The same copy for the lanes named by `mask` only (the others leave their 16 bytes of LDS as they are).
@@ -139,6 +144,7 @@ __device__ __forceinline__ void gather_1k_to_lds_masked(const char* gbase, uint3
     mask = ((uint64_t)mhi << 32) | mlo;                         // wave-uniform by construction; make it scalar registers
     uint64_t saved;
     asm volatile("s_mov_b32 m0, %1\n\t"
+                 "s_mov_b64 %3, %3\n\t"
                  "s_and_saveexec_b64 %0, %4\n\t"
                  "global_load_lds_dwordx4 %2, %3\n\t"
                  "s_mov_b64 exec, %0"

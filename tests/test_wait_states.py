@@ -2,7 +2,9 @@
 writes; it does not look inside inline assembly, so vector memory instructions written by hand have to bring their own.  Read from the disassembled gfx950
 code objects of libgdn_hip.so (CPU: nothing runs).
 
-  a scalar write of M0, then a load into LDS (which takes its place in LDS from M0): one wait state"""
+  a scalar write of M0, then a load into LDS (which takes its place in LDS from M0): one wait state
+  a vector instruction that writes a scalar register, then a vector memory instruction that reads it: five, unless a scalar
+  instruction (which waits by itself) has written the register in between"""
 import collections
 import functools
 import os
@@ -81,5 +83,38 @@ def test_loads_into_lds_wait_for_their_place():
     def test(code, i):
         if _into_lds(code[i]):
             return not any(re.match(r's_\w+ m0\b', before) for before in _before(code, i, 1))
+    failures, seen = _short(test)
+    assert seen > 1000 and not failures, (seen, failures)
+
+
+def _registers(text, kind):
+    found = set()
+    for one, first, last in re.findall(rf'\b{kind}(?:(\d+)\b|\[(\d+):(\d+)\])', text):
+        found |= {int(one)} if one else set(range(int(first), int(last) + 1))
+    return found
+
+
+def _scalars_written_by_a_vector_instruction(instruction):
+    op, _, operands = instruction.partition(' ')
+    operands = operands.split(',')
+    if op.startswith(('v_readfirstlane', 'v_readlane', 'v_cmp')):
+        return _registers(operands[0], 's')
+    if op.startswith(('v_add_co', 'v_addc_co', 'v_sub', 'v_div_scale', 'v_mad_u64', 'v_mad_i64')) and len(operands) > 1:
+        return _registers(operands[1], 's')                                    # (a carry)
+    return set()
+
+
+def test_vector_memory_waits_for_the_scalars_it_reads():
+    def test(code, i):
+        if code[i].startswith(('global_', 'buffer_', 'flat_', 'scratch_')):
+            reads = _registers(code[i], 's')
+            if not reads:
+                return None
+            for before in _before(code, i, 5):
+                if before.startswith('v_') and _scalars_written_by_a_vector_instruction(before) & reads:
+                    return False
+                if before.startswith('s_') and ' ' in before:
+                    reads = reads - _registers(before.split(' ', 1)[1].split(',')[0], 's')
+            return True
     failures, seen = _short(test)
     assert seen > 1000 and not failures, (seen, failures)
