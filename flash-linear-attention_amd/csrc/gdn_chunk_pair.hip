@@ -35,15 +35,19 @@ constexpr int PAIR_THREADS = 512;
 // One 16-byte store per lane at sbase + voff, for the lanes named by `mask` only.  Written in
 // assembly so that the address stays a scalar base plus a 32-bit lane offset, and so that exactly
 // one operation is issued whatever the mask: the execution mask is narrowed around the store by
-// hand instead of by a conditional in the source.
+// hand instead of by a conditional in the source.  (A vector instruction may write the stored registers two wait
+// states after a store of 16 bytes, and the store may read an address that a vector instruction wrote five after it, or behind a
+// scalar one: the compiler does not see to either inside assembly.)
 __device__ __forceinline__ void store16_masked(const char* sbase, uint32_t voff, u32x4 d, uint64_t mask) {
     const uint64_t g = (uint64_t)sbase;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)g), hi = __builtin_amdgcn_readfirstlane((uint32_t)(g >> 32));
     const uint64_t gs = ((uint64_t)hi << 32) | lo;
     uint64_t saved;
-    asm volatile("s_and_saveexec_b64 %0, %1\n\t"
+    asm volatile("s_mov_b64 %4, %4\n\t"
+                 "s_and_saveexec_b64 %0, %1\n\t"
                  "global_store_dwordx4 %2, %3, %4\n\t"
-                 "s_mov_b64 exec, %0"
+                 "s_mov_b64 exec, %0\n\t"
+                 "s_nop 0"
                  : "=&s"(saved) : "s"(mask), "v"(voff), "v"(d), "s"(gs) : "memory", "scc");
 }
 

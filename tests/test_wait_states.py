@@ -4,7 +4,8 @@ code objects of libgdn_hip.so (CPU: nothing runs).
 
   a scalar write of M0, then a load into LDS (which takes its place in LDS from M0): one wait state
   a vector instruction that writes a scalar register, then a vector memory instruction that reads it: five, unless a scalar
-  instruction (which waits by itself) has written the register in between"""
+  instruction (which waits by itself) has written the register in between
+  a store of more than 8 bytes, then a vector instruction that writes the stored registers: two"""
 import collections
 import functools
 import os
@@ -116,5 +117,25 @@ def test_vector_memory_waits_for_the_scalars_it_reads():
                 if before.startswith('s_') and ' ' in before:
                     reads = reads - _registers(before.split(' ', 1)[1].split(',')[0], 's')
             return True
+    failures, seen = _short(test)
+    assert seen > 1000 and not failures, (seen, failures)
+
+
+def _after(code, i, states):
+    """The instructions that may run less than `states` + 1 wait states after instruction i."""
+    while i + 1 < len(code) and states > 0:
+        i += 1
+        if code[i].startswith(('s_branch', 's_endpgm')):
+            return
+        yield code[i]
+        states -= int(code[i].split()[1]) + 1 if code[i].startswith('s_nop') else 1
+
+
+def test_stored_registers_are_not_written_too_soon():
+    def test(code, i):
+        store = re.match(r'(global|flat|scratch|buffer)_store_dwordx[34] (.*)', code[i])
+        if store:
+            data = _registers(store.group(2).split(',')[0 if store.group(1) == 'buffer' else 1], 'v')
+            return not any(after.startswith('v_') and ' ' in after and _registers(after.split(' ', 1)[1].split(',')[0], 'v') & data for after in _after(code, i, 2))
     failures, seen = _short(test)
     assert seen > 1000 and not failures, (seen, failures)
