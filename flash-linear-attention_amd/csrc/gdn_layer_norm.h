@@ -25,6 +25,8 @@ struct NormRow {
     static __device__ __forceinline__ int column(int l, int i, int e) { return (l + LANES * i) * VEC + e; }
 
     template <typename S> using Piece = S __attribute__((ext_vector_type(VEC)));
+    // (in memory, of rows that begin on 16-byte boundaries: eight fp32 values lie on no others, either)
+    template <typename S> using WholePiece = S __attribute__((ext_vector_type(VEC), aligned(16)));
     // (rows that do not begin on 16-byte boundaries: the same wide loads and stores at any address, and element by element only where a row ends inside a piece)
     template <typename S> using AnyPiece = S __attribute__((ext_vector_type(VEC), aligned(sizeof(S))));
 
@@ -33,7 +35,7 @@ struct NormRow {
         const int c = column(l, i, 0);
         Piece<S> v{};
         if constexpr (ALIGNED) {
-            if (c < D) v = *(const Piece<S>*)(row + c);
+            if (c < D) v = *(const WholePiece<S>*)(row + c);
         } else if (c + VEC <= D) {
             v = *(const AnyPiece<S>*)(row + c);
         } else if (c < D) {
@@ -46,7 +48,7 @@ struct NormRow {
     static __device__ __forceinline__ void store(S* row, int l, int i, int D, Piece<S> v) {
         const int c = column(l, i, 0);
         if constexpr (ALIGNED) {
-            if (c < D) *(Piece<S>*)(row + c) = v;
+            if (c < D) *(WholePiece<S>*)(row + c) = v;
         } else if (c + VEC <= D) {
             *(AnyPiece<S>*)(row + c) = v;
         } else if (c < D) {

@@ -44,6 +44,7 @@ enum MlpEpilogue { MLP_PLAIN, MLP_GRAD, MLP_GATE };
 constexpr bool is_gate(int epilogue) { return epilogue >= MLP_GATE; }
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8_at16 __attribute__((ext_vector_type(8), aligned(16)));       // (in the workspace, which lies on 16-byte boundaries)
 
 // What becomes of eight neighbours of a result (of both products where there are two), at offset `at` of the outputs; MLP_GRAD: sv, av are the
 // forward's s and a there.
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mlp_gemm_kernel(MlpGemm p) {
 #pragma unroll
             for (int c = 0; c < ROUND; ++c)
 #pragma unroll
-                for (int kind = 0; kind < KINDS; ++kind) *(f32x8*)(sums + (int64_t)((i * ROUND + c) * KINDS + kind) * G::THREADS * 8) = result(i, kind * ROUND + c);
+                for (int kind = 0; kind < KINDS; ++kind) *(f32x8_at16*)(sums + (int64_t)((i * ROUND + c) * KINDS + kind) * G::THREADS * 8) = result(i, kind * ROUND + c);
         return;
     }
     // 32 rows at a time through this wave's share of the LDS, from the lanes' order into rows, so that the rows of 64 (32) columns leave in whole lines.  A row's
@@ -185,11 +186,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mlp_join_kernel(MlpGemm p) {
     constexpr int KINDS = is_gate(EPI) ? 2 : 1, COLS = G::NT / KINDS, CHUNKS = G::MT * COLS * 2;
     const int tile = (int)blockIdx.x / CHUNKS, chunk = (int)blockIdx.x % CHUNKS;
     const float* sums = p.sums + (int64_t)tile * p.parts * (BM * BN) + ((int64_t)(chunk * KINDS) * G::THREADS + threadIdx.x) * 8;
-    f32x8 x = *(const f32x8*)sums, u = x;
-    if (KINDS == 2) u = *(const f32x8*)(sums + G::THREADS * 8);
+    f32x8 x = *(const f32x8_at16*)sums, u = x;
+    if (KINDS == 2) u = *(const f32x8_at16*)(sums + G::THREADS * 8);
     for (int s = 1; s < p.parts; ++s) {
-        x += *(const f32x8*)(sums + (int64_t)s * (BM * BN));
-        if (KINDS == 2) u += *(const f32x8*)(sums + (int64_t)s * (BM * BN) + G::THREADS * 8);
+        x += *(const f32x8_at16*)(sums + (int64_t)s * (BM * BN));
+        if (KINDS == 2) u += *(const f32x8_at16*)(sums + (int64_t)s * (BM * BN) + G::THREADS * 8);
     }
     const MlpTile at = mlp_tile(p, p.full + tile);
     const int64_t to = mlp_place<G>(p, at, chunk / 2 / COLS, chunk / 2 % COLS, chunk % 2);
@@ -642,8 +643,8 @@ extern "C" int gdn_gated_mlp_fwd(const void* x, const void* wg, const void* wu, 
     if (rc != GDN_OK) return rc;
     if (M == 0) return GDN_OK;
     GDN_CHECK_ARG(x && wg && wu && wd && y && h && !s == !a, GDN_ERR_INVALID, "%s: x, the weights, y and h are required, s goes with a", who);
-    GDN_CHECK_ARG(few || (((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h) & 15) == 0,
-                  GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
+    GDN_CHECK_ARG(few || (((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)y | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h |
+                           (uintptr_t)workspace) & 15) == 0, GDN_ERR_INVALID, "%s: tensors and workspace must be 16-byte aligned", who);
     hipStream_t q = (hipStream_t)stream;
     const Workspace ws{workspace, workspace_bytes};
     return dtype == GDN_DTYPE_BF16 ? mlp_fwd<bf16_t>(x, wg, wu, wd, y, s, a, h, ws, M, D, F, activation, q)
@@ -660,8 +661,8 @@ extern "C" int gdn_gated_mlp_bwd(const void* dy, const void* x, const void* wg, 
     GDN_CHECK_ARG(M == 0 || (dy && (!inner || (wd && s && a && dg && du)) && (!dx || (wg && wu)) && ((!dwg && !dwu) || x) && (!dwd || h)), GDN_ERR_INVALID,
                   "%s: a tensor that the asked gradients need is missing", who);
     GDN_CHECK_ARG((((uintptr_t)dy | (uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu | (uintptr_t)wd | (uintptr_t)s | (uintptr_t)a | (uintptr_t)h | (uintptr_t)dg |
-                    (uintptr_t)du | (uintptr_t)dx | (uintptr_t)dwg | (uintptr_t)dwu | (uintptr_t)dwd) & 15) == 0,
-                  GDN_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
+                    (uintptr_t)du | (uintptr_t)dx | (uintptr_t)dwg | (uintptr_t)dwu | (uintptr_t)dwd | (uintptr_t)workspace) & 15) == 0,
+                  GDN_ERR_INVALID, "%s: tensors and workspace must be 16-byte aligned", who);
     hipStream_t q = (hipStream_t)stream;
     const Workspace ws{workspace, workspace_bytes};
     return dtype == GDN_DTYPE_BF16 ? mlp_bwd<bf16_t>(dy, x, wg, wu, wd, s, a, h, dg, du, dx, dwg, dwu, dwd, ws, M, D, F, q)

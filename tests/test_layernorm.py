@@ -179,6 +179,26 @@ def test_strides_shapes_and_orders():
 
 
 @gpu
+@pytest.mark.parametrize('D', [64, 512, 2048])
+def test_fp32_tensors_on_every_16_byte_boundary(D):
+    """16-bit rows with the stream, its gradient, weight and bias in fp32, each four elements off a boundary of 32 bytes."""
+    t = _inputs(21, D, BF, FP, FP, True)
+    for name in ('residual', 'dres', 'weight', 'bias'):
+        v = t[name]
+        t[name] = torch.cat([v.new_zeros(4), v.flatten()])[4:].view(v.shape)
+        assert t[name].data_ptr() % 32 == 16
+    mods = _mods()
+    keep = {k: v.requires_grad_(True) for k, v in t.items() if k in ('x', 'residual', 'weight', 'bias')}
+    y, stream = mods.layer_norm(*(keep[k] for k in ('x', 'weight', 'bias')), residual=keep['residual'], prenorm=True)
+    grads = torch.autograd.grad([y, stream], list(keep.values()), [t['dy'], t['dres']])
+    want = {k: v.detach().clone().requires_grad_(True) for k, v in keep.items()}
+    y1, stream1 = mods.layer_norm(*(want[k] for k in ('x', 'weight', 'bias')), residual=want['residual'], prenorm=True)
+    assert torch.equal(y, y1) and torch.equal(stream, stream1)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad([y1, stream1], list(want.values()), [t['dy'], t['dres'].clone()])))
+    _check(_inputs(21, D, BF, FP, FP, True), False)
+
+
+@gpu
 def test_gradients_that_are_asked_for():
     mods = _mods()
     t = _inputs(50, 384, BF, FP, FP, True)

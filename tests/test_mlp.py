@@ -435,6 +435,19 @@ def test_the_entry_points_refuse():
     assert lib.gdn_gated_mlp_workspace_bytes(-1, 8, 8, 0) == lib.gdn_gated_mlp_workspace_bytes(8, 12, 8, 1) == 0
 
 
+def test_a_workspace_between_16_byte_boundaries_is_refused():
+    """By the library's host code: nothing is launched.  (Up to 16 rows there is none to look at.)"""
+    from fla_hip import _lib
+    try:
+        lib = _lib.load()
+    except _lib.GDNLibraryError:
+        pytest.skip('not built in this checkout')
+    P, n = 1 << 20, 1 << 40
+    for off in (4, 8, 12):
+        assert lib.gdn_gated_mlp_fwd(*[P] * 5, None, None, P, P + off, n, 48, 2048, 64, 1, 0, None) == _lib.GDN_ERR_INVALID
+        assert lib.gdn_gated_mlp_bwd(*[P] * 14, P + off, n, 48, 2048, 64, 0, None) == _lib.GDN_ERR_INVALID
+
+
 @gpu
 def test_matrices_of_other_sizes():
     """gdn_pad_rows: zeros where there is no source, several matrices in a launch, nothing beside them."""
