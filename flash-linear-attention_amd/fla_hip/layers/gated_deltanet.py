@@ -22,13 +22,12 @@ import warnings
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.nn.modules.module import _has_any_global_hook
-from torch.utils._device import DeviceContext
 
 from fla_hip import _lib
 from fla_hip.modules import FusedRMSNormGated, ShortConvolution
 from fla_hip.ops.backends import has_backends
 from fla_hip.ops.gated_delta_rule import chunk_gated_delta_rule, fused_recurrent_gated_delta_rule
+from fla_hip.utils import calls_are_watched, calls_nothing_else
 
 
 _STEP_LINEARS = ('q_proj', 'k_proj', 'v_proj', 'a_proj', 'b_proj', 'g_proj', 'o_proj')
@@ -46,11 +45,7 @@ _CALLS = _calls()
 
 
 def _watched() -> bool:
-    """Whether something looks at, or stands in for, the calls between all modules: hooks on every module, torch's dispatch and
-    function modes (a default device is none of those), one of ``_CALLS`` patched."""
-    n = torch._C._len_torch_function_stack()
-    return (_has_any_global_hook() or torch._C._len_torch_dispatch_stack() > 0 or _calls() != _CALLS
-            or (n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))))
+    return calls_are_watched() or _calls() != _CALLS
 
 
 class LayerCache:
@@ -176,12 +171,9 @@ class GatedDeltaNet(nn.Module):
         for cls, names in _PARTS:
             for name in names:
                 m = mods[name]
-                d = m.__dict__
-                # calling m is cls.forward and nothing else: no other class, no hooks, no `forward` of its own, not compiled
-                if (type(m) is not cls or d['_forward_hooks'] or d['_forward_pre_hooks'] or d['_backward_hooks'] or d['_backward_pre_hooks']
-                        or 'forward' in d or 'step' in d or '_compiled_call_impl' in d):
+                if not calls_nothing_else(m, cls) or 'step' in m.__dict__:
                     return None
-                params = d['_parameters']
+                params = m.__dict__['_parameters']
                 w = params.get('weight')
                 if type(w) is not nn.Parameter or (cls is nn.Linear and params.get('bias') is not None):
                     return None

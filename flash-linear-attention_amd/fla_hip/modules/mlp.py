@@ -9,6 +9,7 @@ import torch.nn.functional as F
 
 from fla_hip import _lib
 from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, ptr, require_gpu
+from fla_hip.utils import calls_are_watched, calls_nothing_else
 
 _ACTIVATIONS = {'swish': _lib.ACT_SILU, 'silu': _lib.ACT_SILU, 'sigmoid': _lib.ACT_SIGMOID, 'gelu_tanh': _lib.ACT_GELU_TANH}
 
@@ -127,9 +128,20 @@ def gated_mlp(
     return y.reshape(x.shape)
 
 
+def _calls() -> tuple:
+    return nn.Module.__call__, F.linear, nn.Linear.forward
+
+
+# The calls that the operator stands for.  Where a caller has replaced one of them - here, on a module or around every module - the
+# block runs projection by projection and makes it.
+_CALLS = _calls()
+
+
 class GatedMLP(nn.Module):
     """The feed-forward block as the reference's layer of that name builds it: no biases, the inner width ``hidden_ratio`` times two thirds of the hidden
-    size, rounded up to a multiple of 256, unless it is given.  ``fuse_swiglu`` is taken for the reference's sake: there is one path."""
+    size, rounded up to a multiple of 256, unless it is given.  ``fuse_swiglu`` is taken for the reference's sake: there is one path.  That path is
+    ``gated_mlp`` on the three weights, as long as calling the projections would do nothing else; adapters in their places, biases, hooks and the like are
+    called, with the activation and the product in fp32 torch between them."""
 
     def __init__(
         self,
@@ -156,5 +168,28 @@ class GatedMLP(nn.Module):
         self.up_proj = nn.Linear(hidden_size, intermediate_size, bias=False, **kwargs)
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False, **kwargs)
 
+    def _weights(self):
+        """The projections' weights where calling them is a product with those and nothing else, or None."""
+        if calls_are_watched() or _calls() != _CALLS:
+            return None
+        weights = []
+        for name in ('gate_proj', 'up_proj', 'down_proj'):
+            m = self._modules[name]
+            if not calls_nothing_else(m, nn.Linear):
+                return None
+            params = m.__dict__['_parameters']
+            # (torch.func.functional_call puts plain tensors in the parameters' places)
+            if type(params.get('weight')) not in (nn.Parameter, torch.Tensor) or params.get('bias') is not None:
+                return None
+            weights.append(params['weight'])
+        return weights
+
     def forward(self, x: torch.Tensor, **kwargs) -> torch.Tensor:
-        return gated_mlp(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.hidden_act)
+        weights = self._weights()
+        if weights is not None:
+            return gated_mlp(x, *weights, self.hidden_act)
+        require_gpu(x)
+        gate, up = self.gate_proj(x), self.up_proj(x)
+        g = gate.float()
+        act = torch.sigmoid(g) if self.hidden_act == 'sigmoid' else F.gelu(g, approximate='tanh') if self.hidden_act == 'gelu_tanh' else F.silu(g)
+        return self.down_proj((act * up.float()).to(up.dtype))

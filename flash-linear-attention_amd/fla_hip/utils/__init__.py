@@ -13,6 +13,8 @@ from collections import deque
 from typing import Any, Callable
 
 import torch
+from torch.nn.modules.module import _has_any_global_hook
+from torch.utils._device import DeviceContext
 
 logger = logging.getLogger(__name__)
 
@@ -99,6 +101,22 @@ def input_guard(fn: Callable | None = None, *, no_guard_contiguous=False):
 contiguous = input_guard
 
 
+def calls_are_watched() -> bool:
+    """Whether something looks at, or stands in for, the calls between all modules: hooks on every module, torch's dispatch and
+    function modes (a default device is none of those)."""
+    n = torch._C._len_torch_function_stack()
+    return (_has_any_global_hook() or torch._C._len_torch_dispatch_stack() > 0
+            or (n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))))
+
+
+def calls_nothing_else(module: torch.nn.Module, cls: type) -> bool:
+    """Whether calling ``module`` is ``cls.forward`` and nothing besides: no other class, no hooks, no ``forward`` of its own, not
+    compiled."""
+    d = module.__dict__
+    return not (type(module) is not cls or d['_forward_hooks'] or d['_forward_pre_hooks'] or d['_backward_hooks'] or d['_backward_pre_hooks']
+                or 'forward' in d or '_compiled_call_impl' in d)
+
+
 def get_abs_err(x: torch.Tensor, y: torch.Tensor) -> float:
     return (x.detach() - y.detach()).flatten().abs().max().item()
 
@@ -131,4 +149,4 @@ def assert_close(prefix: str, ref: torch.Tensor, tri: torch.Tensor, ratio: float
         warnings.warn(report)
 
 
-__all__ = ['tensor_cache', 'input_guard', 'contiguous', 'get_abs_err', 'get_err_ratio', 'assert_close']
+__all__ = ['tensor_cache', 'input_guard', 'contiguous', 'calls_are_watched', 'calls_nothing_else', 'get_abs_err', 'get_err_ratio', 'assert_close']
