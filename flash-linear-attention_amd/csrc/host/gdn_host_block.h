@@ -16,6 +16,12 @@ variable_list differentiable_once(variable_list grads) {
     return grads;
 }
 
+// A saved tensor as the kernels take it (`saved`), of the type and the number of elements that it had: hooks may have handed back something else.
+at::Tensor restored(const at::Tensor& t, at::ScalarType type, c10::Device dev, int64_t elements) {
+    TORCH_CHECK_VALUE(!t.defined() || t.numel() == elements, "a saved tensor of ", elements, " elements came back with ", t.numel());
+    return saved(t, type, dev);
+}
+
 // ---- normalisation ----
 struct NormCall {
     int64_t rows, D;
@@ -47,7 +53,7 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
         norm_forward(c, x, weight, bias, residual, true, y, stream, mean, rstd);
         ctx->save_for_backward({c.own_stream ? stream : x, weight, mean, rstd});
         ctx->saved_data["call"] = std::vector<int64_t>{c.rows, c.D, c.w_code, c.rms, (int64_t)c.stream_type, (int64_t)x.scalar_type(), weight.defined(), bias.defined(),
-                                                       residual.defined(), bias.defined() ? (int64_t)bias.scalar_type() : 0};
+                                                       residual.defined(), (int64_t)(weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : at::kFloat)};
         ctx->saved_data["shape"] = x.sizes().vec();
         ctx->saved_data["device"] = x.device();
         ctx->set_materialize_grads(false);
@@ -62,9 +68,11 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
         const std::vector<int64_t> n = ctx->saved_data["call"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
         const int64_t rows = n[0], D = n[1];
         const at::ScalarType stream_type = (at::ScalarType)n[4], type = (at::ScalarType)n[5];
+        const at::ScalarType ptype = (at::ScalarType)n[9];            // (weight and bias are of one type)
         auto s = ctx->get_saved_variables();
-        s[0] = saved(s[0], stream_type, dev);
-        for (int i = 1; i < 4; ++i) s[i] = saved(s[i], i == 1 && s[1].defined() ? s[1].scalar_type() : at::kFloat, dev);
+        s[0] = restored(s[0], stream_type, dev, rows * D);
+        s[1] = restored(s[1], ptype, dev, D);
+        for (int i = 2; i < 4; ++i) s[i] = restored(s[i], at::kFloat, dev, rows);
         const at::Tensor &r = s[0], &weight = s[1], &mean = s[2], &rstd = s[3];
         // (inputs that were absent have no edge)
         size_t edge = 0;
@@ -81,7 +89,6 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
         check_rc(p_layer_norm_bwd(dy.data_ptr(), r.data_ptr(), ptr_of(weight), ptr_of<float>(mean), ptr_of<float>(rstd), ptr_of(dstream), ptr_of(dx), ptr_of(dres),
                                   ptr_of<float>(part), rows, D, parts, need_w, need_b, code_of(type), code_of(stream_type), (int)n[2], (int)n[3], stream), "gdn_layer_norm_bwd");
         if (kinds) {
-            const at::ScalarType ptype = need_w ? weight.scalar_type() : (at::ScalarType)n[9];      // (weight and bias are of one type)
             const at::Tensor sums = sum_rows(part, ptype, {kinds, D}, stream);
             if (need_w) dw = sums.select(0, 0);
             if (need_b) db = sums.select(0, kinds - 1);

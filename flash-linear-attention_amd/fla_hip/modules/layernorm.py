@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import differentiable_once, dtype_code, launch, ptr, require_gpu, sum_rows
+from fla_hip.ops.gated_delta_rule._common import differentiable_once, dtype_code, launch, ptr, require_gpu, restored, sum_rows
 
 
 def _stream_dtype(x: torch.Tensor, residual: torch.Tensor | None, residual_dtype: torch.dtype | None) -> torch.dtype:
@@ -138,6 +138,8 @@ class LayerNormFunction(torch.autograd.Function):
         y, mean, rstd, stream = _run(x, weight, bias, residual, eps, residual_in_fp32, is_rms_norm)
         ctx.save_for_backward(stream, weight, bias, mean, rstd)
         ctx.shape, ctx.eps, ctx.is_rms_norm, ctx.has_residual, ctx.x_dtype = shape, eps, is_rms_norm, residual is not None, x.dtype
+        ctx.rows, ctx.device = stream.shape, x.device
+        ctx.dtypes = (stream.dtype, *(None if t is None else t.dtype for t in (weight, bias)))
         ctx.set_materialize_grads(False)
         if not prenorm:
             return y.view(shape)
@@ -147,11 +149,12 @@ class LayerNormFunction(torch.autograd.Function):
     @staticmethod
     @differentiable_once
     def backward(ctx, dy, dstream=None):
-        stream, weight, bias, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
-        rows = stream.shape
         if dy is None and dstream is None:
             return (None,) * 8
+        need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
+        rows, dtypes = ctx.rows, (*ctx.dtypes, torch.float32, torch.float32)
+        shapes = (rows, rows[1:], rows[1:], rows[:1], rows[:1])
+        stream, weight, bias, mean, rstd = (restored(t, dt, shape, ctx.device) for t, dt, shape in zip(ctx.saved_tensors, dtypes, shapes))
         dy = torch.zeros(rows, dtype=ctx.x_dtype, device=stream.device) if dy is None else dy.reshape(rows)
         dstream = None if dstream is None else dstream.reshape(rows)
         dx, dw, db, dres = layer_norm_bwd(dy, stream, weight, bias, ctx.eps, mean, rstd, dstream, ctx.has_residual, ctx.is_rms_norm, ctx.x_dtype,

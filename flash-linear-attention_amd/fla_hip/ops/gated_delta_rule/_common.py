@@ -54,6 +54,15 @@ def aligned16(x: torch.Tensor | None) -> torch.Tensor | None:
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def restored(x: torch.Tensor | None, dtype: torch.dtype, shape, device: torch.device) -> torch.Tensor | None:
+    """A saved tensor as the kernels take it: of the type, the place and the layout that it had (saved-tensor hooks may hand back others), 16-byte aligned."""
+    if x is None:
+        return None
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError(f'a saved tensor {tuple(shape)} came back as {tuple(x.shape)}')
+    return aligned16(x.to(device=device, dtype=dtype).contiguous())
+
+
 def unify_qkv(q, k, v):
     """q, k, v must share one of bf16/fp16/fp32; mixed inputs are cast to q's dtype."""
     dt = q.dtype

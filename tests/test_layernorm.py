@@ -6,6 +6,7 @@ is in fp32.  Statistics are sums of at most 32 terms a lane and 10 steps across 
 magnitudes, and a few operations follow: 64 e times the magnitudes that enter covers both.  Gradients of weight and bias are sums over rows, at most
 ceil(rows / 512) a lane, 16 groups and 64 steps of the last sum: 128 e times the sum of the magnitudes.  Results below the smallest normal number of fp16 are
 off by half its smallest step, 2^-25."""
+import contextlib
 import itertools
 
 import pytest
@@ -218,6 +219,48 @@ def test_gradients_that_are_asked_for():
     assert torch.autograd.grad(y, args['weight'], t['dy'])[0].shape == (384,)
     with torch.no_grad():
         assert not mods.layer_norm(args['x'], args['weight'], t['bias']).requires_grad
+
+
+@gpu
+@pytest.mark.parametrize('strided', [False, True])
+@pytest.mark.parametrize('rms', [False, True])
+@pytest.mark.parametrize('form', [(BF, BF, BF), (BF, FP, FP), (HF, None, FP), (BF, None, BF)])
+def test_saved_tensors_may_come_back_in_another_layout_type_and_place(form, rms, strided):
+    """Saved-tensor hooks on the native and on the other host path: every tensor goes to the host and comes back strided, in fp32 where it was of 16 bits, and an
+    fp32 weight (of values that bf16 holds) in bf16.  What they hold is the same: so are the gradients' bits."""
+    dtype, res, wdtype = form
+    mods = _mods()
+    t = _inputs(37, 520, dtype, res, wdtype, False)
+    t['weight'] = t['weight'].to(BF).to(wdtype)
+    x = t['x']
+    if strided:
+        x = torch.zeros(37, 528, dtype=dtype, device=DEV)[:, :520].copy_(x)
+
+    def unpack(x):
+        x = x.to(DEV)
+        x = x.to(BF) if x.shape == (520,) and x.dtype == FP else x.float()
+        return torch.stack([x, torch.zeros_like(x)], -1)[..., 0]
+
+    def grads(*hooks):
+        leaves = [v.detach().requires_grad_(True) for v in (x, t['weight'], t['residual']) if v is not None]
+        with torch.autograd.graph.saved_tensors_hooks(*hooks) if hooks else contextlib.nullcontext():
+            out = (mods.rms_norm if rms else mods.layer_norm)(leaves[0], leaves[1], None, residual=leaves[2] if res else None, prenorm=res is not None)
+        return torch.autograd.grad(out, leaves, [t['dy'], t['dres']] if res else t['dy'])
+
+    for i, (a, b) in enumerate(zip(grads(), grads(lambda x: x.cpu(), unpack))):
+        assert a.dtype == b.dtype and torch.equal(a, b), i
+
+
+@gpu
+@pytest.mark.parametrize('strided', [False, True])
+def test_saved_tensors_of_another_size_are_refused(strided):
+    mods = _mods()
+    x = torch.randn(6, 40 + 8 * strided, device=DEV)[:, :40].requires_grad_(True)
+    for lost in ((6, 40), (40,), (6,)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x[:-1] if x.shape == lost else x):
+            y = mods.layer_norm(x, torch.ones(40, device=DEV), None)
+        with pytest.raises(ValueError, match='came back'):
+            y.sum().backward()
 
 
 @gpu
