@@ -42,16 +42,17 @@ struct GemmOperands {
 
 typedef uint32_t gm_rsrc __attribute__((ext_vector_type(4)));
 
-// 64 x 16 bytes from a buffer into LDS at lds_off + 16 lane; places at or past `extent` arrive as zeros.  (s_nop: a load into LDS needs one wait state after the
-// scalar write of M0, which the compiler does not see to inside assembly.  M0 is a reserved register: the compiler writes it itself before every use.)
-__device__ __forceinline__ void buffer_1k_to_lds(uint64_t base, uint32_t extent, uint32_t voff, uint32_t lds_off) {
+// 64 x 16 bytes from a buffer into LDS at slot + place + 16 lane; places at or past `extent` arrive as zeros.  (A load into LDS needs one wait state after the
+// scalar write of M0, which the compiler does not see to inside assembly: s_nop, made up for by the addition straight into M0 - 48 rows of 2048 x 5632 29.5 us
+// against 31 with the sum made outside, 8192 x 4096 x 11008 with its gradients 5107 and 5129.  M0 is a reserved register: the compiler writes it itself before every use.)
+__device__ __forceinline__ void buffer_1k_to_lds(uint64_t base, uint32_t extent, uint32_t voff, uint32_t slot, uint32_t place) {
     gm_rsrc r;
     r[0] = __builtin_amdgcn_readfirstlane((uint32_t)base);
     r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) & 0xffff;
     r[2] = __builtin_amdgcn_readfirstlane(extent);
     r[3] = 0x00020000;
-    lds_off = __builtin_amdgcn_readfirstlane(lds_off);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_off), "v"(voff), "s"(r));
+    slot = __builtin_amdgcn_readfirstlane(slot); place = __builtin_amdgcn_readfirstlane(place);
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" : : "s"(slot), "s"(place), "v"(voff), "s"(r) : "scc");
 }
 
 constexpr uint32_t GM_NOWHERE = 0xffff0000u;
@@ -161,8 +162,8 @@ struct Gemm {
         uint32_t ea = 0, eb = 0;
         auto request = [&](int i) {
             if (i == 0) { ea = extent(A_DOWN, lda2, m0); eb = extent(B_DOWN, ldb2, n0); }
-            if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && SideA::first_k(w * PA + i, lane) >= left ? GM_NOWHERE : va[i < PA ? i : 0], to + 1024 * (w * PA + i));
-            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && SideB::first_k(w * PB + i - PA, lane) >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], slot_of_b(to) + 1024 * (w * PB + i - PA));
+            if (i < PA) buffer_1k_to_lds(wa.at, ea, !A_DOWN && SideA::first_k(w * PA + i, lane) >= left ? GM_NOWHERE : va[i < PA ? i : 0], to, 1024 * (w * PA + i));
+            else buffer_1k_to_lds(wb.at, eb, !B_DOWN && SideB::first_k(w * PB + i - PA, lane) >= left ? GM_NOWHERE : vb[i < PA ? 0 : i - PA], slot_of_b(to), 1024 * (w * PB + i - PA));
             if (i < PA + PB - 1) return;
             ++asked;
             const bool second = asked == until_second;
