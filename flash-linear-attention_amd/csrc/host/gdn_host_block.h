@@ -210,8 +210,8 @@ struct MlpTrain : torch::autograd::Function<MlpTrain> {
         const MlpDims d{n[0], n[1], n[2], 0, (int)n[3]};
         const at::ScalarType type = d.code == GDN_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
         auto s = ctx->get_saved_variables();
-        for (auto& t : s) t = saved(t, type, dev);
-        const int64_t D = n[4], F = n[5];
+        const int64_t D = n[4], F = n[5], elements[] = {d.M * d.D, d.F * d.D, d.F * d.D, d.D * d.F, d.M * d.F, d.M * d.F, d.M * d.F};
+        for (int i = 0; i < 7; ++i) s[i] = restored(s[i], type, dev, elements[i]);
         Resize pad(dev), cut(dev);
         const at::Tensor whole = saved(grads[0], type, dev), dy = pad(whole, d.M, D, d.M, d.D);
         pad.run();

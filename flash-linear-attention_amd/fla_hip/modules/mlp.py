@@ -8,7 +8,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, ptr, require_gpu
+from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, ptr, require_gpu, restored
 from fla_hip.utils import calls_are_watched, calls_nothing_else
 
 _ACTIVATIONS = {'swish': _lib.ACT_SILU, 'silu': _lib.ACT_SILU, 'sigmoid': _lib.ACT_SIGMOID, 'gelu_tanh': _lib.ACT_GELU_TANH}
@@ -58,18 +58,18 @@ class GatedMLPFunction(torch.autograd.Function):
         x_k, wg, wu, wd = ops
         ctx.save_for_backward(x_k if need_g or need_u else None, wg if need_x else None, wu if need_x else None, wd if inner else None,
                               s, a, h if need_d else None)
-        ctx.sizes = (*x.shape, gate_weight.shape[0])
+        ctx.sizes, ctx.kept = (*x.shape, gate_weight.shape[0]), (x.dtype, x.device)
         return y if y.shape == x.shape else y[:, :x.shape[1]].contiguous()
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dy):
-        x, wg, wu, wd, s, a, h = ctx.saved_tensors
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        M, D, inner = ctx.sizes
+        (M, D, inner), (dt, dev) = ctx.sizes, ctx.kept
         D8, F8 = (D + 7) // 8 * 8, (inner + 7) // 8 * 8
-        dev, dt = dy.device, dy.dtype
-        dy = _pad(dy, M, D8)
+        shapes = ((M, D8), (F8, D8), (F8, D8), (D8, F8), *((M, F8),) * 3)
+        x, wg, wu, wd, s, a, h = (restored(t, dt, shape, dev) for t, shape in zip(ctx.saved_tensors, shapes))
+        dy = _pad(dy.to(device=dev, dtype=dt), M, D8)
         dg, du = (torch.empty_like(s), torch.empty_like(s)) if s is not None else (None, None)
 
         def empty(need, *shape):

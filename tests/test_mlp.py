@@ -6,6 +6,8 @@ instruction, parts of a contraction one after the other), and g's share of that 
 most 1.13.  All of it is carried through the products on magnitudes, and the result is rounded once.  Over a whole result of 4096 values or more: k independent
 roundings, each uniform in half a spacing, leave a relative 2-norm of at most sqrt(k / 3) u: k = 2 for y and dwd (h, itself), 3 for the other gradients (s or a;
 dg or du; itself).  Results under fp16's smallest normal number are off by half its smallest step, 2^-25, h and the others too."""
+import contextlib
+
 import pytest
 import torch
 
@@ -210,6 +212,75 @@ def test_gradients_that_are_asked_for(size):
             assert all(torch.equal(g, full['d' + names[i]]) for g, i in zip(got, want)), (want, again)
         some = want[len(want) // 2]
         assert torch.equal(torch.autograd.grad(y, leaves[some], t['dy'])[0], full['d' + names[some]])
+
+
+def _unpack(x):
+    """Strided, between 16-byte boundaries, in fp32."""
+    x = x.to(DEV).float()
+    wide = torch.zeros(*x.shape[:-1], x.shape[-1] + 3, device=DEV)
+    wide[..., 1:-2] = x
+    return wide[..., 1:-2]
+
+
+@gpu
+@pytest.mark.parametrize('path', ['native', 'strided', 'autocast'])
+@pytest.mark.parametrize('size', [(40, 256, 512), (40, 250, 509), (7, 64, 96)])
+def test_saved_tensors_may_come_back_in_another_layout_type_and_place(path, size):
+    """Saved-tensor hooks: every tensor goes to the host and comes back in fp32.  What they hold is the same: so are the gradients' bits."""
+    t = _inputs(*size, BF)
+    x = t['x']
+    if path == 'strided':
+        x = torch.zeros(size[0], size[1] + 8, dtype=BF, device=DEV)[:, :size[1]].copy_(x)
+
+    def grads(*hooks):
+        leaves = [v.detach().requires_grad_(True) for v in (x, t['wg'], t['wu'], t['wd'])]
+        if path == 'autocast':
+            leaves = [v.detach().float().requires_grad_(True) for v in leaves]
+        with torch.autograd.graph.saved_tensors_hooks(*hooks) if hooks else contextlib.nullcontext():
+            with torch.autocast('cuda', dtype=BF, enabled=path == 'autocast'):
+                y = _mods().gated_mlp(*leaves)
+        return torch.autograd.grad(y, leaves, t['dy'])
+
+    for i, (a, b) in enumerate(zip(grads(), grads(lambda x: x.cpu(), _unpack))):
+        assert a.dtype == b.dtype and torch.equal(a, b), i
+
+
+@gpu
+@pytest.mark.parametrize('strided', [False, True])
+def test_saved_tensors_of_another_size_are_refused(strided):
+    t = _inputs(20, 64, 96, BF)
+    x = torch.zeros(20, 64 + 8 * strided, dtype=BF, device=DEV)[:, :64].requires_grad_(True)
+    for shape in ((20, 64), (96, 64), (64, 96), (20, 96)):
+        leaves = [x, *(t[k].clone().requires_grad_(True) for k in ('wg', 'wu', 'wd'))]
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x[:-1] if x.shape == shape else x):
+            y = _mods().gated_mlp(*leaves)
+        with pytest.raises(ValueError, match='came back'):
+            y.sum().backward()
+
+
+def test_what_the_library_gets_of_saved_tensors_that_came_back_otherwise(monkeypatch):
+    """The host path in Python (CPU: the library keeps record): with hooks that hand back fp32, strided, the kernel is still given 16-bit memory, 16-byte aligned."""
+    from fla_hip import _lib
+    from fla_hip.modules import mlp
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    got = []
+    monkeypatch.setattr(_lib, 'load', Library)
+    monkeypatch.setattr(mlp, 'require_gpu', lambda x, *_: x.device)
+    monkeypatch.setattr(mlp, 'ptr', lambda t: got.append(t))
+    monkeypatch.setattr(mlp, 'launch', lambda *a: None)
+    x, wg, wu, wd = (torch.randn(*s).to(BF).requires_grad_(True) for s in ((20, 24), (40, 24), (40, 24), (24, 40)))
+    unpack = lambda t: torch.stack([t.float(), t.float()], -1)[..., 0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = mlp.GatedMLPFunction.apply(x, wg, wu, wd, _lib.ACT_SILU)
+    got.clear()
+    y.sum().backward()
+    assert len(got) >= 14
+    for t in got:
+        assert t is None or (t.dtype in (BF, torch.uint8) and t.is_contiguous() and t.data_ptr() % 16 == 0), (t.dtype, t.stride())
 
 
 @gpu
