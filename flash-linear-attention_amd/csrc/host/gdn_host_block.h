@@ -97,6 +97,12 @@ struct NormTrain : torch::autograd::Function<NormTrain> {
     }
 };
 
+// Dual tensors of forward-mode differentiation, with a gradient asked for or not: the Python path refuses them.
+bool has_tangent(std::initializer_list<const Arg*> args) {
+    for (const Arg* a : args)
+        if (*a && (*a)->_fw_grad(0).defined()) return true;
+    return false;
+}
 bool needs_grad(std::initializer_list<const Arg*> args) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Arg* a : args)
@@ -129,6 +135,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (weight && bias && weight->scalar_type() != bias->scalar_type()) Py_RETURN_NONE;
     c.stream_type = residual ? residual->scalar_type() : in_fp32 ? at::kFloat : type;
     c.own_stream = residual || c.stream_type != type;
+    if (has_tangent({&x, &weight, &bias, &residual})) Py_RETURN_NONE;
     if (prenorm && !c.own_stream) Py_RETURN_NONE;                  // (the stream is x: the Python path says how it leaves)
     at::Tensor y, stream;
     if (needs_grad({&x, &weight, &bias, &residual})) {
@@ -240,6 +247,7 @@ PyObject* gated_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!plain(*t, dev) || (*t)->scalar_type() != type) Py_RETURN_NONE;
     const int64_t D = x->size(-1), F = wg->size(0);
     if (wg->size(1) != D || wu->sizes() != wg->sizes() || wd->size(0) != D || wd->size(1) != F || F == 0) Py_RETURN_NONE;
+    if (has_tangent({&x, &wg, &wu, &wd})) Py_RETURN_NONE;
     const bool train = needs_grad({&x, &wg, &wu, &wd});
     MlpDims d{};
     d.M = x->numel() / D;

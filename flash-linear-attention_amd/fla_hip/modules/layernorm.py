@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import differentiable_once, dtype_code, launch, ptr, require_gpu, restored, sum_rows
+from fla_hip.ops.gated_delta_rule._common import differentiable_once, dtype_code, launch, no_forward_mode, ptr, require_gpu, restored, sum_rows
 
 
 def _stream_dtype(x: torch.Tensor, residual: torch.Tensor | None, residual_dtype: torch.dtype | None) -> torch.dtype:
@@ -187,6 +187,7 @@ def layer_norm(
     out = _lib.host().layer_norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, is_rms_norm)
     if out is not None:
         return out
+    no_forward_mode('layer_norm', x, weight, bias, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LayerNormFunction.apply(x, weight, bias, residual, eps, prenorm, residual_in_fp32, is_rms_norm)
     y, _, _, stream = _run(x, weight, bias, residual, eps, residual_in_fp32, is_rms_norm)

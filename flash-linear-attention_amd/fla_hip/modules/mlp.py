@@ -8,7 +8,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from fla_hip import _lib
-from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, ptr, require_gpu, restored
+from fla_hip.ops.gated_delta_rule._common import aligned16, differentiable_once, dtype_code, launch, no_forward_mode, ptr, require_gpu, restored
 from fla_hip.utils import calls_are_watched, calls_nothing_else
 
 _ACTIVATIONS = {'swish': _lib.ACT_SILU, 'silu': _lib.ACT_SILU, 'sigmoid': _lib.ACT_SIGMOID, 'gelu_tanh': _lib.ACT_GELU_TANH}
@@ -111,6 +111,7 @@ def gated_mlp(
     if 0 in gate_weight.shape:
         raise ValueError(f'the weights hold nothing: {tuple(gate_weight.shape)}')
     require_gpu(x, gate_weight, up_weight, down_weight)
+    no_forward_mode('gated_mlp', x, gate_weight, up_weight, down_weight)
     if torch.is_autocast_enabled():
         x, gate_weight, up_weight, down_weight = (t.to(torch.get_autocast_dtype('cuda')) for t in (x, gate_weight, up_weight, down_weight))
     if any(w.dtype != x.dtype for w in (gate_weight, up_weight, down_weight)):

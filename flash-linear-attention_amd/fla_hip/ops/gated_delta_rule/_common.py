@@ -143,6 +143,13 @@ def forward_only(what: str, *activations: torch.Tensor | None) -> None:
         raise NotImplementedError(f'{what} has no backward in fla_hip: run it under torch.no_grad() or on detached inputs')
 
 
+def no_forward_mode(what: str, *tensors: torch.Tensor | None) -> None:
+    """Operators without a forward-mode derivative refuse dual tensors, whether they require a gradient or not, instead of returning a result without
+    a tangent."""
+    if any(x is not None and torch.autograd.forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise NotImplementedError(f'{what} has no forward-mode derivative in fla_hip: its gradients are taken in reverse')
+
+
 def sum_rows(part: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """``part.sum(0)`` of an fp32 tensor of partial sums, in ``dtype`` (added up in fp32, in a fixed order)."""
     out = torch.empty(part.shape[1:], dtype=dtype if dtype in _DTYPE_CODE else torch.float32, device=part.device)
