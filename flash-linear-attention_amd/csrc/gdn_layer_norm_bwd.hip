@@ -12,9 +12,12 @@ struct LayerNormBwdParams {
     bool rms, with_dw, with_db;
 };
 
-// (rows of more than 16384 16-bit elements run a form whose registers spill: 8192 x 16384 bf16 does not, and takes 407 us with its forward, 5.3 TB/s)
+// Registers: up to 512 lanes a row's pieces and its parameters' sums fit (asked to leave room for a second workgroup of 512 lanes a CU, rows at any address spilled 118 to
+// 319 registers: 8192 x 7001 bf16 627 us, 762 with a bias, now 175 and 177).  1024 lanes have 128 registers each.  Two pieces spill a few of them where there is a bias
+// or an fp32 stream (8192 x 16384 bf16 none, 195 us, 5.5 TB/s; with a bias 1, 206 us; with a bias and an fp32 stream 54, 590 us, 3.6 TB/s; 167 at
+// any address, 8192 x 8203 490 us, 2.2 TB/s), and four pieces 100 to 600.
 template <typename T, typename RT, int LANES, int PIECES, bool ALIGNED, bool BIAS>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES, LANES >= 512 && !ALIGNED ? 4 : 1) void layer_norm_bwd_kernel(LayerNormBwdParams p) {
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void layer_norm_bwd_kernel(LayerNormBwdParams p) {
     typedef NormRow<T, LANES, ALIGNED> R;
     constexpr int VEC = R::VEC, WIDTH = LANES * PIECES * VEC;
     __shared__ float red[2][16][2];

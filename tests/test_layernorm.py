@@ -102,6 +102,56 @@ def test_against_the_oracle(D, form, rms, bias):
     _check(_inputs(37, D, dtype, res, wdtype, bias), rms)
 
 
+# rows of 769 to 1024 pieces of 16 bytes that begin anywhere: 512 lanes of two
+@gpu
+@pytest.mark.parametrize('bias', [False, True])
+@pytest.mark.parametrize('rms', [False, True])
+@pytest.mark.parametrize(('dtype', 'res', 'D'), [(t, r, D) for t, widths in ((BF, (6145, 6151, 7837, 8191)), (HF, (6145, 7001, 8191)), (FP, (3073, 3077, 4095))) for D in widths
+                                                 for r in {t, FP, None}])
+def test_rows_of_512_lanes_at_any_address(dtype, res, D, rms, bias):
+    _check(_inputs(21, D, dtype, res, FP if bias else dtype, bias), rms)
+
+
+@gpu
+@pytest.mark.parametrize(('dtype', 'D'), [(BF, 6152), (BF, 8192), (FP, 3076), (FP, 4096)])
+def test_rows_of_512_lanes_between_16_byte_boundaries(dtype, D):
+    t = _inputs(13, D, dtype, dtype, dtype, True)
+    for k in ('x', 'residual', 'weight', 'bias', 'dy', 'dres'):
+        t[k] = torch.cat([t[k].new_zeros(1), t[k].flatten()])[1:].view(t[k].shape)
+    lib, dev = _lib_and_device()
+    y, s, dx = (torch.empty_like(t['x']) for _ in range(3))
+    mean, rstd = torch.empty(13, device=DEV), torch.empty(13, device=DEV)
+    parts = lib.gdn_layer_norm_bwd_parts(13, D, _code(dtype))
+    part = torch.empty(parts, 2, D, device=DEV)
+    c = _code(dtype)
+    ptr = lambda x: x.data_ptr()
+    from fla_hip.ops.gated_delta_rule._common import launch
+    launch(lib.gdn_layer_norm_fwd, dev, *map(ptr, (t['x'], t['residual'], t['weight'], t['bias'], y, s, mean, rstd)), 13, D, 1e-5, c, c, c, 0)
+    launch(lib.gdn_layer_norm_bwd, dev, *map(ptr, (t['dy'], s, t['weight'], mean, rstd, t['dres'], dx)), None, ptr(part), 13, D, parts, 1, 1, c, c, c, 0)
+    r, w, b = s.double(), t['weight'].double(), t['bias'].double()
+    ref, _, rs = M.layer_norm(r, w, b, 1e-5)
+    unit = (r.abs() + r.abs().mean(-1, keepdim=True)) * rs
+    _near('stream', s, t['x'].double() + t['residual'].double(), (t['x'].double() + t['residual'].double()).abs(), 2)
+    _near('y', y, ref, unit * w.abs() + b.abs())
+    dr, dw, db = M.layer_norm_grads(r, w, t['dy'], t['dres'], 1e-5)
+    dy = t['dy'].double().abs()
+    g = dy * w.abs()
+    _near('dx', dx, dr, rs * (g + g.mean(-1, keepdim=True) + unit * (g * unit).mean(-1, keepdim=True)) * 2 + t['dres'].double().abs())
+    sums = part.double().sum(0).float()
+    _near('dweight', sums[0], dw, (dy * unit).sum(0), 128)
+    _near('dbias', sums[1], db, dy.sum(0), 128)
+
+
+def _lib_and_device():
+    from fla_hip import _lib
+    return _lib.load(), torch.device('cuda', torch.cuda.current_device())
+
+
+def _code(dtype):
+    from fla_hip.ops.gated_delta_rule._common import dtype_code
+    return dtype_code(dtype)
+
+
 @gpu
 @pytest.mark.parametrize('rows', [1, 3, 4, 15, 16, 17, 63, 512, 513, 1030, 4099])
 @pytest.mark.parametrize('D', [64, 200, 1024, 2048])

@@ -35,16 +35,19 @@ def _code_objects(data):
         at = data.find(BUNDLE, at + 1)
 
 
-@functools.lru_cache(maxsize=1)
-def _listing():
-    """[(function, [instruction])] of the library."""
+def library_code_objects():
     from fla_hip import _lib
     if not os.path.exists(_lib.LIB_PATH) or not os.path.exists(OBJDUMP):
         pytest.skip('not built in this checkout')
-    functions = []
     with open(_lib.LIB_PATH, 'rb') as f:
-        data = f.read()
-    for code in _code_objects(data):
+        return list(_code_objects(f.read()))
+
+
+@functools.lru_cache(maxsize=1)
+def _listing():
+    """[(function, [instruction])] of the library."""
+    functions = []
+    for code in library_code_objects():
         text = subprocess.run([OBJDUMP, '-d', '--no-show-raw-insn', '-'], input=code, capture_output=True, check=True).stdout.decode()
         for line in text.splitlines():
             if line.endswith('>:'):
