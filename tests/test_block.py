@@ -100,3 +100,21 @@ def test_a_padded_batch():
     for b, n in ((0, 60), (1, 100), (2, 1)):
         alone = block(x[b:b + 1, 100 - n:])[0]
         assert get_err_ratio(alone.float(), got[b:b + 1, 100 - n:].float()) <= 5e-3, b
+
+
+@pytest.mark.parametrize('dtype', [BF, torch.float16])
+def test_under_autocast(dtype):
+    """fp32 weights and an fp32 residual stream, as a training loop under autocast has them: against the same block's weights and input in the 16-bit type.
+    The two differ by the roundings of the weights of the norms and of the streams to 16 bits, each u / sqrt(3) in the 2-norm and carried on to the end: the stream
+    twice, its sum, the norms' weights twice: within 4 u.  The stream stays in fp32, and every parameter gets a gradient of its own type."""
+    block = _block().float().train()
+    u = torch.finfo(dtype).eps / 2
+    x = torch.randn(2, 130, 256, device=DEV).to(dtype).float().requires_grad_(True)
+    with torch.autocast('cuda', dtype=dtype):
+        y = block(x)[0]
+        assert get_err_ratio(y.detach(), block.eval()(x)[0]) <= 4 * u
+    assert y.dtype == torch.float32
+    grads = torch.autograd.grad(y, [x, *block.parameters()], torch.randn(y.shape, device=DEV, generator=torch.Generator(DEV).manual_seed(1)))
+    assert all(g.dtype == torch.float32 and bool(g.isfinite().all()) and bool(g.any()) for g in grads)
+    low = _block().to(dtype).eval()
+    assert get_err_ratio(low(x.detach().to(dtype))[0].float(), y.detach()) <= 4 * u

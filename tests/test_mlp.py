@@ -555,6 +555,33 @@ def test_the_resizing_entry_point_refuses():
 
 
 @gpu
+@pytest.mark.parametrize('rows', [1, 2, 4, 5, 16, 17, 300])
+@pytest.mark.parametrize(('which', 'dtype'), [(w, HF) for w in ('x', 'wg', 'wu', 'wd', 'all weights')] + [(w, BF) for w in ('x', 'wg', 'wu')])
+def test_operands_below_the_smallest_normal_number(rows, which, dtype):
+    """fp16 numbers under 2^-14 and bf16 numbers under 2^-126 count with all their bits in every form: weights like that against rows that make up for
+    them, and rows like that."""
+    D, F = 264, 520
+    low, high = (2.0 ** -15, 2.0 ** 12) if dtype == HF else (2.0 ** -127, 2.0 ** 120)
+    t = _inputs(rows, D, F, dtype)
+    for k in (('wg', 'wu', 'wd') if which == 'all weights' else (which,)):
+        t[k] = (t[k].double() / t[k].double().abs().max() * low).to(dtype)
+        assert (t[k] != 0).sum() > 0.9 * t[k].numel()
+    if which in ('wg', 'wu', 'all weights'):
+        t['x'] = (t['x'].float() * high).to(dtype)
+    if which == 'x':
+        t['wg'], t['wu'] = ((t[k].float() * high).to(dtype) for k in ('wg', 'wu'))
+    ref = _reference(t, 'swish')['y']
+    tol = _u(dtype) * ref[0].abs() + (1 + _u(dtype)) * ref[1] + TINY
+    if which != 'all weights':
+        assert (ref[0].abs() > tol).double().mean() > 0.5                        # (operands taken as zeros would be seen)
+    with torch.no_grad():
+        y = _mods().gated_mlp(t['x'], t['wg'], t['wu'], t['wd'])
+    assert y.any()
+    worst = ((y.double() - ref[0]).abs() / tol).max().item()
+    assert worst <= 1, worst
+
+
+@gpu
 @pytest.mark.parametrize('rows', [1, 3, 16])
 @pytest.mark.parametrize(('D', 'F'), [(1, 1), (7, 9), (31, 33), (250, 1001), (1003, 517), (2049, 40)])
 def test_few_rows_of_any_width_at_any_address(rows, D, F):
