@@ -208,17 +208,22 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 
 // How the products of a launch are cut: the tiles, and over how many workgroups the contraction of each tile is shared out that does not fill a round of the
 // chip (`rest` tiles of `parts` workgroups after `full` of one): the least of the times that the launch would take by these figures.
-//   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)   a round's begin and end, more with an activation or
-//   256 x 256   8      1 a CU       1.55                                  1.05                            8, 4                          the inner gradients
-//   128 x 128   4      2 a CU       1.0                                   0.6                             4, 3      five slots of LDS: half the CU's
-//   128 x 128   8      1 a CU       0.58                                  0.4                             4.5, 2.5  eight: more in flight, for few workgroups
-//   64 x 64     2      2 a CU       0.45                                  0.28                            4, 2.5    the same, where no operand is read down its columns
-// In between a stage's time grows with the workgroups: a full chip is held back by its caches and its clock, too.  Joining parts takes 5.5 us and
-// their bytes, written and read, at 4 TB/s.  Measured (8192, 32768 x 2048 x 5632; 48 to 2000 rows of 2048 x 5632, 1024 x 2816, 4096 x 11008,
-// forward): 48 rows 61 us in 128 x 128 tiles, 28 us; 333 rows 85 -> 49 us; 2000 rows 213 us in 256 x 256 tiles, 155 us.  The weights' gradients of 8192 x 2048 x
-// 5632 are 528 tiles of 256 x 256, two rounds and 16 tiles: those in 8 parts each, the backward 1186 -> 1026 us.
-struct MlpTiles { int side, waves_m, waves_n, slots, per_cu; double full, least, round, more; };
-constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 5, 1, 1.55, 1.05, 8, 4}, {128, 2, 2, 5, 2, 1.0, 0.6, 4, 3}, {128, 4, 2, 8, 1, 0.58, 0.4, 4.5, 2.5}, {64, 2, 1, 8, 2, 0.45, 0.28, 4, 2.5}};
+//   tiles       waves  workgroups   us for a stage of 64, the chip full   and at least (few workgroups)   a round's begin and end
+//   256 x 256   8      1 a CU       1.54                                  1.18                            6
+//   128 x 128   4      2 a CU       0.95                                  0.67                            4.3    five slots of LDS: half the CU's
+//   128 x 128   8      1 a CU       0.55                                  0.55                            5      eight: more in flight, for few workgroups
+//   64 x 64     2      2 a CU       0.42                                  0.42                            4.4    the same, where no operand is read down its columns
+// In between a stage's time grows with the workgroups: a full chip is held back by its caches and its clock, too.  What a round's results are read and written with
+// (8 bytes a result for the inner gradients, 2 otherwise: between those of h alone and of h, s and a) goes at 2.5 TB/s where all workgroups end together; of the rounds
+// before the last a fifth of it is seen.  Joining parts takes 4.3 us, 0.3 a part and their bytes, written and read, at 5.2 TB/s.
+// Fitted to 2481 cuts - every tile and up to 16 parts of the six launches of a forward and a training step, 29 sizes from 20 x 4096 x 11008 and 3000 x 512 x 1408 to
+// 8192 x 4096 x 11008 and 30000 x 1024 x 1024 -, each the geometric mean of its times on operands in the caches and behind 600 MB of other data: met within a tenth
+// (root mean square of the logarithms); the chosen cut takes 2.2 % longer than the best one in the mean, 24 % at worst (dh of 3000 x 512 x 1408).  Both projections of
+// 48 x 2048 x 5632 take 16 us in 64 x 64 tiles, 21 in 128 x 128; down of 300 x 4096 x 11008 50 in 128 x 128 in four parts, 76 in 64 x 64; dh of 2999 x 1008 x 2696 41 in
+// 128 x 128 in four parts, 48 in 132 of 256 x 256; the weights' gradients of 8192 x 2048 x 5632, 528 tiles of 256 x 256, 456 with the last 16 in ten parts, 569 in 128 x 128
+// (operands in the caches).
+struct MlpTiles { int side, waves_m, waves_n, slots, per_cu; double full, least, round; };
+constexpr MlpTiles MLP_TILES[] = {{256, 2, 4, 5, 1, 1.54, 1.18, 6}, {128, 2, 2, 5, 2, 0.95, 0.67, 4.3}, {128, 4, 2, 8, 1, 0.55, 0.55, 5}, {64, 2, 1, 8, 2, 0.42, 0.42, 4.4}};
 struct MlpPlan { int tiles, full, rest, parts; };
 static MlpPlan plan_gemm(const MlpGemm& p, int epilogue, bool rows) {
     const int kinds = is_gate(epilogue) ? 2 : 1;
@@ -234,11 +239,12 @@ static MlpPlan plan_gemm(const MlpGemm& p, int epilogue, bool rows) {
         }
         if (tiles >= (1ll << 31)) continue;
         const int64_t rest = tiles % slots;
-        const double round = k.round + (epilogue == MLP_PLAIN ? 0 : k.more), before = (double)(tiles / slots) * (stages * k.full + round);
+        const double results = (double)k.side * k.side * (epilogue == MLP_GRAD ? 8 : 2) / 2.5e6;          // us, a tile's
+        const double before = (double)(tiles / slots) * (stages * k.full + k.round + 0.2 * slots * results);
         for (int64_t parts = 1; parts <= 16 && (parts == 1 || (rest > 0 && rest * parts <= slots && stages / parts >= 2)); ++parts) {
             double us = before;
-            if (rest) us += (stages + parts - 1) / parts * std::max(k.least, k.full * (rest * parts) / slots) + round;
-            if (parts > 1) us += 5.5 + (double)(rest * parts) * k.side * k.side * 8 / 4e6;
+            if (rest) us += (stages + parts - 1) / parts * std::max(k.least, k.full * (rest * parts) / slots) + k.round + rest * results;
+            if (parts > 1) us += 4.3 + 0.3 * parts + (double)(rest * parts) * k.side * k.side * 8 / 5.2e6;
             if (us < best_us) {
                 best_us = us;
                 best = MlpPlan{t, (int)(parts > 1 ? tiles - rest : tiles), (int)(parts > 1 ? rest : 0), (int)parts};
