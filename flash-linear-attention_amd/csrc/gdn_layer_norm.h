@@ -5,8 +5,8 @@
 //   xh = (r - mean) rstd;  y = xh w + b
 //   dr = rstd (dy w - xh mean(dy w xh) - [layer norm: mean(dy w)]) + dstream;  dw = sum over rows of dy xh;  db = sum over rows of dy
 //
-// The stream is a tensor of its own type, and that tensor is normalised: forward and backward see the same numbers, and the gradients of the
-// parameters are as exact as their sums.
+// The stream is a tensor of its own type, and that tensor is normalised, whether it is handed on or not: forward and backward see the same numbers (the
+// backward keeps one tensor of the stream's type, not two), y is the same with prenorm and without, and the gradients of the parameters are as exact as their sums.
 //
 // A few operations an element: bound by memory, every element read and written once.  Measured with the stream handed on: 32768 x 2048 bf16 forward 96 us
 // (5.6 TB/s; a copy of 1 GB runs at 5.1), with the backward 207 us (5.2); 16384 x 4096 bf16 with an fp32 stream, both, 353 us (4.6).  A row belongs to LANES lanes - part of a wave, a wave, a
@@ -56,7 +56,7 @@ struct NormRow {
             for (int e = 0; e < VEC; ++e) if (c + e < D) row[c + e] = v[e];
         }
     }
-    // weight or bias, of T's type or fp32; `fill` where there is none and past the end
+    // weight or bias, of T's type or fp32: `fill` where there is none, zeros past the end of the one there is
     static __device__ __forceinline__ void params(const void* w, int dtype, float fill, int l, int i, int D, float (&out)[VEC]) {
         if (!w) {
 #pragma unroll

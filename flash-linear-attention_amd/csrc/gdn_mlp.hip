@@ -3,10 +3,12 @@
 //   g = x Wg^T, u = x Wu^T;  h = act(g) u;  y = h Wd^T             x [M][D]; Wg, Wu [F][D]; Wd [D][F]
 //   dh = dy Wd;  dg = dh s, du = dh a  with  s = act'(g) u, a = act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
-// For the backward the forward keeps s and a, each rounded once from the accumulators, where g and u would do: of those, two roundings (and a slope's
-// steepness) would go into dg, and the backward would work the activation out again.  With the one rounding of s or a, that of dg and du and that of the result the
-// gradients come out 1.7 times as far from the exact ones as their own rounding (bf16: 2.9e-3 against 1.7e-3, 2-norms).  More bits of s and a would be
-// more memory held from the forward to the backward, which is what training runs out of.
+// Roundings to 16 bits besides the results': h, dg and du, because they are operands of matrix products, whose instructions take 16-bit operands (with h in two halves of 16 bits the
+// down projection would be two products); s and a, to hold half of what 32 bits would from the forward to the backward.  Each is rounded once, from 32-bit sums.  y and
+// dWd come out 1.4 times as far from the exact ones as their own rounding, the other gradients 1.7 times (bf16: 2.3e-3 and 2.9e-3 against 1.7e-3, 2-norms).
+//
+// Three tensors of M x F are held for the backward, s, a and h: 541 MB at 8192 x 11008.  g and u would be two, 361 MB; but of those two roundings (and a slope's
+// steepness) would go into dg, and the backward would work the activation out again, and h for dWd.
 //
 // Forward two launches (both projections with the activation and the product on top; the down projection), backward three (dh with dg and du on top; dx;
 // the weights' gradients together).  Many rows are bound by the matrix cores: gdn_gemm.h.
@@ -218,7 +220,7 @@ static GemmOperands operands(const void* A, const void* B, int64_t lda, int64_t 
 // before the last a fifth of it is seen.  Joining parts takes 4.3 us, 0.3 a part and their bytes, written and read, at 5.2 TB/s.
 // Fitted to 2481 cuts - every tile and up to 16 parts of the six launches of a forward and a training step, 29 sizes from 20 x 4096 x 11008 and 3000 x 512 x 1408 to
 // 8192 x 4096 x 11008 and 30000 x 1024 x 1024 -, each the geometric mean of its times on operands in the caches and behind 600 MB of other data: met within a tenth
-// (root mean square of the logarithms); the chosen cut takes 2.2 % longer than the best one in the mean, 24 % at worst (dh of 3000 x 512 x 1408).  Both projections of
+// (root mean square of the logarithms); the chosen cut takes 2 % longer than the best one in the mean, 24 % at worst (dh of 3000 x 512 x 1408).  Both projections of
 // 48 x 2048 x 5632 take 16 us in 64 x 64 tiles, 21 in 128 x 128; down of 300 x 4096 x 11008 50 in 128 x 128 in four parts, 76 in 64 x 64; dh of 2999 x 1008 x 2696 41 in
 // 128 x 128 in four parts, 48 in 132 of 256 x 256; the weights' gradients of 8192 x 2048 x 5632, 528 tiles of 256 x 256, 456 with the last 16 in ten parts, 569 in 128 x 128
 // (operands in the caches).

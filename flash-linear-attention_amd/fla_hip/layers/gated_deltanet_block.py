@@ -1,7 +1,7 @@
 """One block of a Gated DeltaNet model, with the parameter names and the call signature of the reference's ``GatedDeltaNetBlock``
 (fla/models/gated_deltanet/modeling_gated_deltanet.py): normalisation, token mixing, normalisation of the residual stream that the mixing is added to, gated
-feed-forward block.  Additions, normalisations and the feed-forward block run in this package's HIP kernels, forward and backward; the mixing layer is
-``GatedDeltaNet`` with its caches and its modes."""
+feed-forward block.  Normalisations, the addition in front of the second one and the feed-forward block run in this package's HIP kernels, forward and backward; the
+last addition is torch's; the mixing layer is ``GatedDeltaNet`` with its caches and its modes."""
 from __future__ import annotations
 
 import contextlib

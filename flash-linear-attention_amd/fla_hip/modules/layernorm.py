@@ -2,8 +2,9 @@
 ``layer_norm_bwd``, the differentiable ``layer_norm`` / ``rms_norm`` and the ``LayerNorm`` / ``RMSNorm`` layers (one group; weights as torch's).  All compute
 is done by ``gdn_layer_norm_fwd``, ``gdn_layer_norm_bwd`` and ``gdn_sum_rows`` of the HIP library.
 
-What is normalised is the residual stream as it is handed on, in the stream's own type (the reference normalises the sum before it is rounded): the backward
-sees the numbers the forward saw, and ``prenorm`` calls equal an addition followed by a normalisation."""
+What is normalised is the residual stream as it is handed on, in the stream's own type, with ``prenorm`` and without (the reference normalises the sum before it is
+rounded): the backward sees the numbers the forward saw and keeps one tensor of them, and every call equals an addition followed by a normalisation.  With a stream of 16 bits that is
+one rounding more than the sum in 32 bits would have; an fp32 stream has none."""
 from __future__ import annotations
 
 import torch

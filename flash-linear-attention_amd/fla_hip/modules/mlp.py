@@ -95,6 +95,7 @@ def gated_mlp(
 ) -> torch.Tensor:
     """``(act(x @ gate_weight.T) * (x @ up_weight.T)) @ down_weight.T`` with ``x`` ``[..., D]``, ``gate_weight`` and ``up_weight`` ``[F, D]``,
     ``down_weight`` ``[D, F]``, all bf16 or all fp16; ``activation``: 'swish' / 'silu', 'sigmoid' or 'gelu_tanh'.  Differentiable in all four.
+    Sums, activation and product are in fp32; the inner activation, what is kept for the backward and the inner gradients are rounded to the operands' type once each.
     Under autocast the operands are cast to its type first.  Without gradients up to 16 rows are read where they are, D and F of any
     size; otherwise D and F that are no multiples of 8 are zero-padded (copies of the weights per call)."""
     if activation not in _ACTIVATIONS:
