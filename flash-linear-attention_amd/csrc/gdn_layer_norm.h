@@ -9,7 +9,7 @@
 // backward keeps one tensor of the stream's type, not two), y is the same with prenorm and without, and the gradients of the parameters are as exact as their sums.
 //
 // A few operations an element: bound by memory, every element read and written once.  Measured with the stream handed on: 32768 x 2048 bf16 forward 96 us
-// (5.6 TB/s; a copy of 1 GB runs at 5.1), with the backward 207 us (5.2); 16384 x 4096 bf16 with an fp32 stream, both, 353 us (4.6).  A row belongs to LANES lanes - part of a wave, a wave, a
+// (5.6 TB/s; a copy of 1 GB runs at 5.1), with the backward 207 to 217 us (5.2 to 4.9); 16384 x 4096 bf16 with an fp32 stream, both, 343 to 347 us (4.7).  A row belongs to LANES lanes - part of a wave, a wave, a
 // workgroup - each of which holds PIECES pieces of 16 bytes (of x) in registers.
 #pragma once
 #include "gdn_common.h"
@@ -96,7 +96,7 @@ struct NormRow {
 };
 
 // The forms of a row that there are kernels for, by the pieces of 16 bytes in it: f(LANES, PIECES, ALIGNED) as integral constants.  The lanes that a row does not
-// fill wait: 8000 x 4097 bf16 (513 pieces) forward and backward 220 us on 512 lanes of two pieces, 164 us on 256 of three.  Rows that begin on 16-byte
+// fill wait: 8000 x 4097 bf16 (513 pieces) forward and backward 191 us on 512 lanes of two pieces, 143 us on 256 of three.  Rows that begin on 16-byte
 // boundaries would run as the others do, too: forward the same, backward 2 % slower (32768 x 2048 bf16 207 -> 211 us).  Element by element, as the others once
 // ran, 1929 x 7837 fp32 took 223 us, now 105.
 template <int LANES, int PIECES, bool ALIGNED, typename F>
