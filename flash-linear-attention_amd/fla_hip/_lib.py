@@ -5,7 +5,7 @@ import ctypes
 import importlib.util
 import os
 import threading
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _ELSEWHERE = os.environ.get('FLA_HIP_LIBRARY')
@@ -181,6 +181,43 @@ SIGNATURES['gdn_gated_mlp_fwd'] = (c_int, [c_void_p] * 9 + [c_size_t] + [c_int64
 SIGNATURES['gdn_gated_mlp_bwd'] = (c_int, [c_void_p] * 15 + [c_size_t] + [c_int64] * 3 + [c_int, c_void_p])     # dy x wg wu wd s a h dg du dx dwg dwu dwd
 SIGNATURES['gdn_pad_rows'] = (c_int, [c_void_p, c_int, c_void_p])     # segments count
 SIGNATURES['gdn_calib_rmw'] = (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p])
+
+
+class RotaryRows(Structure):
+    _fields_ = [('x', c_void_p), ('y', c_void_p), ('heads', c_int64), ('x_stride', c_int64 * 3), ('y_stride', c_int64 * 3)]
+
+
+class RotaryCall(Structure):
+    _fields_ = [(n, c_void_p) for n in ('cos', 'sin', 'positions', 'offsets', 'cu_seqlens')] + [
+        (n, c_int64) for n in ('table_rows', 'table_stride', 'offset', 'B', 'T', 'N', 'D', 'rotary_dim')] + [
+        ('dtype', c_int32), ('table_dtype', c_int32), ('flags', c_uint32), ('reserved', c_uint32)]
+
+
+class PagedCache(Structure):
+    _fields_ = [(n, c_void_p) for n in ('k', 'v', 'page_table', 'context')] + [('k_stride', c_int64 * 3), ('v_stride', c_int64 * 3)] + [
+        (n, c_int64) for n in ('pages', 'page_size', 'heads', 'dim', 'table_cols', 'table_stride')] + [('dtype', c_int32), ('context_int32', c_int32)]
+
+
+class PagedAttnCall(Structure):
+    _fields_ = [(n, c_void_p) for n in ('q', 'o', 'cu_seqlens', 'mask')] + [('q_stride', c_int64 * 3)] + [
+        (n, c_int64) for n in ('mask_seq_stride', 'mask_row_stride', 'mask_cols', 'B', 'T', 'N', 'HQ', 'max_rows')] + [('scale', c_float), ('flags', c_uint32)]
+
+
+class DraftsCall(Structure):
+    _fields_ = [(n, c_void_p) for n in ('p', 'q', 'tokens', 'uniforms', 'parents', 'lengths', 'next_token', 'accepted', 'rows')] + [
+        ('p_stride', c_int64 * 2), ('q_stride', c_int64 * 2)] + [(n, c_int64) for n in ('parents_stride', 'N', 'R', 'V')] + [
+        ('p_dtype', c_int32), ('q_dtype', c_int32), ('flags', c_uint32), ('reserved', c_uint32)]
+
+
+SIGNATURES['gdn_rotary'] = (c_int, [POINTER(RotaryRows), c_int, POINTER(RotaryCall), c_void_p])
+SIGNATURES['gdn_paged_append'] = (c_int, [POINTER(PagedCache)] + [POINTER(RotaryRows)] * 3 + [POINTER(RotaryCall), c_void_p])    # cache q k v
+SIGNATURES['gdn_paged_keep'] = (c_int, [POINTER(PagedCache), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p])     # cache rows rows_stride R kept N
+SIGNATURES['gdn_paged_attn_workspace_bytes'] = (c_size_t, [POINTER(PagedCache), POINTER(PagedAttnCall)])
+SIGNATURES['gdn_paged_attn'] = (c_int, [POINTER(PagedCache), POINTER(PagedAttnCall), c_void_p, c_size_t, c_void_p])
+SIGNATURES['gdn_verify_drafts_workspace_bytes'] = (c_size_t, [POINTER(DraftsCall)])
+SIGNATURES['gdn_verify_drafts'] = (c_int, [POINTER(DraftsCall), c_void_p, c_size_t, c_void_p])
+ROTARY_INTERLEAVED, ROTARY_BACK, ROTARY_POSITIONS_INT32, ROTARY_OFFSETS_INT32 = 1 << 24, 1 << 25, 1 << 26, 1 << 27
+DRAFTS_TOKENS_INT64 = 1 << 24
 CHUNK_STATIC_WORKSPACE_BYTES = 64 << 20
 CONV_BWD_TILES_PER_PART = 8
 MLP_FEW_ROWS = 16

@@ -1,0 +1,266 @@
+"""Rotary positions, with the names of the reference's fla/modules/rotary.py: ``rotary_embedding`` (differentiable) and ``RotaryEmbedding``; ``rotary_embedding_qk``
+turns queries and keys in one launch.  All compute is done by ``gdn_rotary`` of the HIP library; the tables are made once, by torch.
+
+The tables are kept in fp32 from angles in 64 bits (the reference keeps them in the rows' type, from angles in 32): at position 100000 the fastest pair's angle is then
+right to 1e-11 instead of 4e-3.  Tables of the rows' type are taken as well."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+import torch.nn as nn
+
+from fla_hip import _lib
+from fla_hip.ops.gated_delta_rule._common import as_index, dtype_code, forward_only, launch, no_forward_mode, ptr, require_gpu, unit_rows, written
+from fla_hip.ops.utils.index import check_cu_seqlens
+
+
+def rows_of(x: torch.Tensor, y: torch.Tensor | None) -> _lib.RotaryRows:
+    return _lib.RotaryRows(ptr(x), ptr(y), x.shape[2], (ctypes.c_int64 * 3)(*x.stride()[:3]), (ctypes.c_int64 * 3)(*(y if y is not None else x).stride()[:3]))
+
+
+def check_tables(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos, sin ``[positions, R / 2]`` of one type, x's or fp32, their rows equally far apart."""
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError(f'cos and sin must be [positions, rotary_dim / 2], got {tuple(cos.shape)} and {tuple(sin.shape)}')
+    if cos.shape[1] == 0 or 2 * cos.shape[1] > x.shape[-1]:
+        raise ValueError(f'cos and sin turn {2 * cos.shape[1]} elements of heads of {x.shape[-1]}')
+    if cos.dtype != sin.dtype or cos.dtype not in (x.dtype, torch.float32):
+        cos, sin = cos.float(), sin.float()
+    cos, sin = unit_rows(cos), unit_rows(sin)
+    if cos.stride(0) != sin.stride(0) or cos.stride(0) < cos.shape[1]:
+        cos, sin = cos.contiguous(), sin.contiguous()
+    return cos, sin
+
+
+def rotary_call(x: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, interleaved: bool, back: bool, positions: torch.Tensor | None,
+                offsets: torch.Tensor | None, offset: int, cu_seqlens: torch.Tensor | None) -> _lib.RotaryCall:
+    """Everything of a call but its tensors; the indices are as ``as_index`` leaves them."""
+    B, T, _, D = x.shape
+    call = _lib.RotaryCall(ptr(cos), ptr(sin), ptr(positions), ptr(offsets), ptr(cu_seqlens), B=B, T=T, D=D, offset=offset,
+                           N=B if cu_seqlens is None else cu_seqlens.numel() - 1, dtype=dtype_code(x.dtype))
+    if cos is not None:
+        call.table_rows, call.table_stride, call.rotary_dim, call.table_dtype = cos.shape[0], cos.stride(0), 2 * cos.shape[1], dtype_code(cos.dtype)
+    else:
+        call.table_dtype = call.dtype
+    flags = (_lib.ROTARY_INTERLEAVED if interleaved else 0) | (_lib.ROTARY_BACK if back else 0)
+    for t, flag in ((positions, _lib.ROTARY_POSITIONS_INT32), (offsets, _lib.ROTARY_OFFSETS_INT32), (cu_seqlens, _lib.FLAG_CU_INT32)):
+        if t is not None and t.dtype == torch.int32:
+            flags |= flag
+    call.flags = flags
+    return call
+
+
+def _turn(xs: tuple, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace: bool) -> tuple:
+    xs = tuple(unit_rows(x) for x in xs)
+    ys = xs if inplace else tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+    call = rotary_call(xs[0], cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens)
+    rows = (_lib.RotaryRows * len(xs))(*(rows_of(x, y) for x, y in zip(xs, ys)))
+    launch(_lib.load().gdn_rotary, xs[0].device, rows, len(xs), ctypes.byref(call))
+    return ys
+
+
+class RotaryFunction(torch.autograd.Function):
+    """A turn by the tables' angles; its gradient is the turn back, which is this function again (and so differentiable itself)."""
+
+    @staticmethod
+    def forward(ctx, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace, *xs):
+        ctx.save_for_backward(cos, sin, positions, offsets, cu_seqlens)
+        ctx.call = (interleaved, back, offset)
+        ctx.like = [(x.shape, x.dtype, x.device) for x in xs]
+        ctx.set_materialize_grads(False)
+        if inplace:
+            ctx.mark_dirty(*xs)
+        return _turn(xs, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace)
+
+    @staticmethod
+    def backward(ctx, *dys):
+        (interleaved, back, offset), (cos, sin, positions, offsets, cu_seqlens) = ctx.call, ctx.saved_tensors
+        at = [i for i, dy in enumerate(dys) if dy is not None]
+        dxs = [None] * len(dys)
+        if at:
+            grads = RotaryFunction.apply(cos, sin, interleaved, not back, positions, offsets, offset, cu_seqlens, False, *(dys[i].to(ctx.like[i][1]) for i in at))
+            for i, dx in zip(at, grads):
+                dxs[i] = dx
+        return (None,) * 9 + tuple(dxs)
+
+
+def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlens, max_seqlen, positions) -> tuple:
+    x = xs[0]
+    dev = require_gpu(*xs, cos, sin)
+    for other in xs:
+        if other.dim() != 4:
+            raise ValueError(f'rotary positions take [B, T, heads, dim], got {tuple(other.shape)}')
+        if other.shape[:2] != x.shape[:2] or other.shape[3] != x.shape[3] or other.dtype != x.dtype:
+            raise ValueError(f'queries and keys must agree in batch, length, head size and type, got {tuple(x.shape)} {x.dtype} and {tuple(other.shape)} {other.dtype}')
+    dtype_code(x.dtype)
+    cos, sin = check_tables(x, cos, sin)
+    forward_only('a gradient of the tables of rotary positions', cos, sin)
+    no_forward_mode('rotary positions', *xs, cos, sin)
+    B, T = x.shape[:2]
+    N, longest = B, T
+    if cu_seqlens is not None:
+        if B != 1:
+            raise ValueError(f'The batch size is expected to be 1 rather than {B} when using `cu_seqlens`.')
+        N = cu_seqlens.numel() - 1
+        if N < 1:
+            raise ValueError('cu_seqlens must hold N + 1 >= 2 boundaries')
+        if max_seqlen is None:
+            check_cu_seqlens(cu_seqlens, T)
+        longest = max_seqlen
+        cu_seqlens = as_index(cu_seqlens, dev, 'cu_seqlens', (N + 1,))
+    offsets, offset = None, 0
+    if positions is not None:
+        positions = as_index(positions, dev, 'positions', (B, T))
+        if isinstance(seqlen_offsets, torch.Tensor) or seqlen_offsets:
+            raise ValueError('positions take the place of seqlen_offsets: give one of the two')
+    elif isinstance(seqlen_offsets, torch.Tensor):
+        offsets = as_index(seqlen_offsets, dev, 'seqlen_offsets', (N,))
+    else:
+        offset = int(seqlen_offsets)
+        if longest is not None and (offset < 0 or offset + longest > cos.shape[0]):
+            raise ValueError(f'the tables have {cos.shape[0]} positions, positions {offset} to {offset + longest - 1} are needed')
+    if inplace:
+        for x in xs:
+            if x.stride(-1) != 1 and x.shape[-1] > 1:
+                raise ValueError('inplace=True needs heads whose elements lie in a row')
+            if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                raise ValueError('inplace=True needs a tensor that does not overlap itself')
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        return RotaryFunction.apply(cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace, *xs)
+    ys = _turn(tuple(x.detach() for x in xs), cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace)
+    if inplace:
+        written(*xs)
+        return xs
+    return ys
+
+
+def rotary_embedding(
+    x: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    interleaved: bool = False,
+    inplace: bool = False,
+    seqlen_offsets: int | torch.Tensor = 0,
+    cu_seqlens: torch.Tensor | None = None,
+    max_seqlen: int | None = None,
+    positions: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """x ``[B, T, H, D]`` turned by the angles of its positions: ``(x1 cos - x2 sin, x1 sin + x2 cos)`` for the pairs ``(j, j + R/2)``, or ``(2j, 2j + 1)`` with
+    ``interleaved``; cos, sin ``[positions, R/2]``, elements behind R pass through.  Row i of a sequence is at position ``i + seqlen_offsets`` (a number, or
+    ``[N]``), or at ``positions [B, T]``.  ``cu_seqlens [N + 1]``: a packed batch; with ``max_seqlen`` (at least the longest sequence) its boundaries are not read by the host.
+    A position that only the GPU knows and the tables do not have gives NaN; rows of no sequence are handed on as they are.  Differentiable in x, any number of times."""
+    return _rotary((x,), cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlens, max_seqlen, positions)[0]
+
+
+def rotary_embedding_qk(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    interleaved: bool = False,
+    inplace: bool = False,
+    seqlen_offsets: int | torch.Tensor = 0,
+    cu_seqlens: torch.Tensor | None = None,
+    max_seqlen: int | None = None,
+    positions: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rotary_embedding`` of queries and keys (of their own numbers of heads) in one launch."""
+    return _rotary((q, k), cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlens, max_seqlen, positions)
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+    """(angles per position of the ``dim / 2`` pairs in 64 bits, factor of cos and sin).  ``scaling``: ``{'type': 'linear' | 'ntk' | 'yarn', 'factor': s, ...}`` for
+    contexts s times the trained one - every angle divided by s; the base times ``s ** (dim / (dim - 2))``; or (with ``original_max_position_embeddings``, and
+    ``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor`` 0.1 ln s + 1) the pairs that turn less than beta_slow times in the trained context divided by s, those that
+    turn more than beta_fast times left alone, and in between a ramp."""
+    if dim <= 0 or dim % 2:
+        raise ValueError(f'the turned part of a head must be even, got {dim}')
+    inverse = lambda b: b ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if scaling is None:
+        return inverse(base), 1.0
+    kind, factor = scaling.get('type', scaling.get('rope_type')), float(scaling['factor'])
+    if not factor >= 1:
+        raise ValueError(f'the factor of a scaled context must be at least 1, got {factor}')
+    if kind == 'linear':
+        return inverse(base) / factor, 1.0
+    if kind == 'ntk':
+        if dim <= 2:
+            raise ValueError('scaling by the base needs more than one pair')
+        return inverse(base * factor ** (dim / (dim - 2))), 1.0
+    if kind == 'yarn':
+        trained = scaling['original_max_position_embeddings']
+        at = lambda turns: dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low = max(math.floor(at(scaling.get('beta_fast', 32))), 0)
+        high = min(math.ceil(at(scaling.get('beta_slow', 1))), dim - 1)
+        ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inverse(base)
+        return inv / factor * ramp + inv * (1 - ramp), float(scaling.get('attention_factor', 0.1 * math.log(factor) + 1.0))
+    raise ValueError(f"scaling must be of type 'linear', 'ntk' or 'yarn', got {kind!r}")
+
+
+class RotaryEmbedding(nn.Module):
+    """Queries and keys turned by their positions (``fla.modules.RotaryEmbedding``), ``dim`` elements of each head.  ``scale_base``: the turned pairs of queries are scaled by
+    ``s ** ((t - T // 2) / scale_base)``, those of keys by its inverse, ``s = (2j + 0.4 dim) / (1.4 dim)``.  ``scaling``: see ``rotary_frequencies``.  The tables grow with
+    the positions asked for and are no part of the state."""
+
+    def __init__(self, dim: int, base: float = 10000.0, scale_base: float | None = None, interleaved: bool = False, pos_idx_in_fp32: bool = True,
+                 device: torch.device | None = None, scaling: dict | None = None):
+        super().__init__()
+        if not pos_idx_in_fp32:
+            raise NotImplementedError('angles are formed in 64 bits: pos_idx_in_fp32=False is not offered')
+        self.dim, self.base, self.scale_base, self.interleaved, self.scaling = dim, float(base), scale_base, interleaved, scaling
+        inv_freq, self.attention_factor = rotary_frequencies(dim, self.base, scaling)
+        self.register_buffer('inv_freq', inv_freq.float().to(device), persistent=False)
+        self._tables = None
+
+    def extra_repr(self) -> str:
+        return f'dim={self.dim}, base={self.base}, interleaved={self.interleaved}' + (f', scale_base={self.scale_base}' if self.scale_base is not None else '') + (
+            f', scaling={self.scaling}' if self.scaling is not None else '')
+
+    def tables(self, positions: int, device: torch.device) -> tuple[torch.Tensor, ...]:
+        """cos, sin for at least this many positions (and, with ``scale_base``, the keys' cos, sin), fp32."""
+        device = torch.device(device)
+        kept = self._tables
+        if kept is not None and kept[0].device == device and (kept[0].shape[0] >= positions if self.scale_base is None else kept[0].shape[0] == positions):
+            return kept
+        if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f'the tables of {positions} positions are not made yet: call RotaryEmbedding.tables({positions}, device) before the capture')
+        if kept is not None and kept[0].device == device and self.scale_base is None:
+            positions = max(positions, 2 * kept[0].shape[0])             # (asked for position after position: seldom made)
+        inv, factor = rotary_frequencies(self.dim, self.base, self.scaling)
+        # Made on the host and copied while it waits: whatever stream reads them, they are there.
+        with torch.no_grad(), torch.inference_mode(False):
+            t = torch.arange(positions, dtype=torch.float64)
+            angle = t[:, None] * inv
+            cos, sin = angle.cos() * factor, angle.sin() * factor
+            if self.scale_base is None:
+                tables = (cos, sin)
+            else:
+                s = (torch.arange(0, self.dim, 2, dtype=torch.float64) + 0.4 * self.dim) / (1.4 * self.dim)
+                scale = s ** ((t - positions // 2) / self.scale_base)[:, None]
+                tables = (cos * scale, sin * scale, cos / scale, sin / scale)
+            self._tables = tuple(x.float().to(device) for x in tables)
+        return self._tables
+
+    def forward(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        seqlen_offset: int | torch.Tensor = 0,
+        cu_seqlens: torch.Tensor | None = None,
+        max_seqlen: int | None = None,
+        positions: torch.Tensor | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """q, k ``[B, T, heads, D]``.  Where positions are known to the GPU alone (``seqlen_offset`` or ``positions`` a tensor) ``max_seqlen`` says how many the tables
+        have to have."""
+        known = not isinstance(seqlen_offset, torch.Tensor) and positions is None
+        if not known and max_seqlen is None:
+            raise ValueError('max_seqlen is needed where seqlen_offset or positions are tensors: the number of positions that the tables have to have')
+        count = (max_seqlen if max_seqlen is not None else q.shape[1]) + (int(seqlen_offset) if known else 0)
+        tables = self.tables(count, q.device)
+        call = dict(interleaved=self.interleaved, seqlen_offsets=seqlen_offset, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen if cu_seqlens is not None else None, positions=positions)
+        if self.scale_base is None:
+            return rotary_embedding_qk(q, k, *tables, **call)
+        return rotary_embedding(q, *tables[:2], **call), rotary_embedding(k, *tables[2:], **call)

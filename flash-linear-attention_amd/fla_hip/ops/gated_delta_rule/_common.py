@@ -176,3 +176,26 @@ def differentiable_once(backward):
         return tuple(outs)
 
     return wrapper
+
+
+def as_index(x: torch.Tensor, dev: torch.device, name: str, shape: tuple) -> torch.Tensor:
+    """A tensor of whole numbers as the kernels read it: int32 or int64, contiguous, of this shape, on the operands' device."""
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError(f'{name} must be {list(shape)}, got {list(x.shape)}')
+    if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
+        raise ValueError(f'{name} must hold whole numbers, got {x.dtype}')
+    if x.dtype not in (torch.int32, torch.int64):
+        x = x.long()
+    return x.to(dev).contiguous()
+
+
+def unit_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` with the elements of its last dimension in a row (a copy only where they are not)."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def written(*tensors: torch.Tensor) -> None:
+    """Says of tensors that a kernel has written into that they changed: a backward that saved one raises, as behind torch's own in-place operators."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)

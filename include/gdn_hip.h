@@ -709,6 +709,107 @@ typedef struct gdn_pad_segment {
 int gdn_pad_rows(const gdn_pad_segment* segments, int count, void* stream);
 
 /*
+ * Rotary positions: (y1, y2) = (x1 c - x2 s, x1 s + x2 c) for the pairs (j, j + R/2) of a head, or (2j, 2j + 1) with GDN_ROTARY_INTERLEAVED, j < R/2; the
+ * head's elements behind R are handed on as they are.  c, s: row `position` of the tables.  Replaces rotary_embedding_fwdbwd (fla/modules/rotary.py);
+ * the gradient is the same call with GDN_ROTARY_BACK (s negated).
+ *   rows: one or two tensors (queries and keys), x and y [B,T,heads,D] of `dtype` with strides in elements, a head's elements in a row; y may be x
+ *   cos, sin [table_rows, R/2], rows table_stride elements apart, of dtype or fp32 (table_dtype)
+ *   position of row i of sequence n: positions[b,t] where given, else i + seqlen_offsets[n] (or `offset` for all).  A position that the tables do not have gives
+ *   NaN.  cu_seqlens [N+1]: a packed batch (B = 1); rows of no sequence are handed on as they are.
+ *   Products and sums in fp32, one rounding.
+ */
+#define GDN_ROTARY_INTERLEAVED     (1u << 24)
+#define GDN_ROTARY_BACK            (1u << 25)
+#define GDN_ROTARY_POSITIONS_INT32 (1u << 26)
+#define GDN_ROTARY_OFFSETS_INT32   (1u << 27)
+#define GDN_ROTARY_MAX_DIM   1024
+#define GDN_ROTARY_MAX_HEADS 65536
+typedef struct gdn_rotary_rows {
+    const void* x; void* y;
+    int64_t heads;
+    int64_t x_stride[3], y_stride[3];       /* batch, token, head */
+} gdn_rotary_rows;
+typedef struct gdn_rotary_call {
+    const void* cos; const void* sin; const void* positions; const void* offsets; const void* cu_seqlens;
+    int64_t table_rows, table_stride, offset, B, T, N, D, rotary_dim;
+    int32_t dtype, table_dtype;
+    uint32_t flags, reserved;
+} gdn_rotary_call;
+int gdn_rotary(const gdn_rotary_rows* rows, int count, const gdn_rotary_call* call, void* stream);
+
+/*
+ * A cache of keys and values in pages: slot p of sequence n is slot p % page_size of page page_table[n][p / page_size].
+ *   k, v [pages, page_size, heads, dim] of dtype, strides in elements (page, slot, head), a head's elements in a row
+ *   page_table [N, table_cols] int32, rows table_stride apart; an entry outside [0, pages) is no page (so -1 behind a sequence's last)
+ *   context [N] (int32 or int64): slots that held a token before this step; row i of the step has slot context + i
+ * A slot without a page, or behind the table's row, is neither read nor written.
+ */
+typedef struct gdn_paged_cache {
+    void* k; void* v;
+    const int32_t* page_table; const void* context;
+    int64_t k_stride[3], v_stride[3];
+    int64_t pages, page_size, heads, dim, table_cols, table_stride;
+    int32_t dtype, context_int32;
+} gdn_paged_cache;
+
+/*
+ * The keys and values of a step's rows to their slots, turned on the way where rotary_dim > 0 (the default position is the slot), and the step's queries
+ * turned beside them (q may be NULL).  k->y and v->y, call->offsets and call->offset are not read.
+ */
+int gdn_paged_append(const gdn_paged_cache* cache, const gdn_rotary_rows* q, const gdn_rotary_rows* k, const gdn_rotary_rows* v,
+                     const gdn_rotary_call* call, void* stream);
+
+/*
+ * The rows of a step that stay, moved to the front: slot context + i = slot context + rows[n][i] for i < kept[n] (in keys and values).  rows [N, R]
+ * with rows[n][i] >= i (the path down a tree; any other entry leaves its slot as it is), kept [N] (held to R).
+ */
+int gdn_paged_keep(const gdn_paged_cache* cache, const int32_t* rows, int64_t rows_stride, int64_t R, const int32_t* kept, int64_t N, void* stream);
+
+/*
+ * Attention of a step's rows over the paged cache: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that row i sees: the context's, and of the
+ * step's own (which are in the cache by then) those with mask[i][j], or j <= i without a mask.  A row that sees none gets 0.
+ *   q [B,T,HQ,D] with strides in elements (batch, token, head), o [B,T,HQ,D] contiguous, of the cache's dtype (bf16 or fp16); HQ a multiple of the cache's heads
+ *   cu_seqlens [N+1] (GDN_FLAG_CU_INT32) or NULL (N = B sequences of T rows); max_rows: at least the rows of the longest sequence
+ *   mask: bytes, row i of sequence n at n * mask_seq_stride + i * mask_row_stride (with cu_seqlens at (cu[n] + i) * mask_row_stride); key j >= mask_cols is not seen
+ *   Scores, statistics and sums in fp32; the probabilities are rounded to dtype for their product with v.  Rows of no sequence get 0.
+ */
+typedef struct gdn_paged_attn_call {
+    const void* q; void* o; const void* cu_seqlens; const uint8_t* mask;
+    int64_t q_stride[3];
+    int64_t mask_seq_stride, mask_row_stride, mask_cols;
+    int64_t B, T, N, HQ, max_rows;
+    float scale;
+    uint32_t flags;
+} gdn_paged_attn_call;
+size_t gdn_paged_attn_workspace_bytes(const gdn_paged_cache* cache, const gdn_paged_attn_call* call);
+int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn_call* call, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Which drafted tokens stand.  Row 0 of a sequence is its last token, row r > 0 a draft that follows row parents[r] < r (parents NULL: the row before).
+ * From row 0 on: the drafts that follow the row come to are asked in order; draft c stands if u[c] q(x_c) < p(x_c), and the walk goes on from it; else p
+ * becomes (p - q)+, brought to a sum of 1 (as it was where that is 0), and the next is asked.  When none is left, the next token is the first word with
+ * sum_{w <= v} p(w) > u[0] sum p (-1 where p has no mass: all zero or NaN).  p, q: the target's and the draft's probabilities after the row come to; q NULL: drafts that
+ * were not sampled (q is 1 at the draft and 0 elsewhere).  Comparisons and sums in 64 bits; negative and NaN probabilities count as 0.
+ *   p, q [N,R,V] (bf16, fp16 or fp32) with strides in elements (sequence, row); tokens [N,R] (int32, or int64 with GDN_DRAFTS_TOKENS_INT64); u [N,R] fp32;
+ *   parents [N,R] int32 with parents_stride (0: one tree for all); lengths [N] int32 or NULL: rows of a sequence (at least 1)
+ *   next_token [N] int64, accepted [N] int32 (rows that stand, row 0 among them), rows [N,R] int32 (which, in order; -1 behind them)
+ *   A draft outside the vocabulary, and a row whose parent is not before it, is never taken.
+ */
+#define GDN_DRAFTS_TOKENS_INT64 (1u << 24)
+#define GDN_DRAFTS_MAX_ROWS 1024
+#define GDN_DRAFTS_MAX_WORDS 4194304
+typedef struct gdn_drafts_call {
+    const void* p; const void* q; const void* tokens; const float* uniforms; const int32_t* parents; const int32_t* lengths;
+    int64_t* next_token; int32_t* accepted; int32_t* rows;
+    int64_t p_stride[2], q_stride[2], parents_stride;
+    int64_t N, R, V;
+    int32_t p_dtype, q_dtype;
+    uint32_t flags, reserved;
+} gdn_drafts_call;
+size_t gdn_verify_drafts_workspace_bytes(const gdn_drafts_call* call);
+int gdn_verify_drafts(const gdn_drafts_call* call, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Measurement aid with no counterpart in the reference (bench.py --workload calib_rmw): the memory traffic and the
  * dependency of a decode step without its arithmetic.  Every 64 KB block of `data` (n_floats a multiple of 16384)
  * is read, reduced across its workgroup and written back in place.  xcd_run > 0: every XCD works on runs of that

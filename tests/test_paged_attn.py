@@ -1,0 +1,331 @@
+"""Attention of a step's rows over the paged cache (fla_hip.ops.attn.paged_attn) against the 64-bit oracle, element by element.
+
+Tolerance, u = half the spacing of the operands' type relative to it, e = 2^-24, L keys.  A score is a sum of D exact products in fp32 and a scaling: off by (D + 4) e S, S the
+largest sum of |q_d k_d| scale; its distance from the maximum and the exponential add 4 e (spread + 1).  So a weight is off by d = 2 ((D + 4) e S + 4 e (spread + 1)) of itself, the sum of the
+weights by as much, and for the product with v a weight is rounded once to the operands' type, u.  Both sums have L terms in some order, with the parts' sums rescaled at most
+L / 16 times: 2 L e of the sum of the magnitudes A = sum w |v|.  The result is rounded once, u |ref|; a weight below the smallest normal number of fp16 is off by
+2^-25 of the largest, of which at most L meet some |v|: L 2^-25 max |v|."""
+import pytest
+import torch
+
+from oracle import serving_oracle as O
+from paged_inputs import DEV, cache, pages_for, table
+
+gpu = pytest.mark.gpu
+E = 2.0 ** -24
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _attn():
+    from fla_hip.ops import attn
+    return attn
+
+
+def _near(got, ref, size, dots, spread, L, D, v_max):
+    assert tuple(got.shape) == tuple(ref.shape)
+    got = got.cpu()
+    u = torch.finfo(got.dtype).eps / 2
+    d = 2 * ((D + 4) * E * dots + 4 * E * (spread + 1))[..., None]
+    tol = u * ref.abs() * (1 + 1e-3) + (2 * d + u + 2 * (L + 64) * E) * size + (L * v_max + 1) * (2.0 ** -25 if got.dtype == HF else 2.0 ** -130)
+    err = (got.double() - ref).abs()
+    assert bool((err <= tol).all()), f'{(err / tol).nan_to_num(nan=1e9).max().item():.2f} of the tolerance'
+
+
+class Step:
+    """A step over a paged cache: tensors on the GPU and what the oracle takes."""
+
+    def __init__(self, contexts, rows, page_size, HQ, HK, D, dtype, packed=False, mask=None, layout='slots', index=torch.int32, seed=0, spoil=None, q_std=1.0, room=0):
+        self.contexts, self.rows, self.packed, self.D, self.HQ, self.room = contexts, rows, packed, D, HQ, room
+        lengths = [c + r for c, r in zip(contexts, rows)]
+        self.L = max(lengths)
+        pages = pages_for(lengths, page_size)
+        self.k_cache, self.v_cache = cache(pages, page_size, HK, D, dtype, seed, layout)
+        self.t = table(lengths, page_size, pages, seed)
+        if spoil:
+            spoil(self)
+        gen = torch.Generator().manual_seed(seed + 77)
+        self.firsts = [0, *torch.tensor(rows).cumsum(0).tolist()]
+        shape = (1, sum(rows) + room) if packed else (len(rows), rows[0])
+        self.q = (torch.randn(*shape, HQ, D, generator=gen) * q_std).to(dtype).to(DEV)
+        self.mask = mask                                          # [B,T,cols], [T,cols] or packed [rows,cols], on the CPU
+        self.index = index
+        self.scale = D ** -0.5
+
+    def call(self, **kw):
+        cu = torch.tensor(self.firsts, dtype=self.index, device=DEV) if self.packed else None
+        return _attn().paged_attn(kw.pop('q', self.q), self.k_cache, self.v_cache, self.t.to(DEV), torch.tensor(self.contexts, dtype=self.index, device=DEV),
+                                  tree_mask=None if self.mask is None else self.mask.to(DEV), cu_seqlens=cu, **kw)
+
+    def sees(self, n, i, j):
+        if self.mask is None:
+            return j <= i
+        row = self.mask[self.firsts[n] + i] if self.packed else self.mask[i] if self.mask.dim() == 2 else self.mask[n, i]
+        return j < len(row) and bool(row[j])
+
+    def check(self, o=None, scale=None, **kw):
+        o = self.call(scale=scale, **kw) if o is None else o
+        spans = list(zip(self.firsts[:-1], self.firsts[1:]))
+        ref, size, dots, spread = O.paged_attn(self.q.flatten(0, 1), self.k_cache, self.v_cache, self.t, self.contexts, spans, self.sees, self.scale if scale is None else scale)
+        _near(o.flatten(0, 1), ref, size, dots, spread, self.L, self.D, self.v_cache.abs().nan_to_num(0).max().item())
+        return o
+
+
+def _tree(gen, R):
+    sees = torch.zeros(R, R, dtype=torch.bool)
+    for i in range(R):
+        if i:
+            sees[i] |= sees[int(torch.randint(0, i, (1,), generator=gen))]
+        sees[i, i] = True
+    return sees
+
+
+# head sizes and types, groups of one to many heads, pages from a slot to many
+@gpu
+@pytest.mark.parametrize(('HQ', 'HK', 'D', 'page_size', 'dtype'), [
+    (4, 4, 64, 16, BF), (8, 2, 128, 16, BF), (16, 4, 128, 64, HF), (6, 3, 80, 10, HF), (2, 1, 256, 32, BF), (32, 1, 64, 1, BF), (5, 5, 128, 7, HF), (24, 3, 96, 128, BF), (3, 1, 8, 16, BF), (7, 7, 200, 100, HF),
+    (40, 2, 128, 48, BF), (71, 1, 64, 16, HF)])
+def test_steps_of_one_token(HQ, HK, D, page_size, dtype):
+    Step([0], [1], page_size, HQ, HK, D, dtype).check()
+    Step([700, 0, 31, 64, 1, 15], [1] * 6, page_size, HQ, HK, D, dtype, seed=1).check()
+
+
+@gpu
+@pytest.mark.parametrize(('rows', 'HQ', 'HK', 'D', 'page_size', 'dtype'), [
+    (2, 4, 4, 64, 16, BF), (8, 8, 2, 128, 16, BF), (17, 8, 8, 128, 64, HF), (33, 4, 2, 80, 10, HF), (64, 8, 1, 128, 32, BF), (100, 3, 1, 256, 16, BF), (130, 8, 2, 64, 5, HF), (31, 2, 2, 128, 1, BF), (70, 5, 5, 40, 64, BF),
+    (200, 16, 2, 128, 16, BF)])
+@pytest.mark.parametrize('kind', ['chain', 'tree', 'trees', 'packed', 'packed_trees'])
+def test_steps_of_many_rows(kind, rows, HQ, HK, D, page_size, dtype):
+    gen = torch.Generator().manual_seed(rows)
+    contexts, counts = [300, 0, 77], [rows] * 3
+    mask = None
+    if kind.startswith('packed'):
+        counts = [rows, 1, max(1, rows // 3)]
+    if kind == 'tree':
+        mask = _tree(gen, rows)
+    elif kind == 'trees':
+        mask = torch.stack([_tree(gen, rows) for _ in range(3)])
+    elif kind == 'packed_trees':
+        mask = torch.cat([torch.nn.functional.pad(_tree(gen, c), (0, rows - c)) for c in counts])
+    step = Step(contexts, counts, page_size, HQ, HK, D, dtype, kind.startswith('packed'), mask, seed=rows)
+    step.check()
+
+
+@gpu
+@pytest.mark.parametrize('D', [64, 128, 256])
+@pytest.mark.parametrize('packed', [False, True])
+def test_long_contexts_of_all_lengths(packed, D):
+    """Long enough for a sequence's keys to be shared out, and some that are too short for it."""
+    contexts = [20000, 3, 0, 900, 5111, 64]
+    Step(contexts, [1] * 6, 64, 4, 2, D, BF, packed, seed=3).check()
+    Step(contexts[:3], [3] * 3, 16, 8, 2, D, HF, packed, seed=4).check()
+
+
+@gpu
+@pytest.mark.parametrize('rows', [1, 5, 40])
+def test_every_length_around_the_tiles(rows):
+    """Contexts and pages that end anywhere inside a tile of keys."""
+    contexts = list(range(0, 70)) + [127, 128, 129, 255, 256, 257]
+    for page_size in (16, 24, 9):
+        Step(contexts, [rows] * len(contexts), page_size, 4, 2, 64, BF, seed=page_size).check()
+
+
+@gpu
+@pytest.mark.parametrize('rows', [3, 40])
+def test_rows_that_see_nothing_and_columns_that_are_missing(rows):
+    mask = torch.zeros(3, rows, rows, dtype=torch.bool)
+    mask[0, 1, 0] = True
+    mask[1] = _tree(torch.Generator().manual_seed(0), rows)
+    step = Step([0, 0, 5], [rows] * 3, 16, 4, 2, 64, BF, mask=mask)
+    o = step.check()
+    assert not o[0, 0].any() and not o[0, 2:].any() and o[2].any()
+    Step([0, 9, 33], [rows] * 3, 16, 4, 2, 64, BF, mask=mask[:, :, :2]).check()
+    wide = torch.ones(rows, rows + 50, dtype=torch.bool)         # (columns behind the rows: nothing there)
+    Step([0, 9, 33], [rows] * 3, 16, 4, 2, 64, BF, mask=wide).check()
+    inner = torch.zeros(rows, 3, rows, 2, dtype=torch.bool)       # (a mask with strides of its own)
+    inner[..., 1] = mask.transpose(0, 1)
+    want = step.call()
+    step.mask = inner.transpose(0, 1)[..., 1]
+    assert torch.equal(step.call(), want)
+
+
+@gpu
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize(('rows', 'page_size', 'D'), [(1, 16, 64), (6, 16, 128), (6, 10, 128), (40, 64, 128), (80, 7, 64), (24, 16, 256)])
+def test_numbers_in_masked_places(rows, page_size, D, bad):
+    """NaN and infinities in slots that no row sees - behind the last, in pages of nobody - and in drafts that some rows do not see."""
+    contexts = [50, 0, 33]
+    gen = torch.Generator().manual_seed(1)
+    for mask in (None, torch.stack([_tree(gen, rows) for _ in range(3)])):
+        def spoil(step):
+            used = torch.zeros(step.k_cache.shape[:2], dtype=torch.bool)
+            for n, c in enumerate(contexts):
+                for j in range(c + rows):
+                    used[O.slot_of(step.t, n, j, *step.k_cache.shape[:2])] = True
+            for c in (step.k_cache, step.v_cache):
+                c[~used.to(DEV)] = bad
+            step.clean = step.k_cache.clone(), step.v_cache.clone()
+
+        step = Step(contexts, [rows] * 3, page_size, 4, 2, D, BF, mask=mask, spoil=spoil)
+        step.check()
+        # a draft that is not a number: the rows that do not see it get what they got, bit for bit
+        want = step.call()
+        j = rows // 2
+        for cache in (step.k_cache, step.v_cache):
+            cache[O.slot_of(step.t, 0, contexts[0] + j, *cache.shape[:2])] = bad
+        got = step.call()
+        blind = torch.tensor([not step.sees(0, i, j) for i in range(rows)])
+        assert torch.equal(got[0, blind], want[0, blind]) and torch.equal(got[1:], want[1:])
+        if bad != bad:
+            assert got[0, ~blind].isnan().all()
+        # ... and one whose key is a number while its value is not: the element of the value that is not a number, in the rows that see it
+        step.k_cache.copy_(step.clean[0]), step.v_cache.copy_(step.clean[1])
+        step.v_cache[O.slot_of(step.t, 0, contexts[0] + j, *cache.shape[:2])][:, 3] = bad
+        got = step.call()
+        assert torch.equal(got[0, blind], want[0, blind]) and torch.equal(got[0, :, :, 4:], want[0, :, :, 4:])
+        seen = got[0, ~blind][..., 3].float()
+        assert seen.isnan().all() if bad != bad else (seen == bad).all()
+
+
+@gpu
+def test_scores_of_any_size():
+    """Scores that overflow an exponential without the maximum, all keys alike, a single key, scale zero and negative."""
+    Step([300, 2], [4, 4], 16, 4, 2, 128, BF, q_std=300.0).check()
+    step = Step([300, 2], [4, 4], 16, 4, 2, 128, BF)
+    for scale in (0.0, -0.3, 3.0, 1e-6):
+        step.check(scale=scale)
+    step.k_cache[:] = step.k_cache[:1, :1]
+    step.check()
+
+
+@gpu
+@pytest.mark.parametrize('layout', ['heads', 'one', 'odd'])
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+@pytest.mark.parametrize('rows', [1, 50])
+def test_layouts_and_strides(rows, layout, index):
+    step = Step([100, 31], [rows] * 2, 16, 4, 2, 64, BF, layout=layout, index=index)
+    want = step.check()
+    q = step.q
+    wide = torch.zeros(*q.shape[:2], 12, 64, dtype=BF, device=DEV)
+    wide[:, :, 4:8] = q
+    assert torch.equal(step.call(q=wide[:, :, 4:8]), want)
+    assert torch.equal(step.call(q=q.transpose(1, 2).contiguous().transpose(1, 2)), want)
+    assert torch.equal(step.call(q=torch.cat([q.new_zeros(1), q.flatten()])[1:].view(q.shape)), want)
+    assert torch.equal(step.call(q=q.transpose(2, 3).contiguous().transpose(2, 3)), want)
+    table = step.t
+    step.t = torch.full((2, table.shape[1] + 9), 3, dtype=torch.int64)[:, 4:4 + table.shape[1]].copy_(table)
+    assert torch.equal(step.call(), want)
+
+
+def _no_pages(step):
+    step.t[0, 2], step.t[1, 0], step.t[2, 1] = -1, 10 ** 8, -2 ** 31
+
+
+@gpu
+@pytest.mark.parametrize('rows', [1, 30])
+@pytest.mark.parametrize('page_size', [16, 5, 64])
+def test_keys_without_a_page_are_not_seen(page_size, rows):
+    Step([150, 130, 70], [rows] * 3, page_size, 4, 2, 64, BF, spoil=_no_pages).check()
+    step = Step([150, 130, 70], [rows] * 3, page_size, 4, 2, 64, BF)
+    step.t = step.t[:, :2].clone()                               # (slots behind the table's row)
+    step.check()
+    step.t = torch.full((3, 4), -1, dtype=torch.int32)
+    assert not step.call().any()
+    step.t = torch.zeros(3, 0, dtype=torch.int32)
+    assert not step.call().any()
+
+
+@gpu
+@pytest.mark.parametrize('rows', [[1, 1, 1], [3, 0, 50], [0, 0, 1], [90, 2, 0]])
+def test_packed_batches_with_rows_of_no_sequence(rows):
+    step = Step([20, 300, 0], rows, 16, 4, 2, 64, BF, packed=True, room=5)
+    for max_seqlen in (None, max(rows), 1, sum(rows) + 5):      # (a hint: the result does not go by it)
+        o = step.call(max_seqlen=max_seqlen)
+        assert not o[:, sum(rows):].any()
+    spans = list(zip(step.firsts[:-1], step.firsts[1:]))
+    ref, size, dots, spread = O.paged_attn(step.q[0, :sum(rows)], step.k_cache, step.v_cache, step.t, step.contexts, spans, step.sees, step.scale)
+    for max_seqlen in (None, 1):
+        _near(step.call(max_seqlen=max_seqlen)[0, :sum(rows)], ref, size, dots, spread, step.L, 64, step.v_cache.abs().max().item())
+
+
+@gpu
+def test_lengths_that_only_the_gpu_knows():
+    """Contexts below zero and beyond the table are held to what is there; boundaries that lead outside of the batch read nothing."""
+    step = Step([40, 40], [2, 2], 16, 4, 2, 64, BF)
+    want = step.call()
+    a = lambda context, cu=None, q=step.q: _attn().paged_attn(q, step.k_cache, step.v_cache, step.t.to(DEV), torch.tensor(context, device=DEV),
+                                                             cu_seqlens=None if cu is None else torch.tensor(cu, device=DEV), max_seqlen=None if cu is None else 4)
+    got = a([40, 2 ** 40])
+    assert torch.equal(got[0], want[0]) and got.isfinite().all()
+    got = a([40, -5])
+    assert torch.equal(got[0], want[0]) and not got[1].any()
+    packed = step.q.view(1, 4, 4, 64)
+    for cu in ([0, 2, 2 ** 40], [-7, 2, 4], [0, 9, 4], [0, 2, -1]):
+        assert a([40, 40], cu, packed).shape == packed.shape     # (finishes; rows of such sequences are not defined)
+
+
+@gpu
+def test_empty_batches():
+    step = Step([40, 40], [2, 2], 16, 4, 2, 64, BF)
+    assert step.call(q=step.q[:, :0]).shape == (2, 0, 4, 64)
+    none = torch.zeros(0, 3, 4, 64, dtype=BF, device=DEV)
+    assert _attn().paged_attn(none, step.k_cache, step.v_cache, step.t[:0].to(DEV), torch.zeros(0, dtype=torch.int32, device=DEV)).shape == none.shape
+    o = _attn().paged_attn(step.q, step.k_cache[:0], step.v_cache[:0], step.t.to(DEV), torch.tensor([40, 40], device=DEV))
+    assert not o.any()
+
+
+@gpu
+def test_cache_beyond_32_bit_offsets():
+    """Pages whose elements lie more than 2^31 elements (and 2^32 bytes) into the cache."""
+    page_size, HK, D = 64, 8, 128
+    pages = 2 ** 31 // (page_size * HK * D) + 40
+    k_cache, v_cache = (torch.zeros(pages, page_size, HK, D, dtype=BF, device=DEV) for _ in range(2))
+    small = Step([200, 90], [3, 3], page_size, HK, HK, D, BF)
+    far = pages - small.k_cache.shape[0]
+    k_cache[far:], v_cache[far:] = small.k_cache, small.v_cache
+    want = small.call()
+    small.k_cache, small.v_cache, small.t = k_cache, v_cache, torch.where(small.t >= 0, small.t + far, -1).int()
+    assert torch.equal(small.call(), want)
+
+
+@gpu
+def test_the_same_call_twice_and_on_another_stream():
+    step = Step([5000, 20, 900], [4] * 3, 16, 8, 2, 128, BF)
+    want = step.call()
+    assert torch.equal(step.call(), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [step.call() for _ in range(3)]
+    others = [step.call() for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs + others)
+
+
+def _step_call(step, k, v, q, cos, sin, t, context):
+    """Append, attend: what an attention layer does in a step."""
+    q = _attn().paged_append(k, v, step.k_cache, step.v_cache, t, context, q=q, cos=cos, sin=sin)
+    return _attn().paged_attn(q, step.k_cache, step.v_cache, t, context)
+
+
+@gpu
+def test_replayed_graphs_that_share_the_cache():
+    step = Step([4000, 20, 900], [2] * 3, 16, 8, 2, 128, BF)
+    t, context = step.t.to(DEV), torch.tensor(step.contexts, dtype=torch.int32, device=DEV)
+    angle = torch.arange(5000, dtype=torch.float64, device=DEV)[:, None] * 10000.0 ** (-torch.arange(0, 128, 2, device=DEV, dtype=torch.float64) / 128)
+    cos, sin = angle.cos().float(), angle.sin().float()
+    ins = [[torch.randn(3, 2, h, 128, device=DEV).to(BF) for h in (2, 2, 8)] for _ in range(2)]
+    _step_call(step, *ins[0], cos, sin, t, context)
+    graphs, outs = [], []
+    for k, v, q in ins:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(_step_call(step, k, v, q, cos, sin, t, context))
+    for turn in range(3):
+        context.copy_(torch.tensor([[4000, 20, 900], [3, 4000, 0], [1500, 1, 300]][turn]).clamp(max=torch.tensor(step.contexts)))
+        for x in ins[0] + ins[1]:
+            x.copy_(torch.randn_like(x.float()))
+        for i, g in enumerate(graphs):
+            g.replay()
+            torch.cuda.synchronize()
+            got = outs[i].clone()
+            assert torch.equal(got, _step_call(step, *ins[i], cos, sin, t, context))

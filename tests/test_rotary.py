@@ -1,0 +1,389 @@
+"""Rotary positions (fla_hip.modules: rotary_embedding, rotary_embedding_qk, RotaryEmbedding) against the 64-bit oracle, element by element.
+
+Tolerance, u = half the spacing of the result's type relative to it, e = 2^-24: two products and a sum in fp32, three roundings of at most e of the magnitudes
+that enter (|x1 c| + |x2 s|), and one rounding of the result, u |ref|; results below the smallest normal number of fp16 are off by half its smallest step, 2^-25."""
+import math
+
+import pytest
+import torch
+
+from oracle import serving_oracle as O
+
+gpu = pytest.mark.gpu
+DEV = 'cuda'
+E = 2.0 ** -24
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _mods():
+    import fla_hip.modules as mods
+    return mods
+
+
+def _near(name, got, ref, size):
+    assert tuple(got.shape) == tuple(ref.shape), (name, got.shape, ref.shape)
+    got = got.detach().cpu()
+    assert torch.equal(got.isnan(), ref.isnan()), name
+    ok = ~ref.isnan()
+    u = torch.finfo(got.dtype).eps / 2
+    tol = u * ref.abs() * (1 + 1e-3) + 3 * E * size + (2.0 ** -25 if got.dtype == HF else 2.0 ** -140)
+    worst = ((got.double() - ref).abs()[ok] / tol[ok]).max().item() if ok.any() else 0.0
+    assert worst <= 1, f'{name}: {worst:.2f} of the tolerance'
+
+
+def _tables(positions, R, dtype=FP, seed=0):
+    t = torch.arange(positions, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    return t.cos().to(dtype).to(DEV), t.sin().to(dtype).to(DEV)
+
+
+def _rows(*shape, dtype, seed=0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * 2).to(dtype).to(DEV)
+
+
+# head sizes and turned parts on every side of a thread's 16 bytes
+HEADS = [(2, 2), (8, 8), (64, 64), (64, 32), (80, 80), (72, 72), (128, 128), (128, 2), (128, 50), (100, 100), (256, 256), (256, 64), (96, 90), (34, 18), (1024, 1024)]
+
+
+@gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('dtype', [BF, HF, FP])
+@pytest.mark.parametrize(('D', 'R'), HEADS)
+def test_against_the_oracle(D, R, dtype, interleaved):
+    B, T, HQ, HK = 2, 5, 3, 1
+    cos, sin = _tables(T + 3, R)
+    q, k = _rows(B, T, HQ, D, dtype=dtype, seed=D), _rows(B, T, HK, D, dtype=dtype, seed=R)
+    at = torch.arange(T).expand(B, T) + 3
+    got = _mods().rotary_embedding_qk(q, k, cos, sin, interleaved=interleaved, seqlen_offsets=3)
+    for name, x, y in (('q', q, got[0]), ('k', k, got[1])):
+        assert y.dtype == dtype
+        _near(name, y, *O.rotary(x, cos, sin, at, interleaved))
+
+
+@gpu
+@pytest.mark.parametrize(('T', 'HQ', 'HK', 'D'), [(1, 1, 1, 64), (1, 32, 8, 128), (777, 5, 1, 64), (300, 20, 4, 128), (130, 71, 1, 40), (3000, 8, 8, 128), (9, 300, 7, 256)])
+def test_sizes_from_a_row_to_a_full_chip(T, HQ, HK, D):
+    cos, sin = _tables(T, D)
+    q, k = _rows(1, T, HQ, D, dtype=BF), _rows(1, T, HK, D, dtype=BF, seed=1)
+    got = _mods().rotary_embedding_qk(q, k, cos, sin)
+    for x, y in zip((q, k), got):
+        a, b = x.double()[..., :D // 2], x.double()[..., D // 2:]
+        c, s = cos.double()[:, None], sin.double()[:, None]
+        _near('x', y, torch.cat([a * c - b * s, a * s + b * c], -1).cpu(), torch.cat([(a * c).abs() + (b * s).abs(), (a * s).abs() + (b * c).abs()], -1).cpu())
+
+
+@gpu
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+@pytest.mark.parametrize('cu', [[0, 7], [0, 0, 3, 3, 4, 7], [1, 2, 5], [0, 1, 2, 3, 4, 5, 6, 7]])
+def test_packed_batches(cu, index):
+    T = 7
+    cos, sin = _tables(40, 64)
+    x = _rows(1, T, 2, 64, dtype=BF)
+    bounds = torch.tensor(cu, dtype=index, device=DEV)
+    N = len(cu) - 1
+    offsets = torch.arange(N) * 5
+    at = torch.full((1, T), -1)
+    for n in range(N):
+        at[0, cu[n]:cu[n + 1]] = torch.arange(cu[n + 1] - cu[n]) + offsets[n]
+    for max_seqlen in (None, T):
+        y = _mods().rotary_embedding(x, cos, sin, cu_seqlens=bounds, seqlen_offsets=offsets.to(DEV).to(index), max_seqlen=max_seqlen)
+        _near('packed', y, *O.rotary(x, cos, sin, at))
+
+
+@gpu
+@pytest.mark.parametrize('index', [torch.int32, torch.int64, torch.int16])
+def test_positions_and_those_the_tables_do_not_have(index):
+    cos, sin = _tables(10, 32)
+    x = _rows(2, 4, 2, 40, dtype=HF)
+    positions = torch.tensor([[9, 0, 3, 3], [10, 1, 2000, 9]], dtype=index, device=DEV)
+    y = _mods().rotary_embedding(x, cos, sin, positions=positions)
+    _near('positions', y, *O.rotary(x, cos, sin, positions.cpu()))
+    assert y.isnan().any(-1).sum() == 4
+    y = _mods().rotary_embedding(x, cos, sin, seqlen_offsets=torch.tensor([-1, 6], dtype=torch.int32, device=DEV))
+    assert y[0, 0, :, :32].isnan().all() and torch.equal(y[0, 0, :, 32:], x[0, 0, :, 32:])
+    _near('offsets', y[:, 1:], *O.rotary(x[:, 1:], cos, sin, torch.tensor([[0, 1, 2], [7, 8, 9]])))
+
+
+@gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('dtype', [BF, HF])
+def test_tables_of_the_rows_type(dtype, interleaved):
+    cos, sin = _tables(6, 64, dtype)
+    x = _rows(1, 6, 3, 64, dtype=dtype)
+    _near('x', _mods().rotary_embedding(x, cos, sin, interleaved=interleaved), *O.rotary(x, cos, sin, torch.arange(6)[None], interleaved))
+
+
+def _strided(x, how):
+    """The numbers of x at other places."""
+    B, T, H, D = x.shape
+    if how == 'heads_first':
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    if how == 'between_16_bytes':
+        return torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)
+    if how == 'part_of_a_row':                                   # the middle of a wider projection
+        wide = torch.zeros(B, T, 3 * H * D + 5, dtype=x.dtype, device=x.device)
+        wide[..., H * D:2 * H * D] = x.flatten(2)
+        return wide[..., H * D:2 * H * D].view(B, T, H, D)
+    return x.transpose(2, 3).contiguous().transpose(2, 3)        # a head's elements apart
+
+
+@gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('how', ['heads_first', 'between_16_bytes', 'part_of_a_row', 'elements_apart'])
+def test_strides_and_alignments(how, interleaved):
+    cos, sin = _tables(9, 64)
+    x = _rows(2, 9, 4, 64, dtype=BF)
+    want = _mods().rotary_embedding(x, cos, sin, interleaved=interleaved)
+    view = _strided(x, how)
+    assert torch.equal(view, x)
+    assert torch.equal(_mods().rotary_embedding(view, cos, sin, interleaved=interleaved), want)
+    wide = torch.zeros(9, 200, device=DEV)                       # tables as parts of a wider tensor, at any address
+    wide[:, 3:35], wide[:, 40:72] = cos, sin
+    assert torch.equal(_mods().rotary_embedding(x, wide[:, 3:35], wide[:, 40:72], interleaved=interleaved), want)
+    if how != 'elements_apart':
+        assert _mods().rotary_embedding(view, cos, sin, interleaved=interleaved, inplace=True) is view
+        assert torch.equal(view, want)
+
+
+@gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize(('dtype', 'D', 'R'), [(BF, 128, 128), (HF, 64, 32), (FP, 36, 34)])
+def test_gradients_of_a_packed_batch(dtype, D, R, interleaved):
+    T, cu = 11, [0, 4, 4, 9]
+    cos, sin = _tables(30, R)
+    q, k = (_rows(1, T, h, D, dtype=dtype, seed=h).requires_grad_() for h in (3, 1))
+    offsets = torch.tensor([0, 7, 20], device=DEV)
+    at = torch.tensor([[0, 1, 2, 3, 20, 21, 22, 23, 24, -1, -1]])
+    out = _mods().rotary_embedding_qk(q, k, cos, sin, interleaved=interleaved, seqlen_offsets=offsets, cu_seqlens=torch.tensor(cu, device=DEV))
+    douts = [_rows(1, T, h, D, dtype=dtype, seed=10 + h) for h in (3, 1)]
+    grads = torch.autograd.grad(out, [q, k], douts)
+    for x, y, dy, dx in zip((q, k), out, douts, grads):
+        _near('y', y, *O.rotary(x.detach(), cos, sin, at, interleaved))
+        assert dx.dtype == dtype
+        _near('dx', dx, *O.rotary(dy, cos, sin, at, interleaved, back=True))
+
+
+@gpu
+def test_gradients_against_differences_and_of_gradients():
+    cos, sin = _tables(5, 8)
+    x = _rows(1, 5, 2, 10, dtype=FP).requires_grad_()
+    op = lambda x: _mods().rotary_embedding(x, cos, sin)
+    dy = _rows(1, 5, 2, 10, dtype=FP, seed=1)
+    (dx,) = torch.autograd.grad(op(x), x, dy)
+    for i in range(0, x.numel(), 7):
+        step = torch.zeros(x.numel(), device=DEV)
+        step[i] = 0.5                                            # (linear: any step; the difference of sums of 100 products in fp32)
+        there, back = ((op(x.detach() + s * step.view_as(x)).double() * dy.double()).sum() for s in (1, -1))
+        assert abs((there - back) - dx.flatten()[i].double()) < 1e-4
+    # a gradient of the gradient: the turn itself
+    v = _rows(1, 5, 2, 10, dtype=FP, seed=2).requires_grad_()
+    (dx,) = torch.autograd.grad(op(x), x, v, create_graph=True)
+    (dv,) = torch.autograd.grad(dx, v, dy)
+    assert torch.equal(dv, op(dy))
+
+
+@gpu
+def test_broadcast_and_absent_gradients():
+    cos, sin = _tables(4, 16)
+    q, k = (_rows(2, 4, 2, 16, dtype=BF, seed=s).requires_grad_() for s in (0, 1))
+    a, b = _mods().rotary_embedding_qk(q, k, cos, sin)
+    dq, dk = torch.autograd.grad(a.float().sum(), [q, k], allow_unused=True)     # (a gradient of ones without memory of its own; none for k)
+    assert dk is None
+    _near('dq', dq, *O.rotary(torch.ones_like(q), cos, sin, torch.arange(4).expand(2, 4), back=True))
+    shared = _rows(2, 4, 1, 16, dtype=BF).requires_grad_()
+    y = _mods().rotary_embedding(shared.expand(2, 4, 3, 16), cos, sin)
+    (dx,) = torch.autograd.grad(y, shared, torch.ones_like(y))
+    one, size = O.rotary(torch.ones(2, 4, 1, 16), cos, sin, torch.arange(4).expand(2, 4), back=True)
+    # (three equal gradients in bf16, added up by torch in bf16: two roundings more)
+    assert ((dx.double().cpu() - 3 * one).abs() <= 3 * 2.0 ** -8 * (3 * one).abs() + 9 * E * size).all()
+
+
+@gpu
+def test_in_place_under_autograd():
+    cos, sin = _tables(4, 16)
+    x = _rows(1, 4, 2, 16, dtype=FP)
+    leaf = x.clone().requires_grad_()
+    y = leaf * 1
+    z = _mods().rotary_embedding(y, cos, sin, inplace=True)
+    assert z.data_ptr() == y.data_ptr() and torch.equal(z, _mods().rotary_embedding(x, cos, sin))
+    (dx,) = torch.autograd.grad(z, leaf, x)
+    assert torch.equal(dx, torch.autograd.grad(_mods().rotary_embedding(leaf, cos, sin), leaf, x)[0])
+    with pytest.raises(RuntimeError):
+        _mods().rotary_embedding(leaf, cos, sin, inplace=True)
+    # what a graph has saved and is then turned in place cannot be used by its backward
+    saved = x.clone()
+    loss = (leaf * saved).sum()
+    _mods().rotary_embedding(saved, cos, sin, inplace=True)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
+@gpu
+def test_replayed_graph_of_a_training_step():
+    cos, sin = _tables(64, 64)
+    q, k, dq, dk = (_rows(2, 64, h, 64, dtype=BF, seed=i) for i, h in enumerate((4, 2, 4, 2)))
+    q.requires_grad_(), k.requires_grad_()
+
+    def step():
+        out = _mods().rotary_embedding_qk(q, k, cos, sin, interleaved=True)
+        return [*(y.detach() for y in out), *torch.autograd.grad(out, [q, k], [dq, dk])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(3):
+        with torch.no_grad():
+            for t in (q, k, dq, dk):
+                t.copy_(_rows(*t.shape, dtype=BF, seed=20 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+@gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_module(interleaved):
+    mods = _mods()
+    rope = mods.RotaryEmbedding(64, interleaved=interleaved)
+    q, k = _rows(2, 20, 4, 96, dtype=BF), _rows(2, 20, 2, 96, dtype=BF, seed=1)
+    angle = lambda n: torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    for offset in (0, 100000):
+        a, b = rope(q, k, seqlen_offset=offset)
+        t = angle(offset + 20)
+        at = torch.arange(20).expand(2, 20) + offset
+        cos, sin = t.cos().float(), t.sin().float()
+        _near('q', a, *O.rotary(q, cos, sin, at, interleaved))
+        _near('k', b, *O.rotary(k, cos, sin, at, interleaved))
+    one = rope(q[:, :1], k[:, :1], seqlen_offset=torch.tensor([5, 9], device=DEV), max_seqlen=10)
+    _near('step', one[0], *O.rotary(q[:, :1], cos, sin, torch.tensor([[5], [9]]), interleaved))
+    assert not rope.state_dict() and rope._tables[0].shape[0] == 100020
+    with pytest.raises(ValueError, match='max_seqlen'):
+        rope(q, k, seqlen_offset=torch.tensor([5, 9], device=DEV))
+    # the keys' scale is the inverse of the queries'
+    x = mods.RotaryEmbedding(64, scale_base=512.0, interleaved=interleaved)
+    a, b = x(q.float(), k.float())
+    s = ((torch.arange(0, 64, 2, dtype=torch.float64) + 0.4 * 64) / (1.4 * 64)) ** ((torch.arange(20, dtype=torch.float64) - 10) / 512)[:, None]
+    t = angle(20)
+    at = torch.arange(20).expand(2, 20)
+    _near('q', a, *O.rotary(q.float(), (t.cos() * s).float(), (t.sin() * s).float(), at, interleaved))
+    _near('k', b, *O.rotary(k.float(), (t.cos() / s).float(), (t.sin() / s).float(), at, interleaved))
+
+
+@gpu
+def test_module_under_capture_wants_its_tables_first():
+    rope = _mods().RotaryEmbedding(64)
+    q, k = _rows(1, 8, 2, 64, dtype=BF), _rows(1, 8, 1, 64, dtype=BF)
+    rope(q, k)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match='before the capture'):
+            rope(q, k, seqlen_offset=100)
+        held = rope(q, k)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(held, rope(q, k)))
+
+
+@pytest.mark.parametrize('kind', ['linear', 'ntk', 'yarn'])
+def test_frequencies_of_stretched_contexts(kind):
+    """What each of them is for: the slowest pair turns `factor` times as slowly, and, but for the first, the fastest as fast as before."""
+    from fla_hip.modules.rotary import rotary_frequencies
+    plain, one = rotary_frequencies(128)
+    inv, m = rotary_frequencies(128, scaling=dict(type=kind, factor=4.0, original_max_position_embeddings=8192))
+    assert one == 1.0 and inv.dtype == torch.float64 and torch.equal(plain, 10000.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128))
+    assert inv[-1].item() == pytest.approx(plain[-1].item() / 4, rel=1e-12)
+    assert inv[0].item() == pytest.approx(plain[0].item() / (4 if kind == 'linear' else 1), rel=1e-12)
+    assert (inv <= plain).all() and (inv >= plain / 4 * (1 - 1e-12)).all()
+    assert m == (pytest.approx(0.1 * math.log(4) + 1) if kind == 'yarn' else 1.0)
+    if kind == 'yarn':
+        turns = 8192 * plain / (2 * math.pi)
+        assert torch.equal(inv[turns > 33], plain[turns > 33]) and torch.allclose(inv[turns < 0.8], plain[turns < 0.8] / 4, rtol=1e-12)
+
+
+@pytest.mark.parametrize('scaling', [dict(type='linear', factor=0.5), dict(type='other', factor=2.0), dict(type='linear', factor=math.nan)])
+def test_frequencies_refuse(scaling):
+    from fla_hip.modules.rotary import rotary_frequencies
+    with pytest.raises(ValueError):
+        rotary_frequencies(64, scaling=scaling)
+    with pytest.raises(ValueError):
+        rotary_frequencies(63)
+
+
+class _Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    """The library is a stand-in that keeps record: nothing may be launched for a call that is refused."""
+    from fla_hip import _lib
+    from fla_hip.modules import rotary
+    from fla_hip.ops.gated_delta_rule import _common
+    lib = _Library()
+    monkeypatch.setattr(_lib, 'load', lambda: lib)
+    monkeypatch.setattr(_common, 'current_device', lambda: None)
+    monkeypatch.setattr(_common, 'current_stream_ptr', lambda dev: 0)
+    monkeypatch.setattr(rotary, 'require_gpu', lambda x, *_: x.device)
+    return lib
+
+
+def test_refusals(lib):
+    op = _mods().rotary_embedding
+    x, cos = torch.zeros(2, 4, 3, 16, dtype=BF), torch.zeros(8, 8)
+    assert op(x, cos, cos).shape == x.shape and lib.calls == ['gdn_rotary']
+    bad = [
+        (ValueError, lambda: op(x[0], cos, cos)), (ValueError, lambda: op(x, cos[0], cos[0])), (ValueError, lambda: op(x, cos, cos[:4])),
+        (ValueError, lambda: op(x, torch.zeros(8, 9), torch.zeros(8, 9))), (ValueError, lambda: op(x, torch.zeros(8, 0), torch.zeros(8, 0))),
+        (ValueError, lambda: op(x, cos[:3], cos[:3])), (ValueError, lambda: op(x, cos, cos, seqlen_offsets=5)), (ValueError, lambda: op(x, cos, cos, seqlen_offsets=-1)),
+        (ValueError, lambda: op(x, cos, cos, seqlen_offsets=torch.zeros(3, dtype=torch.int32))), (ValueError, lambda: op(x, cos, cos, seqlen_offsets=torch.zeros(2))),
+        (ValueError, lambda: op(x, cos, cos, positions=torch.zeros(4, dtype=torch.int32))), (ValueError, lambda: op(x, cos, cos, positions=torch.zeros(2, 4, dtype=torch.int32), seqlen_offsets=1)),
+        (ValueError, lambda: op(x, cos, cos, cu_seqlens=torch.tensor([0, 4]))), (ValueError, lambda: op(x[:1], cos, cos, cu_seqlens=torch.tensor([0, 5]))),
+        (ValueError, lambda: op(x[:1], cos, cos, cu_seqlens=torch.tensor([0]))), (ValueError, lambda: op(x[:1], cos, cos, cu_seqlens=torch.tensor([0, 3, 2]))),
+        (ValueError, lambda: op(x.transpose(2, 3).contiguous().transpose(2, 3), cos, cos, inplace=True)), (ValueError, lambda: op(x[:, :, :1].expand(2, 4, 3, 16), cos, cos, inplace=True)),
+        (NotImplementedError, lambda: op(x.double(), cos, cos)), (NotImplementedError, lambda: op(x, cos.clone().requires_grad_(), cos)),
+        (ValueError, lambda: _mods().rotary_embedding_qk(x, x[:1], cos, cos)), (ValueError, lambda: _mods().rotary_embedding_qk(x, x.float(), cos, cos)),
+        (ValueError, lambda: _mods().rotary_embedding_qk(x, x[..., :8], cos, cos)),
+    ]
+    for error, call in bad:
+        with pytest.raises(error):
+            call()
+    assert lib.calls == ['gdn_rotary']
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            op(torch.autograd.forward_ad.make_dual(x, x), cos, cos)
+    with pytest.raises(NotImplementedError):
+        _mods().RotaryEmbedding(16, pos_idx_in_fp32=False)
+
+
+def test_no_cpu_path():
+    with pytest.raises(RuntimeError, match='ROCm GPU'):
+        _mods().rotary_embedding(torch.zeros(1, 1, 1, 8), torch.zeros(1, 4), torch.zeros(1, 4))
+
+
+def test_library_refuses():
+    """Sizes that no kernel is made for, at the C entry: an error before any launch."""
+    import ctypes
+    from fla_hip import _lib
+    lib = _lib.load()
+    rows = _lib.RotaryRows(1, 1, 1)
+
+    def call(**kw):
+        c = _lib.RotaryCall(cos=16, sin=16, table_rows=4, table_stride=8, B=1, T=1, N=1, D=16, rotary_dim=16, dtype=0, table_dtype=2)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return lib.gdn_rotary(ctypes.byref(rows), 1, ctypes.byref(c), None)
+
+    invalid = [dict(B=-1), dict(T=-1), dict(D=0), dict(rotary_dim=15), dict(rotary_dim=18), dict(table_stride=7), dict(cos=None), dict(cu_seqlens=16, B=2), dict(cu_seqlens=16, N=0), dict(table_dtype=1)]
+    assert [call(**kw) for kw in invalid] == [_lib.GDN_ERR_INVALID] * len(invalid)
+    unsupported = [dict(D=1026), dict(dtype=3), dict(D=17, flags=_lib.ROTARY_INTERLEAVED)]
+    assert [call(**kw) for kw in unsupported] == [_lib.GDN_ERR_UNSUPPORTED] * len(unsupported)
+    assert lib.gdn_rotary(ctypes.byref(rows), 3, ctypes.byref(_lib.RotaryCall(B=1, T=1, D=16)), None) == _lib.GDN_ERR_INVALID
+    assert lib.gdn_rotary(ctypes.byref(rows), 1, None, None) == _lib.GDN_ERR_INVALID
+    assert call(B=0) == call(T=0) == _lib.GDN_OK
