@@ -2,95 +2,467 @@
 //
 //   o_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),   s_ij = scale q_i . k_j over the keys that row i sees, m_i their maximum
 //
-// One pass over the keys with the running maximum and sum: a wave for a row and a head, a lane for a key of 64, then for the head's elements.
+// One pass over the keys with the running maximum and sum.  The rows of a sequence that share a head of the cache (its tokens times the heads of a group, row m = token * group +
+// head) stand side by side, so a key is read once for all of them.  Both products have the rows as columns:
+//
+//   S^T [keys x rows] = K Q^T,   O^T [elements x rows] += V^T P^T,
+//
+// so a lane has the scores of one row, which are the second product's operand where they are (the order of the keys in a contraction is free, as long as V has
+// the same), the row's statistics are the lane's, and nothing goes through LDS: K is the first operand as it lies in memory; a lane asks for eight elements of
+// eight keys of V and exchanges them in its registers (one v_perm_b32 per pair).
+//
+// A wave takes tiles of 32 keys by itself, without barriers: K of the next tile is asked for when the scores of this one are formed, V of the next when it is added up, the
+// pages' numbers a tile earlier.  The sequence's keys are shared out over `splits` workgroups and their waves; waves are joined through LDS at the end,
+// workgroups by paged_attn_join_kernel.  The memory system bounds it up to 128 rows.
 #include "gdn_paged.h"
+#include "gdn_chunk_common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace gdn {
 
-constexpr int PA_MAX_DIM = 256;
+constexpr int PA_MAX_DIM = 256, PA_TILE = 32;
 
 struct PagedAttnParams {
     PagedCache cache;
     const void* q; void* o; const void* cu; const uint8_t* mask;
+    float* part_o; float* part_ml;           // [splits][B T HQ][D], [splits][B T HQ][2]: sums, maximum and sum of the weights of a part of the keys
     int64_t qb, qt, qh;
-    int64_t mask_seq, mask_row, mask_cols;
-    int64_t B, T, N;
-    int HQ, HK, D;
-    float scale;
+    int64_t mask_seq, mask_row;
+    int64_t T, total;                        // rows of a sequence (dense), of the batch
+    uint32_t page_magic; int page_shift;     // slot / page_size = slot * page_magic >> page_shift
+    int N, HQ, HK, D, group, mask_cols;
+    int tiles, splits, row_groups;
+    float scale2;                            // scale log2(e)
     bool cu_i32;
 };
 
-template <typename T>
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnParams p) {
-    __shared__ float sq[PA_MAX_DIM], sp[64];
-    __shared__ int64_t at[64];
-    const int lane = threadIdx.x;
-    const int64_t token = blockIdx.x;
-    const int h = blockIdx.y, hk = h / (p.HQ / p.HK);
-    const int64_t b = token / p.T, t = token - b * p.T;
-    int64_t n = b, i = t, rows = p.T;
+typedef uint16_t pa_half __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint16_t pa_whole __attribute__((ext_vector_type(8), aligned(2)));
+
+template <typename T> __device__ __forceinline__ bool not_a_number(uint16_t bits) {
+    constexpr uint16_t EXP = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
+    return (bits & EXP) == EXP;
+}
+
+// What a step's sequence is.
+struct PagedSequence {
+    int64_t first;                           // its first row in the batch
+    int rows;
+    int64_t context;
+    int keys;                                // slots that may be seen: [0, keys)
+};
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedAttnParams& p, int64_t n) {
+    PagedSequence s;
+    s.first = n * p.T;
+    int64_t rows = p.T;
     if (p.cu) {
-        n = sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); });
-        if (n < 0) {
-            for (int d = lane; d < p.D; d += 64) ((T*)p.o)[(token * p.HQ + h) * p.D + d] = (T)0.f;
-            return;
-        }
-        const int64_t first = load_index(p.cu, n, p.cu_i32);
-        i = token - first;
-        rows = load_index(p.cu, n + 1, p.cu_i32) - first;
+        s.first = load_index_uniform(p.cu, n, p.cu_i32);
+        rows = load_index_uniform(p.cu, n + 1, p.cu_i32) - s.first;
+        if (s.first < 0 || s.first > p.total) { s.first = 0; rows = 0; }
+        rows = min(rows, p.total - s.first);
     }
-    const T* q = (const T*)p.q + b * p.qb + t * p.qt + h * p.qh;
-    for (int d = lane; d < p.D; d += 64) sq[d] = (float)q[d];
-    __syncthreads();
-    const int64_t context = load_index(p.cache.context, n, p.cache.context_i32);
-    const uint8_t* mask = p.mask ? p.mask + (p.cu ? token * p.mask_row : n * p.mask_seq + i * p.mask_row) : nullptr;
-    const int64_t keys = std::min<int64_t>(context + rows, p.cache.pages.capacity);
-    float m = -INFINITY, l = 0.f, acc[PA_MAX_DIM / 64] = {};
-    for (int64_t from = 0; from < keys; from += 64) {
-        const int64_t key = from + lane, fresh = key - context;
-        bool sees = key < keys;
-        if (sees && fresh >= 0) sees = mask ? fresh < p.mask_cols && mask[fresh] : fresh <= i;
-        const int page = sees ? page_of(p.cache.pages, n, key) : -1;
-        sees = page >= 0;
-        float s = -INFINITY;
-        if (sees) {
-            const int64_t in_page = key % p.cache.pages.page_size;
-            const T* k = (const T*)p.cache.k + page * p.cache.k_page + in_page * p.cache.k_slot + hk * p.cache.k_head;
-            s = 0.f;
-            for (int d = 0; d < p.D; ++d) s += sq[d] * (float)k[d];
-            s *= p.scale;
-            at[lane] = page * p.cache.v_page + in_page * p.cache.v_slot + hk * p.cache.v_head;
+    s.rows = (int)max(rows, (int64_t)0);
+    s.context = load_index_uniform(p.cache.context, n, p.cache.context_i32);
+    const int64_t capacity = p.cache.pages.pages > 0 ? p.cache.pages.capacity : 0;
+    // (in this order: a context near the end of 64 bits does not overflow)
+    s.context = max(min(s.context, capacity), (int64_t)-0x40000000);
+    s.keys = (int)max(min(s.context + s.rows, capacity), (int64_t)0);
+    return s;
+}
+
+// The places of a tile's keys.  UNIFORM (pages of a multiple of 16 slots): a page for each 16 keys, the same for all lanes.  Else a place for each key, in lane key % 32.
+template <bool UNIFORM> struct TilePlaces;
+template <> struct TilePlaces<true> {
+    int64_t k[2], v[2];                      // first key of either half, in elements
+    uint32_t there;                          // bit per key: its page is one of the cache
+};
+template <> struct TilePlaces<false> {
+    int64_t k, v;
+    uint32_t there;
+};
+
+template <typename T, int DT, int RT, bool UNIFORM>
+struct PagedWave {
+    typedef typename Mma<T>::V8 V8;
+    static constexpr int LD = DT + 4;
+    static constexpr int KS = DT / 32, VE = DT >= 128 ? 8 : 4, VC = DT / 16 / VE, MT = DT / 16;     // steps of a score; elements of V at a place, places, products per row tile
+    const PagedAttnParams& p;
+    const PagedSequence& s;
+    const int64_t n;
+    const int hk, lane, c16, g;
+    typedef std::conditional_t<VE == 8, pa_whole, pa_half> VPiece;
+    V8 q[RT][KS], k[2][KS];
+    VPiece v[8][VC];
+    f32x4 o[RT][MT];
+    float m[RT], l[RT];
+    int token[RT];                           // row of the sequence that the lane's column is; -1: none
+    bool odd;                                // infinities and NaN of V are in LDS
+    float* const sums;                       // the wave's place there, [16 RT][LD]
+
+    __device__ __forceinline__ PagedWave(const PagedAttnParams& p, const PagedSequence& s, int64_t n, int hk, float* sums)
+        : p(p), s(s), n(n), hk(hk), lane(threadIdx.x & 63), c16(lane & 15), g(lane >> 4), odd(false), sums(sums) {}
+
+    __device__ __forceinline__ int page_index(int slot) const { return (int)(((uint64_t)(uint32_t)slot * p.page_magic) >> p.page_shift); }
+
+    __device__ __forceinline__ TilePlaces<UNIFORM> places(int tile) const {
+        TilePlaces<UNIFORM> t;
+        const PagedCache& c = p.cache;
+        if constexpr (UNIFORM) {
+            t.there = 0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int slot = tile * PA_TILE + 16 * b, index = page_index(slot);
+                int page = -1;
+                if (slot < s.keys) page = (int)load_index_uniform(c.pages.table, n * c.pages.table_stride + index, true);
+                const bool there = page >= 0 && page < c.pages.pages;
+                const int inside = there ? slot - index * c.pages.page_size : 0;
+                page = there ? page : 0;
+                t.there |= there ? 0xffffu << 16 * b : 0;
+                t.k[b] = page * c.k_page + inside * c.k_slot + hk * c.k_head;
+                t.v[b] = page * c.v_page + inside * c.v_slot + hk * c.v_head;
+            }
         } else {
-            at[lane] = -1;
+            const int slot = tile * PA_TILE + (lane & 31), index = page_index(slot);
+            int page = -1;
+            if (slot < s.keys) page = c.pages.table[n * c.pages.table_stride + index];
+            const bool there = page >= 0 && page < c.pages.pages;
+            const int inside = there ? slot - index * c.pages.page_size : 0;
+            page = there ? page : 0;
+            t.there = (uint32_t)__ballot(there);
+            t.k = page * c.k_page + inside * c.k_slot + hk * c.k_head;
+            t.v = page * c.v_page + inside * c.v_slot + hk * c.v_head;
         }
-        float most = s;
-        for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x, 64));
-        const float now = fmaxf(m, most);
-        // (no maximum yet: nothing is seen, or what is seen is not a number and makes the row's sums so)
-        const float base = now == -INFINITY ? 0.f : now, keep = expf(m - base), w = sees ? expf(s - base) : 0.f;
-        float sum = w;
-        for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x, 64);
-        l = l * keep + sum;
-        m = now;
-        __syncthreads();
-        sp[lane] = w;
-        __syncthreads();
+        return t;
+    }
+
+    __device__ __forceinline__ void load_k(const TilePlaces<UNIFORM>& t) {
 #pragma unroll
-        for (int e = 0; e < PA_MAX_DIM / 64; ++e) acc[e] *= keep;
-        for (int j = 0; j < 64; ++j) {
-            if (at[j] < 0) continue;
-            const T* v = (const T*)p.cache.v + at[j];
+        for (int b = 0; b < 2; ++b) {
+            const uint16_t* at;
+            if constexpr (UNIFORM) at = (const uint16_t*)p.cache.k + t.k[b] + (uint32_t)(c16 * (int)p.cache.k_slot + 8 * g);
+            else at = (const uint16_t*)p.cache.k + __shfl(t.k, 16 * b + c16, 64) + 8 * g;
 #pragma unroll
-            for (int e = 0; e < PA_MAX_DIM / 64; ++e)
-                if (e * 64 + lane < p.D) acc[e] += sp[j] * (float)v[e * 64 + lane];
+            for (int ks = 0; ks < KS; ++ks) {
+                pa_whole x = {};
+                if (32 * ks + 8 * g < p.D) x = *(const pa_whole*)(at + 32 * ks);
+                k[b][ks] = __builtin_bit_cast(V8, x);
+            }
+        }
+    }
+
+    // Lane (c16, g): elements VE c16 .. of keys 16 b + 4 g + e, which are contraction indices 8 g + 4 b + e.
+    __device__ __forceinline__ void load_v(const TilePlaces<UNIFORM>& t) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint16_t* at;
+                if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + (uint32_t)((4 * g + e) * (int)p.cache.v_slot + VE * c16);
+                else at = (const uint16_t*)p.cache.v + __shfl(t.v, 16 * b + 4 * g + e, 64) + VE * c16;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    VPiece x = {};
+                    if (128 * c + VE * c16 < p.D) x = *(const VPiece*)(at + 128 * c);
+                    v[4 * b + e][c] = x;
+                }
+            }
+    }
+
+    __device__ __forceinline__ void start(int row0) {
+        const int rows = s.rows * p.group;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = row0 + 16 * r + c16;
+            token[r] = row < rows ? row / p.group : -1;
+            const int h = hk * p.group + (row < rows ? row - token[r] * p.group : 0);
+            const int64_t t = token[r] < 0 ? 0 : token[r];
+            const uint16_t* at = (const uint16_t*)p.q + (p.cu ? (s.first + t) * p.qt : n * p.qb + t * p.qt) + h * p.qh + 8 * g;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                pa_whole x = {};
+                if (token[r] >= 0 && 32 * ks + 8 * g < p.D) x = *(const pa_whole*)(at + 32 * ks);
+                q[r][ks] = __builtin_bit_cast(V8, x);
+            }
+            m[r] = -INFINITY; l[r] = 0.f;
+#pragma unroll
+            for (int t2 = 0; t2 < MT; ++t2) o[r][t2] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // Which keys of a tile row token[r] sees of those whose pages are there: bit 4 b + e for key 16 b + 4 g + e.
+    __device__ __forceinline__ uint32_t seen(int r, int tile, uint32_t there) const {
+        const int fresh = (int)(tile * PA_TILE + 4 * g - s.context), most = p.mask ? min(p.mask_cols, s.rows) : token[r] + 1;
+        const uint8_t* mask = p.mask;
+        if (mask) mask += (p.cu ? (s.first + token[r]) * p.mask_row : n * p.mask_seq + token[r] * p.mask_row);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = 16 * (i / 4) + i % 4, f = fresh + at;
+            bool is = f < most;
+            if (mask && is && f >= 0 && token[r] >= 0) is = mask[f] != 0;
+            bits |= is && there >> (4 * g + at) & 1 ? 1u << i : 0;
+        }
+        return bits;
+    }
+
+    // The scores of a tile become weights in place: x[r][b][e] of key 16 b + 4 g + e.
+    template <typename Next>
+    __device__ __forceinline__ void tile(int tile, const TilePlaces<UNIFORM>& at, Next&& next_k) {
+        f32x4 x[RT][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                x[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) x[r][b] = Mma<T>::run(k[b][ks], q[r][ks], x[r][b]);
+                x[r][b] *= p.scale2;
+            }
+        next_k();
+        // The keys of the context whose pages are there are seen by every row; the tiles behind them are few.
+        const bool whole = (int64_t)(tile + 1) * PA_TILE <= s.context && at.there == 0xffffffffu;
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t bits = seen(r, tile, at.there);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[r][i / 4][i % 4] = bits >> i & 1 ? x[r][i / 4][i % 4] : -INFINITY;
+            }
+        }
+        V8 w[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    most = fmaxf(most, x[r][b][e]);
+                }
+            most = fmaxf(most, __shfl_xor(most, 16, 64));
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            if (__any(most > m[r])) {
+                const float now = fmaxf(m[r], most), keep = __builtin_amdgcn_exp2f(m[r] - (now == -INFINITY ? 0.f : now));
+                m[r] = now;
+                l[r] *= keep;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) o[r][t] *= keep;
+            }
+            // (no maximum yet: nothing is seen, or what is seen is not a number and makes the row's sums so)
+            const float base = m[r] == -INFINITY ? 0.f : m[r];
+            float sum = 0.f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = __builtin_amdgcn_exp2f(x[r][b][e] - base);
+                    sum += y;
+                    w[r][4 * b + e] = (T)y;
+                }
+            l[r] += sum;
+        }
+        if (!whole && __any(odd_values())) clean(w, at);
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int t = 0; t < VE; ++t) {
+                pa_whole a;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) a[j] = v[j][c][t];
+                const V8 va = __builtin_bit_cast(V8, a);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) o[r][c * VE + t] = Mma<T>::run(va, w[r], o[r][c * VE + t]);
+            }
+    }
+
+    // Infinities and NaN in V, in tiles whose keys not every row sees: a weight of zero does not keep them out of a product.
+    __device__ __forceinline__ bool odd_values() const {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int t = 0; t < VE; ++t) odd = odd || not_a_number<T>(v[j][c][t]);
+        return odd;
+    }
+    // They are taken out of V and added to the rows that see the key in the wave's place in LDS: sums of infinities and NaN, which no later maximum changes.
+    __device__ __forceinline__ void clean(const V8 (&w)[RT], const TilePlaces<UNIFORM>& at) {
+        if (!odd) {
+            for (int i = lane; i < 16 * RT * LD; i += 64) sums[i] = 0.f;
+            odd = true;
+        }
+        uint32_t rows[RT];                                                  // the keys that the lane's row has weights for
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            rows[r] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rows[r] |= (float)w[r][i] != 0.f ? 1u << (16 * (i / 4) + 4 * g + i % 4) : 0;
+            rows[r] |= __shfl_xor(rows[r], 16, 64);
+            rows[r] |= __shfl_xor(rows[r], 32, 64);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int t = 0; t < VE; ++t) v[j][c][t] = not_a_number<T>(v[j][c][t]) ? (uint16_t)0 : v[j][c][t];
+#pragma nounroll
+        for (int key = 0; key < PA_TILE; ++key) {
+            if (!(at.there >> key & 1)) continue;
+            const uint16_t* from;
+            if constexpr (UNIFORM) from = (const uint16_t*)p.cache.v + (key < 16 ? at.v[0] : at.v[1]) + (key & 15) * p.cache.v_slot;
+            else from = (const uint16_t*)p.cache.v + __shfl(at.v, key, 64);
+#pragma nounroll
+            for (int d0 = 0; d0 < p.D; d0 += 64) {
+                const int d = d0 + lane;
+                const uint16_t bits = d < p.D ? from[d] : (uint16_t)0;
+                const bool is = not_a_number<T>(bits);
+                if (!__any(is)) continue;
+                const float value = (float)__builtin_bit_cast(T, bits);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma nounroll
+                    for (int row = 0; row < 16; ++row)
+                        if ((__shfl(rows[r], row, 64) >> key & 1) && is) sums[(16 * r + row) * LD + d] += value;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void run(int first, int last, int step) {
+        if (first >= last) return;
+        TilePlaces<UNIFORM> now = places(first), next = places(first + step);
+        load_k(now);
+        load_v(now);
+        for (int t = first; t < last; t += step) {
+            const bool more = t + step < last;
+            tile(t, now, [&] { if (more) load_k(next); });
+            if (more) load_v(next);
+            now = next;
+            next = places(t + 2 * step);
+        }
+    }
+};
+
+template <typename T, int DT, int RT, bool UNIFORM>
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
+    typedef PagedWave<T, DT, RT, UNIFORM> Wave;
+    constexpr int VE = Wave::VE, LD = Wave::LD;
+    extern __shared__ float lds[];                               // [4 waves][16 RT][LD], then [4 waves][16 RT][2]
+    const int64_t n = blockIdx.z;
+    const int hk = blockIdx.y, split = blockIdx.x % p.splits, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int rg = wave % p.row_groups, kg = wave / p.row_groups, key_groups = 4 / p.row_groups;
+    const PagedSequence s = paged_sequence(p, n);
+    if (p.cu && blockIdx.x == 0) {
+        // rows of no sequence
+        if (n == 0 || n == p.N - 1) {
+            const int64_t from = n == 0 ? 0 : max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), to = n == 0 ? min(load_index_uniform(p.cu, 0, p.cu_i32), p.total) : p.total;
+            auto clear = [&](int64_t from, int64_t to) {
+                const int width = p.group * p.D;
+                for (int64_t row = from; row < to; ++row)
+                    for (int d = threadIdx.x; d < width; d += 256) ((T*)p.o)[(row * p.HQ + hk * p.group) * p.D + d] = (T)0.f;
+            };
+            clear(from, to);
+            if (n == 0 && p.N == 1) clear(max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), p.total);
+        }
+    }
+    const int all = (s.keys + PA_TILE - 1) / PA_TILE, rows = s.rows * p.group, height = 16 * RT * p.row_groups;
+    const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+    for (int tile = blockIdx.x / p.splits; tile * height < rows; tile += p.tiles) {
+        Wave w(p, s, n, hk, lds + wave * 16 * RT * LD);
+        const int row0 = tile * height + rg * 16 * RT;
+        w.start(row0);
+        w.run(t0 + kg, t1, key_groups);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            w.l[r] += __shfl_xor(w.l[r], 16, 64);
+            w.l[r] += __shfl_xor(w.l[r], 32, 64);
+        }
+        // The waves that share rows, joined: each leaves its sums with its maximum.
+        float* const ml = lds + 4 * 16 * RT * LD;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = wave * 16 * RT + 16 * r + w.c16;
+#pragma unroll
+            for (int c = 0; c < Wave::VC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int t = 0; t < VE; t += 4) {
+                        f32x4* const to = (f32x4*)(lds + row * LD + 128 * c + VE * (4 * w.g + e) + t);
+                        f32x4 sum = {w.o[r][c * VE + t][e], w.o[r][c * VE + t + 1][e], w.o[r][c * VE + t + 2][e], w.o[r][c * VE + t + 3][e]};
+                        if (w.odd) sum += *to;
+                        *to = sum;
+                    }
+            if (w.g == 0) { ml[2 * row] = w.m[r]; ml[2 * row + 1] = w.l[r]; }
+        }
+        __syncthreads();
+        constexpr int PIECES = DT / 4;
+        for (int i = threadIdx.x; i < height * PIECES; i += 256) {
+            const int row = i / PIECES, d = 4 * (i % PIECES), at = row + tile * height;
+            if (at >= rows || d >= p.D) continue;
+            float m = -INFINITY;
+            for (int k = 0; k < key_groups; ++k) m = fmaxf(m, ml[2 * (row + k * height)]);
+            const float base = m == -INFINITY ? 0.f : m;
+            float l = 0.f;
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < key_groups; ++k) {
+                const int from = row + k * height;
+                const float keep = __builtin_amdgcn_exp2f(ml[2 * from] - base);
+                l += ml[2 * from + 1] * keep;
+                sum += *(const f32x4*)(lds + from * LD + d) * keep;
+            }
+            const int token = at / p.group;
+            const int64_t out = (s.first + token) * p.HQ + hk * p.group + (at - token * p.group);
+            if (p.splits == 1) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                typedef T piece __attribute__((ext_vector_type(4)));
+                *(piece*)((T*)p.o + out * p.D + d) = piece{(T)(sum[0] * inv), (T)(sum[1] * inv), (T)(sum[2] * inv), (T)(sum[3] * inv)};
+            } else {
+                const int64_t part = split * (p.total * p.HQ) + out;
+                *(f32x4*)(p.part_o + part * p.D + d) = sum;
+                if (d == 0) { p.part_ml[2 * part] = m; p.part_ml[2 * part + 1] = l; }
+            }
         }
         __syncthreads();
     }
-    T* o = (T*)p.o + (token * p.HQ + h) * p.D;
+}
+
+// The parts of a row's keys, joined: a wave per row, a part's weight in the lane of its number.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnParams p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64, rows = p.total * p.HQ;
+    if (row >= rows) return;
+    if (p.cu) {
+        const int64_t token = row / p.HQ;
+        if (sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); }) < 0) return;
+    }
+    float m = -INFINITY, l = 0.f;
+    if (lane < p.splits) {
+        const float* ml = p.part_ml + 2 * (lane * rows + row);
+        m = ml[0]; l = ml[1];
+    }
+    float most = m;
 #pragma unroll
-    for (int e = 0; e < PA_MAX_DIM / 64; ++e)
-        if (e * 64 + lane < p.D) o[e * 64 + lane] = (T)(l == 0.f ? 0.f : acc[e] / l);
+    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+    const float keep = __builtin_amdgcn_exp2f(m - (most == -INFINITY ? 0.f : most));
+    l *= keep;
+    float all = l;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
+    const uint64_t some = __ballot(lane < p.splits && l != 0.f);
+    const int d = 4 * lane;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (uint64_t left = some; left; left &= left - 1) {
+        const int part = __builtin_ctzll(left);
+        const float weight = __shfl(keep, part, 64);
+        if (d < p.D) sum += *(const f32x4*)(p.part_o + (part * rows + row) * p.D + d) * weight;
+    }
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    typedef T piece __attribute__((ext_vector_type(4)));
+    if (d < p.D) *(piece*)((T*)p.o + row * p.D + d) = piece{(T)(sum[0] * inv), (T)(sum[1] * inv), (T)(sum[2] * inv), (T)(sum[3] * inv)};
 }
 
 static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_paged_attn_call* c, PagedCache& out) {
@@ -98,15 +470,38 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     const int rc = check_cache(who, cache, c->N, out);
     if (rc != GDN_OK) return rc;
     GDN_CHECK_ARG(c->HQ % cache->heads == 0, GDN_ERR_INVALID, "%s: the queries' heads are a multiple of the cache's", who);
-    GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of up to %d elements", who, PA_MAX_DIM);
+    GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM && cache->dim % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of a multiple of 8 up to %d elements", who, PA_MAX_DIM);
+    GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->T * c->HQ < (1ll << 31) && cache->heads <= 65535 && c->N <= 65535 && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
+                  "%s: up to 65535 sequences and heads of the cache, rows times heads below 2^31", who);
     return GDN_OK;
+}
+
+// How the work is cut.
+struct PagedAttnPlan { int dim, row_tiles, row_groups, tiles, splits; };
+static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_attn_call* c) {
+    PagedAttnPlan plan;
+    const int64_t rows = std::max<int64_t>(1, std::min(c->max_rows, c->T)) * (c->HQ / cache->heads);
+    plan.dim = cache->dim <= 64 ? 64 : cache->dim <= 128 ? 128 : 256;
+    plan.row_tiles = plan.dim == 256 || rows <= 16 ? 1 : 2;
+    const int64_t each = 16 * plan.row_tiles;
+    plan.row_groups = rows <= each ? 1 : rows <= 2 * each ? 2 : 4;
+    plan.tiles = (int)((rows + each * plan.row_groups - 1) / (each * plan.row_groups));
+    const int64_t units = std::max<int64_t>(1, c->N * cache->heads * plan.tiles), key_tiles = (cache->table_cols * cache->page_size + PA_TILE - 1) / PA_TILE;
+    const int64_t most = std::max<int64_t>(1, key_tiles / (2 * (4 / plan.row_groups)));
+    plan.splits = (int)std::min<int64_t>(std::min<int64_t>(64, most), std::max<int64_t>(1, (2048 + units - 1) / units));
+    return plan;
 }
 
 }  // namespace gdn
 
 using namespace gdn;
 
-extern "C" size_t gdn_paged_attn_workspace_bytes(const gdn_paged_cache*, const gdn_paged_attn_call*) { return 0; }
+extern "C" size_t gdn_paged_attn_workspace_bytes(const gdn_paged_cache* cache, const gdn_paged_attn_call* c) {
+    PagedCache view;
+    if (check_attn("gdn_paged_attn_workspace_bytes", cache, c, view) != GDN_OK || c->B * c->T * c->HQ == 0) return 0;
+    const PagedAttnPlan plan = attn_plan(cache, c);
+    return plan.splits == 1 ? 0 : (size_t)plan.splits * (size_t)(c->B * c->T * c->HQ) * (size_t)(cache->dim + 2) * sizeof(float);
+}
 
 extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "gdn_paged_attn";
@@ -115,13 +510,44 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     if (rc != GDN_OK) return rc;
     if (c->B * c->T * c->HQ == 0) return GDN_OK;
     GDN_CHECK_ARG(c->q && c->o, GDN_ERR_INVALID, "%s: missing tensors", who);
-    GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->HQ <= 65535, GDN_ERR_UNSUPPORTED, "%s: too many rows", who);
+    const PagedAttnPlan plan = attn_plan(cache, c);
+    const size_t need = gdn_paged_attn_workspace_bytes(cache, c);
+    GDN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), GDN_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned", who, need);
     p.q = c->q; p.o = c->o; p.cu = c->cu_seqlens; p.mask = c->mask;
     p.qb = c->q_stride[0]; p.qt = c->q_stride[1]; p.qh = c->q_stride[2];
-    p.mask_seq = c->mask_seq_stride; p.mask_row = c->mask_row_stride; p.mask_cols = c->mask_cols;
-    p.B = c->B; p.T = c->T; p.N = c->N; p.HQ = (int)c->HQ; p.HK = (int)cache->heads; p.D = (int)cache->dim; p.scale = c->scale; p.cu_i32 = c->flags & GDN_FLAG_CU_INT32;
-    const dim3 grid((unsigned)(c->B * c->T), (unsigned)c->HQ);
-    if (cache->dtype == GDN_DTYPE_BF16) hipLaunchKernelGGL(paged_attn_kernel<bf16_t>, grid, dim3(64), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(paged_attn_kernel<f16_t>, grid, dim3(64), 0, (hipStream_t)stream, p);
-    return check_launch("paged_attn_kernel");
+    p.mask_seq = c->mask_seq_stride; p.mask_row = c->mask_row_stride; p.mask_cols = (int)c->mask_cols;
+    p.T = c->T; p.total = c->B * c->T; p.N = (int)c->N; p.HQ = (int)c->HQ; p.HK = (int)cache->heads; p.D = (int)cache->dim; p.group = p.HQ / p.HK;
+    p.cu_i32 = c->flags & GDN_FLAG_CU_INT32;
+    p.scale2 = c->scale * 1.4426950408889634f;
+    p.tiles = plan.tiles; p.splits = plan.splits; p.row_groups = plan.row_groups;
+    p.part_o = (float*)workspace;
+    p.part_ml = p.part_o + (size_t)plan.splits * (size_t)(p.total * p.HQ) * (size_t)p.D;
+    // slot / page_size for slots below 2^31: ceil(2^(31 + l) / page_size), l = ceil(log2 page_size), is below 2^32 and exact
+    int l = 0;
+    while ((1ll << l) < cache->page_size) ++l;
+    p.page_shift = 31 + l;
+    p.page_magic = (uint32_t)(((1ull << p.page_shift) + cache->page_size - 1) / cache->page_size);
+    // (a page for 16 keys; places inside of them in 32 bits)
+    const bool uniform = cache->page_size % 16 == 0 && std::max(cache->k_stride[1], cache->v_stride[1]) < (1ll << 24) && std::min(cache->k_stride[1], cache->v_stride[1]) >= 0;
+    const dim3 grid((unsigned)(plan.tiles * plan.splits), (unsigned)cache->heads, (unsigned)c->N);
+    auto go = [&](auto t, auto dim, auto row_tiles) {
+        typedef decltype(t) T;
+        constexpr int DT = decltype(dim)::value, RT = decltype(row_tiles)::value;
+        const size_t smem = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float);
+        const void* kernel = uniform ? (const void*)paged_attn_kernel<T, DT, RT, true> : (const void*)paged_attn_kernel<T, DT, RT, false>;
+        const int made = ensure_dynamic_smem_for(kernel, smem, who);
+        if (made != GDN_OK) return made;
+        if (uniform) hipLaunchKernelGGL((paged_attn_kernel<T, DT, RT, true>), grid, dim3(256), smem, (hipStream_t)stream, p);
+        else hipLaunchKernelGGL((paged_attn_kernel<T, DT, RT, false>), grid, dim3(256), smem, (hipStream_t)stream, p);
+        const int ran = check_launch("paged_attn_kernel");
+        if (ran != GDN_OK || plan.splits == 1) return ran;
+        hipLaunchKernelGGL(paged_attn_join_kernel<T>, dim3((unsigned)((p.total * p.HQ + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+        return check_launch("paged_attn_join_kernel");
+    };
+    auto dims = [&](auto t) {
+        if (plan.dim == 256) return go(t, std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+        auto tiles = [&](auto dim) { return plan.row_tiles == 1 ? go(t, dim, std::integral_constant<int, 1>()) : go(t, dim, std::integral_constant<int, 2>()); };
+        return plan.dim == 64 ? tiles(std::integral_constant<int, 64>()) : tiles(std::integral_constant<int, 128>());
+    };
+    return cache->dtype == GDN_DTYPE_BF16 ? dims(bf16_t{}) : dims(f16_t{});
 }
