@@ -17,6 +17,7 @@
 #include "gdn_paged.h"
 #include "gdn_chunk_common.h"
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace gdn {
@@ -33,16 +34,20 @@ struct PagedAttnParams {
     uint32_t page_magic; int page_shift;     // slot / page_size = slot * page_magic >> page_shift
     int N, HQ, HK, D, group, mask_cols;
     int tiles, splits, row_groups;
-    float scale2;                            // scale log2(e)
-    bool cu_i32;
+    float scale2;                            // |scale| log2(e)
+    bool cu_i32, negative;                   // negative: of a negative scale the queries take the sign
 };
 
-typedef uint16_t pa_half __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint16_t pa_whole __attribute__((ext_vector_type(8), aligned(2)));
 
-template <typename T> __device__ __forceinline__ bool not_a_number(uint16_t bits) {
-    constexpr uint16_t EXP = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
-    return (bits & EXP) == EXP;
+// Infinities and NaN: an exponent of ones.  In a pair: its upper bit carries into the sign's place.
+template <typename T> constexpr uint32_t PA_EXPONENT = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
+template <typename T> constexpr uint32_t PA_CARRY = std::is_same_v<T, bf16_t> ? 0x0080 : 0x0400;
+template <typename T> __device__ __forceinline__ bool not_a_number(uint16_t bits) { return (bits & PA_EXPONENT<T>) == PA_EXPONENT<T>; }
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T two __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, two));
 }
 
 // What a step's sequence is.
@@ -82,7 +87,7 @@ template <> struct TilePlaces<false> {
     uint32_t there;
 };
 
-template <typename T, int DT, int RT, bool UNIFORM>
+template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
 struct PagedWave {
     typedef typename Mma<T>::V8 V8;
     static constexpr int LD = DT + 4;
@@ -91,9 +96,9 @@ struct PagedWave {
     const PagedSequence& s;
     const int64_t n;
     const int hk, lane, c16, g;
-    typedef std::conditional_t<VE == 8, pa_whole, pa_half> VPiece;
+    typedef uint32_t VPiece __attribute__((ext_vector_type(VE / 2), aligned(2)));
     V8 q[RT][KS], k[2][KS];
-    VPiece v[8][VC];
+    VPiece v[8][VC];                         // pairs of elements
     f32x4 o[RT][MT];
     float m[RT], l[RT];
     int token[RT];                           // row of the sequence that the lane's column is; -1: none
@@ -144,9 +149,10 @@ struct PagedWave {
             else at = (const uint16_t*)p.cache.k + __shfl(t.k, 16 * b + c16, 64) + 8 * g;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                pa_whole x = {};
-                if (32 * ks + 8 * g < p.D) x = *(const pa_whole*)(at + 32 * ks);
-                k[b][ks] = __builtin_bit_cast(V8, x);
+                // (behind the head: nothing, from a place that is there)
+                const bool inside = FULL || 32 * ks + 8 * g < p.D;
+                const pa_whole x = *(const pa_whole*)(at + (inside ? 32 * ks : -8 * g));
+                k[b][ks] = __builtin_bit_cast(V8, inside ? x : pa_whole{});
             }
         }
     }
@@ -161,11 +167,8 @@ struct PagedWave {
                 if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + (uint32_t)((4 * g + e) * (int)p.cache.v_slot + VE * c16);
                 else at = (const uint16_t*)p.cache.v + __shfl(t.v, 16 * b + 4 * g + e, 64) + VE * c16;
 #pragma unroll
-                for (int c = 0; c < VC; ++c) {
-                    VPiece x = {};
-                    if (128 * c + VE * c16 < p.D) x = *(const VPiece*)(at + 128 * c);
-                    v[4 * b + e][c] = x;
-                }
+                for (int c = 0; c < VC; ++c)
+                    v[4 * b + e][c] = *(const VPiece*)(at + (FULL || 128 * c + VE * c16 < p.D ? 128 * c : -VE * c16));
             }
     }
 
@@ -182,7 +185,7 @@ struct PagedWave {
             for (int ks = 0; ks < KS; ++ks) {
                 pa_whole x = {};
                 if (token[r] >= 0 && 32 * ks + 8 * g < p.D) x = *(const pa_whole*)(at + 32 * ks);
-                q[r][ks] = __builtin_bit_cast(V8, x);
+                q[r][ks] = __builtin_bit_cast(V8, p.negative ? x ^ (uint16_t)0x8000 : x);
             }
             m[r] = -INFINITY; l[r] = 0.f;
 #pragma unroll
@@ -193,20 +196,26 @@ struct PagedWave {
     // Which keys of a tile row token[r] sees of those whose pages are there: bit 4 b + e for key 16 b + 4 g + e.
     __device__ __forceinline__ uint32_t seen(int r, int tile, uint32_t there) const {
         const int fresh = (int)(tile * PA_TILE + 4 * g - s.context), most = p.mask ? min(p.mask_cols, s.rows) : token[r] + 1;
-        const uint8_t* mask = p.mask;
-        if (mask) mask += (p.cu ? (s.first + token[r]) * p.mask_row : n * p.mask_seq + token[r] * p.mask_row);
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int at = 16 * (i / 4) + i % 4, f = fresh + at;
-            bool is = f < most;
-            if (mask && is && f >= 0 && token[r] >= 0) is = mask[f] != 0;
-            bits |= is && there >> (4 * g + at) & 1 ? 1u << i : 0;
+            const int at = 16 * (i / 4) + i % 4;
+            bits |= fresh + at < most && there >> (4 * g + at) & 1 ? 1u << i : 0;
+        }
+        if (p.mask) {
+            // (all asked for at once, inside of the row)
+            const int64_t row = max(token[r], 0);
+            const uint8_t* mask = p.mask + (p.cu ? (s.first + row) * p.mask_row : n * p.mask_seq + row * p.mask_row);
+            uint8_t is[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) is[i] = mask[min(max(fresh + 16 * (i / 4) + i % 4, 0), most - 1)];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (fresh + 16 * (i / 4) + i % 4 >= 0 && !is[i]) bits &= ~(1u << i);
         }
         return bits;
     }
 
-    // The scores of a tile become weights in place: x[r][b][e] of key 16 b + 4 g + e.
     template <typename Next>
     __device__ __forceinline__ void tile(int tile, const TilePlaces<UNIFORM>& at, Next&& next_k) {
         f32x4 x[RT][2];
@@ -217,17 +226,17 @@ struct PagedWave {
                 x[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) x[r][b] = Mma<T>::run(k[b][ks], q[r][ks], x[r][b]);
-                x[r][b] *= p.scale2;
             }
         next_k();
         // The keys of the context whose pages are there are seen by every row; the tiles behind them are few.
         const bool whole = (int64_t)(tile + 1) * PA_TILE <= s.context && at.there == 0xffffffffu;
+        uint32_t bits[RT];
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const uint32_t bits = seen(r, tile, at.there);
+                bits[r] = seen(r, tile, at.there);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[r][i / 4][i % 4] = bits >> i & 1 ? x[r][i / 4][i % 4] : -INFINITY;
+                for (int i = 0; i < 8; ++i) x[r][i / 4][i % 4] = bits[r] >> i & 1 ? x[r][i / 4][i % 4] : -INFINITY;
             }
         }
         V8 w[RT];
@@ -235,41 +244,37 @@ struct PagedWave {
         for (int r = 0; r < RT; ++r) {
             float most = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    most = fmaxf(most, x[r][b][e]);
-                }
-            most = fmaxf(most, __shfl_xor(most, 16, 64));
-            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, x[r][i / 4][i % 4]);
+            // (the maximum is the same in the four lanes of a row; it seldom moves once a few tiles are seen)
             if (__any(most > m[r])) {
-                const float now = fmaxf(m[r], most), keep = __builtin_amdgcn_exp2f(m[r] - (now == -INFINITY ? 0.f : now));
+                most = fmaxf(most, __shfl_xor(most, 16, 64));
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+                const float now = fmaxf(m[r], most), keep = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[r] - now) * p.scale2);
                 m[r] = now;
                 l[r] *= keep;
 #pragma unroll
                 for (int t = 0; t < MT; ++t) o[r][t] *= keep;
             }
             // (no maximum yet: nothing is seen, or what is seen is not a number and makes the row's sums so)
-            const float base = m[r] == -INFINITY ? 0.f : m[r];
-            float sum = 0.f;
+            const float base = m[r] == -INFINITY ? 0.f : m[r] * p.scale2;
+            float y[8];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i / 4][i % 4], p.scale2, -base));
+            if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = __builtin_amdgcn_exp2f(x[r][b][e] - base);
-                    sum += y;
-                    w[r][4 * b + e] = (T)y;
-                }
-            l[r] += sum;
+                for (int i = 0; i < 8; ++i) y[i] = bits[r] >> i & 1 ? y[i] : 0.f;
+            }
+            l[r] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+            w[r] = __builtin_bit_cast(V8, u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])});
         }
         if (!whole && __any(odd_values())) clean(w, at);
 #pragma unroll
         for (int c = 0; c < VC; ++c)
 #pragma unroll
             for (int t = 0; t < VE; ++t) {
-                pa_whole a;
+                u32x4 a;                                                     // element t of the eight keys
 #pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] = v[j][c][t];
+                for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c][t / 2], v[2 * j][c][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
                 const V8 va = __builtin_bit_cast(V8, a);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) o[r][c * VE + t] = Mma<T>::run(va, w[r], o[r][c * VE + t]);
@@ -278,14 +283,14 @@ struct PagedWave {
 
     // Infinities and NaN in V, in tiles whose keys not every row sees: a weight of zero does not keep them out of a product.
     __device__ __forceinline__ bool odd_values() const {
-        bool odd = false;
+        uint32_t carried = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int c = 0; c < VC; ++c)
 #pragma unroll
-                for (int t = 0; t < VE; ++t) odd = odd || not_a_number<T>(v[j][c][t]);
-        return odd;
+                for (int t = 0; t < VE / 2; ++t) carried |= (v[j][c][t] & PA_EXPONENT<T> * 0x10001u) + PA_CARRY<T> * 0x10001u;
+        return carried & 0x80008000u;
     }
     // They are taken out of V and added to the rows that see the key in the wave's place in LDS: sums of infinities and NaN, which no later maximum changes.
     __device__ __forceinline__ void clean(const V8 (&w)[RT], const TilePlaces<UNIFORM>& at) {
@@ -307,7 +312,8 @@ struct PagedWave {
 #pragma unroll
             for (int c = 0; c < VC; ++c)
 #pragma unroll
-                for (int t = 0; t < VE; ++t) v[j][c][t] = not_a_number<T>(v[j][c][t]) ? (uint16_t)0 : v[j][c][t];
+                for (int t = 0; t < VE / 2; ++t)
+                    v[j][c][t] &= (not_a_number<T>((uint16_t)v[j][c][t]) ? 0u : 0xffffu) | (not_a_number<T>((uint16_t)(v[j][c][t] >> 16)) ? 0u : 0xffff0000u);
 #pragma nounroll
         for (int key = 0; key < PA_TILE; ++key) {
             if (!(at.there >> key & 1)) continue;
@@ -345,9 +351,9 @@ struct PagedWave {
     }
 };
 
-template <typename T, int DT, int RT, bool UNIFORM>
+template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
-    typedef PagedWave<T, DT, RT, UNIFORM> Wave;
+    typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
     constexpr int VE = Wave::VE, LD = Wave::LD;
     extern __shared__ float lds[];                               // [4 waves][16 RT][LD], then [4 waves][16 RT][2]
     const int64_t n = blockIdx.z;
@@ -395,7 +401,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
                         if (w.odd) sum += *to;
                         *to = sum;
                     }
-            if (w.g == 0) { ml[2 * row] = w.m[r]; ml[2 * row + 1] = w.l[r]; }
+            if (w.g == 0) { ml[2 * row] = w.m[r] == -INFINITY ? -INFINITY : w.m[r] * p.scale2; ml[2 * row + 1] = w.l[r]; }
         }
         __syncthreads();
         constexpr int PIECES = DT / 4;
@@ -518,7 +524,7 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     p.mask_seq = c->mask_seq_stride; p.mask_row = c->mask_row_stride; p.mask_cols = (int)c->mask_cols;
     p.T = c->T; p.total = c->B * c->T; p.N = (int)c->N; p.HQ = (int)c->HQ; p.HK = (int)cache->heads; p.D = (int)cache->dim; p.group = p.HQ / p.HK;
     p.cu_i32 = c->flags & GDN_FLAG_CU_INT32;
-    p.scale2 = c->scale * 1.4426950408889634f;
+    p.scale2 = std::fabs(c->scale) * 1.4426950408889634f; p.negative = c->scale < 0;
     p.tiles = plan.tiles; p.splits = plan.splits; p.row_groups = plan.row_groups;
     p.part_o = (float*)workspace;
     p.part_ml = p.part_o + (size_t)plan.splits * (size_t)(p.total * p.HQ) * (size_t)p.D;
@@ -534,11 +540,15 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
         typedef decltype(t) T;
         constexpr int DT = decltype(dim)::value, RT = decltype(row_tiles)::value;
         const size_t smem = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float);
-        const void* kernel = uniform ? (const void*)paged_attn_kernel<T, DT, RT, true> : (const void*)paged_attn_kernel<T, DT, RT, false>;
-        const int made = ensure_dynamic_smem_for(kernel, smem, who);
+        auto launch = [&](auto uniform_, auto full_) {
+            const auto kernel = paged_attn_kernel<T, DT, RT, decltype(uniform_)::value, decltype(full_)::value>;
+            const int made = ensure_dynamic_smem_for((const void*)kernel, smem, who);
+            if (made == GDN_OK) hipLaunchKernelGGL(kernel, grid, dim3(256), smem, (hipStream_t)stream, p);
+            return made;
+        };
+        auto full = [&](auto uniform_) { return p.D == DT ? launch(uniform_, std::true_type()) : launch(uniform_, std::false_type()); };
+        const int made = uniform ? full(std::true_type()) : full(std::false_type());
         if (made != GDN_OK) return made;
-        if (uniform) hipLaunchKernelGGL((paged_attn_kernel<T, DT, RT, true>), grid, dim3(256), smem, (hipStream_t)stream, p);
-        else hipLaunchKernelGGL((paged_attn_kernel<T, DT, RT, false>), grid, dim3(256), smem, (hipStream_t)stream, p);
         const int ran = check_launch("paged_attn_kernel");
         if (ran != GDN_OK || plan.splits == 1) return ran;
         hipLaunchKernelGGL(paged_attn_join_kernel<T>, dim3((unsigned)((p.total * p.HQ + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
