@@ -33,12 +33,13 @@ struct PagedAttnParams {
     int64_t T, total;                        // rows of a sequence (dense), of the batch
     uint32_t page_magic; int page_shift;     // slot / page_size = slot * page_magic >> page_shift
     int N, HQ, HK, D, group, mask_cols;
-    int tiles, splits, row_groups;
+    int tiles, splits, row_groups, odd_at;
     float scale2;                            // |scale| log2(e)
     bool cu_i32, negative;                   // negative: of a negative scale the queries take the sign
 };
 
 typedef uint16_t pa_whole __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint16_t pa_aligned __attribute__((ext_vector_type(8)));
 
 // Infinities and NaN: an exponent of ones.  In a pair: its upper bit carries into the sign's place.
 template <typename T> constexpr uint32_t PA_EXPONENT = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
@@ -90,7 +91,7 @@ template <> struct TilePlaces<false> {
 template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
 struct PagedWave {
     typedef typename Mma<T>::V8 V8;
-    static constexpr int LD = DT + 4;
+    static constexpr int LD = DT + 4, ODD = DT / 32, ROW = 2 * DT, SWIZZLE = DT == 64 ? 7 : 15;
     static constexpr int KS = DT / 32, VE = DT >= 128 ? 8 : 4, VC = DT / 16 / VE, MT = DT / 16;     // steps of a score; elements of V at a place, places, products per row tile
     const PagedAttnParams& p;
     const PagedSequence& s;
@@ -103,10 +104,10 @@ struct PagedWave {
     float m[RT], l[RT];
     int token[RT];                           // row of the sequence that the lane's column is; -1: none
     bool odd;                                // infinities and NaN of V are in LDS
-    float* const sums;                       // the wave's place there, [16 RT][LD]
+    uint64_t* const odd_bits;                // the wave's place there, [16 RT][ODD]: for each 64 elements those up, those down
 
-    __device__ __forceinline__ PagedWave(const PagedAttnParams& p, const PagedSequence& s, int64_t n, int hk, float* sums)
-        : p(p), s(s), n(n), hk(hk), lane(threadIdx.x & 63), c16(lane & 15), g(lane >> 4), odd(false), sums(sums) {}
+    __device__ __forceinline__ PagedWave(const PagedAttnParams& p, const PagedSequence& s, int64_t n, int hk, uint64_t* odd_bits)
+        : p(p), s(s), n(n), hk(hk), lane(threadIdx.x & 63), c16(lane & 15), g(lane >> 4), odd(false), odd_bits(odd_bits) {}
 
     __device__ __forceinline__ int page_index(int slot) const { return (int)(((uint64_t)(uint32_t)slot * p.page_magic) >> p.page_shift); }
 
@@ -193,9 +194,15 @@ struct PagedWave {
         }
     }
 
+    // What is formed of the result is formed where it is used: the rare paths' places held in registers through the whole loop would not leave the loop enough.
+    static __device__ __forceinline__ int unhoisted(int x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    }
+
     // Which keys of a tile row token[r] sees of those whose pages are there: bit 4 b + e for key 16 b + 4 g + e.
     __device__ __forceinline__ uint32_t seen(int r, int tile, uint32_t there) const {
-        const int fresh = (int)(tile * PA_TILE + 4 * g - s.context), most = p.mask ? min(p.mask_cols, s.rows) : token[r] + 1;
+        const int g = unhoisted(lane) >> 4, fresh = (int)(tile * PA_TILE + 4 * g - s.context), most = p.mask ? min(p.mask_cols, s.rows) : token[r] + 1;
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -204,7 +211,7 @@ struct PagedWave {
         }
         if (p.mask) {
             // (all asked for at once, inside of the row)
-            const int64_t row = max(token[r], 0);
+            const int64_t row = max(unhoisted(token[r]), 0);
             const uint8_t* mask = p.mask + (p.cu ? (s.first + row) * p.mask_row : n * p.mask_seq + row * p.mask_row);
             uint8_t is[8];
 #pragma unroll
@@ -216,8 +223,16 @@ struct PagedWave {
         return bits;
     }
 
+    // stage: where the tile lies in LDS (NULL: nowhere); next_k: asked for between the two products
     template <typename Next>
-    __device__ __forceinline__ void tile(int tile, const TilePlaces<UNIFORM>& at, Next&& next_k) {
+    __device__ __forceinline__ void tile(int tile, const TilePlaces<UNIFORM>& at, const char* stage, Next&& next_k) {
+        // The keys of the context whose pages are there are seen by every row; the tiles behind them are few.
+        const bool whole = (int64_t)(tile + 1) * PA_TILE <= s.context && at.there == 0xffffffffu;
+        uint32_t bits[RT];
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) bits[r] = seen(r, tile, at.there);
+        }
         f32x4 x[RT][2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -228,16 +243,11 @@ struct PagedWave {
                 for (int ks = 0; ks < KS; ++ks) x[r][b] = Mma<T>::run(k[b][ks], q[r][ks], x[r][b]);
             }
         next_k();
-        // The keys of the context whose pages are there are seen by every row; the tiles behind them are few.
-        const bool whole = (int64_t)(tile + 1) * PA_TILE <= s.context && at.there == 0xffffffffu;
-        uint32_t bits[RT];
         if (!whole) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                bits[r] = seen(r, tile, at.there);
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[r][i / 4][i % 4] = bits[r] >> i & 1 ? x[r][i / 4][i % 4] : -INFINITY;
-            }
         }
         V8 w[RT];
 #pragma unroll
@@ -260,14 +270,14 @@ struct PagedWave {
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i / 4][i % 4], p.scale2, -base));
-            if (!whole) {
+            if (!whole) {                                                   // (of a scale of zero nothing is -inf)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = bits[r] >> i & 1 ? y[i] : 0.f;
+                for (int i = 0; i < 8; ++i) y[i] = x[r][i / 4][i % 4] == -INFINITY ? 0.f : y[i];
             }
             l[r] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
             w[r] = __builtin_bit_cast(V8, u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])});
         }
-        if (!whole && __any(odd_values())) clean(w, at);
+        if (!whole && __any(odd_values())) clean(w, at, stage);
 #pragma unroll
         for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -281,6 +291,7 @@ struct PagedWave {
             }
     }
 
+    static __device__ __forceinline__ uint32_t carry(uint32_t pair) { return ((pair & PA_EXPONENT<T> * 0x10001u) + PA_CARRY<T> * 0x10001u) & 0x80008000u; }
     // Infinities and NaN in V, in tiles whose keys not every row sees: a weight of zero does not keep them out of a product.
     __device__ __forceinline__ bool odd_values() const {
         uint32_t carried = 0;
@@ -289,50 +300,130 @@ struct PagedWave {
 #pragma unroll
             for (int c = 0; c < VC; ++c)
 #pragma unroll
-                for (int t = 0; t < VE / 2; ++t) carried |= (v[j][c][t] & PA_EXPONENT<T> * 0x10001u) + PA_CARRY<T> * 0x10001u;
-        return carried & 0x80008000u;
+                for (int t = 0; t < VE / 2; ++t) carried |= carry(v[j][c][t]);
+        return carried;
     }
-    // They are taken out of V and added to the rows that see the key in the wave's place in LDS: sums of infinities and NaN, which no later maximum changes.
-    __device__ __forceinline__ void clean(const V8 (&w)[RT], const TilePlaces<UNIFORM>& at) {
+    // They are taken out of V and kept in LDS for the rows that see the key, a bit for each row and element: what a sum of infinities and NaN will be, whatever is
+    // added to it (both bits: NaN).
+    __device__ __forceinline__ void clean(const V8 (&w)[RT], const TilePlaces<UNIFORM>& at, const char* stage) {
+        const int lane = unhoisted(this->lane), c16 = lane & 15, g = lane >> 4;
+        uint64_t* const mine = odd_bits + (16 * g + c16) * ODD;                 // (lanes of g < RT: row 16 g + c16)
         if (!odd) {
-            for (int i = lane; i < 16 * RT * LD; i += 64) sums[i] = 0.f;
+            if (g < RT)
+                for (int i = 0; i < ODD; ++i) mine[i] = 0;
             odd = true;
         }
-        uint32_t rows[RT];                                                  // the keys that the lane's row has weights for
+        uint32_t row = 0;                                                   // the keys that the lane's row has weights for
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            rows[r] = 0;
+            uint32_t keys = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rows[r] |= (float)w[r][i] != 0.f ? 1u << (16 * (i / 4) + 4 * g + i % 4) : 0;
-            rows[r] |= __shfl_xor(rows[r], 16, 64);
-            rows[r] |= __shfl_xor(rows[r], 32, 64);
+            for (int i = 0; i < 8; ++i) keys |= (float)w[r][i] != 0.f ? 1u << (16 * (i / 4) + 4 * g + i % 4) : 0;
+            keys |= __shfl_xor(keys, 16, 64);
+            keys |= __shfl_xor(keys, 32, 64);
+            if (g == r) row = keys;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int c = 0; c < VC; ++c)
 #pragma unroll
-                for (int t = 0; t < VE / 2; ++t)
-                    v[j][c][t] &= (not_a_number<T>((uint16_t)v[j][c][t]) ? 0u : 0xffffu) | (not_a_number<T>((uint16_t)(v[j][c][t] >> 16)) ? 0u : 0xffff0000u);
+                for (int t = 0; t < VE / 2; ++t) v[j][c][t] &= ~((carry(v[j][c][t]) >> 15) * 0xffffu);
 #pragma nounroll
         for (int key = 0; key < PA_TILE; ++key) {
             if (!(at.there >> key & 1)) continue;
             const uint16_t* from;
-            if constexpr (UNIFORM) from = (const uint16_t*)p.cache.v + (key < 16 ? at.v[0] : at.v[1]) + (key & 15) * p.cache.v_slot;
+            if (stage) from = (const uint16_t*)(stage + PA_TILE * ROW + key * ROW);
+            else if constexpr (UNIFORM) from = (const uint16_t*)p.cache.v + (key < 16 ? at.v[0] : at.v[1]) + (key & 15) * p.cache.v_slot;
             else from = (const uint16_t*)p.cache.v + __shfl(at.v, key, 64);
 #pragma nounroll
-            for (int d0 = 0; d0 < p.D; d0 += 64) {
-                const int d = d0 + lane;
-                const uint16_t bits = d < p.D ? from[d] : (uint16_t)0;
-                const bool is = not_a_number<T>(bits);
-                if (!__any(is)) continue;
-                const float value = (float)__builtin_bit_cast(T, bits);
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma nounroll
-                    for (int row = 0; row < 16; ++row)
-                        if ((__shfl(rows[r], row, 64) >> key & 1) && is) sums[(16 * r + row) * LD + d] += value;
+            for (int i = 0; i < DT / 64; ++i) {
+                const int d = 64 * i + lane;
+                uint16_t bits = 0;
+                if (d < p.D) bits = from[stage ? d ^ (key & SWIZZLE) * 8 : d];
+                const bool is = not_a_number<T>(bits), nan = is && (bits & ~PA_EXPONENT<T> & 0x7fffu);
+                const uint64_t up = __ballot(is && (nan || !(bits >> 15))), down = __ballot(is && (nan || bits >> 15));
+                if ((up | down) && g < RT && row >> key & 1) { mine[2 * i] |= up; mine[2 * i + 1] |= down; }
             }
+        }
+    }
+    // What they make of element d of a row of the wave: infinity, minus infinity, NaN, or nothing.
+    __device__ __forceinline__ float odd_sum(int row, int d) const {
+        const uint64_t* at = odd_bits + row * ODD + 2 * (d / 64);
+        const bool up = at[0] >> (d & 63) & 1, down = at[1] >> (d & 63) & 1;
+        return up && down ? __builtin_nanf("") : up ? INFINITY : down ? -INFINITY : 0.f;
+    }
+
+    // ---- four waves on the same keys: tiles through LDS ----
+    // A stage holds K, then V, of a tile as they lie in memory, the 16-byte pieces of row r XORed with r (so that 16 rows of a column meet no bank twice).
+    static constexpr int PIECES = PA_TILE * ROW / 1024, STAGE = 2 * PA_TILE * ROW, STAGES = 4;
+
+    // This wave's quarter of a tile: copies straight into LDS, 1 KB each, asked for by inline assembly (counted by hand).
+    __device__ __forceinline__ void ask(const TilePlaces<true>& t, uint32_t stage, int wave) {
+        const uint16_t* kb = (const uint16_t*)p.cache.k + (wave < 2 ? t.k[0] : t.k[1]);
+        const uint16_t* vb = (const uint16_t*)p.cache.v + (wave < 2 ? t.v[0] : t.v[1]);
+        constexpr int EACH = PIECES / 4, KEYS = 1024 / ROW;                 // copies of K (and of V), keys of one
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int piece = wave * EACH + i, key = piece * KEYS + lane * 16 / ROW;
+            int element = 8 * ((lane % (ROW / 16)) ^ (key & SWIZZLE));
+            if (!FULL && element >= p.D) element = 0;
+            gather_1k_to_lds((const char*)kb, 2 * ((key & 15) * (uint32_t)p.cache.k_slot + element), stage + piece * 1024);
+            gather_1k_to_lds((const char*)vb, 2 * ((key & 15) * (uint32_t)p.cache.v_slot + element), stage + PA_TILE * ROW + piece * 1024);
+        }
+    }
+    __device__ __forceinline__ void read_k(const char* stage) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const pa_aligned x = *(const pa_aligned*)(stage + (16 * b + c16) * ROW + 16 * ((4 * ks + g) ^ (c16 & SWIZZLE)));
+                k[b][ks] = __builtin_bit_cast(V8, FULL || 32 * ks + 8 * g < p.D ? x : pa_aligned{});
+            }
+    }
+    __device__ __forceinline__ void read_v(const char* stage) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    const int row = 16 * b + 4 * g + e, piece = VE == 8 ? 16 * c + c16 : c16 / 2;
+                    typedef uint32_t Aligned __attribute__((ext_vector_type(VE / 2)));
+                    v[4 * b + e][c] = *(const Aligned*)(stage + PA_TILE * ROW + row * ROW + 16 * (piece ^ (row & SWIZZLE)) + (VE == 8 ? 0 : 8 * (c16 & 1)));
+                }
+    }
+
+    // Tiles first .. last - 1, all four waves on each.
+    __device__ __forceinline__ void run_shared(int first, int last, int wave, char* stages) {
+        if (first >= last) return;
+        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)stages;
+        constexpr int COPIES = 2 * PIECES / 4;
+        TilePlaces<true> at = {}, next = places(first);
+        uint32_t there[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) {
+            there[i] = next.there;
+            if (first + i < last) ask(next, base + i * STAGE, wave);
+            next = places(first + i + 1);
+        }
+        int stage = 0;
+        for (int t = first; t < last; ++t) {
+            const int behind = last - 1 - t;                     // tiles asked for after this one
+            if (behind >= 2) wait_vm_at_most<2 * COPIES>();
+            else if (behind == 1) wait_vm_at_most<COPIES>();
+            else wait_vm_at_most<0>();
+            lds_barrier();
+            there[STAGES - 1] = next.there;
+            if (t + STAGES - 1 < last) ask(next, base + (stage + STAGES - 1) % STAGES * STAGE, wave);
+            next = places(t + STAGES);
+            const char* from = stages + stage * STAGE;
+            read_k(from);
+            at.there = there[0];
+            tile(t, at, from, [&] { read_v(from); });
+#pragma unroll
+            for (int i = 0; i < STAGES - 1; ++i) there[i] = there[i + 1];
+            stage = (stage + 1) % STAGES;
         }
     }
 
@@ -343,7 +434,7 @@ struct PagedWave {
         load_v(now);
         for (int t = first; t < last; t += step) {
             const bool more = t + step < last;
-            tile(t, now, [&] { if (more) load_k(next); });
+            tile(t, now, nullptr, [&] { if (more) load_k(next); });
             if (more) load_v(next);
             now = next;
             next = places(t + 2 * step);
@@ -351,9 +442,10 @@ struct PagedWave {
     }
 };
 
-template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
+template <typename T, int DT, int RT, bool UNIFORM, bool FULL, bool SHARED>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
     typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
+    static_assert(!SHARED || UNIFORM, "copies of whole pieces");
     constexpr int VE = Wave::VE, LD = Wave::LD;
     extern __shared__ float lds[];                               // [4 waves][16 RT][LD], then [4 waves][16 RT][2]
     const int64_t n = blockIdx.z;
@@ -373,13 +465,21 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
             if (n == 0 && p.N == 1) clear(max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), p.total);
         }
     }
-    const int all = (s.keys + PA_TILE - 1) / PA_TILE, rows = s.rows * p.group, height = 16 * RT * p.row_groups;
-    const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+    const int rows = s.rows * p.group, height = 16 * RT * p.row_groups;
     for (int tile = blockIdx.x / p.splits; tile * height < rows; tile += p.tiles) {
-        Wave w(p, s, n, hk, lds + wave * 16 * RT * LD);
+        Wave w(p, s, n, hk, (uint64_t*)((char*)lds + p.odd_at) + wave * 16 * RT * Wave::ODD);
         const int row0 = tile * height + rg * 16 * RT;
         w.start(row0);
-        w.run(t0 + kg, t1, key_groups);
+        // (without a mask a row sees no row behind it: nor do the keys behind the last row's matter)
+        const int last_token = min((tile * height + height - 1) / p.group, s.rows - 1);
+        const int keys = p.mask ? s.keys : (int)min((int64_t)s.keys, max(s.context + last_token + 1, (int64_t)0)), all = (keys + PA_TILE - 1) / PA_TILE;
+        const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+        if constexpr (SHARED) {
+            w.run_shared(t0, t1, wave, (char*)lds);
+            __syncthreads();
+        } else {
+            w.run(t0 + kg, t1, key_groups);
+        }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             w.l[r] += __shfl_xor(w.l[r], 16, 64);
@@ -387,21 +487,25 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
         }
         // The waves that share rows, joined: each leaves its sums with its maximum.
         float* const ml = lds + 4 * 16 * RT * LD;
+        const int lane = Wave::unhoisted(w.lane), c16 = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const int row = wave * 16 * RT + 16 * r + w.c16;
+            const int row = wave * 16 * RT + 16 * r + c16;
 #pragma unroll
             for (int c = 0; c < Wave::VC; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int t = 0; t < VE; t += 4) {
-                        f32x4* const to = (f32x4*)(lds + row * LD + 128 * c + VE * (4 * w.g + e) + t);
+                        f32x4* const to = (f32x4*)(lds + row * LD + 128 * c + VE * (4 * g + e) + t);
                         f32x4 sum = {w.o[r][c * VE + t][e], w.o[r][c * VE + t + 1][e], w.o[r][c * VE + t + 2][e], w.o[r][c * VE + t + 3][e]};
-                        if (w.odd) sum += *to;
+                        if (w.odd) {
+                            const int d = 128 * c + VE * (4 * g + e) + t;
+                            sum += f32x4{w.odd_sum(16 * r + c16, d), w.odd_sum(16 * r + c16, d + 1), w.odd_sum(16 * r + c16, d + 2), w.odd_sum(16 * r + c16, d + 3)};
+                        }
                         *to = sum;
                     }
-            if (w.g == 0) { ml[2 * row] = w.m[r] == -INFINITY ? -INFINITY : w.m[r] * p.scale2; ml[2 * row + 1] = w.l[r]; }
+            if (g == 0) { ml[2 * row] = w.m[r] == -INFINITY ? -INFINITY : w.m[r] * p.scale2; ml[2 * row + 1] = w.l[r]; }
         }
         __syncthreads();
         constexpr int PIECES = DT / 4;
@@ -535,19 +639,30 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     p.page_magic = (uint32_t)(((1ull << p.page_shift) + cache->page_size - 1) / cache->page_size);
     // (a page for 16 keys; places inside of them in 32 bits)
     const bool uniform = cache->page_size % 16 == 0 && std::max(cache->k_stride[1], cache->v_stride[1]) < (1ll << 24) && std::min(cache->k_stride[1], cache->v_stride[1]) >= 0;
+    // (rows on 16-byte boundaries: copies into LDS)
+    const PagedCache& v = p.cache;
+    const bool whole_pieces = (((uintptr_t)v.k | (uintptr_t)v.v) & 15) == 0 && ((v.k_page | v.k_slot | v.k_head | v.v_page | v.v_slot | v.v_head) & 7) == 0;
     const dim3 grid((unsigned)(plan.tiles * plan.splits), (unsigned)cache->heads, (unsigned)c->N);
     auto go = [&](auto t, auto dim, auto row_tiles) {
         typedef decltype(t) T;
         constexpr int DT = decltype(dim)::value, RT = decltype(row_tiles)::value;
-        const size_t smem = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float);
-        auto launch = [&](auto uniform_, auto full_) {
-            const auto kernel = paged_attn_kernel<T, DT, RT, decltype(uniform_)::value, decltype(full_)::value>;
+        auto launch = [&](auto uniform_, auto full_, auto shared_) {
+            constexpr bool UNIFORM = decltype(uniform_)::value, FULL = decltype(full_)::value, SHARED = decltype(shared_)::value;
+            typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
+            const size_t joined = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float), room = SHARED ? std::max<size_t>(joined, Wave::STAGES * Wave::STAGE) : joined,
+                         smem = room + (size_t)4 * 16 * RT * Wave::ODD * sizeof(uint64_t);
+            p.odd_at = (int)room;
+            const auto kernel = paged_attn_kernel<T, DT, RT, UNIFORM, FULL, SHARED>;
             const int made = ensure_dynamic_smem_for((const void*)kernel, smem, who);
             if (made == GDN_OK) hipLaunchKernelGGL(kernel, grid, dim3(256), smem, (hipStream_t)stream, p);
             return made;
         };
-        auto full = [&](auto uniform_) { return p.D == DT ? launch(uniform_, std::true_type()) : launch(uniform_, std::false_type()); };
-        const int made = uniform ? full(std::true_type()) : full(std::false_type());
+        auto full = [&](auto uniform_, auto shared_) { return p.D == DT ? launch(uniform_, std::true_type(), shared_) : launch(uniform_, std::false_type(), shared_); };
+        int made;
+        if (!uniform) made = full(std::false_type(), std::false_type());
+        else if (plan.row_groups < 4 || !whole_pieces) made = full(std::true_type(), std::false_type());
+        else if constexpr (RT == 2 || DT == 256) made = full(std::true_type(), std::true_type());
+        else made = GDN_ERR_UNSUPPORTED;
         if (made != GDN_OK) return made;
         const int ran = check_launch("paged_attn_kernel");
         if (ran != GDN_OK || plan.splits == 1) return ran;
