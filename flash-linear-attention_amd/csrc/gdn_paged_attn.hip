@@ -34,6 +34,7 @@ struct PagedAttnParams {
     uint32_t page_magic; int page_shift;     // slot / page_size = slot * page_magic >> page_shift
     int N, HQ, HK, D, group, mask_cols;
     int tiles, splits, row_groups, odd_at;
+    uint32_t k_page, k_slot, k_head, v_page, v_slot, v_head;     // the cache's strides where they are below 2^32 (UNIFORM)
     float scale2;                            // |scale| log2(e)
     bool cu_i32, negative;                   // negative: of a negative scale the queries take the sign
 };
@@ -57,6 +58,7 @@ struct PagedSequence {
     int rows;
     int64_t context;
     int keys;                                // slots that may be seen: [0, keys)
+    int whole;                               // tiles that lie in the context
 };
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedAttnParams& p, int64_t n) {
     PagedSequence s;
@@ -74,13 +76,14 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedAttnParams& p
     // (in this order: a context near the end of 64 bits does not overflow)
     s.context = max(min(s.context, capacity), (int64_t)-0x40000000);
     s.keys = (int)max(min(s.context + s.rows, capacity), (int64_t)0);
+    s.whole = (int)max(s.context, (int64_t)0) / PA_TILE;
     return s;
 }
 
 // The places of a tile's keys.  UNIFORM (pages of a multiple of 16 slots): a page for each 16 keys, the same for all lanes.  Else a place for each key, in lane key % 32.
 template <bool UNIFORM> struct TilePlaces;
 template <> struct TilePlaces<true> {
-    int64_t k[2], v[2];                      // first key of either half, in elements
+    uint64_t k[2], v[2];                     // first key of either half, in elements
     uint32_t there;                          // bit per key: its page is one of the cache
 };
 template <> struct TilePlaces<false> {
@@ -91,7 +94,7 @@ template <> struct TilePlaces<false> {
 template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
 struct PagedWave {
     typedef typename Mma<T>::V8 V8;
-    static constexpr int LD = DT + 4, ODD = DT / 32, ROW = 2 * DT, SWIZZLE = DT == 64 ? 7 : 15;
+    static constexpr int LD = DT + 4, ODD = DT / 32, ROW = 2 * DT, SWIZZLE = DT == 64 ? 7 : 15;   // LDS: floats of a row of sums, words of odd_bits, bytes of a key
     static constexpr int KS = DT / 32, VE = DT >= 128 ? 8 : 4, VC = DT / 16 / VE, MT = DT / 16;     // steps of a score; elements of V at a place, places, products per row tile
     const PagedAttnParams& p;
     const PagedSequence& s;
@@ -111,6 +114,9 @@ struct PagedWave {
 
     __device__ __forceinline__ int page_index(int slot) const { return (int)(((uint64_t)(uint32_t)slot * p.page_magic) >> p.page_shift); }
 
+    __device__ __forceinline__ uint64_t k_place(uint32_t page, uint32_t inside) const { return (uint64_t)page * p.k_page + (uint64_t)inside * p.k_slot + (uint64_t)hk * p.k_head; }
+    __device__ __forceinline__ uint64_t v_place(uint32_t page, uint32_t inside) const { return (uint64_t)page * p.v_page + (uint64_t)inside * p.v_slot + (uint64_t)hk * p.v_head; }
+
     __device__ __forceinline__ TilePlaces<UNIFORM> places(int tile) const {
         TilePlaces<UNIFORM> t;
         const PagedCache& c = p.cache;
@@ -125,8 +131,8 @@ struct PagedWave {
                 const int inside = there ? slot - index * c.pages.page_size : 0;
                 page = there ? page : 0;
                 t.there |= there ? 0xffffu << 16 * b : 0;
-                t.k[b] = page * c.k_page + inside * c.k_slot + hk * c.k_head;
-                t.v[b] = page * c.v_page + inside * c.v_slot + hk * c.v_head;
+                t.k[b] = k_place(page, inside);
+                t.v[b] = v_place(page, inside);
             }
         } else {
             const int slot = tile * PA_TILE + (lane & 31), index = page_index(slot);
@@ -146,7 +152,7 @@ struct PagedWave {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint16_t* at;
-            if constexpr (UNIFORM) at = (const uint16_t*)p.cache.k + t.k[b] + (uint32_t)(c16 * (int)p.cache.k_slot + 8 * g);
+            if constexpr (UNIFORM) at = (const uint16_t*)p.cache.k + t.k[b] + (c16 * p.k_slot + 8 * g);
             else at = (const uint16_t*)p.cache.k + __shfl(t.k, 16 * b + c16, 64) + 8 * g;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -165,7 +171,7 @@ struct PagedWave {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint16_t* at;
-                if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + (uint32_t)((4 * g + e) * (int)p.cache.v_slot + VE * c16);
+                if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + ((4 * g + e) * p.v_slot + VE * c16);
                 else at = (const uint16_t*)p.cache.v + __shfl(t.v, 16 * b + 4 * g + e, 64) + VE * c16;
 #pragma unroll
                 for (int c = 0; c < VC; ++c)
@@ -227,7 +233,7 @@ struct PagedWave {
     template <typename Next>
     __device__ __forceinline__ void tile(int tile, const TilePlaces<UNIFORM>& at, const char* stage, Next&& next_k) {
         // The keys of the context whose pages are there are seen by every row; the tiles behind them are few.
-        const bool whole = (int64_t)(tile + 1) * PA_TILE <= s.context && at.there == 0xffffffffu;
+        const bool whole = tile < s.whole && at.there == 0xffffffffu;
         uint32_t bits[RT];
         if (!whole) {
 #pragma unroll
@@ -237,11 +243,14 @@ struct PagedWave {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                x[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int r = 0; r < RT; ++r) x[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // (a product waits for the one before it in its own sum: the sums take turns)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) x[r][b] = Mma<T>::run(k[b][ks], q[r][ks], x[r][b]);
-            }
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) x[r][b] = Mma<T>::run(k[b][ks], q[r][ks], x[r][b]);
         next_k();
         if (!whole) {
 #pragma unroll
@@ -333,7 +342,7 @@ struct PagedWave {
         for (int key = 0; key < PA_TILE; ++key) {
             if (!(at.there >> key & 1)) continue;
             const uint16_t* from;
-            if (stage) from = (const uint16_t*)(stage + PA_TILE * ROW + key * ROW);
+            if (stage) from = (const uint16_t*)(stage + TILE + key * ROW);
             else if constexpr (UNIFORM) from = (const uint16_t*)p.cache.v + (key < 16 ? at.v[0] : at.v[1]) + (key & 15) * p.cache.v_slot;
             else from = (const uint16_t*)p.cache.v + __shfl(at.v, key, 64);
 #pragma nounroll
@@ -354,76 +363,81 @@ struct PagedWave {
         return up && down ? __builtin_nanf("") : up ? INFINITY : down ? -INFINITY : 0.f;
     }
 
-    // ---- four waves on the same keys: tiles through LDS ----
-    // A stage holds K, then V, of a tile as they lie in memory, the 16-byte pieces of row r XORed with r (so that 16 rows of a column meet no bank twice).
-    static constexpr int PIECES = PA_TILE * ROW / 1024, STAGE = 2 * PA_TILE * ROW, STAGES = 4;
+    // ---- four waves on the same keys: 64 at a time through LDS ----
+    // A stage holds K, then V, of two tiles as they lie in memory, the 16-byte pieces of row r XORed with r (so that 16 rows of a column meet no bank twice).  Copies are
+    // of 1 KB, straight into LDS, asked for by inline assembly and waited for by hand; a wave makes those of 16 keys, so of one page.
+    static constexpr int TILE = PA_TILE * ROW, STAGE = 4 * TILE, STAGES = 2;
 
-    // This wave's quarter of a tile: copies straight into LDS, 1 KB each, asked for by inline assembly (counted by hand).
-    __device__ __forceinline__ void ask(const TilePlaces<true>& t, uint32_t stage, int wave) {
-        const uint16_t* kb = (const uint16_t*)p.cache.k + (wave < 2 ? t.k[0] : t.k[1]);
-        const uint16_t* vb = (const uint16_t*)p.cache.v + (wave < 2 ? t.v[0] : t.v[1]);
-        constexpr int EACH = PIECES / 4, KEYS = 1024 / ROW;                 // copies of K (and of V), keys of one
+    struct Block { int page, inside; };
+    __device__ __forceinline__ Block block_of(int stage, int wave) const {
+        const int slot = 64 * stage + 16 * wave, index = page_index(slot);
+        int page = -1;
+        if (slot < s.keys) page = (int)load_index_uniform(p.cache.pages.table, n * p.cache.pages.table_stride + index, true);
+        return Block{page, slot - index * p.cache.pages.page_size};
+    }
+    // there: a half word for each wave's keys, all ones where their page is one of the cache
+    __device__ __forceinline__ void ask(const Block& from, uint32_t to, uint16_t* there, int wave) {
+        const bool is = from.page >= 0 && from.page < p.cache.pages.pages;
+        const uint32_t page = is ? from.page : 0, inside = is ? from.inside : 0;
+        const char* kb = p.cache.k + 2 * k_place(page, inside);
+        const char* vb = p.cache.v + 2 * v_place(page, inside);
+        constexpr int EACH = 16 * ROW / 1024, KEYS = 1024 / ROW;            // copies of K (and of V), keys of one
+        const uint32_t k0 = to + wave / 2 * (2 * TILE) + (wave & 1) * 16 * ROW;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int piece = wave * EACH + i, key = piece * KEYS + lane * 16 / ROW;
+            const int key = i * KEYS + lane * 16 / ROW;
             int element = 8 * ((lane % (ROW / 16)) ^ (key & SWIZZLE));
             if (!FULL && element >= p.D) element = 0;
-            gather_1k_to_lds((const char*)kb, 2 * ((key & 15) * (uint32_t)p.cache.k_slot + element), stage + piece * 1024);
-            gather_1k_to_lds((const char*)vb, 2 * ((key & 15) * (uint32_t)p.cache.v_slot + element), stage + PA_TILE * ROW + piece * 1024);
+            gather_1k_to_lds(kb, 2 * (key * p.k_slot + element), k0 + i * 1024);
+            gather_1k_to_lds(vb, 2 * (key * p.v_slot + element), k0 + TILE + i * 1024);
         }
+        if (lane == 0) there[wave] = is ? 0xffff : 0;
     }
-    __device__ __forceinline__ void read_k(const char* stage) {
+    __device__ __forceinline__ void read_k(const char* at) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const pa_aligned x = *(const pa_aligned*)(stage + (16 * b + c16) * ROW + 16 * ((4 * ks + g) ^ (c16 & SWIZZLE)));
+                const pa_aligned x = *(const pa_aligned*)(at + (16 * b + c16) * ROW + 16 * ((4 * ks + g) ^ (c16 & SWIZZLE)));
                 k[b][ks] = __builtin_bit_cast(V8, FULL || 32 * ks + 8 * g < p.D ? x : pa_aligned{});
             }
     }
-    __device__ __forceinline__ void read_v(const char* stage) {
+    __device__ __forceinline__ void read_v(const char* at) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
-                    const int row = 16 * b + 4 * g + e, piece = VE == 8 ? 16 * c + c16 : c16 / 2;
+                    const int row = 4 * g + e, piece = VE == 8 ? 16 * c + c16 : c16 / 2;
                     typedef uint32_t Aligned __attribute__((ext_vector_type(VE / 2)));
-                    v[4 * b + e][c] = *(const Aligned*)(stage + PA_TILE * ROW + row * ROW + 16 * (piece ^ (row & SWIZZLE)) + (VE == 8 ? 0 : 8 * (c16 & 1)));
+                    v[4 * b + e][c] = *(const Aligned*)(at + TILE + (16 * b + row) * ROW + 16 * (piece ^ (row & SWIZZLE)) + (VE == 8 ? 0 : 8 * (c16 & 1)));
                 }
     }
 
-    // Tiles first .. last - 1, all four waves on each.
-    __device__ __forceinline__ void run_shared(int first, int last, int wave, char* stages) {
+    // Stages first .. last - 1, all four waves on each.  there: [STAGES][4]
+    __device__ __forceinline__ void run_shared(int first, int last, int wave, char* stages, uint16_t* there) {
         if (first >= last) return;
         const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)stages;
-        constexpr int COPIES = 2 * PIECES / 4;
-        TilePlaces<true> at = {}, next = places(first);
-        uint32_t there[STAGES];
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) {
-            there[i] = next.there;
-            if (first + i < last) ask(next, base + i * STAGE, wave);
-            next = places(first + i + 1);
-        }
-        int stage = 0;
-        for (int t = first; t < last; ++t) {
-            const int behind = last - 1 - t;                     // tiles asked for after this one
-            if (behind >= 2) wait_vm_at_most<2 * COPIES>();
-            else if (behind == 1) wait_vm_at_most<COPIES>();
-            else wait_vm_at_most<0>();
+        ask(block_of(first, wave), base, there, wave);
+        Block next = block_of(first + 1, wave);
+        int now = 0;
+        for (int i = first; i < last; ++i) {
+            wait_vm_at_most<0>();
             lds_barrier();
-            there[STAGES - 1] = next.there;
-            if (t + STAGES - 1 < last) ask(next, base + (stage + STAGES - 1) % STAGES * STAGE, wave);
-            next = places(t + STAGES);
-            const char* from = stages + stage * STAGE;
-            read_k(from);
-            at.there = there[0];
-            tile(t, at, from, [&] { read_v(from); });
-#pragma unroll
-            for (int i = 0; i < STAGES - 1; ++i) there[i] = there[i + 1];
-            stage = (stage + 1) % STAGES;
+            const uint64_t all = *(const uint64_t*)(there + 4 * now);
+            if (i + 1 < last) ask(next, base + (now ^ 1) * STAGE, there + 4 * (now ^ 1), wave);
+            next = block_of(i + 2, wave);
+            TilePlaces<true> at = {};
+#pragma nounroll
+            for (int half = 0; half < 2; ++half) {
+                const char* from = stages + now * STAGE + half * (2 * TILE);
+                at.there = __builtin_amdgcn_readfirstlane((uint32_t)(all >> 32 * half));
+                if (!at.there) continue;
+                read_k(from);
+                tile(2 * i + half, at, from, [&] { read_v(from); });
+            }
+            now ^= 1;
         }
     }
 
@@ -465,6 +479,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
             if (n == 0 && p.N == 1) clear(max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), p.total);
         }
     }
+    constexpr int STEP = SHARED ? 2 * PA_TILE : PA_TILE;         // keys that the splits share out
     const int rows = s.rows * p.group, height = 16 * RT * p.row_groups;
     for (int tile = blockIdx.x / p.splits; tile * height < rows; tile += p.tiles) {
         Wave w(p, s, n, hk, (uint64_t*)((char*)lds + p.odd_at) + wave * 16 * RT * Wave::ODD);
@@ -472,10 +487,10 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
         w.start(row0);
         // (without a mask a row sees no row behind it: nor do the keys behind the last row's matter)
         const int last_token = min((tile * height + height - 1) / p.group, s.rows - 1);
-        const int keys = p.mask ? s.keys : (int)min((int64_t)s.keys, max(s.context + last_token + 1, (int64_t)0)), all = (keys + PA_TILE - 1) / PA_TILE;
+        const int keys = p.mask ? s.keys : (int)min((int64_t)s.keys, max(s.context + last_token + 1, (int64_t)0)), all = (keys + STEP - 1) / STEP;
         const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
         if constexpr (SHARED) {
-            w.run_shared(t0, t1, wave, (char*)lds);
+            w.run_shared(t0, t1, wave, (char*)lds, (uint16_t*)((char*)lds + p.odd_at - 64));
             __syncthreads();
         } else {
             w.run(t0 + kg, t1, key_groups);
@@ -637,8 +652,12 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     while ((1ll << l) < cache->page_size) ++l;
     p.page_shift = 31 + l;
     p.page_magic = (uint32_t)(((1ull << p.page_shift) + cache->page_size - 1) / cache->page_size);
-    // (a page for 16 keys; places inside of them in 32 bits)
-    const bool uniform = cache->page_size % 16 == 0 && std::max(cache->k_stride[1], cache->v_stride[1]) < (1ll << 24) && std::min(cache->k_stride[1], cache->v_stride[1]) >= 0;
+    // (a page for 16 keys; strides in 32 bits)
+    bool uniform = cache->page_size % 16 == 0 && std::max(cache->k_stride[1], cache->v_stride[1]) < (1ll << 24);
+    for (int i = 0; i < 3; ++i)
+        for (int64_t stride : {cache->k_stride[i], cache->v_stride[i]}) uniform = uniform && stride >= 0 && stride < (1ll << 32);
+    p.k_page = (uint32_t)cache->k_stride[0]; p.k_slot = (uint32_t)cache->k_stride[1]; p.k_head = (uint32_t)cache->k_stride[2];
+    p.v_page = (uint32_t)cache->v_stride[0]; p.v_slot = (uint32_t)cache->v_stride[1]; p.v_head = (uint32_t)cache->v_stride[2];
     // (rows on 16-byte boundaries: copies into LDS)
     const PagedCache& v = p.cache;
     const bool whole_pieces = (((uintptr_t)v.k | (uintptr_t)v.v) & 15) == 0 && ((v.k_page | v.k_slot | v.k_head | v.v_page | v.v_slot | v.v_head) & 7) == 0;
@@ -649,7 +668,7 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
         auto launch = [&](auto uniform_, auto full_, auto shared_) {
             constexpr bool UNIFORM = decltype(uniform_)::value, FULL = decltype(full_)::value, SHARED = decltype(shared_)::value;
             typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
-            const size_t joined = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float), room = SHARED ? std::max<size_t>(joined, Wave::STAGES * Wave::STAGE) : joined,
+            const size_t joined = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float), room = 64 + (SHARED ? std::max<size_t>(joined, Wave::STAGES * Wave::STAGE) : joined),
                          smem = room + (size_t)4 * 16 * RT * Wave::ODD * sizeof(uint64_t);
             p.odd_at = (int)room;
             const auto kernel = paged_attn_kernel<T, DT, RT, UNIFORM, FULL, SHARED>;
