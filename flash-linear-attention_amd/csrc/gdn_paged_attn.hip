@@ -91,10 +91,10 @@ template <> struct TilePlaces<false> {
     uint32_t there;
 };
 
-template <typename T, int DT, int RT, bool UNIFORM, bool FULL>
+template <typename T, int DT, int RT, bool UNIFORM, bool FULL, bool SHARED>
 struct PagedWave {
     typedef typename Mma<T>::V8 V8;
-    static constexpr int LD = DT + 4, ODD = DT / 32, ROW = 2 * DT, SWIZZLE = DT == 64 ? 7 : 15;   // LDS: floats of a row of sums, words of odd_bits, bytes of a key
+    static constexpr int LD = DT + 4, ODD = DT / 32, ROW = 2 * DT, PIECES = ROW / 16;   // LDS: floats of a row of sums, words of odd_bits, bytes and 16-byte pieces of a key
     static constexpr int KS = DT / 32, VE = DT >= 128 ? 8 : 4, VC = DT / 16 / VE, MT = DT / 16;     // steps of a score; elements of V at a place, places, products per row tile
     const PagedAttnParams& p;
     const PagedSequence& s;
@@ -102,7 +102,7 @@ struct PagedWave {
     const int hk, lane, c16, g;
     typedef uint32_t VPiece __attribute__((ext_vector_type(VE / 2), aligned(2)));
     V8 q[RT][KS], k[2][KS];
-    VPiece v[8][VC];                         // pairs of elements
+    uint32_t v[DT / 4];                      // pairs: of elements of a key as they lie in memory (operand()), or of keys of an element (SHARED)
     f32x4 o[RT][MT];
     float m[RT], l[RT];
     int token[RT];                           // row of the sequence that the lane's column is; -1: none
@@ -174,9 +174,24 @@ struct PagedWave {
                 if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + ((4 * g + e) * p.v_slot + VE * c16);
                 else at = (const uint16_t*)p.cache.v + __shfl(t.v, 16 * b + 4 * g + e, 64) + VE * c16;
 #pragma unroll
-                for (int c = 0; c < VC; ++c)
-                    v[4 * b + e][c] = *(const VPiece*)(at + (FULL || 128 * c + VE * c16 < p.D ? 128 * c : -VE * c16));
+                for (int c = 0; c < VC; ++c) {
+                    const VPiece x = *(const VPiece*)(at + (FULL || 128 * c + VE * c16 < p.D ? 128 * c : -VE * c16));
+#pragma unroll
+                    for (int t = 0; t < VE / 2; ++t) v[pair(4 * b + e, c, t)] = x[t];
+                }
             }
+    }
+    static constexpr int pair(int j, int c, int t) { return (j * VC + c) * (VE / 2) + t; }
+
+    // The first operand of product t of a row tile, V^T: 16 elements of the eight keys of the lane's contraction indices.
+    __device__ __forceinline__ V8 operand(int t) const {
+        u32x4 a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (SHARED) a[j] = v[4 * t + j];
+            else a[j] = __builtin_amdgcn_perm(v[pair(2 * j + 1, t / VE, t % VE / 2)], v[pair(2 * j, t / VE, t % VE / 2)], t % 2 ? 0x07060302u : 0x05040100u);
+        }
+        return __builtin_bit_cast(V8, a);
     }
 
     __device__ __forceinline__ void start(int row0) {
@@ -264,8 +279,9 @@ struct PagedWave {
             float most = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; ++i) most = fmaxf(most, x[r][i / 4][i % 4]);
-            // (the maximum is the same in the four lanes of a row; it seldom moves once a few tiles are seen)
-            if (__any(most > m[r])) {
+            // m is a maximum that was passed by 2^8 at most: it is the same in the four lanes of a row and moves a few times only (as the true maximum it would move in
+            // four tiles of ten of the first 4000 keys).  The sums' terms are up to 2^8 then, of 2^128 (of 2^16 where weights are rounded to fp16).
+            if (__any(most * p.scale2 > m[r] * p.scale2 + 8.f || (m[r] == -INFINITY && most > m[r]))) {
                 most = fmaxf(most, __shfl_xor(most, 16, 64));
                 most = fmaxf(most, __shfl_xor(most, 32, 64));
                 const float now = fmaxf(m[r], most), keep = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[r] - now) * p.scale2);
@@ -288,16 +304,11 @@ struct PagedWave {
         }
         if (!whole && __any(odd_values())) clean(w, at, stage);
 #pragma unroll
-        for (int c = 0; c < VC; ++c)
+        for (int t = 0; t < MT; ++t) {
+            const V8 a = operand(t);
 #pragma unroll
-            for (int t = 0; t < VE; ++t) {
-                u32x4 a;                                                     // element t of the eight keys
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_perm(v[2 * j + 1][c][t / 2], v[2 * j][c][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
-                const V8 va = __builtin_bit_cast(V8, a);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) o[r][c * VE + t] = Mma<T>::run(va, w[r], o[r][c * VE + t]);
-            }
+            for (int r = 0; r < RT; ++r) o[r][t] = Mma<T>::run(a, w[r], o[r][t]);
+        }
     }
 
     static __device__ __forceinline__ uint32_t carry(uint32_t pair) { return ((pair & PA_EXPONENT<T> * 0x10001u) + PA_CARRY<T> * 0x10001u) & 0x80008000u; }
@@ -305,11 +316,7 @@ struct PagedWave {
     __device__ __forceinline__ bool odd_values() const {
         uint32_t carried = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int t = 0; t < VE / 2; ++t) carried |= carry(v[j][c][t]);
+        for (int i = 0; i < DT / 4; ++i) carried |= carry(v[i]);
         return carried;
     }
     // They are taken out of V and kept in LDS for the rows that see the key, a bit for each row and element: what a sum of infinities and NaN will be, whatever is
@@ -333,11 +340,7 @@ struct PagedWave {
             if (g == r) row = keys;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int t = 0; t < VE / 2; ++t) v[j][c][t] &= ~((carry(v[j][c][t]) >> 15) * 0xffffu);
+        for (int i = 0; i < DT / 4; ++i) v[i] &= ~((carry(v[i]) >> 15) * 0xffffu);
 #pragma nounroll
         for (int key = 0; key < PA_TILE; ++key) {
             if (!(at.there >> key & 1)) continue;
@@ -349,7 +352,7 @@ struct PagedWave {
             for (int i = 0; i < DT / 64; ++i) {
                 const int d = 64 * i + lane;
                 uint16_t bits = 0;
-                if (d < p.D) bits = from[stage ? d ^ (key & SWIZZLE) * 8 : d];
+                if (d < p.D) bits = from[stage ? d ^ swizzle(key) * 8 : d];
                 const bool is = not_a_number<T>(bits), nan = is && (bits & ~PA_EXPONENT<T> & 0x7fffu);
                 const uint64_t up = __ballot(is && (nan || !(bits >> 15))), down = __ballot(is && (nan || bits >> 15));
                 if ((up | down) && g < RT && row >> key & 1) { mine[2 * i] |= up; mine[2 * i + 1] |= down; }
@@ -364,10 +367,12 @@ struct PagedWave {
     }
 
     // ---- four waves on the same keys: 64 at a time through LDS ----
-    // A stage holds K, then V, of two tiles as they lie in memory, the 16-byte pieces of row r XORed with r (so that 16 rows of a column meet no bank twice).  Copies are
+    // A stage holds K, then V, of two tiles as they lie in memory, the 16-byte pieces of row r in places XORed with twice r
+    // (so that eight rows of a piece, and four rows of two pieces, meet no bank twice).  Copies are
     // of 1 KB, straight into LDS, asked for by inline assembly and waited for by hand; a wave makes those of 16 keys, so of one page.
     static constexpr int TILE = PA_TILE * ROW, STAGE = 4 * TILE, STAGES = 2;
 
+    static __device__ __forceinline__ int swizzle(int row) { return (2 * (row & 7) + (row >> 3 & 1)) & (PIECES - 1) & 15; }
     struct Block { int page, inside; };
     __device__ __forceinline__ Block block_of(int stage, int wave) const {
         const int slot = 64 * stage + 16 * wave, index = page_index(slot);
@@ -386,7 +391,7 @@ struct PagedWave {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int key = i * KEYS + lane * 16 / ROW;
-            int element = 8 * ((lane % (ROW / 16)) ^ (key & SWIZZLE));
+            int element = 8 * ((lane % PIECES) ^ swizzle(key));
             if (!FULL && element >= p.D) element = 0;
             gather_1k_to_lds(kb, 2 * (key * p.k_slot + element), k0 + i * 1024);
             gather_1k_to_lds(vb, 2 * (key * p.v_slot + element), k0 + TILE + i * 1024);
@@ -398,21 +403,21 @@ struct PagedWave {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const pa_aligned x = *(const pa_aligned*)(at + (16 * b + c16) * ROW + 16 * ((4 * ks + g) ^ (c16 & SWIZZLE)));
+                const pa_aligned x = *(const pa_aligned*)(at + (16 * b + c16) * ROW + 16 * ((4 * ks + g) ^ swizzle(c16)));
                 k[b][ks] = __builtin_bit_cast(V8, FULL || 32 * ks + 8 * g < p.D ? x : pa_aligned{});
             }
     }
+    // Transposed on the way: lane c16 of a group of 16 names four elements of key 4 g + c16 / 4 and receives element 16 t + c16 of the group's four keys.
     __device__ __forceinline__ void read_v(const char* at) {
+        const int row = 4 * g + c16 / 4;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < VC; ++c) {
-                    const int row = 4 * g + e, piece = VE == 8 ? 16 * c + c16 : c16 / 2;
-                    typedef uint32_t Aligned __attribute__((ext_vector_type(VE / 2)));
-                    v[4 * b + e][c] = *(const Aligned*)(at + TILE + (16 * b + row) * ROW + 16 * (piece ^ (row & SWIZZLE)) + (VE == 8 ? 0 : 8 * (c16 & 1)));
-                }
+            for (int b = 0; b < 2; ++b) {
+                const auto x = Mma<T>::tr_read((const T*)(at + TILE + (16 * b + row) * ROW + 16 * ((2 * t + (c16 & 3) / 2) ^ swizzle(row)) + 8 * (c16 & 1)));
+                const u32x2 two = __builtin_bit_cast(u32x2, x);
+                v[4 * t + 2 * b] = two[0]; v[4 * t + 2 * b + 1] = two[1];
+            }
     }
 
     // Stages first .. last - 1, all four waves on each.  there: [STAGES][4]
@@ -458,7 +463,7 @@ struct PagedWave {
 
 template <typename T, int DT, int RT, bool UNIFORM, bool FULL, bool SHARED>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
-    typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
+    typedef PagedWave<T, DT, RT, UNIFORM, FULL, SHARED> Wave;
     static_assert(!SHARED || UNIFORM, "copies of whole pieces");
     constexpr int VE = Wave::VE, LD = Wave::LD;
     extern __shared__ float lds[];                               // [4 waves][16 RT][LD], then [4 waves][16 RT][2]
@@ -506,20 +511,19 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = wave * 16 * RT + 16 * r + c16;
+            auto put = [&](int d, f32x4 sum) {
+                if (w.odd) sum += f32x4{w.odd_sum(16 * r + c16, d), w.odd_sum(16 * r + c16, d + 1), w.odd_sum(16 * r + c16, d + 2), w.odd_sum(16 * r + c16, d + 3)};
+                *(f32x4*)(lds + row * LD + d) = sum;
+            };
+            if constexpr (SHARED) {
 #pragma unroll
-            for (int c = 0; c < Wave::VC; ++c)
+                for (int t = 0; t < Wave::MT; ++t) put(16 * t + 4 * g, w.o[r][t]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int t = 0; t < Wave::MT; t += 4)
 #pragma unroll
-                    for (int t = 0; t < VE; t += 4) {
-                        f32x4* const to = (f32x4*)(lds + row * LD + 128 * c + VE * (4 * g + e) + t);
-                        f32x4 sum = {w.o[r][c * VE + t][e], w.o[r][c * VE + t + 1][e], w.o[r][c * VE + t + 2][e], w.o[r][c * VE + t + 3][e]};
-                        if (w.odd) {
-                            const int d = 128 * c + VE * (4 * g + e) + t;
-                            sum += f32x4{w.odd_sum(16 * r + c16, d), w.odd_sum(16 * r + c16, d + 1), w.odd_sum(16 * r + c16, d + 2), w.odd_sum(16 * r + c16, d + 3)};
-                        }
-                        *to = sum;
-                    }
+                    for (int e = 0; e < 4; ++e) put(128 * (t / VE) + VE * (4 * g + e) + t % VE, f32x4{w.o[r][t][e], w.o[r][t + 1][e], w.o[r][t + 2][e], w.o[r][t + 3][e]});
+            }
             if (g == 0) { ml[2 * row] = w.m[r] == -INFINITY ? -INFINITY : w.m[r] * p.scale2; ml[2 * row + 1] = w.l[r]; }
         }
         __syncthreads();
@@ -667,7 +671,7 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
         constexpr int DT = decltype(dim)::value, RT = decltype(row_tiles)::value;
         auto launch = [&](auto uniform_, auto full_, auto shared_) {
             constexpr bool UNIFORM = decltype(uniform_)::value, FULL = decltype(full_)::value, SHARED = decltype(shared_)::value;
-            typedef PagedWave<T, DT, RT, UNIFORM, FULL> Wave;
+            typedef PagedWave<T, DT, RT, UNIFORM, FULL, SHARED> Wave;
             const size_t joined = (size_t)4 * 16 * RT * (DT + 4 + 2) * sizeof(float), room = 64 + (SHARED ? std::max<size_t>(joined, Wave::STAGES * Wave::STAGE) : joined),
                          smem = room + (size_t)4 * 16 * RT * Wave::ODD * sizeof(uint64_t);
             p.odd_at = (int)room;
