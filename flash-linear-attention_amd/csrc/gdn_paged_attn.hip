@@ -12,8 +12,7 @@
 // eight keys of V and exchanges them in its registers (one v_perm_b32 per pair).
 //
 // A wave takes tiles of 32 keys by itself, without barriers: K of the next tile is asked for when the scores of this one are formed, V of the next when it is added up, the
-// pages' numbers a tile earlier.  The sequence's keys are shared out over `splits` workgroups and their waves; waves are joined through LDS at the end,
-// workgroups by paged_attn_join_kernel.  The memory system bounds it up to 128 rows.
+// pages' numbers a tile earlier.  Waves that share rows are joined through LDS at the end, workgroups by paged_attn_join_kernel.  The memory system bounds it up to 128 rows.
 #include "gdn_paged.h"
 #include "gdn_chunk_common.h"
 #include <algorithm>
@@ -27,13 +26,14 @@ constexpr int PA_MAX_DIM = 256, PA_TILE = 32;
 struct PagedAttnParams {
     PagedCache cache;
     const void* q; void* o; const void* cu; const uint8_t* mask;
-    float* part_o; float* part_ml;           // [splits][B T HQ][D], [splits][B T HQ][2]: sums, maximum and sum of the weights of a part of the keys
+    int64_t* before;                         // [N + 1]: the work of the sequences before (PagedWork), for the join
+    float* part_o; float* part_ml;           // [2 workgroups][height][D], [..][2]: sums, maximum and sum of the weights of a part of a unit's keys
     int64_t qb, qt, qh;
     int64_t mask_seq, mask_row;
     int64_t T, total;                        // rows of a sequence (dense), of the batch
     uint32_t page_magic; int page_shift;     // slot / page_size = slot * page_magic >> page_shift
     int N, HQ, HK, D, group, mask_cols;
-    int tiles, splits, row_groups, odd_at;
+    int height, step, overhead, groups, row_groups, odd_at;      // rows of a unit; keys of a step, what a unit's beginning and end count as; workgroups; of four waves, those with rows of their own
     uint32_t k_page, k_slot, k_head, v_page, v_slot, v_head;     // the cache's strides where they are below 2^32 (UNIFORM)
     float scale2;                            // |scale| log2(e)
     bool cu_i32, negative;                   // negative: of a negative scale the queries take the sign
@@ -46,6 +46,12 @@ typedef uint16_t pa_aligned __attribute__((ext_vector_type(8)));
 template <typename T> constexpr uint32_t PA_EXPONENT = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
 template <typename T> constexpr uint32_t PA_CARRY = std::is_same_v<T, bf16_t> ? 0x0080 : 0x0400;
 template <typename T> __device__ __forceinline__ bool not_a_number(uint16_t bits) { return (bits & PA_EXPONENT<T>) == PA_EXPONENT<T>; }
+
+// (the same in every lane by construction)
+__device__ __forceinline__ int64_t scalar(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     typedef T two __attribute__((ext_vector_type(2)));
@@ -60,24 +66,87 @@ struct PagedSequence {
     int keys;                                // slots that may be seen: [0, keys)
     int whole;                               // tiles that lie in the context
 };
+template <bool UNIFORM = true>
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedAttnParams& p, int64_t n) {
+    auto load = [](const void* at, int64_t i, bool is_i32) { return UNIFORM ? load_index_uniform(at, i, is_i32) : load_index(at, i, is_i32); };
     PagedSequence s;
     s.first = n * p.T;
     int64_t rows = p.T;
     if (p.cu) {
-        s.first = load_index_uniform(p.cu, n, p.cu_i32);
-        rows = load_index_uniform(p.cu, n + 1, p.cu_i32) - s.first;
+        s.first = load(p.cu, n, p.cu_i32);
+        rows = load(p.cu, n + 1, p.cu_i32) - s.first;
         if (s.first < 0 || s.first > p.total) { s.first = 0; rows = 0; }
         rows = min(rows, p.total - s.first);
     }
     s.rows = (int)max(rows, (int64_t)0);
-    s.context = load_index_uniform(p.cache.context, n, p.cache.context_i32);
+    s.context = load(p.cache.context, n, p.cache.context_i32);
     const int64_t capacity = p.cache.pages.pages > 0 ? p.cache.pages.capacity : 0;
     // (in this order: a context near the end of 64 bits does not overflow)
     s.context = max(min(s.context, capacity), (int64_t)-0x40000000);
     s.keys = (int)max(min(s.context + s.rows, capacity), (int64_t)0);
     s.whole = (int)max(s.context, (int64_t)0) / PA_TILE;
     return s;
+}
+
+// How the work is shared out.  A unit is `height` rows of a sequence at a head of the cache; it counts as its steps of keys and `overhead` (for its beginning and end).
+// The units stand in a row, by sequence, head and rows, and every workgroup takes as much of the row as any other, wherever that begins and ends: contexts of all lengths
+// keep all of them busy to the end, in one round of the chip.  What a workgroup has of a unit that others have parts of goes to the workspace: at most the end of one unit
+// (part 2 w) and the beginning of another (part 2 w + 1).
+struct PagedWork {
+    int tiles, steps;                        // units per head; steps of each
+    int64_t all;
+};
+__device__ __forceinline__ PagedWork paged_work(const PagedAttnParams& p, const PagedSequence& s) {
+    PagedWork w;
+    w.tiles = (s.rows * p.group + p.height - 1) / p.height;
+    w.steps = (s.keys + p.step - 1) / p.step;
+    w.all = (int64_t)p.HK * w.tiles * (w.steps + p.overhead);
+    return w;
+}
+// Workgroup w of `groups` has all w / groups (rounded down) and up to where the next begins: none is empty, because no more of them work than there are places.
+__device__ __forceinline__ int64_t paged_groups(const PagedAttnParams& p, int64_t all) { return min((int64_t)p.groups, all); }
+__device__ __forceinline__ int paged_owner(int64_t x, int64_t all, int64_t groups) { return (int)(((x + 1) * groups - 1) / all); }
+
+// Where a workgroup begins: the sequence with place `from` of the row, and the work before it.  by all 256 threads
+struct PagedStart { int64_t n, before, from, to; };
+__device__ __forceinline__ PagedStart paged_start(const PagedAttnParams& p, int group) {
+    __shared__ int64_t sums[4], found[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    auto work = [&](int64_t n) { return n < p.N ? paged_work(p, paged_sequence<false>(p, n)).all : (int64_t)0; };
+    const int64_t first = work(threadIdx.x);
+    int64_t mine = first;
+    for (int64_t n = threadIdx.x + 256; n < p.N; n += 256) mine += work(n);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d, 64);
+    if (lane == 0) sums[wave] = mine;
+    __syncthreads();
+    const int64_t all = sums[0] + sums[1] + sums[2] + sums[3];
+    const int64_t groups = max(paged_groups(p, all), (int64_t)1);
+    PagedStart at{p.N, 0, group < groups ? all * group / groups : all, group < groups ? all * (group + 1) / groups : all};
+    if (group == 0 && threadIdx.x == 0) p.before[p.N] = all;
+    int64_t before = 0;
+    for (int64_t n0 = 0; n0 < p.N; n0 += 256) {
+        const int64_t n = n0 + threadIdx.x, x = n0 ? work(n) : first;
+        int64_t upto = x;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int64_t y = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += y;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wave] = upto;
+        if (threadIdx.x == 0) found[0] = -1;
+        __syncthreads();
+        upto += before;
+        for (int w = 0; w < wave; ++w) upto += sums[w];
+        if (group == 0 && n < p.N) p.before[n] = upto - x;
+        if (upto - x <= at.from && at.from < upto) { found[0] = n; found[1] = upto - x; }
+        before += sums[0] + sums[1] + sums[2] + sums[3];
+        __syncthreads();
+        if (found[0] >= 0) { at.n = found[0]; at.before = found[1]; }
+        if (group != 0 && before > at.from) break;
+    }
+    return at;
 }
 
 // The places of a tile's keys.  UNIFORM (pages of a multiple of 16 slots): a page for each 16 keys, the same for all lanes.  Else a place for each key, in lane key % 32.
@@ -467,38 +536,40 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
     static_assert(!SHARED || UNIFORM, "copies of whole pieces");
     constexpr int VE = Wave::VE, LD = Wave::LD;
     extern __shared__ float lds[];                               // [4 waves][16 RT][LD], then [4 waves][16 RT][2]
-    const int64_t n = blockIdx.z;
-    const int hk = blockIdx.y, split = blockIdx.x % p.splits, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int rg = wave % p.row_groups, kg = wave / p.row_groups, key_groups = 4 / p.row_groups;
-    const PagedSequence s = paged_sequence(p, n);
-    if (p.cu && blockIdx.x == 0) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = blockIdx.x;
+    const int rg = wave % p.row_groups, kg = wave / p.row_groups, key_groups = 4 / p.row_groups, height = p.height;
+    if (p.cu) {
         // rows of no sequence
-        if (n == 0 || n == p.N - 1) {
-            const int64_t from = n == 0 ? 0 : max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), to = n == 0 ? min(load_index_uniform(p.cu, 0, p.cu_i32), p.total) : p.total;
-            auto clear = [&](int64_t from, int64_t to) {
-                const int width = p.group * p.D;
-                for (int64_t row = from; row < to; ++row)
-                    for (int d = threadIdx.x; d < width; d += 256) ((T*)p.o)[(row * p.HQ + hk * p.group) * p.D + d] = (T)0.f;
-            };
-            clear(from, to);
-            if (n == 0 && p.N == 1) clear(max(load_index_uniform(p.cu, p.N, p.cu_i32), (int64_t)0), p.total);
-        }
+        const int64_t first = max(min(load_index_uniform(p.cu, 0, p.cu_i32), p.total), (int64_t)0), last = max(load_index_uniform(p.cu, p.N, p.cu_i32), first), width = (int64_t)p.HQ * p.D;
+        for (int64_t row = group; row < p.total; row += p.groups)
+            if (row < first || row >= last)
+                for (int64_t d = threadIdx.x; d < width; d += 256) ((T*)p.o)[row * width + d] = (T)0.f;
     }
-    constexpr int STEP = SHARED ? 2 * PA_TILE : PA_TILE;         // keys that the splits share out
-    const int rows = s.rows * p.group, height = 16 * RT * p.row_groups;
-    for (int tile = blockIdx.x / p.splits; tile * height < rows; tile += p.tiles) {
+    const PagedStart start = paged_start(p, group);
+    int64_t n = scalar(start.n), before = scalar(start.before), x = scalar(start.from);
+    const int64_t to = scalar(start.to);
+    while (x < to && n < p.N) {
+        const PagedSequence s = paged_sequence(p, n);
+        const PagedWork work = paged_work(p, s);
+        if (x >= before + work.all) { before += work.all; ++n; continue; }
+        const int per = work.steps + p.overhead, unit = (int)((x - before) / per);
+        const int64_t begins = before + (int64_t)unit * per, ends = min(to, begins + per);
+        const int first = max((int)(x - begins) - p.overhead, 0), last = max((int)(ends - begins) - p.overhead, 0);
+        const bool all_of_it = first == 0 && last == work.steps;
+        const int hk = unit / work.tiles, tile = unit - hk * work.tiles, rows = s.rows * p.group;
+        const bool its_start = x == begins;
+        x = ends;
+        if (first == last && !(work.steps == 0 && its_start)) continue;
         Wave w(p, s, n, hk, (uint64_t*)((char*)lds + p.odd_at) + wave * 16 * RT * Wave::ODD);
-        const int row0 = tile * height + rg * 16 * RT;
-        w.start(row0);
+        w.start(tile * height + rg * 16 * RT);
         // (without a mask a row sees no row behind it: nor do the keys behind the last row's matter)
         const int last_token = min((tile * height + height - 1) / p.group, s.rows - 1);
-        const int keys = p.mask ? s.keys : (int)min((int64_t)s.keys, max(s.context + last_token + 1, (int64_t)0)), all = (keys + STEP - 1) / STEP;
-        const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+        const int keys = p.mask ? s.keys : (int)min((int64_t)s.keys, max(s.context + last_token + 1, (int64_t)0));
         if constexpr (SHARED) {
-            w.run_shared(t0, t1, wave, (char*)lds, (uint16_t*)((char*)lds + p.odd_at - 64));
+            w.run_shared(first, min(last, (keys + 2 * PA_TILE - 1) / (2 * PA_TILE)), wave, (char*)lds, (uint16_t*)((char*)lds + p.odd_at - 64));
             __syncthreads();
         } else {
-            w.run(t0 + kg, t1, key_groups);
+            w.run(first * key_groups + kg, min(last * key_groups, (keys + PA_TILE - 1) / PA_TILE), key_groups);
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -544,12 +615,12 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
             }
             const int token = at / p.group;
             const int64_t out = (s.first + token) * p.HQ + hk * p.group + (at - token * p.group);
-            if (p.splits == 1) {
+            if (all_of_it) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 typedef T piece __attribute__((ext_vector_type(4)));
                 *(piece*)((T*)p.o + out * p.D + d) = piece{(T)(sum[0] * inv), (T)(sum[1] * inv), (T)(sum[2] * inv), (T)(sum[3] * inv)};
             } else {
-                const int64_t part = split * (p.total * p.HQ) + out;
+                const int64_t part = (int64_t)(2 * group + (first == 0)) * height + row;
                 *(f32x4*)(p.part_o + part * p.D + d) = sum;
                 if (d == 0) { p.part_ml[2 * part] = m; p.part_ml[2 * part + 1] = l; }
             }
@@ -558,38 +629,64 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attn_kernel(Page
     }
 }
 
-// The parts of a row's keys, joined: a wave per row, a part's weight in the lane of its number.
-template <typename T>
+// The parts of a row's keys, joined, where several workgroups have some: by a wave, or by four where a unit has many parts.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnParams p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64, rows = p.total * p.HQ;
-    if (row >= rows) return;
-    if (p.cu) {
-        const int64_t token = row / p.HQ;
-        if (sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); }) < 0) return;
-    }
-    float m = -INFINITY, l = 0.f;
-    if (lane < p.splits) {
-        const float* ml = p.part_ml + 2 * (lane * rows + row);
-        m = ml[0]; l = ml[1];
-    }
-    float most = m;
+    constexpr int AHEAD = 4;
+    __shared__ f32x4 sums[WAVES][64];
+    __shared__ float weights[WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), sub = wave % WAVES;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+    if (row >= p.total * p.HQ) return;                           // (four waves of a row end together)
+    const int64_t token = row / p.HQ;
+    const int h = (int)(row - token * p.HQ), hk = h / p.group;
+    const int64_t n = p.cu ? sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); }) : token / p.T;
+    if (n < 0) return;
+    const PagedSequence s = paged_sequence<false>(p, n);
+    const PagedWork work = paged_work(p, s);
+    const int64_t i = (token - s.first) * p.group + h - hk * p.group;
+    if (work.steps == 0 || i < 0 || i >= (int64_t)s.rows * p.group) return;
+    const int tile = (int)(i / p.height), at = (int)(i - (int64_t)tile * p.height);
+    const int64_t all = p.before[p.N], groups = paged_groups(p, all), begins = p.before[n] + ((int64_t)hk * work.tiles + tile) * (work.steps + p.overhead) + p.overhead;
+    const int first = paged_owner(begins, all, groups), last = paged_owner(begins + work.steps - 1, all, groups);
+    if (first == last) return;
+    auto part = [&](int w) { return (int64_t)(2 * w + (w == first)) * p.height + at; };
+    float m = -INFINITY;
+    for (int w = first + lane; w <= last; w += 64) m = fmaxf(m, p.part_ml[2 * part(w)]);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
-    const float keep = __builtin_amdgcn_exp2f(m - (most == -INFINITY ? 0.f : most));
-    l *= keep;
-    float all = l;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
-    const uint64_t some = __ballot(lane < p.splits && l != 0.f);
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const float base = m == -INFINITY ? 0.f : m;
     const int d = 4 * lane;
+    float l = 0.f;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (uint64_t left = some; left; left &= left - 1) {
-        const int part = __builtin_ctzll(left);
-        const float weight = __shfl(keep, part, 64);
-        if (d < p.D) sum += *(const f32x4*)(p.part_o + (part * rows + row) * p.D + d) * weight;
+    for (int w = first + sub; w <= last; w += AHEAD * WAVES) {
+        f32x4 x[AHEAD];
+        float ml[AHEAD][2];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int we = w + e * WAVES;
+            const int64_t from = part(min(we, last));
+            ml[e][0] = we <= last ? p.part_ml[2 * from] : -INFINITY;
+            ml[e][1] = p.part_ml[2 * from + 1];
+            x[e] = d < p.D ? *(const f32x4*)(p.part_o + from * p.D + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            if (w + e * WAVES > last) continue;
+            const float keep = __builtin_amdgcn_exp2f(ml[e][0] - base);
+            l += ml[e][1] * keep;
+            sum += x[e] * keep;
+        }
     }
-    const float inv = all == 0.f ? 0.f : 1.f / all;
+    if constexpr (WAVES > 1) {
+        sums[sub][lane] = sum;
+        if (lane == 0) weights[sub] = l;
+        __syncthreads();
+        if (sub) return;
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) { sum += sums[k][lane]; l += weights[k]; }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     typedef T piece __attribute__((ext_vector_type(4)));
     if (d < p.D) *(piece*)((T*)p.o + row * p.D + d) = piece{(T)(sum[0] * inv), (T)(sum[1] * inv), (T)(sum[2] * inv), (T)(sum[3] * inv)};
 }
@@ -600,25 +697,42 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     if (rc != GDN_OK) return rc;
     GDN_CHECK_ARG(c->HQ % cache->heads == 0, GDN_ERR_INVALID, "%s: the queries' heads are a multiple of the cache's", who);
     GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM && cache->dim % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of a multiple of 8 up to %d elements", who, PA_MAX_DIM);
-    GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->T * c->HQ < (1ll << 31) && cache->heads <= 65535 && c->N <= 65535 && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
-                  "%s: up to 65535 sequences and heads of the cache, rows times heads below 2^31", who);
+    GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->B * c->T * c->HQ < (1ll << 31) && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
+                  "%s: rows times heads below 2^31, up to 2^30 slots of a sequence", who);
     return GDN_OK;
 }
 
-// How the work is cut.
-struct PagedAttnPlan { int dim, row_tiles, row_groups, tiles, splits; };
-static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_attn_call* c) {
+struct PagedAttnPlan { int dim, row_tiles, row_groups, height, step, overhead, groups; bool many_parts; size_t bytes; };
+static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, bool shares) {
     PagedAttnPlan plan;
     const int64_t rows = std::max<int64_t>(1, std::min(c->max_rows, c->T)) * (c->HQ / cache->heads);
     plan.dim = cache->dim <= 64 ? 64 : cache->dim <= 128 ? 128 : 256;
     plan.row_tiles = plan.dim == 256 || rows <= 16 ? 1 : 2;
     const int64_t each = 16 * plan.row_tiles;
     plan.row_groups = rows <= each ? 1 : rows <= 2 * each ? 2 : 4;
-    plan.tiles = (int)((rows + each * plan.row_groups - 1) / (each * plan.row_groups));
-    const int64_t units = std::max<int64_t>(1, c->N * cache->heads * plan.tiles), key_tiles = (cache->table_cols * cache->page_size + PA_TILE - 1) / PA_TILE;
-    const int64_t most = std::max<int64_t>(1, key_tiles / (2 * (4 / plan.row_groups)));
-    plan.splits = (int)std::min<int64_t>(std::min<int64_t>(64, most), std::max<int64_t>(1, (2048 + units - 1) / units));
+    plan.height = (int)(each * plan.row_groups);
+    plan.step = shares && plan.row_groups == 4 ? 2 * PA_TILE : PA_TILE * (4 / plan.row_groups);
+    // What a unit costs besides its keys, in steps.  Measured, us a call (1, 2, 4, 6, 8 steps): 16 sequences of up to 8000 keys with trees of 64 rows 219, 189, 166, 148, 149 (through
+    // LDS); 32 of up to 8000 with 8 rows 142, 129, 131, 131, 133; 256 of up to 1000 with one row 115, 117, 123, 123, 124.
+    plan.overhead = shares && plan.row_groups == 4 ? 6 : plan.row_tiles;
+    // One round of the chip: two workgroups share a CU (one where a head of 256 takes a wave's registers), but no more than there can be steps.
+    const int64_t units = std::max<int64_t>(1, c->N) * cache->heads * ((rows + plan.height - 1) / plan.height);
+    const int64_t steps = std::max<int64_t>(1, (cache->table_cols * cache->page_size + plan.step - 1) / plan.step);
+    plan.groups = (int)std::min<int64_t>(plan.dim == 256 ? 256 : 512, units * steps);
+    plan.many_parts = plan.groups > 8 * units;
+    plan.bytes = ((size_t)c->N + 2) / 2 * 16 + (size_t)2 * plan.groups * plan.height * (cache->dim + 2) * sizeof(float);
     return plan;
+}
+// Rows on 16-byte boundaries: copies into LDS.
+static bool whole_pieces(const PagedCache& v) {
+    return (((uintptr_t)v.k | (uintptr_t)v.v) & 15) == 0 && ((v.k_page | v.k_slot | v.k_head | v.v_page | v.v_slot | v.v_head) & 7) == 0;
+}
+// A page for 16 keys; strides in 32 bits.
+static bool uniform_tiles(const gdn_paged_cache* c) {
+    bool is = c->page_size % 16 == 0 && std::max(c->k_stride[1], c->v_stride[1]) < (1ll << 24);
+    for (int i = 0; i < 3; ++i)
+        for (int64_t stride : {c->k_stride[i], c->v_stride[i]}) is = is && stride >= 0 && stride < (1ll << 32);
+    return is;
 }
 
 }  // namespace gdn
@@ -628,8 +742,7 @@ using namespace gdn;
 extern "C" size_t gdn_paged_attn_workspace_bytes(const gdn_paged_cache* cache, const gdn_paged_attn_call* c) {
     PagedCache view;
     if (check_attn("gdn_paged_attn_workspace_bytes", cache, c, view) != GDN_OK || c->B * c->T * c->HQ == 0) return 0;
-    const PagedAttnPlan plan = attn_plan(cache, c);
-    return plan.splits == 1 ? 0 : (size_t)plan.splits * (size_t)(c->B * c->T * c->HQ) * (size_t)(cache->dim + 2) * sizeof(float);
+    return attn_plan(cache, c, uniform_tiles(cache) && whole_pieces(view)).bytes;
 }
 
 extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, void* workspace, size_t workspace_bytes, void* stream) {
@@ -639,33 +752,26 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     if (rc != GDN_OK) return rc;
     if (c->B * c->T * c->HQ == 0) return GDN_OK;
     GDN_CHECK_ARG(c->q && c->o, GDN_ERR_INVALID, "%s: missing tensors", who);
-    const PagedAttnPlan plan = attn_plan(cache, c);
-    const size_t need = gdn_paged_attn_workspace_bytes(cache, c);
-    GDN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), GDN_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned", who, need);
+    const bool uniform = uniform_tiles(cache), shares = uniform && whole_pieces(p.cache);
+    const PagedAttnPlan plan = attn_plan(cache, c, shares);
+    GDN_CHECK_ARG(workspace && workspace_bytes >= plan.bytes && (uintptr_t)workspace % 16 == 0, GDN_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned", who, plan.bytes);
     p.q = c->q; p.o = c->o; p.cu = c->cu_seqlens; p.mask = c->mask;
     p.qb = c->q_stride[0]; p.qt = c->q_stride[1]; p.qh = c->q_stride[2];
     p.mask_seq = c->mask_seq_stride; p.mask_row = c->mask_row_stride; p.mask_cols = (int)c->mask_cols;
     p.T = c->T; p.total = c->B * c->T; p.N = (int)c->N; p.HQ = (int)c->HQ; p.HK = (int)cache->heads; p.D = (int)cache->dim; p.group = p.HQ / p.HK;
     p.cu_i32 = c->flags & GDN_FLAG_CU_INT32;
     p.scale2 = std::fabs(c->scale) * 1.4426950408889634f; p.negative = c->scale < 0;
-    p.tiles = plan.tiles; p.splits = plan.splits; p.row_groups = plan.row_groups;
-    p.part_o = (float*)workspace;
-    p.part_ml = p.part_o + (size_t)plan.splits * (size_t)(p.total * p.HQ) * (size_t)p.D;
+    p.overhead = plan.overhead; p.height = plan.height; p.step = plan.step; p.groups = plan.groups; p.row_groups = plan.row_groups;
+    p.before = (int64_t*)workspace;
+    p.part_o = (float*)((char*)workspace + (c->N + 2) / 2 * 16);
+    p.part_ml = p.part_o + (size_t)2 * plan.groups * plan.height * (size_t)p.D;
     // slot / page_size for slots below 2^31: ceil(2^(31 + l) / page_size), l = ceil(log2 page_size), is below 2^32 and exact
     int l = 0;
     while ((1ll << l) < cache->page_size) ++l;
     p.page_shift = 31 + l;
     p.page_magic = (uint32_t)(((1ull << p.page_shift) + cache->page_size - 1) / cache->page_size);
-    // (a page for 16 keys; strides in 32 bits)
-    bool uniform = cache->page_size % 16 == 0 && std::max(cache->k_stride[1], cache->v_stride[1]) < (1ll << 24);
-    for (int i = 0; i < 3; ++i)
-        for (int64_t stride : {cache->k_stride[i], cache->v_stride[i]}) uniform = uniform && stride >= 0 && stride < (1ll << 32);
     p.k_page = (uint32_t)cache->k_stride[0]; p.k_slot = (uint32_t)cache->k_stride[1]; p.k_head = (uint32_t)cache->k_stride[2];
     p.v_page = (uint32_t)cache->v_stride[0]; p.v_slot = (uint32_t)cache->v_stride[1]; p.v_head = (uint32_t)cache->v_stride[2];
-    // (rows on 16-byte boundaries: copies into LDS)
-    const PagedCache& v = p.cache;
-    const bool whole_pieces = (((uintptr_t)v.k | (uintptr_t)v.v) & 15) == 0 && ((v.k_page | v.k_slot | v.k_head | v.v_page | v.v_slot | v.v_head) & 7) == 0;
-    const dim3 grid((unsigned)(plan.tiles * plan.splits), (unsigned)cache->heads, (unsigned)c->N);
     auto go = [&](auto t, auto dim, auto row_tiles) {
         typedef decltype(t) T;
         constexpr int DT = decltype(dim)::value, RT = decltype(row_tiles)::value;
@@ -677,19 +783,20 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
             p.odd_at = (int)room;
             const auto kernel = paged_attn_kernel<T, DT, RT, UNIFORM, FULL, SHARED>;
             const int made = ensure_dynamic_smem_for((const void*)kernel, smem, who);
-            if (made == GDN_OK) hipLaunchKernelGGL(kernel, grid, dim3(256), smem, (hipStream_t)stream, p);
+            if (made == GDN_OK) hipLaunchKernelGGL(kernel, dim3((unsigned)plan.groups), dim3(256), smem, (hipStream_t)stream, p);
             return made;
         };
         auto full = [&](auto uniform_, auto shared_) { return p.D == DT ? launch(uniform_, std::true_type(), shared_) : launch(uniform_, std::false_type(), shared_); };
         int made;
         if (!uniform) made = full(std::false_type(), std::false_type());
-        else if (plan.row_groups < 4 || !whole_pieces) made = full(std::true_type(), std::false_type());
+        else if (plan.row_groups < 4 || !shares) made = full(std::true_type(), std::false_type());
         else if constexpr (RT == 2 || DT == 256) made = full(std::true_type(), std::true_type());
         else made = GDN_ERR_UNSUPPORTED;
         if (made != GDN_OK) return made;
         const int ran = check_launch("paged_attn_kernel");
-        if (ran != GDN_OK || plan.splits == 1) return ran;
-        hipLaunchKernelGGL(paged_attn_join_kernel<T>, dim3((unsigned)((p.total * p.HQ + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
+        if (ran != GDN_OK || plan.groups == 1) return ran;
+        if (plan.many_parts) hipLaunchKernelGGL((paged_attn_join_kernel<T, 4>), dim3((unsigned)(p.total * p.HQ)), dim3(256), 0, (hipStream_t)stream, p);
+        else hipLaunchKernelGGL((paged_attn_join_kernel<T, 1>), dim3((unsigned)((p.total * p.HQ + 3) / 4)), dim3(256), 0, (hipStream_t)stream, p);
         return check_launch("paged_attn_join_kernel");
     };
     auto dims = [&](auto t) {
