@@ -21,7 +21,7 @@ OUT_DIR = os.path.join(HERE, 'fla_hip', '_C')
 LIB = os.path.join(OUT_DIR, 'libgdn_hip.so')
 OBJ_DIR = os.path.join(HERE, 'build', 'obj')
 HOST_SRC = os.path.join(CSRC, 'host', 'gdn_host.cpp')
-HOST_HDRS = [os.path.join(CSRC, 'host', name) for name in ('gdn_host_train.h', 'gdn_host_block.h')]
+HOST_HDRS = [os.path.join(CSRC, 'host', name) for name in ('gdn_host_train.h', 'gdn_host_block.h', 'gdn_host_serving.h')]
 HOST_LIB = os.path.join(OUT_DIR, 'gdn_host.so')
 HOST_TORCH = os.path.join(OBJ_DIR, 'gdn_host.torch')      # the torch that HOST_LIB was built with
 

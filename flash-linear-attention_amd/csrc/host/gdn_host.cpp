@@ -44,6 +44,13 @@ decltype(&gdn_gated_mlp_fwd) p_gated_mlp_fwd;
 decltype(&gdn_gated_mlp_bwd) p_gated_mlp_bwd;
 decltype(&gdn_gated_mlp_workspace_bytes) p_gated_mlp_workspace_bytes;
 decltype(&gdn_pad_rows) p_pad_rows;
+decltype(&gdn_rotary) p_rotary;
+decltype(&gdn_paged_append) p_paged_append;
+decltype(&gdn_paged_keep) p_paged_keep;
+decltype(&gdn_paged_attn) p_paged_attn;
+decltype(&gdn_paged_attn_workspace_bytes) p_paged_attn_workspace_bytes;
+decltype(&gdn_verify_drafts) p_verify_drafts;
+decltype(&gdn_verify_drafts_workspace_bytes) p_verify_drafts_workspace_bytes;
 decltype(&gdn_last_error) p_last_error;
 
 PyObject* bind(PyObject*, PyObject* table) {
@@ -61,7 +68,9 @@ PyObject* bind(PyObject*, PyObject* table) {
         !take("gdn_causal_conv1d_fwd", p_conv_fwd) || !take("gdn_causal_conv1d_bwd_runs", p_conv_bwd_runs) || !take("gdn_gate_bwd", p_gate_bwd) ||
         !take("gdn_layer_norm_fwd", p_layer_norm_fwd) || !take("gdn_layer_norm_bwd", p_layer_norm_bwd) || !take("gdn_layer_norm_bwd_parts", p_layer_norm_bwd_parts) ||
         !take("gdn_gated_mlp_fwd", p_gated_mlp_fwd) || !take("gdn_gated_mlp_bwd", p_gated_mlp_bwd) || !take("gdn_gated_mlp_workspace_bytes", p_gated_mlp_workspace_bytes) ||
-        !take("gdn_pad_rows", p_pad_rows) ||
+        !take("gdn_pad_rows", p_pad_rows) || !take("gdn_rotary", p_rotary) || !take("gdn_paged_append", p_paged_append) || !take("gdn_paged_keep", p_paged_keep) ||
+        !take("gdn_paged_attn", p_paged_attn) || !take("gdn_paged_attn_workspace_bytes", p_paged_attn_workspace_bytes) ||
+        !take("gdn_verify_drafts", p_verify_drafts) || !take("gdn_verify_drafts_workspace_bytes", p_verify_drafts_workspace_bytes) ||
         !take("gdn_sum_rows", p_sum_rows) || !take("gdn_last_error", p_last_error))
         return nullptr;
     Py_RETURN_NONE;
@@ -400,6 +409,7 @@ PyObject* layer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #include "gdn_host_train.h"
 #include "gdn_host_block.h"
+#include "gdn_host_serving.h"
 
 PyMethodDef methods[] = {
     {"chunk_train", (PyCFunction)(void*)chunk_train, METH_FASTCALL, "chunked operator with gradients; None: not a call for the native path"},
@@ -407,6 +417,11 @@ PyMethodDef methods[] = {
     {"layer_step", (PyCFunction)(void*)layer_step, METH_FASTCALL, "one decode step of the layer; None: not a call for the native path"},
     {"layer_norm", (PyCFunction)(void*)layer_norm, METH_FASTCALL, "normalisation with the residual stream; None: not a call for the native path"},
     {"gated_mlp", (PyCFunction)(void*)gated_mlp, METH_FASTCALL, "the gated feed-forward block; None: not a call for the native path"},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, "rotary positions; None: not a call for the native path"},
+    {"paged_append", (PyCFunction)(void*)paged_append, METH_FASTCALL, "rows into the paged cache; None: not a call for the native path"},
+    {"paged_attn", (PyCFunction)(void*)paged_attn, METH_FASTCALL, "attention over the paged cache; None: not a call for the native path"},
+    {"paged_keep", (PyCFunction)(void*)paged_keep, METH_FASTCALL, "rows moved in the paged cache; None: not a call for the native path"},
+    {"verify_drafts", (PyCFunction)(void*)verify_drafts, METH_FASTCALL, "verification of drafts; None: not a call for the native path"},
     {"bind", bind, METH_O, "bind({name: address}) - entry points of libgdn_hip.so"},
     {"fused_recurrent", (PyCFunction)(void*)fused_recurrent, METH_FASTCALL, "token recurrence; None: not a call for the native path"},
     {"chunk_fwd", (PyCFunction)(void*)chunk_fwd, METH_FASTCALL, "chunked forward; None: not a call for the native path"},

@@ -264,6 +264,7 @@ class _PythonHost:
         return None
 
     fused_recurrent = chunk_fwd = chunk_train = layer_step = layer_train = layer_norm = gated_mlp = _leave
+    rotary = paged_append = paged_attn = paged_keep = verify_drafts = _leave
 
 
 _host = None

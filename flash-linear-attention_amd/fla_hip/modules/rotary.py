@@ -87,6 +87,10 @@ class RotaryFunction(torch.autograd.Function):
 
 
 def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlens, max_seqlen, positions) -> tuple:
+    if not inplace:
+        ys = _lib.host().rotary(xs[0], xs[1] if len(xs) > 1 else None, cos, sin, interleaved, seqlen_offsets, cu_seqlens, max_seqlen, positions)
+        if ys is not None:
+            return ys
     x = xs[0]
     dev = require_gpu(*xs, cos, sin)
     for other in xs:

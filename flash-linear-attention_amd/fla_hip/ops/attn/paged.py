@@ -80,6 +80,9 @@ def paged_append(
     turned on the way (``fla_hip.modules.rotary_embedding``), and so are the queries ``q [B, T, query heads, dim]``, which are returned (None without q): at
     ``positions [B, T]``, by default the slot's number.  Rows whose slot has no page, and rows of no sequence, write nothing.  In the type of the cache; forward only.
     A page that is written belongs to one sequence."""
+    done = _lib.host().paged_append(k, v, k_cache, v_cache, page_table, context_lens, cu_seqlens, max_seqlen, q, cos, sin, positions, interleaved)
+    if done is not None:
+        return done[0]
     dev = require_gpu(k, v, k_cache, v_cache, page_table, context_lens, *(t for t in (q, cos, sin, positions, cu_seqlens) if t is not None))
     if k.dim() != 4 or v.shape != k.shape or (q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3])):
         raise ValueError(f'k and v must be [B, T, heads, dim] and q agree with them, got {tuple(k.shape)}, {tuple(v.shape)}' + ('' if q is None else f' and {tuple(q.shape)}'))
@@ -125,6 +128,9 @@ def paged_attn(
     truth values ``[T, columns]`` (one tree for all), ``[B, T, columns]``, or ``[rows, columns]`` of a packed batch; row i sees row j of its sequence where ``tree_mask[.., i, j]``,
     columns that are missing are not seen.  A row that sees nothing, and one of no sequence, gets 0.  ``scale``: default ``dim ** -0.5``.  ``max_seqlen`` (packed): at
     least the longest sequence's rows, then the boundaries are not read by the host.  bf16 or fp16, dim a multiple of 8 up to 256; forward only."""
+    o = _lib.host().paged_attn(q, k_cache, v_cache, page_table, context_lens, tree_mask, scale, cu_seqlens, max_seqlen)
+    if o is not None:
+        return o
     dev = require_gpu(q, k_cache, v_cache, page_table, context_lens, *(t for t in (tree_mask, cu_seqlens) if t is not None))
     if q.dim() != 4 or k_cache.dim() != 4 or q.shape[3] != k_cache.shape[3]:
         raise ValueError(f'q must be [B, T, heads, dim] with the dim of the cache, got {tuple(q.shape)} and {tuple(k_cache.shape)}')
@@ -171,6 +177,8 @@ def paged_keep(
     """The rows of a step that stand, moved to the front of its slots: slot ``context_lens[n] + i`` becomes what slot ``context_lens[n] + rows[n, i]`` was, for
     ``i < num_kept[n]`` (rows ``[N, R]`` int32 with ``rows[n, i] >= i``, num_kept ``[N]``: the path and the count that ``verify_drafts`` returns).  Any other entry, and one whose
     slots have no page, leaves its slot as it is.  The positions that keys were turned by stay: a node of a tree is at the same depth before and after."""
+    if _lib.host().paged_keep(k_cache, v_cache, page_table, context_lens, rows, num_kept) is not None:
+        return
     dev = require_gpu(k_cache, v_cache, page_table, context_lens, rows, num_kept)
     if rows.dim() != 2:
         raise ValueError(f'rows must be [N, R], got {list(rows.shape)}')

@@ -29,6 +29,9 @@ def verify_drafts(
 
     Returns ``(next_token [N] int64, num_accepted [N] int32, rows [N, R] int32)``: the token to go on with (-1 where p has no finite mass), the number of rows that stand, row 0
     among them, and which, in order, -1 behind them.  Computed in 64 bits; nothing of it is differentiable."""
+    out = _lib.host().verify_drafts(target_probs, draft_tokens, uniforms, parents, draft_probs, lengths)
+    if out is not None:
+        return out
     dev = require_gpu(target_probs, draft_tokens, uniforms, *(t for t in (parents, draft_probs, lengths) if t is not None))
     if target_probs.dim() != 3 or target_probs.shape[1] < 1 or target_probs.shape[2] < 1:
         raise ValueError(f'target_probs must be [N, R, V], got {list(target_probs.shape)}')

@@ -276,6 +276,7 @@ def lib(monkeypatch):
     from fla_hip.ops.gated_delta_rule import _common
     lib = _Library()
     monkeypatch.setattr(_lib, 'load', lambda: lib)
+    monkeypatch.setattr(_lib, 'host', lambda: _lib._PythonHost)
     monkeypatch.setattr(_common, 'current_device', lambda: None)
     monkeypatch.setattr(_common, 'current_stream_ptr', lambda dev: 0)
     monkeypatch.setattr(paged, 'require_gpu', lambda x, *_: x.device)
