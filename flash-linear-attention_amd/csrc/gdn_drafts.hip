@@ -10,7 +10,7 @@
 // The sums are kept for every SEGMENT words: the token is found in the segment where the running sum crosses u_0 times the whole, by reading it again.
 //
 // Everything that decides is in 64 bits and in a fixed order.  Bounded by the memory system for many sequences and words, by latency for few: the first pass, for most
-// sequences the only one, is shared out over workgroups (drafts_first_kernel), each of which walks to it by itself, and one workgroup per sequence finishes.
+// sequences the only one, is shared out over workgroups (drafts_round_kernel), each of which walks to it by itself, and one workgroup per sequence finishes.
 #include "gdn_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -25,7 +25,9 @@ struct DraftParams {
     int64_t p_seq, p_row, q_seq, q_row, parents_stride;
     int R, V, segments;
     bool tokens64;
-    double* sums;                                  // [N][segments]: of the first pass, or NULL
+    double* sums;                                  // [rounds][N][segments]: of the first passes
+    int64_t N;
+    int rounds;
 };
 
 // Where a sequence has come to.
@@ -50,6 +52,8 @@ __device__ __forceinline__ double weight(bool sampled, double a, double b, doubl
     const double w = sampled ? a * p - b * q : a * p;
     return w > 0.0 ? w : 0.0;
 }
+
+__device__ __forceinline__ int rows_of(const DraftParams& p, int64_t n) { return p.lengths ? min(max(p.lengths[n], 1), p.R) : p.R; }
 
 template <typename T>
 __device__ void draft_tests(const DraftParams& p, int64_t n, int rows, DraftShared& s) {
@@ -155,29 +159,6 @@ __device__ double segment_sum(const DraftParams& p, int64_t n, const DraftShared
     return sum;
 }
 
-// The sums of all segments into s.sums, by the whole workgroup, and their sum (in order, by wave 0 into s.total).  `from`: they are in memory already.
-template <typename T>
-__device__ void draft_pass(const DraftParams& p, int64_t n, DraftShared& s, const DraftWeights& w, const double* from) {
-    const int waves = blockDim.x / 64, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    if (from) {
-        for (int k = threadIdx.x; k < p.segments; k += blockDim.x) s.sums[k] = from[k];
-    } else {
-        for (int k = wave; k < p.segments; k += waves) {
-            const double sum = p.q ? segment_sum<T, true>(p, n, s, w, k) : segment_sum<T, false>(p, n, s, w, k);
-            if (lane == 0) s.sums[k] = sum;
-        }
-    }
-    __syncthreads();
-    if (wave == 0) {
-        double sum = 0.0;
-        for (int k = lane; k < p.segments; k += 64) sum += s.sums[k];
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-        if (lane == 0) s.total = sum;
-    }
-    __syncthreads();
-}
-
 __device__ __forceinline__ double scan_add(double x) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -211,23 +192,39 @@ __device__ int draft_word(const DraftParams& p, int64_t n, const DraftShared& s,
     if (!found) segment = filled;
     if (segment < 0) return -1;
     constexpr int EACH = DRAFT_SEGMENT / 64;
+    constexpr int VEC = 16 / sizeof(T);
     const T* pr = (const T*)p.p + n * p.p_seq + w.here * p.p_row;
     const T* qr = (const T*)p.q + n * p.q_seq + w.here * p.q_row;
     const int first = segment * DRAFT_SEGMENT + lane * EACH;
     double x[EACH], sum = 0.0;
     int last = -1;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int v = first + e;
-        x[e] = 0.0;
-        if (v < p.V) {
-            x[e] = weight(p.q != nullptr, w.a, w.b, mass_of(pr[v]), p.q ? mass_of(qr[v]) : 0.0);
-            if (!p.q)
-                for (int j = 0; j < w.refused; ++j)
-                    if (s.refused[j] == v) x[e] = 0.0;
+    for (int k = 0; k < EACH; k += VEC) {
+        Words<T, VEC> a = {}, b = {};
+        if (first + k + VEC <= p.V) {
+            a = *(const Words<T, VEC>*)(pr + first + k);
+            if (p.q) b = *(const Words<T, VEC>*)(qr + first + k);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                a.e[e] = first + k + e < p.V ? pr[first + k + e] : (T)0.f;
+                if (p.q) b.e[e] = first + k + e < p.V ? qr[first + k + e] : (T)0.f;
+            }
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[k + e] = weight(p.q != nullptr, w.a, w.b, mass_of(a.e[e]), p.q ? mass_of(b.e[e]) : 0.0);
+    }
+    if (!p.q)
+        for (int j = 0; j < w.refused; ++j) {
+            const int at = s.refused[j] - first;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+                if (e == at) x[e] = 0.0;
+        }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
         sum += x[e];
-        if (x[e] > 0.0) last = v;
+        if (x[e] > 0.0) last = first + e;
     }
     const double upto = before + scan_add(sum);
     const uint64_t passed = __ballot(found && upto > t && sum > 0.0);
@@ -249,79 +246,92 @@ __device__ int draft_word(const DraftParams& p, int64_t n, const DraftShared& s,
     return last;
 }
 
-__device__ __forceinline__ int rows_of(const DraftParams& p, int64_t n) { return p.lengths ? min(max(p.lengths[n], 1), p.R) : p.R; }
 
-__device__ __forceinline__ void start_walk(DraftShared& s) {
+// A sequence's walk from pass to pass, the same in every workgroup that makes it: pass i is taken from memory where an earlier launch made it, else `make(weights)` makes
+// it, or says that it ends here (false).  `finish(walk, weights)`: the last pass has been made.
+template <typename T, typename Make, typename Finish>
+__device__ __forceinline__ void draft_passes(const DraftParams& p, int64_t n, DraftShared& s, int made, Make&& make, Finish&& finish) {
+    const int rows = rows_of(p, n);
+    draft_tests<T>(p, n, rows, s);
     if (threadIdx.x == 0) {
         s.walk = DraftWalk{0, 0, 1, 0, 0, 1.0, 0.0};
         s.path[0] = 0;
     }
+    __syncthreads();
+    bool again = false;                                            // nothing was left: what was there before, added up again
+    for (int pass = 0;; ++pass) {
+        if (!again) {
+            if (threadIdx.x < 64) draft_walk(p, rows, s);
+            __syncthreads();
+        }
+        DraftWalk walk = s.walk;
+        const DraftWeights w = weights_of(walk, walk.asks);
+        if (pass < made) {
+            const double* from = p.sums + (pass * p.N + n) * p.segments;
+            for (int k = threadIdx.x; k < p.segments; k += blockDim.x) s.sums[k] = from[k];
+        } else if (!make(w)) {
+            return;
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            double sum = 0.0;
+            for (int k = threadIdx.x; k < p.segments; k += 64) sum += s.sums[k];
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+            if (threadIdx.x == 0) s.total = sum;
+        }
+        __syncthreads();
+        // (every wave looks: rows asked later that follow the same row)
+        const bool more = walk.asks && next_draft(s, walk.here, walk.last, rows) < rows;
+        const bool some = s.total > 0.0;
+        if (again || (!more && (some || !walk.asks))) {
+            finish(walk, w);
+            return;
+        }
+        if (some) { walk.a /= s.total; walk.b = (walk.b + 1.0) / s.total; ++walk.refused; }
+        again = !more;
+        walk.asks = 0;
+        __syncthreads();
+        if (threadIdx.x == 0) s.walk = walk;
+        __syncthreads();
+    }
 }
 
-// The first pass of every sequence (blockIdx.y), its segments shared out.
+// Pass p.rounds of every sequence (blockIdx.y) that comes to it, its segments shared out.
 template <typename T>
-__global__ __launch_bounds__(256) void drafts_first_kernel(DraftParams p) {
+__global__ __launch_bounds__(256) void drafts_round_kernel(DraftParams p) {
     __shared__ DraftShared s;
     const int64_t n = blockIdx.y;
-    const int rows = rows_of(p, n), lane = threadIdx.x & 63;
-    draft_tests<T>(p, n, rows, s);
-    start_walk(s);
-    __syncthreads();
-    if (threadIdx.x < 64) draft_walk(p, rows, s);
-    __syncthreads();
-    const DraftWeights w = weights_of(s.walk, s.walk.asks);
-    for (int k = blockIdx.x * 4 + threadIdx.x / 64; k < p.segments; k += gridDim.x * 4) {
-        const double sum = p.q ? segment_sum<T, true>(p, n, s, w, k) : segment_sum<T, false>(p, n, s, w, k);
-        if (lane == 0) p.sums[n * p.segments + k] = sum;
-    }
+    draft_passes<T>(p, n, s, p.rounds, [&](const DraftWeights& w) {
+        double* const to = p.sums + (p.rounds * p.N + n) * p.segments;
+        for (int k = blockIdx.x * 4 + threadIdx.x / 64; k < p.segments; k += gridDim.x * 4) {
+            const double sum = p.q ? segment_sum<T, true>(p, n, s, w, k) : segment_sum<T, false>(p, n, s, w, k);
+            if ((threadIdx.x & 63) == 0) to[k] = sum;
+        }
+        return false;
+    }, [](const DraftWalk&, const DraftWeights&) {});
 }
 
 template <typename T>
 __global__ __launch_bounds__(1024) void drafts_kernel(DraftParams p) {
     __shared__ DraftShared s;
     const int64_t n = blockIdx.x;
-    const int rows = rows_of(p, n);
-    draft_tests<T>(p, n, rows, s);
-    start_walk(s);
-    __syncthreads();
-    const double* from = p.sums ? p.sums + n * p.segments : nullptr;
-    for (;;) {
-        if (threadIdx.x < 64) draft_walk(p, rows, s);
-        __syncthreads();
-        DraftWalk walk = s.walk;
-        DraftWeights w = weights_of(walk, walk.asks);
-        draft_pass<T>(p, n, s, w, from);
-        from = nullptr;
-        const bool more = walk.asks && [&] {
-            // (every wave looks: rows asked later that follow the same row)
-            return next_draft(s, walk.here, walk.last, rows) < rows;
-        }();
-        if (walk.asks) {
-            const bool some = s.total > 0.0;
-            if (some) { walk.a /= s.total; walk.b = (walk.b + 1.0) / s.total; ++walk.refused; }
-            walk.asks = 0;
-            if (!some && !more) {                                  // nothing left: what was there before, added up again
-                w = weights_of(walk, 0);
-                __syncthreads();
-                draft_pass<T>(p, n, s, w, nullptr);
+    draft_passes<T>(p, n, s, p.rounds, [&](const DraftWeights& w) {
+        for (int k = threadIdx.x / 64; k < p.segments; k += 16) {
+            const double sum = p.q ? segment_sum<T, true>(p, n, s, w, k) : segment_sum<T, false>(p, n, s, w, k);
+            if ((threadIdx.x & 63) == 0) s.sums[k] = sum;
+        }
+        return true;
+    }, [&](const DraftWalk& walk, const DraftWeights& w) {
+        if (threadIdx.x < 64) {
+            const int word = s.total > 0.0 && s.total < __builtin_inf() ? draft_word<T>(p, n, s, w, (double)s.u[0] * s.total) : -1;
+            if (threadIdx.x == 0) {
+                p.next[n] = word;
+                p.accepted[n] = walk.depth;
             }
         }
-        if (!more) {
-            if (threadIdx.x < 64) {
-                const double total = s.total;
-                const int word = total > 0.0 && total < __builtin_inf() ? draft_word<T>(p, n, s, w, (double)s.u[0] * total) : -1;
-                if (threadIdx.x == 0) {
-                    p.next[n] = word;
-                    p.accepted[n] = walk.depth;
-                }
-            }
-            for (int r = threadIdx.x; r < p.R; r += blockDim.x) p.rows[n * p.R + r] = r < walk.depth ? s.path[r] : -1;
-            return;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) s.walk = walk;
-        __syncthreads();
-    }
+        for (int r = threadIdx.x; r < p.R; r += 1024) p.rows[n * p.R + r] = r < walk.depth ? s.path[r] : -1;
+    });
 }
 
 static int check_drafts(const char* who, const gdn_drafts_call* c) {
@@ -333,11 +343,12 @@ static int check_drafts(const char* who, const gdn_drafts_call* c) {
     return GDN_OK;
 }
 
-// Workgroups of the first pass per sequence; 0: the finishing workgroup makes it.
-static int64_t first_parts(const gdn_drafts_call* c) {
+// Passes that are shared out over workgroups, a launch for each, and workgroups per sequence: the first one, of which a chain has no other, and two more of trees.
+struct DraftPlan { int rounds, parts; };
+static DraftPlan draft_plan(const gdn_drafts_call* c) {
     const int64_t segments = (c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT;
-    const int64_t parts = std::min<int64_t>((segments + 3) / 4, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, c->N)));
-    return parts > 1 ? parts : 0;
+    if (segments <= 32 || c->N >= 192) return {0, 0};
+    return {c->parents ? 3 : 1, (int)std::min<int64_t>((segments + 3) / 4, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, c->N)))};
 }
 
 }  // namespace gdn
@@ -345,8 +356,8 @@ static int64_t first_parts(const gdn_drafts_call* c) {
 using namespace gdn;
 
 extern "C" size_t gdn_verify_drafts_workspace_bytes(const gdn_drafts_call* c) {
-    if (check_drafts("gdn_verify_drafts_workspace_bytes", c) != GDN_OK || c->N == 0 || first_parts(c) == 0) return 0;
-    return (size_t)(c->N * ((c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT)) * sizeof(double);
+    if (check_drafts("gdn_verify_drafts_workspace_bytes", c) != GDN_OK || c->N == 0) return 0;
+    return (size_t)draft_plan(c).rounds * (size_t)(c->N * ((c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT)) * sizeof(double);
 }
 
 extern "C" int gdn_verify_drafts(const gdn_drafts_call* c, void* workspace, size_t workspace_bytes, void* stream) {
@@ -358,13 +369,14 @@ extern "C" int gdn_verify_drafts(const gdn_drafts_call* c, void* workspace, size
     const size_t need = gdn_verify_drafts_workspace_bytes(c);
     GDN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0), GDN_ERR_WORKSPACE, "%s: workspace of %zu bytes, 8-byte aligned", who, need);
     DraftParams p{c->p, c->q, c->tokens, c->uniforms, c->parents, c->lengths, c->next_token, c->accepted, c->rows, c->p_stride[0], c->p_stride[1], c->q_stride[0], c->q_stride[1],
-                  c->parents_stride, (int)c->R, (int)c->V, (int)((c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT), (c->flags & GDN_DRAFTS_TOKENS_INT64) != 0, need ? (double*)workspace : nullptr};
+                  c->parents_stride, (int)c->R, (int)c->V, (int)((c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT), (c->flags & GDN_DRAFTS_TOKENS_INT64) != 0, (double*)workspace, c->N, 0};
     auto go = [&](auto t) {
         typedef decltype(t) T;
-        if (need) {
-            hipLaunchKernelGGL(drafts_first_kernel<T>, dim3((unsigned)first_parts(c), (unsigned)c->N), dim3(256), 0, (hipStream_t)stream, p);
-            const int first = check_launch("drafts_first_kernel");
-            if (first != GDN_OK) return first;
+        const DraftPlan plan = draft_plan(c);
+        for (; p.rounds < plan.rounds; ++p.rounds) {
+            hipLaunchKernelGGL(drafts_round_kernel<T>, dim3((unsigned)plan.parts, (unsigned)c->N), dim3(256), 0, (hipStream_t)stream, p);
+            const int ran = check_launch("drafts_round_kernel");
+            if (ran != GDN_OK) return ran;
         }
         hipLaunchKernelGGL(drafts_kernel<T>, dim3((unsigned)c->N), dim3(1024), 0, (hipStream_t)stream, p);
         return check_launch("drafts_kernel");

@@ -48,7 +48,7 @@ def _inputs(N, R, V, dtype=FP, sampled=True, tree=False, seed=0, apart=0.7):
 @gpu
 @pytest.mark.parametrize('tree', [False, True])
 @pytest.mark.parametrize('sampled', [False, True])
-@pytest.mark.parametrize(('N', 'R', 'V'), [(1, 1, 1), (1, 2, 5), (5, 3, 64), (3, 8, 2047), (3, 8, 2048), (3, 8, 2049), (2, 7, 9001), (70, 20, 33), (1, 100, 40), (2, 1024, 10), (2, 6, 50257)])
+@pytest.mark.parametrize(('N', 'R', 'V'), [(1, 1, 1), (1, 2, 5), (5, 3, 64), (3, 8, 2047), (3, 8, 2048), (3, 8, 2049), (2, 7, 9001), (70, 20, 33), (1, 100, 40), (2, 1024, 10), (2, 6, 50257), (2, 9, 131073), (200, 5, 70001)])
 def test_against_the_oracle(N, R, V, sampled, tree):
     for seed in range(3):
         _same(**_inputs(N, R, V, sampled=sampled, tree=tree, seed=seed))
@@ -240,7 +240,7 @@ def test_library_refuses():
         _verify(torch.zeros(1, 1, 1), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 1))
 
     def call(**kw):
-        c = _lib.DraftsCall(p=16, tokens=16, uniforms=16, next_token=16, accepted=16, rows=16, N=1, R=2, V=10000, p_dtype=2)
+        c = _lib.DraftsCall(p=16, tokens=16, uniforms=16, next_token=16, accepted=16, rows=16, N=1, R=2, V=100000, p_dtype=2)
         for k, v in kw.items():
             setattr(c, k, v)
         return lib.gdn_verify_drafts(ctypes.byref(c), None, 0, None)
