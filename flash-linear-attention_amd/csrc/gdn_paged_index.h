@@ -14,7 +14,7 @@ namespace gdn {
 struct PageTable {
     const int32_t* table;
     int64_t table_stride;
-    int64_t capacity;                // slots that a row of the table can name: table_cols * page_size
+    int64_t capacity;                // slots that a row of the table can name: table_cols * page_size, below 2^31
     int32_t pages, page_size;
 };
 
@@ -22,9 +22,11 @@ struct PageTable {
 // for a slot outside the row.
 GDN_ANYWHERE int32_t page_of(const PageTable& t, int64_t n, int64_t slot) {
     if (slot < 0 || slot >= t.capacity) return -1;
-    const int32_t page = t.table[n * t.table_stride + slot / t.page_size];
+    const int32_t page = t.table[n * t.table_stride + (uint32_t)slot / (uint32_t)t.page_size];
     return page >= 0 && page < t.pages ? page : -1;
 }
+// The slot's place in its page (of a slot that has one).
+GDN_ANYWHERE uint32_t place_in_page(const PageTable& t, int64_t slot) { return (uint32_t)slot % (uint32_t)t.page_size; }
 
 // The sequence that a row of a packed batch belongs to, or -1: cu [N + 1] are the boundaries, rows before the first and behind the last
 // belong to none.  (Boundaries that decrease give some sequence or none, and read nothing else.)

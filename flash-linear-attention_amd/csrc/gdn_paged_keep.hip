@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void paged_keep_kernel(KeepParams p, int per_u
     auto place = [&](int64_t slot) -> U* {
         const int page = page_of(p.cache.pages, n, slot);
         if (page < 0) return nullptr;
-        return (U*)data + (page * page_stride + slot % p.cache.pages.page_size * slot_stride + inside) / per_unit + c;
+        return (U*)data + (page * page_stride + (int64_t)place_in_page(p.cache.pages, slot) * slot_stride + inside) / per_unit + c;
     };
     for (int i = 0; i < kept; i += AHEAD) {
         U held[AHEAD];

@@ -2,9 +2,10 @@
 //
 //   (y1, y2) = (x1 c - x2 s, x1 s + x2 c)      c, s = cos, sin of the row's position, pair (j, j + R/2) or (2j, 2j + 1), j < R/2 <= D/2
 //
-// The gradient is the turn back (s negated).  Every element is read once and written once; the rows of the tables are read once per row of heads.  The memory
-// system bounds it: a thread turns V elements of either half (or V / 2 pairs side by side) for up to four heads of its token, all asked for
-// before the first is stored, and keeps the tables' values in registers for them.
+// The gradient is the turn back (s negated).  Every element is read once and written once; the rows of the tables are read once per row of heads.  The memory system bounds
+// it: a thread turns 16 bytes of either half (or of pairs side by side) for two or three heads of its token, asked for before anything that says where the token stands, and
+// keeps the tables' values in registers for them.  Loads and stores past the caches: 32768 tokens of 20 heads of 128 83 -> 64 us (5.5 TB/s), prompts of 14000 tokens of
+// 48 heads into the cache 116 -> 89, with the rows asked for first 75.
 #include "gdn_paged.h"
 #include <algorithm>
 #include <type_traits>
@@ -29,22 +30,50 @@ struct RotaryParams {
     int half, D;
     float sign;
     bool pos_i32, off_i32, cu_i32;
-    int chunks, chunk_lanes, head_lanes, tokens;
+    int chunks, chunk_lanes, head_lanes, tokens, each;           // each: heads of a thread at a time
     PagedCache cache;
 };
 
 template <typename T, int V, int ALIGN = (V * sizeof(T) > 16 ? 16 : V * sizeof(T))> struct alignas(ALIGN) Pack { T e[V]; };
 
-template <typename T, typename TT, int V, bool INTER, bool CACHE>
+// (past the caches: a call's rows are more than they hold, or too few to matter)
+template <typename P, typename T> __device__ __forceinline__ P load_streamed(const T* at) {
+    if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_nontemporal_load((const u32x4*)at));
+    else return *(const P*)at;
+}
+template <typename P, typename T> __device__ __forceinline__ void store_streamed(T* at, const P& x) {
+    if constexpr (sizeof(P) == 16) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, x), (u32x4*)at);
+    else *(P*)at = x;
+}
+
+// HEADS: of a thread at a time, at most
+template <typename T, typename TT, int V, bool INTER, bool CACHE, int HEADS>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     // (the narrowest form of the interleaved layout takes pairs at any address)
     typedef std::conditional_t<INTER && V == 2, Pack<T, V, sizeof(T)>, Pack<T, V>> P;
-    constexpr int HEADS = 4, PAIRS = INTER ? V / 2 : V;
+    constexpr int PAIRS = INTER ? V / 2 : V;
     const int lanes = p.head_lanes * p.chunk_lanes, local = threadIdx.x / lanes, at = threadIdx.x - local * lanes;
     const int64_t token = (int64_t)blockIdx.x * p.tokens + local;
     if (local >= p.tokens || token >= p.B * p.T) return;
-    const int64_t b = token / p.T, t = token - b * p.T;
+    const int64_t b = p.B == 1 ? 0 : (uint32_t)token / (uint32_t)p.T, t = token - b * p.T;
     const int h0 = at / p.chunk_lanes, c0 = at - h0 * p.chunk_lanes;
+    const int turned = INTER ? 2 * p.half / V : p.half / V;
+    P a[HEADS], z[HEADS];
+    auto place = [&](int c) { return c < turned ? c * V : 2 * p.half + (c - turned) * V; };
+    auto load = [&](int c, int h) {
+#pragma unroll
+        for (int u = 0; u < HEADS; ++u) {
+            const int hu = h + u * p.head_lanes;
+            if (u >= p.each || hu >= p.heads) continue;
+            const int s = hu < p.rows[0].end ? 0 : hu < p.rows[1].end ? 1 : 2;
+            const RotaryRows& r = p.rows[s];
+            const T* x = (const T*)r.x + b * r.xb + t * r.xt + (hu - (s ? p.rows[s - 1].end : 0)) * r.xh + place(c);
+            a[u] = load_streamed<P>(x);
+            if (!INTER && c < turned) z[u] = load_streamed<P>(x + p.half);
+        }
+    };
+    // The rows are asked for before what says where they stand, which takes several loads one after the other.
+    if (c0 < p.chunks && h0 < p.heads) load(c0, h0);
     int64_t n = b, i = t;
     if (p.cu) {
         n = sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); });
@@ -61,13 +90,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     if constexpr (CACHE) {
         const int page = n >= 0 ? page_of(p.cache.pages, n, slot) : -1;
         stored = page >= 0;
-        const int64_t in_page = stored ? slot % p.cache.pages.page_size : 0;
+        const int64_t in_page = stored ? place_in_page(p.cache.pages, slot) : 0;
         to[0] = page * p.cache.k_page + in_page * p.cache.k_slot;
         to[1] = page * p.cache.v_page + in_page * p.cache.v_slot;
     }
     // (a row of no sequence is handed on as it is; a position that the tables do not have gives NaN)
     const bool inside = n >= 0 && pos >= 0 && pos < p.table_rows;
-    const int turned = INTER ? 2 * p.half / V : p.half / V;
     for (int c = c0; c < p.chunks; c += p.chunk_lanes) {
         const bool pair = c < turned;
         float cs[PAIRS], sn[PAIRS];
@@ -80,23 +108,13 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
 #pragma unroll
             for (int e = 0; e < PAIRS; ++e) cs[e] = sn[e] = __builtin_nanf("");
         }
-        const int first = pair ? c * V : 2 * p.half + (c - turned) * V, second = first + p.half;
-        for (int h = h0; h < p.heads; h += HEADS * p.head_lanes) {
-            P a[HEADS], z[HEADS];
+        const int first = place(c);
+        for (int h = h0; h < p.heads; h += p.each * p.head_lanes) {
+            if (c != c0 || h != h0) load(c, h);
 #pragma unroll
             for (int u = 0; u < HEADS; ++u) {
                 const int hu = h + u * p.head_lanes;
-                if (hu >= p.heads) continue;
-                const int s = hu < p.rows[0].end ? 0 : hu < p.rows[1].end ? 1 : 2;
-                const RotaryRows& r = p.rows[s];
-                const T* x = (const T*)r.x + b * r.xb + t * r.xt + (hu - (s ? p.rows[s - 1].end : 0)) * r.xh;
-                a[u] = *(const P*)(x + first);
-                if (!INTER && pair) z[u] = *(const P*)(x + second);
-            }
-#pragma unroll
-            for (int u = 0; u < HEADS; ++u) {
-                const int hu = h + u * p.head_lanes;
-                if (hu >= p.heads) continue;
+                if (u >= p.each || hu >= p.heads) continue;
                 const int s = hu < p.rows[0].end ? 0 : hu < p.rows[1].end ? 1 : 2;
                 const RotaryRows& r = p.rows[s];
                 const int64_t head = hu - (s ? p.rows[s - 1].end : 0);
@@ -116,8 +134,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
                         else { a[u].e[e] = y1; z[u].e[e] = y2; }
                     }
                 }
-                *(P*)(y + first) = a[u];
-                if (!INTER && pair) *(P*)(y + second) = z[u];
+                store_streamed(y + first, a[u]);
+                if (!INTER && pair) store_streamed(y + first + p.half, z[u]);
             }
         }
     }
@@ -128,15 +146,34 @@ static int launch_rotary(const char* who, RotaryParams& p, bool inter, bool cach
     const int64_t tokens = p.B * p.T;
     p.chunks = (inter ? 2 * p.half : p.half) / V + (p.D - 2 * p.half) / V;
     p.chunk_lanes = std::min(p.chunks, 256);
-    // Where the chip is not full a thread takes one head, else four.
-    const int each = tokens * p.heads * p.chunks <= 256 * 1024 ? 1 : 4;
-    p.head_lanes = std::max(1, std::min((p.heads + each - 1) / each, 256 / p.chunk_lanes));
-    p.tokens = std::max(1, 256 / (p.head_lanes * p.chunk_lanes));
+    // Heads of a thread: one where the chip is not full, else two or three, as leaves the fewest of a block's threads idle (of equals two).  Measured: queries and keys of 20
+    // heads of 128 elements, two heads 64 us, three 70, four 68; 48 heads into the cache 78, 71, 81; 40 heads of 64 turned and 64 other elements with gradients 103, 98, 99.
+    auto lay_out = [&](int each) {
+        p.head_lanes = std::max(1, std::min((p.heads + each - 1) / each, 256 / p.chunk_lanes));
+        p.tokens = std::max(1, 256 / (p.head_lanes * p.chunk_lanes));
+        const int rounds = (p.heads + p.head_lanes * each - 1) / (p.head_lanes * each);
+        return (double)(p.tokens * p.heads * p.chunk_lanes) / (256.0 * each * rounds);
+    };
+    int each = 1;
+    if (tokens * p.heads * p.chunks > 256 * 1024) {
+        const double two = lay_out(2);
+        each = V * sizeof(T) == 16 && lay_out(3) > 1.02 * two ? 3 : 2;
+    }
+    lay_out(each);
+    p.each = each;
     const int64_t blocks = (tokens + p.tokens - 1) / p.tokens;
-    GDN_CHECK_ARG(blocks < (1ll << 31), GDN_ERR_UNSUPPORTED, "%s: too many tokens", who);
+    GDN_CHECK_ARG(tokens < (1ll << 31), GDN_ERR_UNSUPPORTED, "%s: fewer than 2^31 tokens", who);
     auto go = [&](auto inter_, auto cache_) {
         constexpr bool I = decltype(inter_)::value, C = decltype(cache_)::value;
-        if constexpr (!I || V >= 2) hipLaunchKernelGGL((rotary_kernel<T, TT, V, I, C>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        if constexpr (!I || V >= 2) {
+            if constexpr (V * sizeof(T) == 16) {
+                if (each == 3) {
+                    hipLaunchKernelGGL((rotary_kernel<T, TT, V, I, C, 3>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+                    return;
+                }
+            }
+            hipLaunchKernelGGL((rotary_kernel<T, TT, V, I, C, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        }
     };
     auto with_cache = [&](auto inter_) { cache ? go(inter_, std::true_type()) : go(inter_, std::false_type()); };
     inter ? with_cache(std::true_type()) : with_cache(std::false_type());
