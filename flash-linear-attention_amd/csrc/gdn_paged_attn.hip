@@ -113,6 +113,31 @@ __device__ __forceinline__ PagedStart paged_start(const PagedAttnParams& p, int 
     __shared__ int64_t sums[4], found[2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     auto work = [&](int64_t n) { return n < p.N ? paged_work(p, paged_sequence<false>(p, n)).all : (int64_t)0; };
+    auto share = [&](int64_t all) {
+        const int64_t groups = max(paged_groups(p, all), (int64_t)1);
+        return PagedStart{p.N, 0, group < groups ? all * group / groups : all, group < groups ? all * (group + 1) / groups : all};
+    };
+    if (p.N <= 64) {                                             // every wave by itself
+        const int64_t x = work(lane);
+        int64_t upto = x;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int64_t y = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += y;
+        }
+        const int64_t all = __shfl(upto, 63, 64);
+        if (group == 0 && wave == 0) {
+            if (lane < p.N) p.before[lane] = upto - x;
+            if (lane == 0) p.before[p.N] = all;
+        }
+        PagedStart at = share(all);
+        const uint64_t has = __ballot(upto - x <= at.from && at.from < upto);
+        if (has) {
+            at.n = __builtin_ctzll(has);
+            at.before = __shfl(upto - x, (int)at.n, 64);
+        }
+        return at;
+    }
     const int64_t first = work(threadIdx.x);
     int64_t mine = first;
     for (int64_t n = threadIdx.x + 256; n < p.N; n += 256) mine += work(n);
@@ -121,8 +146,7 @@ __device__ __forceinline__ PagedStart paged_start(const PagedAttnParams& p, int 
     if (lane == 0) sums[wave] = mine;
     __syncthreads();
     const int64_t all = sums[0] + sums[1] + sums[2] + sums[3];
-    const int64_t groups = max(paged_groups(p, all), (int64_t)1);
-    PagedStart at{p.N, 0, group < groups ? all * group / groups : all, group < groups ? all * (group + 1) / groups : all};
+    PagedStart at = share(all);
     if (group == 0 && threadIdx.x == 0) p.before[p.N] = all;
     int64_t before = 0;
     for (int64_t n0 = 0; n0 < p.N; n0 += 256) {
@@ -699,6 +723,9 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM && cache->dim % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of a multiple of 8 up to %d elements", who, PA_MAX_DIM);
     GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->B * c->T * c->HQ < (1ll << 31) && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
                   "%s: rows times heads below 2^31, up to 2^30 slots of a sequence", who);
+    // (the work is counted in 64 bits, times the workgroups)
+    GDN_CHECK_ARG((double)c->N * (double)cache->heads * (double)(c->T * (c->HQ / cache->heads) / 16 + 1) * (double)(cache->table_cols * cache->page_size / 32 + 8) < 4e15, GDN_ERR_UNSUPPORTED,
+                  "%s: too much work for one call", who);
     return GDN_OK;
 }
 

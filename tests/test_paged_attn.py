@@ -121,6 +121,17 @@ def test_long_contexts_of_all_lengths(packed, D):
 
 
 @gpu
+@pytest.mark.parametrize('N', [2, 63, 64, 65, 255, 256, 257, 700])
+@pytest.mark.parametrize('packed', [False, True])
+def test_many_sequences(N, packed):
+    """The work is shared out over the sequences by a wave, by a workgroup, in several turns of it; some of them have nothing to do."""
+    contexts = [(i * 37) % 150 if i % 5 else 0 for i in range(N)]
+    contexts[N // 2] = 2500
+    rows = [(i * 7) % 4 for i in range(N)] if packed else [1] * N
+    Step(contexts, rows, 16, 2, 1, 64, BF, packed, seed=N).check()
+
+
+@gpu
 @pytest.mark.parametrize('rows', [1, 5, 40])
 def test_every_length_around_the_tiles(rows):
     """Contexts and pages that end anywhere inside a tile of keys."""

@@ -356,7 +356,8 @@ def test_library_refuses():
     attn = lambda cache=None, **kw: lib.gdn_paged_attn(make(**(cache or {})), ctypes.byref(_lib.PagedAttnCall(**{**dict(q=16, o=16, B=1, T=1, N=1, HQ=2, max_rows=1), **kw})), None, 0, None)
     invalid = [dict(B=-1), dict(T=-1), dict(HQ=-1), dict(N=2), dict(max_rows=-1), dict(q=None), dict(o=None), dict(cu_seqlens=16, B=2, N=2), dict(cu_seqlens=16, N=0), dict(cache=dict(heads=3), HQ=4)]
     assert [attn(**kw) for kw in invalid] == [_lib.GDN_ERR_INVALID] * len(invalid)
-    assert attn(cache=dict(dtype=2)) == attn(cache=dict(dim=264)) == _lib.GDN_ERR_UNSUPPORTED
+    assert attn(cache=dict(dtype=2)) == attn(cache=dict(dim=264)) == attn(cache=dict(dim=12)) == attn(cache=dict(page_size=2 ** 29 + 1)) == _lib.GDN_ERR_UNSUPPORTED
+    assert attn() == _lib.GDN_ERR_WORKSPACE
     assert attn(B=0, N=0) == attn(T=0) == attn(HQ=0) == _lib.GDN_OK
     rows = lambda heads: ctypes.byref(_lib.RotaryRows(16, 16, heads))
     append = lambda k=1, v=1, q=None, cache=None, **kw: lib.gdn_paged_append(make(**(cache or {})), None if q is None else rows(q), rows(k), rows(v),
