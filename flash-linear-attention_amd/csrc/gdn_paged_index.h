@@ -20,10 +20,14 @@ struct PageTable {
 
 // The page of a slot, or -1: the slot lies outside the table's row, or the table names no page of the cache there.  Nothing is read
 // for a slot outside the row.
-GDN_ANYWHERE int32_t page_of(const PageTable& t, int64_t n, int64_t slot) {
+template <typename Load>
+GDN_ANYWHERE int32_t page_of(const PageTable& t, int64_t n, int64_t slot, Load load) {
     if (slot < 0 || slot >= t.capacity) return -1;
-    const int32_t page = t.table[n * t.table_stride + (uint32_t)slot / (uint32_t)t.page_size];
+    const int32_t page = load(t.table, n * t.table_stride + (uint32_t)slot / (uint32_t)t.page_size);
     return page >= 0 && page < t.pages ? page : -1;
+}
+GDN_ANYWHERE int32_t page_of(const PageTable& t, int64_t n, int64_t slot) {
+    return page_of(t, n, slot, [](const int32_t* at, int64_t i) { return at[i]; });
 }
 // The slot's place in its page (of a slot that has one).
 GDN_ANYWHERE uint32_t place_in_page(const PageTable& t, int64_t slot) { return (uint32_t)slot % (uint32_t)t.page_size; }

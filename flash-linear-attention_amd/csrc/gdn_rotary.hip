@@ -74,26 +74,31 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
     };
     // The rows are asked for before what says where they stand, which takes several loads one after the other.
     if (c0 < p.chunks && h0 < p.heads) load(c0, h0);
-    int64_t n = b, i = t;
-    if (p.cu) {
-        n = sequence_of(token, p.N, [&](int64_t j) { return load_index(p.cu, j, p.cu_i32); });
-        i = n < 0 ? 0 : token - load_index(p.cu, n, p.cu_i32);
-    }
-    int64_t slot = -1, pos = 0;
-    if (n >= 0) {
-        const int64_t before = p.offsets ? load_index(p.offsets, n, p.off_i32) : p.offset;
-        pos = p.positions ? load_index(p.positions, token, p.pos_i32) : before + i;
-        slot = before + i;
-    }
-    int64_t to[2] = {0, 0};
+    int64_t n = b, i = t, slot = -1, pos = 0, to[2] = {0, 0};
     bool stored = false;
-    if constexpr (CACHE) {
-        const int page = n >= 0 ? page_of(p.cache.pages, n, slot) : -1;
-        stored = page >= 0;
-        const int64_t in_page = stored ? place_in_page(p.cache.pages, slot) : 0;
-        to[0] = page * p.cache.k_page + in_page * p.cache.k_slot;
-        to[1] = page * p.cache.v_page + in_page * p.cache.v_slot;
-    }
+    auto stand = [&](int64_t token, auto&& index) {
+        if (p.cu) {
+            n = sequence_of(token, p.N, [&](int64_t j) { return index(p.cu, j, p.cu_i32); });
+            i = n < 0 ? 0 : token - index(p.cu, n, p.cu_i32);
+        }
+        if (n >= 0) {
+            const int64_t before = p.offsets ? index(p.offsets, n, p.off_i32) : p.offset;
+            pos = p.positions ? index(p.positions, token, p.pos_i32) : before + i;
+            slot = before + i;
+        }
+        if constexpr (CACHE) {
+            const int page = n >= 0 ? page_of(p.cache.pages, n, slot, [&](const int32_t* at, int64_t j) { return (int32_t)index(at, j, true); }) : -1;
+            stored = page >= 0;
+            const int64_t in_page = stored ? place_in_page(p.cache.pages, slot) : 0;
+            to[0] = page * p.cache.k_page + in_page * p.cache.k_slot;
+            to[1] = page * p.cache.v_page + in_page * p.cache.v_slot;
+        }
+    };
+    // (a wave of one token: scalar loads, a third of the latency of the others)
+    if (p.tokens == 1 || lanes % 64 == 0)
+        stand((int64_t)blockIdx.x * p.tokens + __builtin_amdgcn_readfirstlane(local), [](const void* at, int64_t j, bool is_i32) { return load_index_uniform(at, j, is_i32); });
+    else
+        stand(token, [](const void* at, int64_t j, bool is_i32) { return load_index(at, j, is_i32); });
     // (a row of no sequence is handed on as it is; a position that the tables do not have gives NaN)
     const bool inside = n >= 0 && pos >= 0 && pos < p.table_rows;
     for (int c = c0; c < p.chunks; c += p.chunk_lanes) {
