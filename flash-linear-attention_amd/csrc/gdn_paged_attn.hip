@@ -264,7 +264,7 @@ struct PagedWave {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint16_t* at;
-                if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + t.v[b] + ((4 * g + e) * p.v_slot + VE * c16);
+                if constexpr (UNIFORM) at = (const uint16_t*)p.cache.v + (t.v[b] + (uint64_t)(e * p.v_slot)) + (4 * g * p.v_slot + VE * c16);
                 else at = (const uint16_t*)p.cache.v + __shfl(t.v, 16 * b + 4 * g + e, 64) + VE * c16;
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
@@ -729,19 +729,21 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     return GDN_OK;
 }
 
-struct PagedAttnPlan { int dim, row_tiles, row_groups, height, step, overhead, groups; bool many_parts; size_t bytes; };
-static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, bool shares) {
+struct PagedAttnPlan { int dim, row_tiles, row_groups, height, step, overhead, groups; bool shares, many_parts; size_t bytes; };
+static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, bool uniform, bool shares) {
     PagedAttnPlan plan;
     const int64_t rows = std::max<int64_t>(1, std::min(c->max_rows, c->T)) * (c->HQ / cache->heads);
     plan.dim = cache->dim <= 64 ? 64 : cache->dim <= 128 ? 128 : 256;
-    plan.row_tiles = plan.dim == 256 || rows <= 16 ? 1 : 2;
+    // Two row tiles of a wave where its registers hold them beside the keys under way: heads of the whole 64 or 128 in pages of whole tiles, and tiles through LDS.
+    plan.row_tiles = plan.dim < 256 && rows > 16 && ((uniform && cache->dim == plan.dim) || (shares && rows > 64)) ? 2 : 1;
     const int64_t each = 16 * plan.row_tiles;
     plan.row_groups = rows <= each ? 1 : rows <= 2 * each ? 2 : 4;
     plan.height = (int)(each * plan.row_groups);
-    plan.step = shares && plan.row_groups == 4 ? 2 * PA_TILE : PA_TILE * (4 / plan.row_groups);
+    plan.shares = shares && plan.row_groups == 4 && (plan.row_tiles == 2 || plan.dim == 256);
+    plan.step = plan.shares ? 2 * PA_TILE : PA_TILE * (4 / plan.row_groups);
     // What a unit costs besides its keys, in steps.  Measured, us a call (1, 2, 4, 6, 8 steps): 16 sequences of up to 8000 keys with trees of 64 rows 219, 189, 166, 148, 149 (through
     // LDS); 32 of up to 8000 with 8 rows 142, 129, 131, 131, 133; 256 of up to 1000 with one row 115, 117, 123, 123, 124.
-    plan.overhead = shares && plan.row_groups == 4 ? 6 : plan.row_tiles;
+    plan.overhead = plan.shares ? 6 : plan.row_tiles;
     // One round of the chip: two workgroups share a CU (one where a head of 256 takes a wave's registers), but no more than there can be steps.
     const int64_t units = std::max<int64_t>(1, c->N) * cache->heads * ((rows + plan.height - 1) / plan.height);
     const int64_t steps = std::max<int64_t>(1, (cache->table_cols * cache->page_size + plan.step - 1) / plan.step);
@@ -769,7 +771,8 @@ using namespace gdn;
 extern "C" size_t gdn_paged_attn_workspace_bytes(const gdn_paged_cache* cache, const gdn_paged_attn_call* c) {
     PagedCache view;
     if (check_attn("gdn_paged_attn_workspace_bytes", cache, c, view) != GDN_OK || c->B * c->T * c->HQ == 0) return 0;
-    return attn_plan(cache, c, uniform_tiles(cache) && whole_pieces(view)).bytes;
+    const bool uniform = uniform_tiles(cache);
+    return attn_plan(cache, c, uniform, uniform && whole_pieces(view)).bytes;
 }
 
 extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn_call* c, void* workspace, size_t workspace_bytes, void* stream) {
@@ -779,8 +782,8 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
     if (rc != GDN_OK) return rc;
     if (c->B * c->T * c->HQ == 0) return GDN_OK;
     GDN_CHECK_ARG(c->q && c->o, GDN_ERR_INVALID, "%s: missing tensors", who);
-    const bool uniform = uniform_tiles(cache), shares = uniform && whole_pieces(p.cache);
-    const PagedAttnPlan plan = attn_plan(cache, c, shares);
+    const bool uniform = uniform_tiles(cache);
+    const PagedAttnPlan plan = attn_plan(cache, c, uniform, uniform && whole_pieces(p.cache));
     GDN_CHECK_ARG(workspace && workspace_bytes >= plan.bytes && (uintptr_t)workspace % 16 == 0, GDN_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned", who, plan.bytes);
     p.q = c->q; p.o = c->o; p.cu = c->cu_seqlens; p.mask = c->mask;
     p.qb = c->q_stride[0]; p.qt = c->q_stride[1]; p.qh = c->q_stride[2];
@@ -813,12 +816,18 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
             if (made == GDN_OK) hipLaunchKernelGGL(kernel, dim3((unsigned)plan.groups), dim3(256), smem, (hipStream_t)stream, p);
             return made;
         };
-        auto full = [&](auto uniform_, auto shared_) { return p.D == DT ? launch(uniform_, std::true_type(), shared_) : launch(uniform_, std::false_type(), shared_); };
-        int made;
-        if (!uniform) made = full(std::false_type(), std::false_type());
-        else if (plan.row_groups < 4 || !shares) made = full(std::true_type(), std::false_type());
-        else if constexpr (RT == 2 || DT == 256) made = full(std::true_type(), std::true_type());
-        else made = GDN_ERR_UNSUPPORTED;
+        const std::true_type yes;
+        const std::false_type no;
+        const bool whole_head = p.D == DT;
+        int made = GDN_ERR_UNSUPPORTED;
+        if constexpr (RT == 2 || DT == 256) {
+            if (plan.shares) made = whole_head ? launch(yes, yes, yes) : launch(yes, no, yes);
+        }
+        if (!plan.shares) {
+            if constexpr (RT == 2) made = launch(yes, yes, no);
+            else if (uniform) made = whole_head ? launch(yes, yes, no) : launch(yes, no, no);
+            else made = whole_head ? launch(no, yes, no) : launch(no, no, no);
+        }
         if (made != GDN_OK) return made;
         const int ran = check_launch("paged_attn_kernel");
         if (ran != GDN_OK || plan.groups == 1) return ran;
