@@ -734,12 +734,13 @@ static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_att
     PagedAttnPlan plan;
     const int64_t rows = std::max<int64_t>(1, std::min(c->max_rows, c->T)) * (c->HQ / cache->heads);
     plan.dim = cache->dim <= 64 ? 64 : cache->dim <= 128 ? 128 : 256;
-    // Two row tiles of a wave where its registers hold them beside the keys under way: heads of the whole 64 or 128 in pages of whole tiles, and tiles through LDS.
-    plan.row_tiles = plan.dim < 256 && rows > 16 && ((uniform && cache->dim == plan.dim) || (shares && rows > 64)) ? 2 : 1;
+    // More than 32 rows: the four waves on the same keys, through LDS.  Else by themselves, two row tiles where the registers hold them beside the keys under way (heads
+    // of the whole 64 or 128 elements in pages of whole tiles).
+    plan.shares = shares && rows > 32;
+    plan.row_tiles = plan.dim < 256 && (plan.shares ? rows > 64 : rows > 16 && uniform && cache->dim == plan.dim) ? 2 : 1;
     const int64_t each = 16 * plan.row_tiles;
-    plan.row_groups = rows <= each ? 1 : rows <= 2 * each ? 2 : 4;
+    plan.row_groups = plan.shares || rows > 2 * each ? 4 : rows > each ? 2 : 1;
     plan.height = (int)(each * plan.row_groups);
-    plan.shares = shares && plan.row_groups == 4 && (plan.row_tiles == 2 || plan.dim == 256);
     plan.step = plan.shares ? 2 * PA_TILE : PA_TILE * (4 / plan.row_groups);
     // What a unit costs besides its keys, in steps.  Measured, us a call (1, 2, 4, 6, 8 steps): 16 sequences of up to 8000 keys with trees of 64 rows 219, 189, 166, 148, 149 (through
     // LDS); 32 of up to 8000 with 8 rows 142, 129, 131, 131, 133; 256 of up to 1000 with one row 115, 117, 123, 123, 124.
@@ -820,9 +821,7 @@ extern "C" int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn
         const std::false_type no;
         const bool whole_head = p.D == DT;
         int made = GDN_ERR_UNSUPPORTED;
-        if constexpr (RT == 2 || DT == 256) {
-            if (plan.shares) made = whole_head ? launch(yes, yes, yes) : launch(yes, no, yes);
-        }
+        if (plan.shares) made = whole_head ? launch(yes, yes, yes) : launch(yes, no, yes);
         if (!plan.shares) {
             if constexpr (RT == 2) made = launch(yes, yes, no);
             else if (uniform) made = whole_head ? launch(yes, yes, no) : launch(yes, no, no);
