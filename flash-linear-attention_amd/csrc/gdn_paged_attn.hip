@@ -721,8 +721,9 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     if (rc != GDN_OK) return rc;
     GDN_CHECK_ARG(c->HQ % cache->heads == 0, GDN_ERR_INVALID, "%s: the queries' heads are a multiple of the cache's", who);
     GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM && cache->dim % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of a multiple of 8 up to %d elements", who, PA_MAX_DIM);
-    GDN_CHECK_ARG(c->B * c->T < (1ll << 31) && c->B * c->T * c->HQ < (1ll << 31) && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
-                  "%s: rows times heads below 2^31, up to 2^30 slots of a sequence", who);
+    // (a launch has fewer than 2^32 threads, the last of 64 for each row of a head)
+    GDN_CHECK_ARG(c->B < (1ll << 26) && c->T < (1ll << 26) && c->HQ < (1ll << 26) && c->B * c->T < (1ll << 26) && c->B * c->T * c->HQ < (1ll << 26) && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
+                  "%s: rows times heads below 2^26, up to 2^30 slots of a sequence", who);
     // (the work is counted in 64 bits, times the workgroups)
     GDN_CHECK_ARG((double)c->N * (double)cache->heads * (double)(c->T * (c->HQ / cache->heads) / 16 + 1) * (double)(cache->table_cols * cache->page_size / 32 + 8) < 4e15, GDN_ERR_UNSUPPORTED,
                   "%s: too much work for one call", who);
@@ -749,7 +750,7 @@ static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_att
     const int64_t units = std::max<int64_t>(1, c->N) * cache->heads * ((rows + plan.height - 1) / plan.height);
     const int64_t steps = std::max<int64_t>(1, (cache->table_cols * cache->page_size + plan.step - 1) / plan.step);
     plan.groups = (int)std::min<int64_t>(plan.dim == 256 ? 256 : 512, units * steps);
-    plan.many_parts = plan.groups > 8 * units;
+    plan.many_parts = plan.groups > 8 * units && c->B * c->T * c->HQ < (1 << 24);
     plan.bytes = ((size_t)c->N + 2) / 2 * 16 + (size_t)2 * plan.groups * plan.height * (cache->dim + 2) * sizeof(float);
     return plan;
 }

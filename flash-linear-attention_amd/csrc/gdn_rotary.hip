@@ -167,7 +167,7 @@ static int launch_rotary(const char* who, RotaryParams& p, bool inter, bool cach
     lay_out(each);
     p.each = each;
     const int64_t blocks = (tokens + p.tokens - 1) / p.tokens;
-    GDN_CHECK_ARG(tokens < (1ll << 31), GDN_ERR_UNSUPPORTED, "%s: fewer than 2^31 tokens", who);
+    GDN_CHECK_ARG(blocks < (1 << 24), GDN_ERR_UNSUPPORTED, "%s: fewer than 2^24 workgroups of tokens", who);     // (a launch has fewer than 2^32 threads)
     auto go = [&](auto inter_, auto cache_) {
         constexpr bool I = decltype(inter_)::value, C = decltype(cache_)::value;
         if constexpr (!I || V >= 2) {
@@ -234,6 +234,7 @@ static int rotary_checks(const char* who, RotaryParams& p, const gdn_rotary_call
                   "%s: bad sizes (the turned part of a head is even and at most the head)", who);
     GDN_CHECK_ARG(c->D <= GDN_ROTARY_MAX_DIM, GDN_ERR_UNSUPPORTED, "%s: heads of up to %d elements", who, GDN_ROTARY_MAX_DIM);
     GDN_CHECK_ARG(c->dtype == GDN_DTYPE_BF16 || c->dtype == GDN_DTYPE_F16 || c->dtype == GDN_DTYPE_F32, GDN_ERR_UNSUPPORTED, "%s: unsupported dtype %d", who, c->dtype);
+    GDN_CHECK_ARG(c->B < (1ll << 31) && c->T < (1ll << 31) && c->B * c->T < (1ll << 31), GDN_ERR_UNSUPPORTED, "%s: fewer than 2^31 tokens", who);
     GDN_CHECK_ARG(!c->cu_seqlens || (c->B == 1 && c->N >= 1), GDN_ERR_INVALID, "%s: a packed batch is one row of tokens with N >= 1 sequences", who);
     GDN_CHECK_ARG(c->rotary_dim == 0 || (c->table_rows >= 0 && (c->table_rows == 0 || (c->cos && c->sin)) && c->table_stride >= c->rotary_dim / 2), GDN_ERR_INVALID, "%s: cos and sin are missing", who);
     p.cos = c->cos; p.sin = c->sin; p.table_stride = c->table_stride; p.table_rows = c->rotary_dim ? c->table_rows : (1ll << 62);

@@ -131,6 +131,8 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
                 raise ValueError('inplace=True needs heads whose elements lie in a row')
             if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
                 raise ValueError('inplace=True needs a tensor that does not overlap itself')
+        if len(xs) == 2 and xs[0].numel() and xs[0].data_ptr() == xs[1].data_ptr():
+            raise ValueError('inplace=True needs queries and keys that do not overlap')
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         return RotaryFunction.apply(cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace, *xs)
     ys = _turn(tuple(x.detach() for x in xs), cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace)
@@ -207,7 +209,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
 class RotaryEmbedding(nn.Module):
     """Queries and keys turned by their positions (``fla.modules.RotaryEmbedding``), ``dim`` elements of each head.  ``scale_base``: the turned pairs of queries are scaled by
     ``s ** ((t - T // 2) / scale_base)``, those of keys by its inverse, ``s = (2j + 0.4 dim) / (1.4 dim)``.  ``scaling``: see ``rotary_frequencies``.  The tables grow with
-    the positions asked for and are no part of the state."""
+    the positions asked for and are no part of the state; those that a captured graph reads are kept as long as the module."""
 
     def __init__(self, dim: int, base: float = 10000.0, scale_base: float | None = None, interleaved: bool = False, pos_idx_in_fp32: bool = True,
                  device: torch.device | None = None, scaling: dict | None = None):
@@ -217,7 +219,7 @@ class RotaryEmbedding(nn.Module):
         self.dim, self.base, self.scale_base, self.interleaved, self.scaling = dim, float(base), scale_base, interleaved, scaling
         inv_freq, self.attention_factor = rotary_frequencies(dim, self.base, scaling)
         self.register_buffer('inv_freq', inv_freq.float().to(device), persistent=False)
-        self._tables = None
+        self._tables, self._captured = None, []
 
     def extra_repr(self) -> str:
         return f'dim={self.dim}, base={self.base}, interleaved={self.interleaved}' + (f', scale_base={self.scale_base}' if self.scale_base is not None else '') + (
@@ -226,13 +228,17 @@ class RotaryEmbedding(nn.Module):
     def tables(self, positions: int, device: torch.device) -> tuple[torch.Tensor, ...]:
         """cos, sin for at least this many positions (and, with ``scale_base``, the keys' cos, sin), fp32."""
         device = torch.device(device)
-        kept = self._tables
+        kept, captured = self._tables, device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
         if kept is not None and kept[0].device == device and (kept[0].shape[0] >= positions if self.scale_base is None else kept[0].shape[0] == positions):
+            if captured and not any(t is kept for t in self._captured):
+                self._captured.append(kept)
             return kept
-        if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+        if captured:
             raise RuntimeError(f'the tables of {positions} positions are not made yet: call RotaryEmbedding.tables({positions}, device) before the capture')
         if kept is not None and kept[0].device == device and self.scale_base is None:
             positions = max(positions, 2 * kept[0].shape[0])             # (asked for position after position: seldom made)
+        if kept is not None and kept[0].is_cuda:
+            torch.cuda.synchronize(kept[0].device)                       # (a call on another stream may still read those that go)
         inv, factor = rotary_frequencies(self.dim, self.base, self.scaling)
         # Made on the host and copied while it waits: whatever stream reads them, they are there.
         with torch.no_grad(), torch.inference_mode(False):

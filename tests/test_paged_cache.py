@@ -358,6 +358,7 @@ def test_library_refuses():
     assert [attn(**kw) for kw in invalid] == [_lib.GDN_ERR_INVALID] * len(invalid)
     assert attn(cache=dict(dtype=2)) == attn(cache=dict(dim=264)) == attn(cache=dict(dim=12)) == attn(cache=dict(page_size=2 ** 29 + 1)) == _lib.GDN_ERR_UNSUPPORTED
     assert attn() == _lib.GDN_ERR_WORKSPACE
+    assert [attn(**kw) for kw in (dict(T=2 ** 25), dict(T=2 ** 26, HQ=1), dict(B=2 ** 40, N=2 ** 40), dict(T=2 ** 40))] == [_lib.GDN_ERR_UNSUPPORTED] * 4
     assert attn(B=0, N=0) == attn(T=0) == attn(HQ=0) == _lib.GDN_OK
     rows = lambda heads: ctypes.byref(_lib.RotaryRows(16, 16, heads))
     append = lambda k=1, v=1, q=None, cache=None, **kw: lib.gdn_paged_append(make(**(cache or {})), None if q is None else rows(q), rows(k), rows(v),

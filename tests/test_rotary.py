@@ -287,6 +287,40 @@ def test_module_under_capture_wants_its_tables_first():
     assert all(torch.equal(a, b) for a, b in zip(held, rope(q, k)))
 
 
+@gpu
+@pytest.mark.parametrize('scale_base', [None, 512.0])
+def test_module_keeps_the_tables_of_captured_graphs(scale_base):
+    rope = _mods().RotaryEmbedding(64, scale_base=scale_base)
+    q, k = _rows(1, 8, 2, 64, dtype=BF), _rows(1, 8, 1, 64, dtype=BF)
+    want = rope(q, k)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = rope(q, k)
+    for positions in (300, 50, 4000):
+        rope(*(x.repeat(1, positions, 1, 1) for x in (q, k)))
+        taken = [torch.full((n, 32), 7.0, device=DEV) for n in (8, 8, 8, 8, 300 * 8, 300 * 8)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), positions
+        del taken
+
+
+@gpu
+def test_empty_calls():
+    mods = _mods()
+    cos, sin = torch.ones(4, 8, device=DEV), torch.zeros(4, 8, device=DEV)
+    for shape in ((0, 3, 2, 16), (2, 0, 2, 16), (2, 3, 0, 16)):
+        x = torch.zeros(*shape, dtype=BF, device=DEV, requires_grad=True)
+        y, z = mods.rotary_embedding_qk(x, x.detach(), cos, sin)
+        assert y.shape == z.shape == shape
+        y.sum().backward()
+        assert x.grad.shape == shape
+    # no keys beside the queries
+    q = _rows(2, 3, 2, 16, dtype=BF)
+    y, z = mods.rotary_embedding_qk(q, q[:, :, :0], cos, sin)
+    assert torch.equal(y, q) and z.shape == (2, 3, 0, 16)
+
+
 @pytest.mark.parametrize('kind', ['linear', 'ntk', 'yarn'])
 def test_frequencies_of_stretched_contexts(kind):
     """What each of them is for: the slowest pair turns `factor` times as slowly, and, but for the first, the fastest as fast as before."""
@@ -351,6 +385,7 @@ def test_refusals(lib):
         (NotImplementedError, lambda: op(x.double(), cos, cos)), (NotImplementedError, lambda: op(x, cos.clone().requires_grad_(), cos)),
         (ValueError, lambda: _mods().rotary_embedding_qk(x, x[:1], cos, cos)), (ValueError, lambda: _mods().rotary_embedding_qk(x, x.float(), cos, cos)),
         (ValueError, lambda: _mods().rotary_embedding_qk(x, x[..., :8], cos, cos)),
+        (ValueError, lambda: _mods().rotary_embedding_qk(x, x, cos, cos, inplace=True)),
     ]
     for error, call in bad:
         with pytest.raises(error):
@@ -383,7 +418,7 @@ def test_library_refuses():
 
     invalid = [dict(B=-1), dict(T=-1), dict(D=0), dict(rotary_dim=15), dict(rotary_dim=18), dict(table_stride=7), dict(cos=None), dict(cu_seqlens=16, B=2), dict(cu_seqlens=16, N=0), dict(table_dtype=1)]
     assert [call(**kw) for kw in invalid] == [_lib.GDN_ERR_INVALID] * len(invalid)
-    unsupported = [dict(D=1026), dict(dtype=3), dict(D=17, flags=_lib.ROTARY_INTERLEAVED)]
+    unsupported = [dict(D=1026), dict(dtype=3), dict(D=17, flags=_lib.ROTARY_INTERLEAVED), dict(B=2 ** 31), dict(T=2 ** 31), dict(B=2 ** 16, T=2 ** 16), dict(T=2 ** 28, D=1024)]
     assert [call(**kw) for kw in unsupported] == [_lib.GDN_ERR_UNSUPPORTED] * len(unsupported)
     assert lib.gdn_rotary(ctypes.byref(rows), 3, ctypes.byref(_lib.RotaryCall(B=1, T=1, D=16)), None) == _lib.GDN_ERR_INVALID
     assert lib.gdn_rotary(ctypes.byref(rows), 1, None, None) == _lib.GDN_ERR_INVALID
