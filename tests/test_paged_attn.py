@@ -259,6 +259,18 @@ def test_packed_batches_with_rows_of_no_sequence(rows):
 
 
 @gpu
+@pytest.mark.parametrize('N', [63, 64, 130])
+def test_packed_batches_of_many_sequences(N):
+    g = torch.Generator().manual_seed(N)
+    contexts, rows = (torch.randint(0, n, (N,), generator=g).tolist() for n in (400, 4))
+    step = Step(contexts, rows, 16, 4, 2, 64, BF, packed=True)
+    o = step.call(max_seqlen=3)
+    spans = list(zip(step.firsts[:-1], step.firsts[1:]))
+    ref, size, dots, spread = O.paged_attn(step.q[0, :sum(rows)], step.k_cache, step.v_cache, step.t, step.contexts, spans, step.sees, step.scale)
+    _near(o[0, :sum(rows)], ref, size, dots, spread, step.L, 64, step.v_cache.abs().max().item())
+
+
+@gpu
 def test_lengths_that_only_the_gpu_knows():
     """Contexts below zero and beyond the table are held to what is there; boundaries that lead outside of the batch read nothing."""
     step = Step([40, 40], [2, 2], 16, 4, 2, 64, BF)

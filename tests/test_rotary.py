@@ -90,6 +90,23 @@ def test_packed_batches(cu, index):
 
 
 @gpu
+@pytest.mark.parametrize('heads', [2, 20])
+@pytest.mark.parametrize('N', [1, 63, 64, 130, 700])
+def test_many_sequences(N, heads):
+    """Some of them empty, rows before the first and behind the last; tokens of few threads and of many."""
+    lengths = torch.randint(0, 4, (N,), generator=torch.Generator().manual_seed(N))
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]) + 3
+    T = int(cu[-1]) + 2
+    at = torch.full((1, T), -1)
+    for n in range(N):
+        at[0, cu[n]:cu[n + 1]] = torch.arange(lengths[n]) + n % 30
+    cos, sin = _tables(40, 128)
+    x = _rows(1, T, heads, 128, dtype=BF)
+    y = _mods().rotary_embedding(x, cos, sin, cu_seqlens=cu.to(DEV), seqlen_offsets=(torch.arange(N) % 30).to(DEV), max_seqlen=T)
+    _near('many', y, *O.rotary(x, cos, sin, at))
+
+
+@gpu
 @pytest.mark.parametrize('index', [torch.int32, torch.int64, torch.int16])
 def test_positions_and_those_the_tables_do_not_have(index):
     cos, sin = _tables(10, 32)
