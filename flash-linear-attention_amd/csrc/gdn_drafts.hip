@@ -11,6 +11,7 @@
 //
 // Everything that decides is in 64 bits and in a fixed order.  Bounded by the memory system for many sequences and words, by latency for few: the first pass, for most
 // sequences the only one, is shared out over workgroups (drafts_round_kernel), each of which walks to it by itself, and one workgroup per sequence finishes.
+// Measured: 16 chains of five drafts over 32000 fp32 words 12.3 us; 32 trees of 15 over 131072 words 45 to 65 (three shared passes of 8.4, then 27; one workgroup per sequence for all: 83).
 #include "gdn_common.h"
 #include <algorithm>
 #include <type_traits>

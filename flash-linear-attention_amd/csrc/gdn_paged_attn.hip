@@ -12,7 +12,12 @@
 // eight keys of V and exchanges them in its registers (one v_perm_b32 per pair).
 //
 // A wave takes tiles of 32 keys by itself, without barriers: K of the next tile is asked for when the scores of this one are formed, V of the next when it is added up, the
-// pages' numbers a tile earlier.  Waves that share rows are joined through LDS at the end, workgroups by paged_attn_join_kernel.  The memory system bounds it up to 128 rows.
+// pages' numbers a tile earlier.  From 33 rows on the four waves of a workgroup take the same keys, 64 at a time, from two stages in LDS (four waves asking for the same rows:
+// 417 us for the long trees below, through LDS 318).  Waves that share rows are joined through LDS at the end, workgroups by paged_attn_join_kernel.
+//
+// The memory system bounds it up to 128 rows.  Measured (bf16, heads of 128, 32 query heads on 8): 64 sequences of 3300 keys, a row each 168 us (5.2 TB/s), of up to 8192 keys 176;
+// eight trees of 32 rows over 32768 keys 221 (4.9 TB/s), of it the join 12; four of 8000 with 256 rows 255 (534 TFLOP/s).  Heads of 80 in pages of 10 are bound by the wait for
+// each tile: 33 chains of 7 over 3001 keys 28 us.
 #include "gdn_paged.h"
 #include "gdn_chunk_common.h"
 #include <algorithm>

@@ -5,7 +5,7 @@
 // The gradient is the turn back (s negated).  Every element is read once and written once; the rows of the tables are read once per row of heads.  The memory system bounds
 // it: a thread turns 16 bytes of either half (or of pairs side by side) for two or three heads of its token, asked for before anything that says where the token stands, and
 // keeps the tables' values in registers for them.  Loads and stores past the caches: 32768 tokens of 20 heads of 128 83 -> 64 us (5.5 TB/s), prompts of 14000 tokens of
-// 48 heads into the cache 116 -> 89, with the rows asked for first 75.
+// 48 heads into the cache 116 -> 89, with the rows asked for first 75, with scalar loads of the places 68.7 (5.2 TB/s).
 #include "gdn_paged.h"
 #include <algorithm>
 #include <type_traits>

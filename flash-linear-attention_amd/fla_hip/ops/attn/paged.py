@@ -1,5 +1,5 @@
 """Softmax attention of a serving step over a paged cache of keys and values: what the attention layers of a model that interleaves them with the gated delta
-rule need beside the recurrence's pools of states.  (The reference runs them through flash_attn with a cache of whole tensors, fla/layers/attn.py.)
+rule need beside the recurrence's pools of states.  (The reference keeps a cache of whole tensors, fla/layers/attn.py.)
 
 The cache is ``k_cache, v_cache [pages, page_size, heads, dim]`` (any strides with a head's elements in a row); slot p of sequence n is slot ``p % page_size`` of page
 ``page_table[n, p // page_size]``.  ``context_lens [N]`` says how many slots hold a token before the step; row i of the step's tokens belongs to slot

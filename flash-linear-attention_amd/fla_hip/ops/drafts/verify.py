@@ -1,5 +1,5 @@
 """Verification of drafted tokens: which stand against the target's probabilities, and the token after them.  The count it returns is what the token recurrence takes as
-``num_accepted_tokens`` (with a state per token), the path what ``fla_hip.ops.attn.paged_keep`` takes.  (The reference leaves generation to transformers.)"""
+``num_accepted_tokens`` (with a state per token), the path what ``fla_hip.ops.attn.paged_keep`` takes."""
 from __future__ import annotations
 
 import ctypes

@@ -6,7 +6,8 @@
  * FFI of its own; its boundary for this path is two Python functions.  Each
  * entry point below is what a binding for one of them calls, and cites the
  * reference interface it replaces.  All pointers are DEVICE pointers unless
- * stated otherwise; all tensors are contiguous, token-major, exactly as the
+ * stated otherwise; all tensors are contiguous (but where an entry takes
+ * strides), token-major, exactly as the
  * reference's `input_guard` hands them to its kernels
  * (fla/utils/_decorators.py:99-165).  Calls only enqueue work on `stream`
  * (a hipStream_t passed as void*, NULL = the null stream); they never
