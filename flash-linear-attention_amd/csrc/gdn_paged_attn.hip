@@ -17,7 +17,7 @@
 //
 // The memory system bounds it up to 128 rows.  Measured (bf16, heads of 128, 32 query heads on 8): 64 sequences of 3300 keys, a row each 168 us (5.2 TB/s), of up to 8192 keys 176;
 // eight trees of 32 rows over 32768 keys 221 (4.9 TB/s), of it the join 12; four of 8000 with 256 rows 255 (534 TFLOP/s).  Heads of 80 in pages of 10 are bound by the wait for
-// each tile: 33 chains of 7 over 3001 keys 28 us.
+// each tile: 33 chains of 7 over 3001 keys 27 us.
 #include "gdn_paged.h"
 #include "gdn_chunk_common.h"
 #include <algorithm>
@@ -749,8 +749,9 @@ static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_att
     plan.height = (int)(each * plan.row_groups);
     plan.step = plan.shares ? 2 * PA_TILE : PA_TILE * (4 / plan.row_groups);
     // What a unit costs besides its keys, in steps.  Measured, us a call (1, 2, 4, 6, 8 steps): 16 sequences of up to 8000 keys with trees of 64 rows 219, 189, 166, 148, 149 (through
-    // LDS); 32 of up to 8000 with 8 rows 142, 129, 131, 131, 133; 256 of up to 1000 with one row 115, 117, 123, 123, 124.
-    plan.overhead = plan.shares ? 6 : plan.row_tiles;
+    // LDS); 32 of up to 8000 with 8 rows of 4 heads 142, 129, 131, 131, 133, 33 of up to 3001 with 7 rows of 2 heads 29.4, 27.7, 27.3; 256 of up to 1000 with one row of 4 heads 115,
+    // 117, 123, 123, 124, one of 4000 15.6, 16.6, 16.9.
+    plan.overhead = plan.shares ? 6 : rows > 8 ? 2 : 1;
     // One round of the chip: two workgroups share a CU (one where a head of 256 takes a wave's registers), but no more than there can be steps.
     const int64_t units = std::max<int64_t>(1, c->N) * cache->heads * ((rows + plan.height - 1) / plan.height);
     const int64_t steps = std::max<int64_t>(1, (cache->table_cols * cache->page_size + plan.step - 1) / plan.step);
