@@ -61,14 +61,15 @@ __device__ void draft_tests(const DraftParams& p, int64_t n, int rows, DraftShar
     for (int r = threadIdx.x; r < rows; r += blockDim.x) {
         int parent = r - 1;
         if (p.parents) parent = p.parents[n * p.parents_stride + r];
-        if (r == 0 || parent < 0 || parent >= r) parent = -1;
         const int64_t word = p.tokens64 ? ((const int64_t*)p.tokens)[n * p.R + r] : (int64_t)((const int32_t*)p.tokens)[n * p.R + r];
         const bool known = word >= 0 && word < p.V;
+        // (a word outside the vocabulary was drawn from nothing and takes nothing: its row follows none)
+        if (r == 0 || parent < 0 || parent >= r || !known) parent = -1;
         s.parent[r] = parent;
-        s.word[r] = known ? (int)word : -1;
+        s.word[r] = (int)word;
         s.u[r] = p.u[n * p.R + r];
-        s.p[r] = known && parent >= 0 ? mass_of(((const T*)p.p)[n * p.p_seq + parent * p.p_row + word]) : 0.0;
-        s.q[r] = !p.q ? 1.0 : known && parent >= 0 ? mass_of(((const T*)p.q)[n * p.q_seq + parent * p.q_row + word]) : 0.0;
+        s.p[r] = parent >= 0 ? mass_of(((const T*)p.p)[n * p.p_seq + parent * p.p_row + word]) : 0.0;
+        s.q[r] = !p.q ? 1.0 : parent >= 0 ? mass_of(((const T*)p.q)[n * p.q_seq + parent * p.q_row + word]) : 0.0;
     }
 }
 
@@ -92,7 +93,7 @@ __device__ void draft_walk(const DraftParams& p, int rows, DraftShared& s) {
         if (c >= rows) break;
         w.last = c;
         const int word = s.word[c];
-        double left = word < 0 ? 0.0 : weight(p.q != nullptr, w.a, w.b, s.p[c], s.q[c]);
+        double left = weight(p.q != nullptr, w.a, w.b, s.p[c], s.q[c]);
         if (!p.q)
             for (int k = 0; k < w.refused; ++k)
                 if (s.refused[k] == word) left = 0.0;

@@ -25,7 +25,7 @@ def verify_drafts(
 
     From row 0 on the drafts that follow the row come to are asked in order: a draft x stands where ``u q(x) < p(x)``, and the walk goes on from it; one that does not
     leaves ``p = (p - q)+ / sum`` to the next (without draft_probs: p without x; p as it was where nothing would be left).  When none is left the next token is the first v
-    with ``sum(p[: v + 1]) > u sum(p)``.  So tokens are distributed as the target's own, whatever was drafted.
+    with ``sum(p[: v + 1]) > u sum(p)``.  A draft outside the vocabulary (a padded row, -1) is passed over.  So tokens are distributed as the target's own, whatever was drafted.
 
     Returns ``(next_token [N] int64, num_accepted [N] int32, rows [N, R] int32)``: the token to go on with (-1 where p has no finite mass), the number of rows that stand, row 0
     among them, and which, in order, -1 behind them.  Computed in 64 bits; nothing of it is differentiable."""

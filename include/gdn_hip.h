@@ -794,7 +794,7 @@ int gdn_paged_attn(const gdn_paged_cache* cache, const gdn_paged_attn_call* call
  *   p, q [N,R,V] (bf16, fp16 or fp32) with strides in elements (sequence, row); tokens [N,R] (int32, or int64 with GDN_DRAFTS_TOKENS_INT64); u [N,R] fp32;
  *   parents [N,R] int32 with parents_stride (0: one tree for all); lengths [N] int32 or NULL: rows of a sequence (at least 1)
  *   next_token [N] int64, accepted [N] int32 (rows that stand, row 0 among them), rows [N,R] int32 (which, in order; -1 behind them)
- *   A draft outside the vocabulary, and a row whose parent is not before it, is never taken.
+ *   A draft outside the vocabulary, and a row whose parent is not before it, is passed over: it is never taken and takes nothing from p.
  */
 #define GDN_DRAFTS_TOKENS_INT64 (1u << 24)
 #define GDN_DRAFTS_MAX_ROWS 1024

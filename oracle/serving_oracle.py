@@ -76,19 +76,19 @@ def verify_drafts(p, tokens, u, parents=None, q=None, lengths=None):
         path, left = [0], p[n, 0].clone()
         for r in range(1, count):
             parent = r - 1 if parents is None else int(parents[r] if parents.dim() == 1 else parents[n, r])
-            if parent != path[-1] or parent >= r:
-                continue
             word = int(tokens[n, r])
-            known = 0 <= word < V
-            chance = (1.0 if q is None else float(q[n, parent, word])) if known else 0.0
-            if known and float(u[n, r]) * chance < float(left[word]):
+            # (a word outside the vocabulary was drawn from nothing: there is nothing of it to take from p)
+            if parent != path[-1] or parent >= r or not 0 <= word < V:
+                continue
+            chance = 1.0 if q is None else float(q[n, parent, word])
+            if float(u[n, r]) * chance < float(left[word]):
                 path.append(r)
                 left = p[n, r].clone()
                 continue
             rest = left.clone()
             if q is not None:
                 rest = (rest - q[n, parent]).clamp(min=0)
-            elif known:
+            else:
                 rest[word] = 0
             if float(rest.sum()) > 0:
                 left = rest / rest.sum()

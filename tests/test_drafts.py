@@ -250,3 +250,57 @@ def test_library_refuses():
     unsupported = [dict(R=1025), dict(V=4194305), dict(N=65536), dict(p_dtype=3)]
     assert [call(**kw) for kw in unsupported] == [_lib.GDN_ERR_UNSUPPORTED] * len(unsupported)
     assert call() == _lib.GDN_ERR_WORKSPACE and call(N=0) == _lib.GDN_OK
+
+
+def _outside(sampled, tree, dtype=torch.int32):
+    """Inputs of which every third draft is a word outside the vocabulary, and the same without those rows: rows without a parent."""
+    x = _inputs(40, 12, 300, sampled=sampled, tree=tree, apart=2.0, seed=7)
+    if not tree:
+        x['parents'] = (torch.arange(12) - 1).expand(40, 12).int()
+    x['tokens'], x['u'] = x['tokens'].to(dtype), x['u'] * 0.6
+    out = torch.rand(40, 12, generator=torch.Generator().manual_seed(1)) < 0.3
+    out[:, 0] = False
+    without = dict(x, parents=torch.where(out, -1, x['parents']).int())
+    x['tokens'] = torch.where(out, torch.tensor([-1, 300, 2 ** 31 - 1])[torch.arange(12) % 3].to(dtype), x['tokens'])
+    return x, without
+
+
+@pytest.mark.parametrize('tree', [False, True])
+@pytest.mark.parametrize('sampled', [False, True])
+def test_oracle_of_drafts_outside_the_vocabulary(sampled, tree):
+    """They were drawn from nothing, so they take nothing: the oracle says what it says without their rows."""
+    x, without = _outside(sampled, tree)
+    for a, b in zip(*(O.verify_drafts(d['p'], d['tokens'], d['u'], d['parents'], d['q']) for d in (x, without))):
+        assert torch.equal(a, b)
+    p, q = torch.tensor([0.5, 0.3, 0.2]), torch.tensor([0.2, 0.3, 0.5])
+    u = torch.stack([torch.linspace(0, 1, 1001)[:-1], torch.full((1000,), 0.5)], 1)
+    token = O.verify_drafts(p.expand(1000, 2, 3), torch.tensor([[0, -1]]).expand(1000, 2), u, None, q.expand(1000, 2, 3) if sampled else None)[0]
+    assert ((torch.bincount(token, minlength=3) / 1000 - p).abs() <= 1.5e-3).all()      # (a thousand equal steps: an end of each word off by one)
+
+
+@gpu
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+@pytest.mark.parametrize('tree', [False, True])
+@pytest.mark.parametrize('sampled', [False, True])
+def test_drafts_outside_the_vocabulary_take_nothing(sampled, tree, index):
+    x, without = _outside(sampled, tree, index)
+    want = _same(**without)
+    got = _same(**x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_tokens_of_padded_rows_are_distributed_as_the_targets():
+    """As test_tokens_are_distributed_as_the_targets, with rows that a server has padded by -1 in most of the sequences."""
+    N, V = 20000, 6
+    gen = torch.Generator().manual_seed(4)
+    p, q = torch.softmax(torch.randn(4, V, generator=gen), -1), torch.softmax(torch.randn(4, V, generator=gen), -1)
+    for parents in (torch.tensor([-1, 0, 1, 2]), torch.tensor([-1, 0, 0, 0])):
+        up = parents.clamp(min=0)
+        tokens = torch.stack([torch.multinomial(q[up[r]], N, replacement=True, generator=gen) for r in range(4)], 1)
+        tokens[torch.arange(4) >= torch.randint(1, 5, (N, 1), generator=gen)] = -1
+        u = torch.rand(N, 4, generator=gen)
+        token, accepted, rows = (x.cpu() for x in _verify(p.expand(N, 4, V).to(DEV), tokens.to(DEV), u.to(DEV), parents=parents.to(DEV), draft_probs=q.expand(N, 4, V).to(DEV)))
+        first = torch.where(accepted > 1, tokens[torch.arange(N), rows[:, 1].long().clamp(min=0)], token)
+        share = torch.bincount(first, minlength=V) / N
+        assert ((share - p[0]).abs() <= 5 * (p[0] * (1 - p[0]) / N).sqrt()).all(), (parents, share, p[0])
