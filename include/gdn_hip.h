@@ -771,7 +771,7 @@ int gdn_paged_keep(const gdn_paged_cache* cache, const int32_t* rows, int64_t ro
  * step's own (which are in the cache by then) those with mask[i][j], or j <= i without a mask.  A row that sees none gets 0.
  *   q [B,T,HQ,D] with strides in elements (batch, token, head), o [B,T,HQ,D] contiguous, of the cache's dtype (bf16 or fp16); HQ a multiple of the cache's heads
  *   cu_seqlens [N+1] (GDN_FLAG_CU_INT32) or NULL (N = B sequences of T rows); max_rows: at least the rows of the longest sequence
- *   mask: bytes, row i of sequence n at n * mask_seq_stride + i * mask_row_stride (with cu_seqlens at (cu[n] + i) * mask_row_stride); key j >= mask_cols is not seen
+ *   mask: bytes, row i of sequence n at n * mask_seq_stride + i * mask_row_stride (with cu_seqlens at (cu[n] + i) * mask_row_stride); key j >= mask_cols (at least 1 with a mask) is not seen
  *   Scores, statistics and sums in fp32; the probabilities are rounded to dtype for their product with v.  Rows of no sequence get 0.
  */
 typedef struct gdn_paged_attn_call {

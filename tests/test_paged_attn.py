@@ -352,3 +352,21 @@ def test_replayed_graphs_that_share_the_cache():
             torch.cuda.synchronize()
             got = outs[i].clone()
             assert torch.equal(got, _step_call(step, *ins[i], cos, sin, t, context))
+
+
+def _refusals(**sizes):
+    """(bytes of a workspace, code) of calls at the C entry, without a workspace: nothing is launched."""
+    import ctypes
+    from fla_hip import _lib
+    lib = _lib.load()
+    cache = _lib.PagedCache(k=16, v=16, page_table=16, context=16, pages=2, page_size=4, heads=1, dim=16, table_cols=2, table_stride=2, dtype=0)
+    call = _lib.PagedAttnCall(**{**dict(q=16, o=16, B=1, T=1, N=1, HQ=2, max_rows=1), **sizes})
+    return lib.gdn_paged_attn_workspace_bytes(ctypes.byref(cache), ctypes.byref(call)), lib.gdn_paged_attn(ctypes.byref(cache), ctypes.byref(call), None, 0, None)
+
+
+def test_library_refuses_masks_without_columns():
+    """A mask of no columns has no place in its rows that could be read."""
+    from fla_hip import _lib
+    for cols in (0, -1, -2 ** 40):
+        assert _refusals(mask=16, mask_cols=cols) == (0, _lib.GDN_ERR_INVALID)
+    assert _refusals(mask=16, mask_cols=1)[1] == _refusals(mask_cols=0)[1] == _lib.GDN_ERR_WORKSPACE
