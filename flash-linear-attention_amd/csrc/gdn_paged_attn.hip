@@ -728,9 +728,9 @@ static int check_attn(const char* who, const gdn_paged_cache* cache, const gdn_p
     // (a row's bytes are asked for before it is known which of them count: one of them has to be there)
     GDN_CHECK_ARG(!c->mask || c->mask_cols >= 1, GDN_ERR_INVALID, "%s: a mask has columns", who);
     GDN_CHECK_ARG(cache->dtype != GDN_DTYPE_F32 && cache->dim <= PA_MAX_DIM && cache->dim % 8 == 0, GDN_ERR_UNSUPPORTED, "%s: bf16 or fp16 heads of a multiple of 8 up to %d elements", who, PA_MAX_DIM);
-    // (a launch has fewer than 2^32 threads, the last of 64 for each row of a head)
-    GDN_CHECK_ARG(c->B < (1ll << 26) && c->T < (1ll << 26) && c->HQ < (1ll << 26) && c->B * c->T < (1ll << 26) && c->B * c->T * c->HQ < (1ll << 26) && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
-                  "%s: rows times heads below 2^26, up to 2^30 slots of a sequence", who);
+    // (a launch has fewer than 2^32 threads: 64 for each row of a head, in blocks of 256)
+    GDN_CHECK_ARG(c->B < (1ll << 26) && c->T < (1ll << 26) && c->HQ < (1ll << 26) && c->B * c->T < (1ll << 26) && c->B * c->T * c->HQ <= (1ll << 26) - 4 && cache->table_cols * cache->page_size <= (1ll << 30) && c->mask_cols < (1ll << 31), GDN_ERR_UNSUPPORTED,
+                  "%s: rows times heads up to 2^26 - 4, up to 2^30 slots of a sequence", who);
     // (the work is counted in 64 bits, times the workgroups)
     GDN_CHECK_ARG((double)c->N * (double)cache->heads * (double)(c->T * (c->HQ / cache->heads) / 16 + 1) * (double)(cache->table_cols * cache->page_size / 32 + 8) < 4e15, GDN_ERR_UNSUPPORTED,
                   "%s: too much work for one call", who);

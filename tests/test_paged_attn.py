@@ -370,3 +370,11 @@ def test_library_refuses_masks_without_columns():
     for cols in (0, -1, -2 ** 40):
         assert _refusals(mask=16, mask_cols=cols) == (0, _lib.GDN_ERR_INVALID)
     assert _refusals(mask=16, mask_cols=1)[1] == _refusals(mask_cols=0)[1] == _lib.GDN_ERR_WORKSPACE
+
+
+def test_library_refuses_more_rows_than_a_launch_has_threads():
+    """64 threads for each row of a head, in blocks of 256, below 2^32 in all."""
+    from fla_hip import _lib
+    for rows in (2 ** 26 - 3, 2 ** 26 - 1):
+        assert _refusals(T=rows, HQ=1) == (0, _lib.GDN_ERR_UNSUPPORTED)
+    assert _refusals(T=2 ** 26 - 4, HQ=1)[1] == _lib.GDN_ERR_WORKSPACE
