@@ -379,7 +379,7 @@ struct PagedWave {
             for (int i = 0; i < 8; ++i) most = fmaxf(most, x[r][i / 4][i % 4]);
             // m is a maximum that was passed by 2^8 at most: it is the same in the four lanes of a row and moves a few times only (as the true maximum it would move in
             // four tiles of ten of the first 4000 keys).  The sums' terms are up to 2^8 then, of 2^128 (of 2^16 where weights are rounded to fp16).
-            if (__any(most * p.scale2 > m[r] * p.scale2 + 8.f || (m[r] == -INFINITY && most > m[r]))) {
+            if (__any((most - m[r]) * p.scale2 > 8.f || (m[r] == -INFINITY && most > m[r]))) {
                 most = fmaxf(most, __shfl_xor(most, 16, 64));
                 most = fmaxf(most, __shfl_xor(most, 32, 64));
                 const float now = fmaxf(m[r], most), keep = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[r] - now) * p.scale2);
@@ -389,10 +389,11 @@ struct PagedWave {
                 for (int t = 0; t < MT; ++t) o[r][t] *= keep;
             }
             // (no maximum yet: nothing is seen, or what is seen is not a number and makes the row's sums so)
-            const float base = m[r] == -INFINITY ? 0.f : m[r] * p.scale2;
+            // (the distance from it before the scale: a large score's steps may be far above 1, its distance from itself is 0)
+            const float base = m[r] == -INFINITY ? 0.f : m[r];
             float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i / 4][i % 4], p.scale2, -base));
+            for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f((x[r][i / 4][i % 4] - base) * p.scale2);
             if (!whole) {                                                   // (of a scale of zero nothing is -inf)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = x[r][i / 4][i % 4] == -INFINITY ? 0.f : y[i];

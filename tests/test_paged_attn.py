@@ -378,3 +378,33 @@ def test_library_refuses_more_rows_than_a_launch_has_threads():
     for rows in (2 ** 26 - 3, 2 ** 26 - 1):
         assert _refusals(T=rows, HQ=1) == (0, _lib.GDN_ERR_UNSUPPORTED)
     assert _refusals(T=2 ** 26 - 4, HQ=1)[1] == _lib.GDN_ERR_WORKSPACE
+
+
+@gpu
+@pytest.mark.parametrize('sign', [1, -1])
+@pytest.mark.parametrize(('rows', 'D', 'page_size'), [(1, 64, 16), (7, 128, 10), (40, 128, 16), (80, 64, 16)])
+@pytest.mark.parametrize('dtype', [BF, HF])
+def test_scores_beyond_the_steps_of_an_exponent(dtype, rows, D, page_size, sign):
+    """Scores so large that their own rounding steps are far above 1: keys that are the same share the weight, wherever the largest score comes, and every other key has
+    none.  Equal keys give equal scores in the kernel, so their weights are equal, whatever is lost: the result is the mean of their values, off by its sum in fp32 and the
+    rounding of the weights and of the result."""
+    context = 200
+    first = _attn()
+    for large in (3000.0, 60000.0):
+        for at in ([0, 1, 150], [199], [40, 170, 171, 172]):
+            k = torch.zeros(context + rows, 1, D)
+            k[5::7] = -large                                    # (scores far below)
+            k[3::7] = 0.5 * large
+            k[at] = large
+            v = torch.randn(context + rows, 1, D, generator=torch.Generator().manual_seed(rows)).to(dtype)
+            pages = -(-(context + rows) // page_size)
+            caches = []
+            for x in (k, v):
+                c = torch.zeros(pages * page_size, 1, D, dtype=dtype)
+                c[:context + rows] = x.to(dtype)
+                caches.append(c.view(pages, page_size, 1, D).to(DEV))
+            q = torch.full((1, rows, 2, D), sign * large, dtype=dtype, device=DEV)
+            o = first.paged_attn(q, *caches, torch.arange(pages, dtype=torch.int32, device=DEV)[None], torch.tensor([context], dtype=torch.int32, device=DEV), scale=sign * D ** -0.5)
+            want = v[at].double().mean(0)
+            tol = torch.finfo(dtype).eps / 2 * (want.abs() * (1 + 1e-3) + v[at].double().abs().mean(0)) + 2 * (context + rows + 64) * E * v[at].double().abs().mean(0) + 2.0 ** -25
+            assert bool(((o.cpu().double() - want).abs() <= tol).all()), (large, at, o[0, 0, 0, :4], want[0, :4])
