@@ -50,6 +50,10 @@ typedef uint16_t pa_aligned __attribute__((ext_vector_type(8)));
 // Infinities and NaN: an exponent of ones.  In a pair: its upper bit carries into the sign's place.
 template <typename T> constexpr uint32_t PA_EXPONENT = std::is_same_v<T, bf16_t> ? 0x7f80 : 0x7c00;
 template <typename T> constexpr uint32_t PA_CARRY = std::is_same_v<T, bf16_t> ? 0x0080 : 0x0400;
+// Weights are 2^PA_LIFT at the row's maximum, and up to 2^8 times that before the maximum moves, below fp16's 2^16: rounded to fp16 a weight loses what is below 2^-32 of
+// the maximum's, of which two million keys together make half a step of the largest value. (Without the lift 2^-25: 131071 keys 17.4 below one in their score, 0.36 % of
+// the result, were 0.)  The factor is in the weights' sum, too.  bf16 has the range of fp32.
+template <typename T> constexpr float PA_LIFT = std::is_same_v<T, bf16_t> ? 0.f : 7.f;
 template <typename T> __device__ __forceinline__ bool not_a_number(uint16_t bits) { return (bits & PA_EXPONENT<T>) == PA_EXPONENT<T>; }
 
 // (the same in every lane by construction)
@@ -378,7 +382,7 @@ struct PagedWave {
 #pragma unroll
             for (int i = 0; i < 8; ++i) most = fmaxf(most, x[r][i / 4][i % 4]);
             // m is a maximum that was passed by 2^8 at most: it is the same in the four lanes of a row and moves a few times only (as the true maximum it would move in
-            // four tiles of ten of the first 4000 keys).  The sums' terms are up to 2^8 then, of 2^128 (of 2^16 where weights are rounded to fp16).
+            // four tiles of ten of the first 4000 keys).  The sums' terms are up to 2^8 then (of fp16 2^15, PA_LIFT), of 2^128.
             if (__any((most - m[r]) * p.scale2 > 8.f || (m[r] == -INFINITY && most > m[r]))) {
                 most = fmaxf(most, __shfl_xor(most, 16, 64));
                 most = fmaxf(most, __shfl_xor(most, 32, 64));
@@ -393,7 +397,7 @@ struct PagedWave {
             const float base = m[r] == -INFINITY ? 0.f : m[r];
             float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f((x[r][i / 4][i % 4] - base) * p.scale2);
+            for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][i / 4][i % 4] - base, p.scale2, PA_LIFT<T>));
             if (!whole) {                                                   // (of a scale of zero nothing is -inf)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = x[r][i / 4][i % 4] == -INFINITY ? 0.f : y[i];

@@ -408,3 +408,40 @@ def test_scores_beyond_the_steps_of_an_exponent(dtype, rows, D, page_size, sign)
             want = v[at].double().mean(0)
             tol = torch.finfo(dtype).eps / 2 * (want.abs() * (1 + 1e-3) + v[at].double().abs().mean(0)) + 2 * (context + rows + 64) * E * v[at].double().abs().mean(0) + 2.0 ** -25
             assert bool(((o.cpu().double() - want).abs() <= tol).all()), (large, at, o[0, 0, 0, :4], want[0, :4])
+
+
+def _one_key_above_many(HQ, HK, D, rows, context, dtype, at, score, value, page_size=64, N=1, bad_at=None, bad=None):
+    """N sequences that share the pages of one: the key in slot `at` has score `score` and values `value`, all others score 0 and values from 0.5 to 1.5 (the one in
+    slot bad_at: bad).  (o [N, rows, HQ, D], the oracle's, its magnitudes, dots and spread for one sequence)"""
+    pages = -(-(context + rows) // page_size)
+    gen = torch.Generator().manual_seed(context)
+    k = torch.zeros(pages * page_size, HK, D)
+    k[at, :, 0] = score
+    v = (0.5 + torch.rand(pages * page_size, HK, D, generator=gen)).to(dtype)
+    v[at] = value
+    if bad is not None:
+        v[bad_at, :, 1] = bad
+    k_cache, v_cache = (x.to(dtype).view(pages, page_size, HK, D).to(DEV) for x in (k, v))
+    q = torch.zeros(N, rows, HQ, D, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    order = torch.arange(pages, dtype=torch.int32)
+    o = _attn().paged_attn(q, k_cache, v_cache, order.expand(N, pages).contiguous().to(DEV), torch.full((N,), context, dtype=torch.int32, device=DEV), scale=1.0)
+    ref = O.paged_attn(q[0, :1], k_cache, v_cache, order[None], [context], [(0, 1)], lambda n, i, j: True, 1.0)
+    return o, ref
+
+
+@gpu
+@pytest.mark.parametrize('at', [0, 70000, 131070])
+@pytest.mark.parametrize('rows', [1, 9, 40])
+@pytest.mark.parametrize('dtype', [BF, HF])
+def test_many_small_weights_behind_one_large(dtype, rows, at):
+    """131071 keys e^-17.4375 of one key each, whose own values are 0: what is left of the result are the small ones, together 0.35 % of the weights.  A weight is held
+    relative to 2^7 times the row's maximum, so one below the smallest normal number of fp16 is off by 2^-32 of the largest: L 2^-32 max |v| in the tolerance that the head
+    of this file derives.  (The first row alone is compared: those behind it see a key more each.)"""
+    context = 131071
+    o, (ref, size, dots, spread) = _one_key_above_many(2, 1, 64, rows, context, dtype, at, 17.4375, 0.0, N=600)
+    u, L = torch.finfo(dtype).eps / 2, context + 1
+    d = 2 * (68 * E * dots + 4 * E * (spread + 1))[..., None]
+    tol = u * ref.abs() * (1 + 1e-3) + (2 * d + u + 2 * (L + 64) * E) * size + (L * 1.5 + 1) * (2.0 ** -32 if dtype == HF else 2.0 ** -130)
+    err = (o[:, :1].cpu().double() - ref).abs()
+    assert bool((err <= tol).all()), f'{(err / tol).max().item():.2f} of the tolerance, {(err / ref).max().item():.4f} of the result'
