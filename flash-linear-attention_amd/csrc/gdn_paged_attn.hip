@@ -405,7 +405,7 @@ struct PagedWave {
             l[r] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
             w[r] = __builtin_bit_cast(V8, u32x4{pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])});
         }
-        if (!whole && __any(odd_values())) clean(w, at, stage);
+        if (!whole && __any(odd_values())) clean(bits, at, stage);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             const V8 a = operand(t);
@@ -422,9 +422,9 @@ struct PagedWave {
         for (int i = 0; i < DT / 4; ++i) carried |= carry(v[i]);
         return carried;
     }
-    // They are taken out of V and kept in LDS for the rows that see the key, a bit for each row and element: what a sum of infinities and NaN will be, whatever is
-    // added to it (both bits: NaN).
-    __device__ __forceinline__ void clean(const V8 (&w)[RT], const TilePlaces<UNIFORM>& at, const char* stage) {
+    // They are taken out of V and kept in LDS for the rows that see the key (bits, seen()), however little it weighs: a bit for each row and element: what a sum of
+    // infinities and NaN will be, whatever is added to it (both bits: NaN).
+    __device__ __forceinline__ void clean(const uint32_t (&bits)[RT], const TilePlaces<UNIFORM>& at, const char* stage) {
         const int lane = unhoisted(this->lane), c16 = lane & 15, g = lane >> 4;
         uint64_t* const mine = odd_bits + (16 * g + c16) * ODD;                 // (lanes of g < RT: row 16 g + c16)
         if (!odd) {
@@ -432,12 +432,12 @@ struct PagedWave {
                 for (int i = 0; i < ODD; ++i) mine[i] = 0;
             odd = true;
         }
-        uint32_t row = 0;                                                   // the keys that the lane's row has weights for
+        uint32_t row = 0;                                                   // the keys that the lane's row sees
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             uint32_t keys = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) keys |= (float)w[r][i] != 0.f ? 1u << (16 * (i / 4) + 4 * g + i % 4) : 0;
+            for (int i = 0; i < 8; ++i) keys |= bits[r] >> i & 1 ? 1u << (16 * (i / 4) + 4 * g + i % 4) : 0;
             keys |= __shfl_xor(keys, 16, 64);
             keys |= __shfl_xor(keys, 32, 64);
             if (g == r) row = keys;

@@ -445,3 +445,15 @@ def test_many_small_weights_behind_one_large(dtype, rows, at):
     tol = u * ref.abs() * (1 + 1e-3) + (2 * d + u + 2 * (L + 64) * E) * size + (L * 1.5 + 1) * (2.0 ** -32 if dtype == HF else 2.0 ** -130)
     err = (o[:, :1].cpu().double() - ref).abs()
     assert bool((err <= tol).all()), f'{(err / tol).max().item():.2f} of the tolerance, {(err / ref).max().item():.4f} of the result'
+
+
+@gpu
+@pytest.mark.parametrize('slot', [3, 31, 40, 76, 97, 99])
+@pytest.mark.parametrize('rows', [1, 40])
+@pytest.mark.parametrize('dtype', [BF, HF])
+def test_a_value_that_is_not_a_number_behind_a_small_weight(dtype, rows, slot):
+    """Wherever its key lies, in a tile of the context or in the last, beside the one that outweighs it - all rows see both - an element that is NaN makes the rows' NaN, and an infinity leaves no number."""
+    for D in (64, 128):
+        for bad in (float('nan'), float('inf')):
+            o, _ = _one_key_above_many(2, 1, D, rows, 100, dtype, slot // 32 * 32 + 2, 30.0, 1.0, page_size=16, bad_at=slot, bad=bad)
+            assert (o[..., 1].isnan() if bad != bad else ~o[..., 1].isfinite()).all() and o[..., 0].isfinite().all() and o[..., 2:].isfinite().all(), (D, bad)
