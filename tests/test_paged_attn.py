@@ -457,3 +457,43 @@ def test_a_value_that_is_not_a_number_behind_a_small_weight(dtype, rows, slot):
         for bad in (float('nan'), float('inf')):
             o, _ = _one_key_above_many(2, 1, D, rows, 100, dtype, slot // 32 * 32 + 2, 30.0, 1.0, page_size=16, bad_at=slot, bad=bad)
             assert (o[..., 1].isnan() if bad != bad else ~o[..., 1].isfinite()).all() and o[..., 0].isfinite().all() and o[..., 2:].isfinite().all(), (D, bad)
+
+
+# keys through LDS (more than 32 rows of a head of the cache, pages of whole tiles): parts of a head of 128 and of 256 elements, and fp16
+@gpu
+@pytest.mark.parametrize(('rows', 'HQ', 'HK', 'D', 'page_size', 'dtype'), [(40, 4, 2, 80, 16, HF), (70, 8, 2, 96, 64, BF), (50, 4, 2, 200, 16, HF), (64, 8, 1, 128, 32, HF), (33, 3, 1, 136, 48, BF),
+                                                                          (129, 2, 2, 72, 16, HF), (40, 2, 1, 256, 16, HF), (90, 1, 1, 64, 16, HF), (36, 4, 4, 8, 16, BF)])
+@pytest.mark.parametrize('kind', ['chain', 'trees', 'packed'])
+def test_keys_through_lds(kind, rows, HQ, HK, D, page_size, dtype):
+    gen = torch.Generator().manual_seed(rows)
+    counts = [rows, 1, max(1, rows // 3)] if kind == 'packed' else [rows] * 3
+    mask = torch.stack([_tree(gen, rows) for _ in range(3)]) if kind == 'trees' else None
+    Step([300, 0, 77], counts, page_size, HQ, HK, D, dtype, kind == 'packed', mask, seed=rows).check()
+
+
+@gpu
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize(('rows', 'page_size', 'D', 'dtype'), [(1, 16, 64, HF), (6, 10, 128, HF), (40, 16, 80, HF), (40, 16, 96, BF), (40, 64, 200, BF), (70, 16, 128, HF), (36, 16, 256, HF), (12, 16, 72, HF)])
+def test_numbers_in_masked_places_of_other_heads_and_types(rows, page_size, D, dtype, bad):
+    """NaN and infinities in slots that no row sees, and in a draft that some rows do not see: nothing of them in those rows."""
+    contexts = [50, 0, 33]
+    mask = torch.stack([_tree(torch.Generator().manual_seed(n), rows) for n in range(3)])
+
+    def spoil(step):
+        used = torch.zeros(step.k_cache.shape[:2], dtype=torch.bool)
+        for n, c in enumerate(contexts):
+            for j in range(c + rows):
+                used[O.slot_of(step.t, n, j, *step.k_cache.shape[:2])] = True
+        for c in (step.k_cache, step.v_cache):
+            c[~used.to(DEV)] = bad
+
+    step = Step(contexts, [rows] * 3, page_size, 4, 2, D, dtype, mask=mask, spoil=spoil)
+    want = step.check()
+    j = rows // 2
+    step.v_cache[O.slot_of(step.t, 0, contexts[0] + j, *step.v_cache.shape[:2])][:, 5] = bad
+    got = step.call()
+    sees = torch.tensor([step.sees(0, i, j) for i in range(rows)])
+    assert torch.equal(got[0, ~sees], want[0, ~sees]) and torch.equal(got[1:], want[1:])
+    assert torch.equal(got[0, :, :, :5], want[0, :, :, :5]) and torch.equal(got[0, :, :, 6:], want[0, :, :, 6:])
+    seen = got[0, sees][..., 5].float()
+    assert seen.isnan().all() if bad != bad else (seen == bad).all()
