@@ -56,7 +56,12 @@ struct RotaryTrain : torch::autograd::Function<RotaryTrain> {
         variable_list xs = {a};
         if (b) xs.push_back(*b);
         ctx->save_for_backward({t.cos, t.sin, t.positions, t.offsets, t.cu});
-        ctx->saved_data["call"] = std::vector<int64_t>{t.offset, t.interleaved, t.back, (int64_t)a.scalar_type(), (int64_t)b.has_value()};
+        std::vector<int64_t> call = {t.offset, t.interleaved, t.back, (int64_t)a.scalar_type(), (int64_t)b.has_value(), t.cos.size(1)};
+        for (const at::Tensor* s : {&t.cos, &t.sin, &t.positions, &t.offsets, &t.cu}) {
+            call.push_back(s->defined() ? (int64_t)s->scalar_type() : 0);
+            call.push_back(s->defined() ? s->numel() : 0);
+        }
+        ctx->saved_data["call"] = std::move(call);
         ctx->saved_data["device"] = a.device();
         ctx->set_materialize_grads(false);
         return turn(t, xs);
@@ -68,10 +73,16 @@ struct RotaryTrain : torch::autograd::Function<RotaryTrain> {
         const bool two = n[4];
         variable_list out(3), dys;
         const auto saved = ctx->get_saved_variables();
-        auto here = [&](const at::Tensor& t) { return t.defined() ? t.to(dev) : t; };
-        RotaryTables t{here(saved[0]), here(saved[1]), here(saved[2]), here(saved[3]), here(saved[4]), n[0], (bool)n[1], !n[2]};
-        TORCH_CHECK_VALUE(t.cos.sizes() == t.sin.sizes() && t.cos.dim() == 2, "saved tables of rotary positions came back with other sizes");
-        if (!in_rows(t.cos) || !in_rows(t.sin) || t.cos.stride(0) != t.sin.stride(0)) { t.cos = t.cos.contiguous(); t.sin = t.sin.contiguous(); }
+        // (in the type and the place that they had: saved-tensor hooks may hand back others)
+        auto here = [&](int i) {
+            const at::Tensor& x = saved[i];
+            if (!x.defined()) return x;
+            TORCH_CHECK_VALUE(x.numel() == n[7 + 2 * i], "a saved tensor of ", n[7 + 2 * i], " elements came back with ", x.numel());
+            return x.to(dev, (at::ScalarType)n[6 + 2 * i]);
+        };
+        RotaryTables t{here(0), here(1), here(2), here(3), here(4), n[0], (bool)n[1], !n[2]};
+        TORCH_CHECK_VALUE(t.cos.sizes() == t.sin.sizes() && t.cos.dim() == 2 && t.cos.size(1) == n[5], "saved tables of rotary positions came back with other sizes");
+        if (!in_rows(t.cos) || !in_rows(t.sin) || t.cos.stride(0) != t.sin.stride(0) || t.cos.stride(0) < t.cos.size(1)) { t.cos = t.cos.contiguous(); t.sin = t.sin.contiguous(); }
         for (at::Tensor* index : {&t.positions, &t.offsets, &t.cu})
             if (index->defined()) *index = index->contiguous();
         for (size_t i = 0; i < (two ? 2u : 1u); ++i)

@@ -28,10 +28,24 @@ def check_tables(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> tuple
         raise ValueError(f'cos and sin turn {2 * cos.shape[1]} elements of heads of {x.shape[-1]}')
     if cos.dtype != sin.dtype or cos.dtype not in (x.dtype, torch.float32):
         cos, sin = cos.float(), sin.float()
+    return table_rows(cos, sin)
+
+
+def table_rows(cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tables with their rows equally far apart, a row's elements side by side."""
     cos, sin = unit_rows(cos), unit_rows(sin)
     if cos.stride(0) != sin.stride(0) or cos.stride(0) < cos.shape[1]:
         cos, sin = cos.contiguous(), sin.contiguous()
     return cos, sin
+
+
+def as_saved(x: torch.Tensor | None, dtype: torch.dtype, shape, device: torch.device) -> torch.Tensor | None:
+    """A saved tensor in the type and the place that it had (saved-tensor hooks may hand back others)."""
+    if x is None:
+        return None
+    if x.shape != shape:
+        raise ValueError(f'a saved tensor {tuple(shape)} came back as {tuple(x.shape)}')
+    return x.to(device=device, dtype=dtype)
 
 
 def rotary_call(x: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, interleaved: bool, back: bool, positions: torch.Tensor | None,
@@ -68,7 +82,8 @@ class RotaryFunction(torch.autograd.Function):
     def forward(ctx, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace, *xs):
         ctx.save_for_backward(cos, sin, positions, offsets, cu_seqlens)
         ctx.call = (interleaved, back, offset)
-        ctx.like = [(x.shape, x.dtype, x.device) for x in xs]
+        ctx.saved_as = [None if t is None else (t.dtype, t.shape, t.device) for t in (cos, sin, positions, offsets, cu_seqlens)]
+        ctx.dtype = xs[0].dtype
         ctx.set_materialize_grads(False)
         if inplace:
             ctx.mark_dirty(*xs)
@@ -76,11 +91,14 @@ class RotaryFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *dys):
-        (interleaved, back, offset), (cos, sin, positions, offsets, cu_seqlens) = ctx.call, ctx.saved_tensors
+        interleaved, back, offset = ctx.call
+        cos, sin, positions, offsets, cu_seqlens = (t if was is None else as_saved(t, *was) for t, was in zip(ctx.saved_tensors, ctx.saved_as))
+        cos, sin = table_rows(cos, sin)
+        positions, offsets, cu_seqlens = (None if t is None else t.contiguous() for t in (positions, offsets, cu_seqlens))
         at = [i for i, dy in enumerate(dys) if dy is not None]
         dxs = [None] * len(dys)
         if at:
-            grads = RotaryFunction.apply(cos, sin, interleaved, not back, positions, offsets, offset, cu_seqlens, False, *(dys[i].to(ctx.like[i][1]) for i in at))
+            grads = RotaryFunction.apply(cos, sin, interleaved, not back, positions, offsets, offset, cu_seqlens, False, *(dys[i].to(ctx.dtype) for i in at))
             for i, dx in zip(at, grads):
                 dxs[i] = dx
         return (None,) * 9 + tuple(dxs)

@@ -440,3 +440,61 @@ def test_library_refuses():
     assert lib.gdn_rotary(ctypes.byref(rows), 3, ctypes.byref(_lib.RotaryCall(B=1, T=1, D=16)), None) == _lib.GDN_ERR_INVALID
     assert lib.gdn_rotary(ctypes.byref(rows), 1, None, None) == _lib.GDN_ERR_INVALID
     assert call(B=0) == call(T=0) == _lib.GDN_OK
+
+
+# what a saved-tensor hook may hand back: another type, another place, another layout
+HOOKS = {'types': lambda x: x.double() if x.is_floating_point() else x.to(torch.int64 if x.dtype == torch.int32 else torch.int16), 'layout': lambda x: torch.stack([x, x], -1)[..., 0], 'host': lambda x: x.cpu()}
+
+
+def _seen(c):
+    """What a kernel reads behind the pointers of a call (CPU tensors): tables, positions, offsets, boundaries."""
+    import ctypes
+    read = lambda at, n, of: list((of * n).from_address(at)) if at else None
+    index = lambda at, n, is_i32: read(at, n, ctypes.c_int32 if is_i32 else ctypes.c_int64)
+    tables = [[read(t + 4 * r * c.table_stride, c.rotary_dim // 2, ctypes.c_float) for r in range(c.table_rows)] for t in (c.cos, c.sin)]
+    flags = c.flags
+    return (c.table_dtype, c.table_rows, c.rotary_dim, *tables, index(c.positions, c.B * c.T, flags >> 26 & 1), index(c.offsets, c.N, flags >> 27 & 1), index(c.cu_seqlens, c.N + 1, flags >> 5 & 1))
+
+
+@pytest.mark.parametrize('hook', ['types', 'layout'])
+@pytest.mark.parametrize('how', ['positions', 'packed'])
+def test_saved_tensors_of_other_types_and_layouts_on_the_host(lib, how, hook):
+    """The tables and indices that the gradient's call reads are those of the call itself."""
+    calls = []
+    lib.gdn_rotary = lambda rows, count, call, stream: calls.append(_seen(call._obj)) or 0
+    x = torch.zeros(1, 6, 2, 16, dtype=BF, requires_grad=True)
+    wide = torch.rand(10, 40)
+    cos, sin = wide[:, 1:9], wide[:, 20:28]
+    kw = dict(positions=torch.tensor([[3, 0, 9, 1, 1, 2]], dtype=torch.int32)) if how == 'positions' else dict(cu_seqlens=torch.tensor([0, 2, 6]), seqlen_offsets=torch.tensor([1, 3], dtype=torch.int32))
+    for unpack, error in ((lambda t: t, None), (HOOKS[hook], None), (lambda t: t[:-1] if t.dim() == 1 else t[:, :-1], ValueError)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = _mods().rotary_embedding(x, cos, sin, **kw)
+        if error is None:
+            torch.autograd.grad(y, x, torch.zeros_like(y))
+            assert calls[0] == calls[1] and len(calls) == 2
+        else:
+            with pytest.raises(error, match='came back'):
+                torch.autograd.grad(y, x, torch.zeros_like(y))
+            assert len(calls) == 1
+        calls.clear()
+
+
+@gpu
+@pytest.mark.parametrize('native', [True, False])
+@pytest.mark.parametrize('hook', list(HOOKS))
+def test_saved_tensors_of_other_types_places_and_layouts(hook, native, monkeypatch):
+    from fla_hip import _lib
+    if not native:
+        monkeypatch.setattr(_lib, 'host', lambda: _lib._PythonHost)
+    cos, sin = _tables(30, 64)
+    q, k = (_rows(1, 11, h, 64, dtype=BF, seed=h).requires_grad_() for h in (3, 1))
+    dy = [_rows(1, 11, h, 64, dtype=BF, seed=10 + h) for h in (3, 1)]
+    for kw in (dict(positions=torch.arange(11, dtype=torch.int32, device=DEV)[None] * 2), dict(seqlen_offsets=torch.tensor([0, 7], device=DEV), cu_seqlens=torch.tensor([0, 4, 11], dtype=torch.int32, device=DEV), max_seqlen=7)):
+        want = torch.autograd.grad(_mods().rotary_embedding_qk(q, k, cos, sin, **kw), [q, k], dy)
+        with torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda t: t):
+            out = _mods().rotary_embedding_qk(q, k, cos, sin, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [q, k], dy), want))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1] if t.dim() == 1 else t[:, :-1]):
+            out = _mods().rotary_embedding_qk(q, k, cos, sin, **kw)
+        with pytest.raises(ValueError, match='came back'):
+            torch.autograd.grad(out, [q, k], dy)
