@@ -226,34 +226,40 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
 
 class RotaryEmbedding(nn.Module):
     """Queries and keys turned by their positions (``fla.modules.RotaryEmbedding``), ``dim`` elements of each head.  ``scale_base``: the turned pairs of queries are scaled by
-    ``s ** ((t - T // 2) / scale_base)``, those of keys by its inverse, ``s = (2j + 0.4 dim) / (1.4 dim)``.  ``scaling``: see ``rotary_frequencies``.  The tables grow with
-    the positions asked for and are no part of the state; those that a captured graph reads are kept as long as the module."""
+    ``s ** ((t - c) / scale_base)``, those of keys by its inverse, ``s = (2j + 0.4 dim) / (1.4 dim)``.  c is ``scale_center``; without one it is the middle ``T // 2`` of the call's
+    positions, which holds for whole sequences only: the scales of keys from one call and queries of another would not cancel, so calls that go on from others
+    (``seqlen_offset``, ``positions``) raise.  ``scaling``: see ``rotary_frequencies``.  The tables grow with the positions asked for and are no part of the state; those that a
+    captured graph reads are kept as long as the module."""
 
     def __init__(self, dim: int, base: float = 10000.0, scale_base: float | None = None, interleaved: bool = False, pos_idx_in_fp32: bool = True,
-                 device: torch.device | None = None, scaling: dict | None = None):
+                 device: torch.device | None = None, scaling: dict | None = None, scale_center: int | None = None):
         super().__init__()
         if not pos_idx_in_fp32:
             raise NotImplementedError('angles are formed in 64 bits: pos_idx_in_fp32=False is not offered')
-        self.dim, self.base, self.scale_base, self.interleaved, self.scaling = dim, float(base), scale_base, interleaved, scaling
+        if scale_center is not None and scale_base is None:
+            raise ValueError('scale_center is that of scale_base')
+        self.dim, self.base, self.scale_base, self.interleaved, self.scaling, self.scale_center = dim, float(base), scale_base, interleaved, scaling, scale_center
+        self._prefixes = scale_base is None or scale_center is not None      # (tables of more positions begin with those of fewer)
         inv_freq, self.attention_factor = rotary_frequencies(dim, self.base, scaling)
         self.register_buffer('inv_freq', inv_freq.float().to(device), persistent=False)
         self._tables, self._captured = None, []
 
     def extra_repr(self) -> str:
         return f'dim={self.dim}, base={self.base}, interleaved={self.interleaved}' + (f', scale_base={self.scale_base}' if self.scale_base is not None else '') + (
+            f', scale_center={self.scale_center}' if self.scale_center is not None else '') + (
             f', scaling={self.scaling}' if self.scaling is not None else '')
 
     def tables(self, positions: int, device: torch.device) -> tuple[torch.Tensor, ...]:
         """cos, sin for at least this many positions (and, with ``scale_base``, the keys' cos, sin), fp32."""
         device = torch.device(device)
         kept, captured = self._tables, device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
-        if kept is not None and kept[0].device == device and (kept[0].shape[0] >= positions if self.scale_base is None else kept[0].shape[0] == positions):
+        if kept is not None and kept[0].device == device and (kept[0].shape[0] >= positions if self._prefixes else kept[0].shape[0] == positions):
             if captured and not any(t is kept for t in self._captured):
                 self._captured.append(kept)
             return kept
         if captured:
             raise RuntimeError(f'the tables of {positions} positions are not made yet: call RotaryEmbedding.tables({positions}, device) before the capture')
-        if kept is not None and kept[0].device == device and self.scale_base is None:
+        if kept is not None and kept[0].device == device and self._prefixes:
             positions = max(positions, 2 * kept[0].shape[0])             # (asked for position after position: seldom made)
         if kept is not None and kept[0].is_cuda:
             torch.cuda.synchronize(kept[0].device)                       # (a call on another stream may still read those that go)
@@ -267,7 +273,7 @@ class RotaryEmbedding(nn.Module):
                 tables = (cos, sin)
             else:
                 s = (torch.arange(0, self.dim, 2, dtype=torch.float64) + 0.4 * self.dim) / (1.4 * self.dim)
-                scale = s ** ((t - positions // 2) / self.scale_base)[:, None]
+                scale = s ** ((t - (positions // 2 if self.scale_center is None else self.scale_center)) / self.scale_base)[:, None]
                 tables = (cos * scale, sin * scale, cos / scale, sin / scale)
             self._tables = tuple(x.float().to(device) for x in tables)
         return self._tables
@@ -286,6 +292,8 @@ class RotaryEmbedding(nn.Module):
         known = not isinstance(seqlen_offset, torch.Tensor) and positions is None
         if not known and max_seqlen is None:
             raise ValueError('max_seqlen is needed where seqlen_offset or positions are tensors: the number of positions that the tables have to have')
+        if not self._prefixes and (not known or int(seqlen_offset)):
+            raise ValueError('scales around the middle of a call do not cancel between calls: give RotaryEmbedding a scale_center for calls that go on from others')
         count = (max_seqlen if max_seqlen is not None else q.shape[1]) + (int(seqlen_offset) if known else 0)
         tables = self.tables(count, q.device)
         call = dict(interleaved=self.interleaved, seqlen_offsets=seqlen_offset, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen if cu_seqlens is not None else None, positions=positions)

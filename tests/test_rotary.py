@@ -498,3 +498,40 @@ def test_saved_tensors_of_other_types_places_and_layouts(hook, native, monkeypat
             out = _mods().rotary_embedding_qk(q, k, cos, sin, **kw)
         with pytest.raises(ValueError, match='came back'):
             torch.autograd.grad(out, [q, k], dy)
+
+
+def test_scales_of_calls_that_go_on_from_others(lib):
+    """The scale of a query and that of a key it meets cancel only around the same centre: around the middle of each call, other calls' keys raise; around a given one all
+    tables begin alike."""
+    x = torch.zeros(1, 2, 1, 64, dtype=BF)
+    rope = _mods().RotaryEmbedding(64, scale_base=512.0)
+    assert rope(x, x)[0].shape == x.shape and len(lib.calls) == 2
+    for kw in (dict(seqlen_offset=1), dict(seqlen_offset=torch.zeros(1, dtype=torch.int32), max_seqlen=9), dict(positions=torch.zeros(1, 2, dtype=torch.int32), max_seqlen=9)):
+        with pytest.raises(ValueError, match='scale_center'):
+            rope(x, x, **kw)
+    assert len(lib.calls) == 2
+    with pytest.raises(ValueError, match='scale_base'):
+        _mods().RotaryEmbedding(64, scale_center=0)
+    rope = _mods().RotaryEmbedding(64, scale_base=512.0, scale_center=100)
+    tables = {n: rope.tables(n, 'cpu') for n in (1, 40, 300)}
+    again = _mods().RotaryEmbedding(64, scale_base=512.0, scale_center=100).tables(300, 'cpu')
+    for n, t in tables.items():
+        assert all(a.shape[0] >= n and torch.equal(a[:n], b[:n]) for a, b in zip(t, again))
+    assert rope.tables(250, 'cpu')[0] is rope.tables(300, 'cpu')[0]
+    s = ((torch.arange(0, 64, 2, dtype=torch.float64) + 0.4 * 64) / (1.4 * 64)) ** ((torch.arange(300, dtype=torch.float64) - 100) / 512)[:, None]
+    assert torch.equal(again[0], ((torch.arange(300, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)).cos() * s).float())
+
+
+@gpu
+def test_token_by_token_around_one_centre():
+    """Rows of one whole call, and the same token by token: bit for bit, so every score is the same."""
+    q, k = _rows(2, 40, 4, 64, dtype=BF), _rows(2, 40, 2, 64, dtype=BF, seed=1)
+    whole = _mods().RotaryEmbedding(64, scale_base=512.0, scale_center=20)
+    want = whole(q, k)
+    middle = _mods().RotaryEmbedding(64, scale_base=512.0)(q, k)
+    assert all(torch.equal(a, b) for a, b in zip(want, middle))
+    rope = _mods().RotaryEmbedding(64, scale_base=512.0, scale_center=20)
+    for t in range(40):
+        offset = t if t % 2 else torch.tensor([t, t], device=DEV)
+        got = rope(q[:, t:t + 1], k[:, t:t + 1], seqlen_offset=offset, max_seqlen=1 if t % 2 else 40)
+        assert all(torch.equal(a, b[:, t:t + 1]) for a, b in zip(got, want)), t
