@@ -259,8 +259,16 @@ class RotaryEmbedding(nn.Module):
             return kept
         if captured:
             raise RuntimeError(f'the tables of {positions} positions are not made yet: call RotaryEmbedding.tables({positions}, device) before the capture')
+        center = positions // 2 if self.scale_center is None else self.scale_center
+        if self.scale_base is not None:
+            # ((2/7) ** (distance / scale_base) and its inverse are normal numbers of fp32)
+            reach = int(126 * abs(self.scale_base) / math.log2(3.5))
+            most = center + reach + 1
+            if positions > most or center > reach:
+                raise ValueError(f'scales of positions more than {reach} from their centre {center} leave the range of fp32: {positions} positions were asked for')
         if kept is not None and kept[0].device == device and self._prefixes:
-            positions = max(positions, 2 * kept[0].shape[0])             # (asked for position after position: seldom made)
+            # (asked for position after position: seldom made)
+            positions = max(positions, 2 * kept[0].shape[0] if self.scale_base is None else min(2 * kept[0].shape[0], most))
         if kept is not None and kept[0].is_cuda:
             torch.cuda.synchronize(kept[0].device)                       # (a call on another stream may still read those that go)
         inv, factor = rotary_frequencies(self.dim, self.base, self.scaling)
@@ -273,7 +281,7 @@ class RotaryEmbedding(nn.Module):
                 tables = (cos, sin)
             else:
                 s = (torch.arange(0, self.dim, 2, dtype=torch.float64) + 0.4 * self.dim) / (1.4 * self.dim)
-                scale = s ** ((t - (positions // 2 if self.scale_center is None else self.scale_center)) / self.scale_base)[:, None]
+                scale = s ** ((t - center) / self.scale_base)[:, None]
                 tables = (cos * scale, sin * scale, cos / scale, sin / scale)
             self._tables = tuple(x.float().to(device) for x in tables)
         return self._tables
