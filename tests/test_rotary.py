@@ -539,13 +539,13 @@ def test_token_by_token_around_one_centre():
 
 @pytest.mark.parametrize('center', [None, 0, 3000])
 def test_scales_beyond_the_range_of_their_tables(center):
-    """(2/7) ** (126 scale_base / log2(7/2)) is 2^-126, the smallest normal number of fp32: at scale_base 64 reached 4462 positions from the centre."""
+    """(2/7) ** (126 scale_base / log2(7/2)) is 2^-126, the smallest normal number of fp32: at scale_base 64 reached 4461.8 positions from the centre."""
     rope = _mods().RotaryEmbedding(64, scale_base=64.0, scale_center=center)
-    most = {None: 8924, 0: 4463, 3000: 7463}[center]
+    most = {None: 8923, 0: 4462, 3000: 7462}[center]
     for n in (most // 2 + 1, most):                              # (the second of them would double the first's)
         assert all(t.isfinite().all() and (torch.maximum(t[:, 0].abs(), t[:, 32].abs()) > 0).all() for t in (torch.cat(pair, 1) for pair in zip(*[iter(rope.tables(n, 'cpu'))] * 2)))
     assert rope.tables(most, 'cpu')[0].shape[0] == most
     with pytest.raises(ValueError, match='range of fp32'):
         rope.tables(most + 2, 'cpu')
     with pytest.raises(ValueError, match='range of fp32'):
-        _mods().RotaryEmbedding(64, scale_base=64.0, scale_center=4463).tables(1, 'cpu')
+        _mods().RotaryEmbedding(64, scale_base=64.0, scale_center=4462).tables(1, 'cpu')
