@@ -198,13 +198,18 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
     """(angles per position of the ``dim / 2`` pairs in 64 bits, factor of cos and sin).  ``scaling``: ``{'type': 'linear' | 'ntk' | 'yarn', 'factor': s, ...}`` for
     contexts s times the trained one - every angle divided by s; the base times ``s ** (dim / (dim - 2))``; or (with ``original_max_position_embeddings``, and
     ``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor`` 0.1 ln s + 1) the pairs that turn less than beta_slow times in the trained context divided by s, those that
-    turn more than beta_fast times left alone, and in between a ramp."""
+    turn more than beta_fast times left alone, and in between a ramp.  Any other entry raises: it would make other tables than its model's."""
     if dim <= 0 or dim % 2:
         raise ValueError(f'the turned part of a head must be even, got {dim}')
     inverse = lambda b: b ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
     if scaling is None:
         return inverse(base), 1.0
     kind, factor = scaling.get('type', scaling.get('rope_type')), float(scaling['factor'])
+    if scaling.get('rope_type', kind) != kind:
+        raise ValueError(f"scaling is of type {kind!r} and of rope_type {scaling['rope_type']!r}")
+    taken = {'type', 'rope_type', 'factor', 'original_max_position_embeddings'} | ({'beta_fast', 'beta_slow', 'attention_factor'} if kind == 'yarn' else set())
+    if set(scaling) - taken:
+        raise ValueError(f'scaling of type {kind!r} takes {sorted(taken)}, got {sorted(set(scaling) - taken)} besides')
     if not factor >= 1:
         raise ValueError(f'the factor of a scaled context must be at least 1, got {factor}')
     if kind == 'linear':

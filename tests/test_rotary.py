@@ -549,3 +549,15 @@ def test_scales_beyond_the_range_of_their_tables(center):
         rope.tables(most + 2, 'cpu')
     with pytest.raises(ValueError, match='range of fp32'):
         _mods().RotaryEmbedding(64, scale_base=64.0, scale_center=4462).tables(1, 'cpu')
+
+
+@pytest.mark.parametrize('scaling', [dict(type='yarn', factor=4.0, original_max_position_embeddings=4096, mscale=1.0), dict(type='yarn', factor=4.0, original_max_position_embeddings=4096, mscale_all_dim=0.7),
+                                     dict(type='yarn', factor=4.0, original_max_position_embeddings=4096, truncate=False), dict(type='linear', factor=4.0, beta_fast=16), dict(type='ntk', factor=4.0, attention_factor=1.2),
+                                     dict(rope_type='linear', factor=4.0, low_freq_factor=1.0), dict(type='linear', rope_type='yarn', factor=4.0, original_max_position_embeddings=4096)])
+def test_options_that_are_not_offered(scaling):
+    """What would be dropped in silence makes other tables than the model's."""
+    from fla_hip.modules.rotary import rotary_frequencies
+    with pytest.raises(ValueError):
+        rotary_frequencies(64, scaling=scaling)
+    offered = dict(type='yarn', rope_type='yarn', factor=4.0, original_max_position_embeddings=4096, beta_fast=16, beta_slow=2, attention_factor=1.5)
+    assert rotary_frequencies(64, scaling=offered)[1] == 1.5
