@@ -78,8 +78,10 @@ def _turn(xs: tuple, cos, sin, interleaved, back, positions, offsets, offset, cu
 class RotaryFunction(torch.autograd.Function):
     """A turn by the tables' angles; its gradient is the turn back, which is this function again (and so differentiable itself)."""
 
+    # (the rows first: of a view that is written torch takes the gradient's way through the first operand)
     @staticmethod
-    def forward(ctx, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace, *xs):
+    def forward(ctx, a, b, cos, sin, interleaved, back, positions, offsets, offset, cu_seqlens, inplace):
+        xs = (a,) if b is None else (a, b)
         ctx.save_for_backward(cos, sin, positions, offsets, cu_seqlens)
         ctx.call = (interleaved, back, offset)
         ctx.saved_as = [None if t is None else (t.dtype, t.shape, t.device) for t in (cos, sin, positions, offsets, cu_seqlens)]
@@ -96,12 +98,23 @@ class RotaryFunction(torch.autograd.Function):
         cos, sin = table_rows(cos, sin)
         positions, offsets, cu_seqlens = (None if t is None else t.contiguous() for t in (positions, offsets, cu_seqlens))
         at = [i for i, dy in enumerate(dys) if dy is not None]
-        dxs = [None] * len(dys)
+        dxs = [None, None]
         if at:
-            grads = RotaryFunction.apply(cos, sin, interleaved, not back, positions, offsets, offset, cu_seqlens, False, *(dys[i].to(ctx.dtype) for i in at))
+            turned = [dys[i].to(ctx.dtype) for i in at] + [None]
+            grads = RotaryFunction.apply(*turned[:2], cos, sin, interleaved, not back, positions, offsets, offset, cu_seqlens, False)
             for i, dx in zip(at, grads):
                 dxs[i] = dx
-        return (None,) * 9 + tuple(dxs)
+        return (*dxs, *(None,) * 9)
+
+
+def check_written(x: torch.Tensor) -> None:
+    """What torch refuses to have written in place, before it is written (an autograd function says so when its forward has run)."""
+    if not x.requires_grad:
+        return
+    if x.is_leaf or (x._is_view() and x._base.is_leaf and x._base.requires_grad):
+        raise RuntimeError('inplace=True: a leaf that requires a gradient, or a view of one, cannot be turned in place')
+    if x._is_view() and torch._C._autograd._get_creation_meta(x) != torch._C._autograd.CreationMeta.DEFAULT:
+        raise RuntimeError('inplace=True: a view that came with others (split, unbind), or was made without a graph, cannot be turned in place: slice the tensor, or turn it out of place')
 
 
 def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlens, max_seqlen, positions) -> tuple:
@@ -152,7 +165,13 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
         if len(xs) == 2 and xs[0].numel() and xs[0].data_ptr() == xs[1].data_ptr():
             raise ValueError('inplace=True needs queries and keys that do not overlap')
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        return RotaryFunction.apply(cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace, *xs)
+        if inplace:
+            for x in xs:
+                check_written(x)
+            if len(xs) == 2 and not all(x.requires_grad and not x._is_view() for x in xs):
+                # (torch writes into a view for a function of one result only; a tensor without a gradient stays one)
+                return sum((_rotary((x,), cos, sin, interleaved, True, offset if offsets is None else offsets, cu_seqlens, max_seqlen, positions) for x in xs), ())
+        return RotaryFunction.apply(*(*xs, None)[:2], cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace)
     ys = _turn(tuple(x.detach() for x in xs), cos, sin, interleaved, False, positions, offsets, offset, cu_seqlens, inplace)
     if inplace:
         written(*xs)

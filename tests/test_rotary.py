@@ -561,3 +561,41 @@ def test_options_that_are_not_offered(scaling):
         rotary_frequencies(64, scaling=scaling)
     offered = dict(type='yarn', rope_type='yarn', factor=4.0, original_max_position_embeddings=4096, beta_fast=16, beta_slow=2, attention_factor=1.5)
     assert rotary_frequencies(64, scaling=offered)[1] == 1.5
+
+
+def test_refusals_in_place_come_before_anything_is_written(lib):
+    op, both = _mods().rotary_embedding, _mods().rotary_embedding_qk
+    cos = torch.ones(8, 8)
+    leaf = torch.ones(1, 4, 6, 16, requires_grad=True)
+    fused = leaf * 1
+    with torch.no_grad():
+        quiet = fused[:, :, :2]
+    free = torch.ones(1, 4, 2, 16)
+    for call in (lambda: op(leaf, cos, cos, inplace=True), lambda: op(leaf[:, :, :2], cos, cos, inplace=True), lambda: op(fused.split([4, 2], 2)[0], cos, cos, inplace=True),
+                 lambda: both(*fused.split([4, 2], 2), cos, cos, inplace=True), lambda: both(leaf, free, cos, cos, inplace=True), lambda: both(free, leaf[:, :, 2:], cos, cos, inplace=True),
+                 lambda: both(fused[:, :, 2:], leaf[:, :, 2:], cos, cos, inplace=True), lambda: op(quiet, cos, cos, inplace=True)):
+        with pytest.raises(RuntimeError, match='inplace=True'):
+            call()
+    assert not lib.calls and free._version == 0 and fused._version == 0
+    q, k = both(fused[:, :, :4], fused[:, :, 4:], cos, cos, inplace=True)
+    assert q.requires_grad and k.requires_grad and len(lib.calls) == 2
+    q, k = both(free, fused[:, :, 4:], cos, cos, inplace=True)
+    assert q is free and not free.requires_grad and free._version == 1 and k.requires_grad and len(lib.calls) == 4
+
+
+@gpu
+@pytest.mark.parametrize('how', ['both', 'queries', 'keys'])
+def test_parts_of_one_projection_in_place_under_autograd(how):
+    cos, sin = _tables(9, 64)
+    x, w = _rows(2, 9, 6, 64, dtype=BF).requires_grad_(), _rows(2, 9, 6, 64, dtype=BF, seed=1)
+    other = _rows(2, 9, 2, 64, dtype=BF, seed=2)
+    results = []
+    for inplace in (False, True):
+        fused, free = x * 2, other.clone()
+        q, k = (fused[:, :, :4] if how != 'keys' else free), (fused[:, :, 4:] if how != 'queries' else free)
+        a, b = _mods().rotary_embedding_qk(q, k, cos, sin, inplace=inplace, seqlen_offsets=torch.zeros(2, dtype=torch.int32, device=DEV))
+        whole = torch.cat([a if how != 'keys' else fused[:, :, :4], b if how != 'queries' else fused[:, :, 4:]], 2)
+        if inplace:
+            assert torch.equal(fused, whole) and (how == 'both' or not free.requires_grad)
+        results.append([whole.detach(), a.detach(), b.detach(), *torch.autograd.grad(whole, x, w)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
