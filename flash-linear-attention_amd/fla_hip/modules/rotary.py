@@ -107,6 +107,36 @@ class RotaryFunction(torch.autograd.Function):
         return (*dxs, *(None,) * 9)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one type share an element: whether sum i s - sum j r is the distance of their first elements for some indices i, j within their sizes."""
+    if not a.numel() or not b.numel():
+        return False
+    spans = {}                                                        # stride -> least and largest number of steps
+    for x, sign in ((a, 1), (b, -1)):
+        for size, stride in zip(x.shape, x.stride()):
+            if size > 1 and stride:
+                low, high = spans.get(stride, (0, 0))
+                spans[stride] = (low, high + size - 1) if sign > 0 else (low - (size - 1), high)
+    steps = sorted(((s, *lh) for s, lh in spans.items()), reverse=True)
+    inner = [(0, 0)]                                                  # what the strides behind reach
+    for s, low, high in reversed(steps):
+        inner.insert(0, (inner[0][0] + s * low, inner[0][1] + s * high))
+    left = 10000
+
+    def reached(distance: int, at: int) -> bool:
+        nonlocal left
+        left -= 1
+        if left < 0:                                                  # (strides that fold into each other many times: taken for an overlap)
+            return True
+        if at == len(steps):
+            return distance == 0
+        s, low, high = steps[at]
+        behind = inner[at + 1]
+        return any(reached(distance - n * s, at + 1) for n in range(max(low, -((behind[1] - distance) // s)), min(high, (distance - behind[0]) // s) + 1))
+
+    return reached((b.data_ptr() - a.data_ptr()) // a.element_size(), 0)
+
+
 def check_written(x: torch.Tensor) -> None:
     """What torch refuses to have written in place, before it is written (an autograd function says so when its forward has run)."""
     if not x.requires_grad:
@@ -162,7 +192,7 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
                 raise ValueError('inplace=True needs heads whose elements lie in a row')
             if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
                 raise ValueError('inplace=True needs a tensor that does not overlap itself')
-        if len(xs) == 2 and xs[0].numel() and xs[0].data_ptr() == xs[1].data_ptr():
+        if len(xs) == 2 and overlap(*xs):
             raise ValueError('inplace=True needs queries and keys that do not overlap')
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         if inplace:

@@ -599,3 +599,29 @@ def test_parts_of_one_projection_in_place_under_autograd(how):
             assert torch.equal(fused, whole) and (how == 'both' or not free.requires_grad)
         results.append([whole.detach(), a.detach(), b.detach(), *torch.autograd.grad(whole, x, w)])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_queries_and_keys_that_overlap(lib):
+    """Turned in place at once they would be a race: refused, and only they are - against every element's address."""
+    from fla_hip.modules.rotary import overlap
+    both, cos = _mods().rotary_embedding_qk, torch.ones(9, 8)
+    x = torch.zeros(3, 9, 12, 16, dtype=BF)
+    one = x.flatten()
+    apart = [(x[:, :, :8], x[:, :, 8:]), (x[:, :, ::2], x[:, :, 1::2]), (x[:1], x[2:]), (x[:, :4], x[:, 4:8]), (x.view(3, 9, 4, 3, 16)[:, :, :, 0], x.view(3, 9, 4, 3, 16)[:, :, :, 2]),
+             (one[:640].view(1, 4, 10, 16), one[640:1280].view(1, 4, 10, 16)), (one[:640].view(1, 4, 10, 16), one[640:1024].view(1, 4, 6, 16)), (x.view(3, 9, 6, 32)[..., :16], x.view(3, 9, 6, 32)[..., 16:])]
+    meet = [(x[:, :, :8], x[:, :, 7:]), (x[:, :, 3:5], x), (x[:, :8], x[:, 1:]), (x[:, :, ::2], x[:, :, 2::2]), (x, x), (x.view(3, 9, 4, 3, 16)[:, :, :, 0], x[:, :, 9:]),
+            (one[:640].view(1, 4, 10, 16), one[639:639 + 384].view(1, 4, 6, 16)), (x[:, 8:], x[:, 8:9, 11:]), (x.view(3, 9, 6, 32)[..., :16], x.view(3, 9, 6, 32)[..., 8:24])]
+    for pairs, want in ((apart, False), (meet, True)):
+        for q, k in pairs:
+            places = [set((t.storage_offset() + sum((torch.arange(n) * s).view(-1, *[1] * (3 - i)) for i, (n, s) in enumerate(zip(t.shape, t.stride())))).flatten().tolist()) for t in (q, k)]
+            assert bool(places[0] & places[1]) == overlap(q, k) == overlap(k, q) == want
+            if q.shape[:2] != k.shape[:2]:
+                continue
+            lib.calls.clear()
+            if want:
+                with pytest.raises(ValueError, match='overlap'):
+                    both(q, k, cos, cos, inplace=True)
+            else:
+                both(q, k, cos, cos, inplace=True)
+            assert len(lib.calls) == (not want)
+    assert not overlap(x[:, :0], x) and not overlap(x[:, :, :0], x)
