@@ -14,7 +14,7 @@ struct KeepParams {
     PagedCache cache;
     const int32_t* rows; const int32_t* kept;
     int64_t rows_stride;
-    int R, chunks, heads;
+    int R, chunks, heads, all_heads;                              // all_heads: of keys and values
 };
 
 template <typename U>
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void paged_keep_kernel(KeepParams p, int per_u
     constexpr int AHEAD = 8;
     const int64_t n = blockIdx.y;
     const int lane = blockIdx.x * 256 + threadIdx.x;
-    if (lane >= 2 * p.heads * p.chunks) return;
+    if (lane >= p.all_heads * p.chunks) return;
     const int c = lane % p.chunks, kh = lane / p.chunks, h = kh % p.heads;
     const bool values = kh >= p.heads;
     char* const data = values ? p.cache.v : p.cache.k;
@@ -76,7 +76,9 @@ extern "C" int gdn_paged_keep(const gdn_paged_cache* cache, const int32_t* rows,
     p.rows = rows; p.kept = kept; p.rows_stride = rows_stride; p.R = (int)R;
     GDN_CHECK_ARG(2 * cache->heads * (row_bytes / unit) < (1ll << 30), GDN_ERR_UNSUPPORTED, "%s: rows too long", who);
     p.heads = (int)cache->heads; p.chunks = (int)(row_bytes / unit);
-    const dim3 grid((unsigned)((2 * p.heads * p.chunks + 255) / 256), (unsigned)N);
+    // (one tensor for keys and values, as of latent vectors, is moved once: two threads on the same slots would read what the other has written)
+    p.all_heads = c.k == c.v && c.k_page == c.v_page && c.k_slot == c.v_slot && c.k_head == c.v_head ? p.heads : 2 * p.heads;
+    const dim3 grid((unsigned)((p.all_heads * p.chunks + 255) / 256), (unsigned)N);
     auto go = [&](auto u) { hipLaunchKernelGGL(paged_keep_kernel<decltype(u)>, grid, dim3(256), 0, (hipStream_t)stream, p, unit / size); };
     if (unit == 16) go(u32x4{});
     else if (unit == 4) go(uint32_t{});

@@ -176,7 +176,7 @@ def paged_keep(
 ) -> None:
     """The rows of a step that stand, moved to the front of its slots: slot ``context_lens[n] + i`` becomes what slot ``context_lens[n] + rows[n, i]`` was, for
     ``i < num_kept[n]`` (rows ``[N, R]`` int32 with ``rows[n, i] >= i``, num_kept ``[N]``: the path and the count that ``verify_drafts`` returns).  Any other entry, and one whose
-    slots have no page, leaves its slot as it is.  The positions that keys were turned by stay: a node of a tree is at the same depth before and after."""
+    slots have no page, leaves its slot as it is.  k_cache and v_cache may be one tensor.  The positions that keys were turned by stay: a node of a tree is at the same depth before and after."""
     if _lib.host().paged_keep(k_cache, v_cache, page_table, context_lens, rows, num_kept) is not None:
         return
     dev = require_gpu(k_cache, v_cache, page_table, context_lens, rows, num_kept)

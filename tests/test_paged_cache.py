@@ -365,3 +365,22 @@ def test_library_refuses():
                                                                             ctypes.byref(_lib.RotaryCall(**{**dict(B=1, T=1, N=1, D=16, dtype=0, table_dtype=0), **kw})), None)
     invalid = [dict(k=2), dict(v=2), dict(D=8), dict(dtype=1, table_dtype=1), dict(q=-1), dict(cache=dict(page_size=0)), dict(rotary_dim=16)]
     assert [append(**kw) for kw in invalid] == [_lib.GDN_ERR_INVALID] * len(invalid)
+
+
+@gpu
+@pytest.mark.parametrize(('page_size', 'D', 'heads'), [(16, 128, 1), (4, 64, 5), (1, 576, 1)])
+def test_keep_of_one_tensor_for_keys_and_values(page_size, D, heads):
+    """Every slot is moved once: a path that shifts all of its rows by one or two, so that a row moved twice would have been the next."""
+    N, R = 40, 33
+    contexts = [(7 * n) % 50 for n in range(N)]
+    lengths = [c + R for c in contexts]
+    pages = pages_for(lengths, page_size)
+    one, _ = cache(pages, page_size, heads, D, BF)
+    t = table(lengths, page_size, pages)
+    rows = torch.stack([torch.arange(R - 2) + 1 + n % 2 for n in range(N)]).int()
+    want, now = one.clone().cpu(), one.cpu()
+    for n in range(N):
+        for i in range(R - 2):
+            want[O.slot_of(t, n, contexts[n] + i, pages, page_size)] = now[O.slot_of(t, n, contexts[n] + int(rows[n, i]), pages, page_size)]
+    _attn().paged_keep(one, one, t.to(DEV), torch.tensor(contexts, device=DEV), rows.to(DEV), torch.full((N,), R - 2, device=DEV))
+    assert torch.equal(one.cpu(), want)
