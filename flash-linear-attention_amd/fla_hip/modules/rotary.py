@@ -13,7 +13,7 @@ import torch.nn as nn
 
 from fla_hip import _lib
 from fla_hip.ops.gated_delta_rule._common import as_index, dtype_code, forward_only, launch, no_forward_mode, ptr, require_gpu, unit_rows, written
-from fla_hip.ops.utils.index import check_cu_seqlens
+from fla_hip.ops.utils.index import check_cu_seqlens, max_seq_len
 
 
 def rows_of(x: torch.Tensor, y: torch.Tensor | None) -> _lib.RotaryRows:
@@ -164,7 +164,7 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
     forward_only('a gradient of the tables of rotary positions', cos, sin)
     no_forward_mode('rotary positions', *xs, cos, sin)
     B, T = x.shape[:2]
-    N, longest = B, T
+    N, longest = B, T if max_seqlen is None or cu_seqlens is None else max_seqlen
     if cu_seqlens is not None:
         if B != 1:
             raise ValueError(f'The batch size is expected to be 1 rather than {B} when using `cu_seqlens`.')
@@ -173,7 +173,7 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
             raise ValueError('cu_seqlens must hold N + 1 >= 2 boundaries')
         if max_seqlen is None:
             check_cu_seqlens(cu_seqlens, T)
-        longest = max_seqlen
+            longest = max_seq_len(cu_seqlens)
         cu_seqlens = as_index(cu_seqlens, dev, 'cu_seqlens', (N + 1,))
     offsets, offset = None, 0
     if positions is not None:
@@ -184,7 +184,7 @@ def _rotary(xs: tuple, cos, sin, interleaved, inplace, seqlen_offsets, cu_seqlen
         offsets = as_index(seqlen_offsets, dev, 'seqlen_offsets', (N,))
     else:
         offset = int(seqlen_offsets)
-        if longest is not None and (offset < 0 or offset + longest > cos.shape[0]):
+        if offset < 0 or offset + longest > cos.shape[0]:
             raise ValueError(f'the tables have {cos.shape[0]} positions, positions {offset} to {offset + longest - 1} are needed')
     if inplace:
         for x in xs:

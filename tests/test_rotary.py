@@ -625,3 +625,17 @@ def test_queries_and_keys_that_overlap(lib):
                 both(q, k, cos, cos, inplace=True)
             assert len(lib.calls) == (not want)
     assert not overlap(x[:, :0], x) and not overlap(x[:, :, :0], x)
+
+
+def test_positions_of_a_packed_batch_that_the_tables_do_not_have(lib):
+    """Where the host has read the boundaries it knows the last position of every sequence."""
+    op, x = _mods().rotary_embedding, torch.zeros(1, 7, 2, 16, dtype=BF)
+    cu, cos = torch.tensor([0, 2, 7]), torch.zeros(6, 8)
+    op(x, cos, cos, cu_seqlens=cu, seqlen_offsets=1)
+    op(x, cos[:5], cos[:5], cu_seqlens=cu)
+    op(x, cos, cos, cu_seqlens=cu, max_seqlen=5, seqlen_offsets=1)
+    for call in (lambda: op(x, cos, cos, cu_seqlens=cu, seqlen_offsets=2), lambda: op(x, cos[:4], cos[:4], cu_seqlens=cu), lambda: op(x, cos, cos, cu_seqlens=cu, seqlen_offsets=-1),
+                 lambda: op(x, cos, cos, cu_seqlens=cu, max_seqlen=5, seqlen_offsets=2)):
+        with pytest.raises(ValueError, match='positions'):
+            call()
+    assert len(lib.calls) == 3
