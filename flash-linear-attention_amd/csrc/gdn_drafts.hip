@@ -346,11 +346,21 @@ static int check_drafts(const char* who, const gdn_drafts_call* c) {
 }
 
 // Passes that are shared out over workgroups, a launch for each, and workgroups per sequence: the first one, of which a chain has no other, and two more of trees.
+// Measured, us a call, one workgroup per sequence against shared (5 drafts of a chain; 15 of a tree), fp32:
+//   sequences           1             8 (4)         32 (16)       48            64            96
+//   chain,  32000       12.1  13.6    12.6  15.1    13.2  16.3    14.5  17.0    14.5  17.2    15.4  20.1
+//   chain,  65536       15.0  14.8    16.0  15.4    17.3  16.3    18.4  18.3    18.2  19.7    18.8  22.0
+//   chain, 131072       21.6  14.2    22.6  15.4    25.7  19.6    26.2  22.3    26.3  26.5    30.0  31.0
+//   tree,   32000       22.9  32.3    25.4  34.2    27.8  37.6    29.5  40.1    29.8  41.1    30.4  43.9
+//   tree,   65536       28.0  31.8    36.5  36.2    36.4  36.6    43.9  47.6    44.1  49.2    45.9  54.6
+//   tree,  131072       60.2  38.0    67.9  47.2    71.3  51.3    74.4  63.2    74.8  76.6    82.9  94.1
+// One or two shared passes of a tree of 131072 words: 64.6 and 57.5 of 16 sequences, five 51.7.  512 workgroups in all against 2048 and 8192: the same up to 48 sequences,
+// from 64 on up to a tenth less.
 struct DraftPlan { int rounds, parts; };
 static DraftPlan draft_plan(const gdn_drafts_call* c) {
     const int64_t segments = (c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT;
-    if (segments <= 32 || c->N >= 192) return {0, 0};
-    return {c->parents ? 3 : 1, (int)std::min<int64_t>((segments + 3) / 4, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, c->N)))};
+    if (segments <= 32 || c->N >= 64) return {0, 0};
+    return {c->parents ? 3 : 1, (int)std::min<int64_t>((segments + 3) / 4, std::max<int64_t>(1, 512 / std::max<int64_t>(1, c->N)))};
 }
 
 }  // namespace gdn

@@ -151,8 +151,10 @@ static int launch_rotary(const char* who, RotaryParams& p, bool inter, bool cach
     const int64_t tokens = p.B * p.T;
     p.chunks = (inter ? 2 * p.half : p.half) / V + (p.D - 2 * p.half) / V;
     p.chunk_lanes = std::min(p.chunks, 256);
-    // Heads of a thread: one where the chip is not full, else two or three, as leaves the fewest of a block's threads idle (of equals two).  Measured: queries and keys of 20
-    // heads of 128 elements, two heads 64 us, three 70, four 68; 48 heads into the cache 78, 71, 81; 40 heads of 64 turned and 64 other elements with gradients 103, 98, 99.
+    // Heads of a thread: one where the chip is not full, else two or three, as leaves the fewest of a block's threads idle (of equals two).  Measured, us a call with one, two and
+    // three: 32768 tokens of 20 heads of 128 elements 77.6, 65.3, 70.5; 14000 tokens of 48 heads into the cache 75.3, 70.9, 66.2, of 24 heads 44.3, 38.3, 35.9; 8192 tokens of 24
+    // heads of 64 16.5, 16.0, 13.3, of 9 heads of 256 22.1, 21.8, 19.6; 8191 tokens of 40 heads of 64 interleaved and 64 other elements 45.3, 42.7, 44.9 (the rule says three: 5 %).
+    // Fewer tokens of 20 heads: 820 (131000 threads of a head each) 8.4, 8.7, 8.8, 1640 8.7, 8.7, 9.1, 3280 11.9, 10.1, 10.7.
     auto lay_out = [&](int each) {
         p.head_lanes = std::max(1, std::min((p.heads + each - 1) / each, 256 / p.chunk_lanes));
         p.tokens = std::max(1, 256 / (p.head_lanes * p.chunk_lanes));
