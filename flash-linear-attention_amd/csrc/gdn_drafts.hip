@@ -11,7 +11,7 @@
 //
 // Everything that decides is in 64 bits and in a fixed order.  Bounded by the memory system for many sequences and words, by latency for few: the first pass, for most
 // sequences the only one, is shared out over workgroups (drafts_round_kernel), each of which walks to it by itself, and one workgroup per sequence finishes.
-// Measured: 16 chains of five drafts over 32000 fp32 words 12.3 us; 32 trees of 15 over 131072 words 45 to 65 (three shared passes of 8.4, then 27; one workgroup per sequence for all: 83).
+// Measured: 16 chains of five drafts over 32000 fp32 words 12.3 us; 32 trees of 15 over 131072 words 45 to 65 (three shared passes of 8.5, then 27; one workgroup per sequence for all: 71 to 83).
 #include "gdn_common.h"
 #include <algorithm>
 #include <type_traits>
@@ -346,16 +346,15 @@ static int check_drafts(const char* who, const gdn_drafts_call* c) {
 }
 
 // Passes that are shared out over workgroups, a launch for each, and workgroups per sequence: the first one, of which a chain has no other, and two more of trees.
-// Measured, us a call, one workgroup per sequence against shared (5 drafts of a chain; 15 of a tree), fp32:
-//   sequences           1             8 (4)         32 (16)       48            64            96
-//   chain,  32000       12.1  13.6    12.6  15.1    13.2  16.3    14.5  17.0    14.5  17.2    15.4  20.1
-//   chain,  65536       15.0  14.8    16.0  15.4    17.3  16.3    18.4  18.3    18.2  19.7    18.8  22.0
-//   chain, 131072       21.6  14.2    22.6  15.4    25.7  19.6    26.2  22.3    26.3  26.5    30.0  31.0
-//   tree,   32000       22.9  32.3    25.4  34.2    27.8  37.6    29.5  40.1    29.8  41.1    30.4  43.9
-//   tree,   65536       28.0  31.8    36.5  36.2    36.4  36.6    43.9  47.6    44.1  49.2    45.9  54.6
-//   tree,  131072       60.2  38.0    67.9  47.2    71.3  51.3    74.4  63.2    74.8  76.6    82.9  94.1
-// One or two shared passes of a tree of 131072 words: 64.6 and 57.5 of 16 sequences, five 51.7.  512 workgroups in all against 2048 and 8192: the same up to 48 sequences,
-// from 64 on up to a tenth less.
+// Measured, us a call of a replayed graph, one workgroup per sequence and shared (5 drafts of a chain, 15 of a tree, fp32):
+//   sequences           1             8             32            48            64            96            192
+//   chain,  32000       11.8  12.8    12.5  14.1    13.2  15.2    13.6  16.4    14.6  16.6    15.8  19.4    18.3  23.1
+//   chain,  65536       14.8  12.8    15.8  14.2    17.6  15.9    18.1  18.2    18.2  19.2    18.9  21.9    24.8  31.9
+//   chain, 131072       21.6  12.8    22.5  14.1    25.8  19.5    25.9  21.7    26.4  26.1    30.7  31.1    50.4  52.1
+//   tree,   32000       22.4  29.6    27.8  35.8    28.2  37.8    29.6  39.1    30.1  40.4    30.9  44.3    34.0  51.3
+//   tree,   65536       27.8  28.9    32.2  30.3    43.7  43.1    43.6  46.8    44.1  49.4    46.4  55.1    55.3  83.8
+//   tree,  131072       59.8  36.3    67.5  46.2    70.7  55.7    74.0  61.8    74.9  76.0    82.2  95.4   108.0 133.8
+// One or two shared passes of 32 trees of 131072 words: 66.4 and 61.1, five 56.3.  512 workgroups in all are as fast as 2048 up to 48 sequences.
 struct DraftPlan { int rounds, parts; };
 static DraftPlan draft_plan(const gdn_drafts_call* c) {
     const int64_t segments = (c->V + DRAFT_SEGMENT - 1) / DRAFT_SEGMENT;

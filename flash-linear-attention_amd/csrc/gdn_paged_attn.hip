@@ -15,9 +15,14 @@
 // pages' numbers a tile earlier.  From 33 rows on the four waves of a workgroup take the same keys, 64 at a time, from two stages in LDS (four waves asking for the same rows:
 // 417 us for the long trees below, through LDS 318).  Waves that share rows are joined through LDS at the end, workgroups by paged_attn_join_kernel.
 //
-// The memory system bounds it up to 128 rows.  Measured (bf16, heads of 128, 32 query heads on 8): 64 sequences of 3300 keys, a row each 168 us (5.2 TB/s), of up to 8192 keys 176;
-// eight trees of 32 rows over 32768 keys 221 (4.9 TB/s), of it the join 12; four of 8000 with 256 rows 255 (534 TFLOP/s).  Heads of 80 in pages of 10 are bound by the wait for
-// each tile: 33 chains of 7 over 3001 keys 27 us.
+// The weights are rounded to the operands' type for their product with V, once, as the matrix cores take them; their sum, the statistics and the sums of V are fp32.  (In fp32
+// the second product would have a sixteenth of the rate, by the published peaks.  With bf16 rows the result is 1.2 to 1.4 times as far from the exact one as its own rounding puts it.)
+//
+// The memory system bounds it up to 128 rows.  Measured (bf16, heads of 128, 32 query heads on 8): 64 sequences of 3300 keys, a row each 162 to 168 us (5.2 to 5.4 TB/s), of up to
+// 8192 keys 176; eight trees of 32 rows over 32768 keys 220 to 240, by machine (4.5 to 4.9 TB/s), of it the join 12; four of 8000 with 256 rows 248 (551 TFLOP/s).  Heads of 256, 16 on 4,
+// up to 8000 keys: 32 rows 115 us (4.7 TB/s), 16 trees of 16 rows 99 (3.7 TB/s, 232 TFLOP/s), 128 rows each 724 (374 TFLOP/s).  Heads of 80 in pages of 10 are bound by the wait for
+// each tile: 33 chains of 7 over 3001 keys 27 us.  Whole prompts run, at half the rate of a chunk behind a context and less: seven of 2048 rows 1244 us (193 TFLOP/s), because
+// a unit counts as all keys of its sequence while it stops at its last row.
 #include "gdn_paged.h"
 #include "gdn_chunk_common.h"
 #include <algorithm>
@@ -763,8 +768,9 @@ static PagedAttnPlan attn_plan(const gdn_paged_cache* cache, const gdn_paged_att
     const int64_t units = std::max<int64_t>(1, c->N) * cache->heads * ((rows + plan.height - 1) / plan.height);
     const int64_t steps = std::max<int64_t>(1, (cache->table_cols * cache->page_size + plan.step - 1) / plan.step);
     plan.groups = (int)std::min<int64_t>(plan.dim == 256 ? 256 : 512, units * steps);
-    // The join of a row's parts by four waves in place of one: measured, us a call (parts that a unit may have): heads of 128, 32 rows on one head of the cache 18.8 and 19.1 (3),
-    // 20.1 and 19.9 (8), 30.4 and 26.6 (16), 50.0 and 41.6 (32), 63.4 and 31.4 (256); a row on each of 8 heads 24.6 and 23.9 (4), 20.7 and 20.1 (8), 25.8 and 23.7 (16).
+    // The join of a row's parts by four waves in place of one: measured, us a call of a replayed graph (parts that a unit may have), heads of 128: 32 rows on one head of the
+    // cache 18.3 and 18.3 (3), 19.2 and 18.6 (8), 30.8 and 27.0 (16), 50.6 and 42.5 (32), 64.9 and 31.6 (256); four on each of 8 heads 24.4 and 24.3 (4), 21.3 and 20.6 (8), 26.1 and
+    // 24.1 (16), 43.8 and 35.7 (64).  It has four times the workgroups, so it is for few rows.
     plan.many_parts = plan.groups > 8 * units && c->B * c->T * c->HQ < (1 << 24);
     plan.bytes = ((size_t)c->N + 2) / 2 * 16 + (size_t)2 * plan.groups * plan.height * (cache->dim + 2) * sizeof(float);
     return plan;

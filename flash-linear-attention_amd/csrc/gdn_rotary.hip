@@ -151,10 +151,10 @@ static int launch_rotary(const char* who, RotaryParams& p, bool inter, bool cach
     const int64_t tokens = p.B * p.T;
     p.chunks = (inter ? 2 * p.half : p.half) / V + (p.D - 2 * p.half) / V;
     p.chunk_lanes = std::min(p.chunks, 256);
-    // Heads of a thread: one where the chip is not full, else two or three, as leaves the fewest of a block's threads idle (of equals two).  Measured, us a call with one, two and
-    // three: 32768 tokens of 20 heads of 128 elements 77.6, 65.3, 70.5; 14000 tokens of 48 heads into the cache 75.3, 70.9, 66.2, of 24 heads 44.3, 38.3, 35.9; 8192 tokens of 24
-    // heads of 64 16.5, 16.0, 13.3, of 9 heads of 256 22.1, 21.8, 19.6; 8191 tokens of 40 heads of 64 interleaved and 64 other elements 45.3, 42.7, 44.9 (the rule says three: 5 %).
-    // Fewer tokens of 20 heads: 820 (131000 threads of a head each) 8.4, 8.7, 8.8, 1640 8.7, 8.7, 9.1, 3280 11.9, 10.1, 10.7.
+    // Heads of a thread: one where the chip is not full, else two or three, as leaves the fewest of a block's threads idle (of equals two).  Measured, us a call of a replayed graph
+    // with one, two and three: 32768 tokens of 20 heads of 128 elements 78.0, 65.5, 70.4; 14000 tokens of 48 heads into the cache 76.0, 70.1, 66.5, of 24 heads 44.6, 38.5, 35.2; 8192
+    // tokens of 24 heads of 64 15.9, 15.8, 12.9, of 9 heads of 256 22.3, 21.4, 19.9; 8191 tokens of 40 heads of 64 interleaved and 64 other elements 45.9, 43.0, 44.2 (three is taken).
+    // Fewer tokens of 20 heads: 820 (131000 threads of a head each) 5.3, 6.2, 7.1, 1640 (262000) 6.8, 7.1, 7.8, 3280 11.1, 9.5, 11.3.
     auto lay_out = [&](int each) {
         p.head_lanes = std::max(1, std::min((p.heads + each - 1) / each, 256 / p.chunk_lanes));
         p.tokens = std::max(1, 256 / (p.head_lanes * p.chunk_lanes));
