@@ -250,7 +250,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
     turn more than beta_fast times left alone, and in between a ramp.  Any other entry raises: it would make other tables than its model's."""
     if dim <= 0 or dim % 2:
         raise ValueError(f'the turned part of a head must be even, got {dim}')
-    inverse = lambda b: b ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    inverse = lambda b: b ** (-torch.arange(0, dim, 2, dtype=torch.float64, device='cpu') / dim)
     if scaling is None:
         return inverse(base), 1.0
     kind, factor = scaling.get('type', scaling.get('rope_type')), float(scaling['factor'])
@@ -272,7 +272,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
         at = lambda turns: dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
         low = max(math.floor(at(scaling.get('beta_fast', 32))), 0)
         high = min(math.ceil(at(scaling.get('beta_slow', 1))), dim - 1)
-        ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        ramp = ((torch.arange(dim // 2, dtype=torch.float64, device='cpu') - low) / max(high - low, 1e-3)).clamp(0, 1)
         inv = inverse(base)
         return inv / factor * ramp + inv * (1 - ramp), float(scaling.get('attention_factor', 0.1 * math.log(factor) + 1.0))
     raise ValueError(f"scaling must be of type 'linear', 'ntk' or 'yarn', got {kind!r}")
@@ -294,8 +294,9 @@ class RotaryEmbedding(nn.Module):
             raise ValueError('scale_center is that of scale_base')
         self.dim, self.base, self.scale_base, self.interleaved, self.scaling, self.scale_center = dim, float(base), scale_base, interleaved, scaling, scale_center
         self._prefixes = scale_base is None or scale_center is not None      # (tables of more positions begin with those of fewer)
-        inv_freq, self.attention_factor = rotary_frequencies(dim, self.base, scaling)
-        self.register_buffer('inv_freq', inv_freq.float().to(device), persistent=False)
+        self._frequencies, self.attention_factor = rotary_frequencies(dim, self.base, scaling)
+        # (the reference's buffer, for who reads it: the tables are made from the frequencies in 64 bits)
+        self.register_buffer('inv_freq', self._frequencies.float().to(torch.get_default_device() if device is None else device), persistent=False)
         self._tables, self._captured = None, []
 
     def extra_repr(self) -> str:
@@ -325,16 +326,15 @@ class RotaryEmbedding(nn.Module):
             positions = max(positions, 2 * kept[0].shape[0] if self.scale_base is None else min(2 * kept[0].shape[0], most))
         if kept is not None and kept[0].is_cuda:
             torch.cuda.synchronize(kept[0].device)                       # (a call on another stream may still read those that go)
-        inv, factor = rotary_frequencies(self.dim, self.base, self.scaling)
-        # Made on the host and copied while it waits: whatever stream reads them, they are there.
+        # Made on the host (whatever the default device) and copied while it waits: whatever stream reads them, they are there.
         with torch.no_grad(), torch.inference_mode(False):
-            t = torch.arange(positions, dtype=torch.float64)
-            angle = t[:, None] * inv
-            cos, sin = angle.cos() * factor, angle.sin() * factor
+            t = torch.arange(positions, dtype=torch.float64, device='cpu')
+            angle = t[:, None] * self._frequencies
+            cos, sin = angle.cos() * self.attention_factor, angle.sin() * self.attention_factor
             if self.scale_base is None:
                 tables = (cos, sin)
             else:
-                s = (torch.arange(0, self.dim, 2, dtype=torch.float64) + 0.4 * self.dim) / (1.4 * self.dim)
+                s = (torch.arange(0, self.dim, 2, dtype=torch.float64, device='cpu') + 0.4 * self.dim) / (1.4 * self.dim)
                 scale = s ** ((t - center) / self.scale_base)[:, None]
                 tables = (cos * scale, sin * scale, cos / scale, sin / scale)
             self._tables = tuple(x.float().to(device) for x in tables)

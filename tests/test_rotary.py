@@ -639,3 +639,22 @@ def test_positions_of_a_packed_batch_that_the_tables_do_not_have(lib):
         with pytest.raises(ValueError, match='positions'):
             call()
     assert len(lib.calls) == 3
+
+
+def test_tables_do_not_follow_the_modules_type():
+    """The buffer of frequencies goes with the module; the tables are formed from those in 64 bits, whatever becomes of it."""
+    scaling = dict(type='yarn', factor=4.0, original_max_position_embeddings=64)
+    rope, cast = (_mods().RotaryEmbedding(32, scaling=scaling) for _ in range(2))
+    cast = cast.half()
+    assert cast.inv_freq.dtype == HF and all(torch.equal(a, b) for a, b in zip(rope.tables(300, 'cpu'), cast.tables(300, 'cpu')))
+    assert rope.tables(300, 'cpu')[0][0, 0].item() == pytest.approx(rope.attention_factor)
+
+
+@pytest.mark.parametrize('kw', [dict(), dict(scale_base=512.0, scale_center=10), dict(scaling=dict(type='yarn', factor=4.0, original_max_position_embeddings=64))])
+def test_tables_are_made_on_the_host_whatever_the_default_device(kw):
+    """Formed on a device by default they would be ready on the stream of that moment only (here: a device that holds no numbers at all)."""
+    want = _mods().RotaryEmbedding(32, **kw).tables(50, 'cpu')
+    with torch.device('meta'):
+        rope = _mods().RotaryEmbedding(32, **kw)
+        inside = rope.tables(50, 'cpu')
+    assert rope.inv_freq.is_meta and all(torch.equal(a, b) for a, b in zip(want, inside))
