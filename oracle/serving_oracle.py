@@ -40,7 +40,7 @@ def slot_of(table, n, slot, pages, page_size):
 def paged_attn(q, k_cache, v_cache, table, context, rows, sees, scale):
     """q [rows of all sequences, HQ, D]; rows: [(first, last)] of each sequence; sees(n, i, j) -> whether row i sees row j of its sequence.
 
-    Returns (o, sum_j p_j |v_j|, largest sum_d |q_d k_d| scale over the keys seen, largest |score - maximum|), fp64."""
+    Returns (o, sum_j p_j |v_j|, largest sum_d |q_d k_d scale| over the keys seen, largest |score - maximum|), fp64."""
     q, k_cache, v_cache = q.double().cpu(), k_cache.double().cpu(), v_cache.double().cpu()
     pages, page_size, HK, D = k_cache.shape
     HQ = q.shape[1]
@@ -60,7 +60,7 @@ def paged_attn(q, k_cache, v_cache, table, context, rows, sees, scale):
                 w = w / w.sum()
                 o[first + i, h] = (w[:, None] * v).sum(0)
                 size[first + i, h] = (w[:, None] * v.abs()).sum(0)
-                dots[first + i, h] = (k * x).abs().sum(1).max() * scale
+                dots[first + i, h] = (k * x).abs().sum(1).max() * abs(scale)
                 spread[first + i, h] = (s.max() - s).max()
     return o, size, dots, spread
 

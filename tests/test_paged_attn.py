@@ -497,3 +497,44 @@ def test_numbers_in_masked_places_of_other_heads_and_types(rows, page_size, D, d
     assert torch.equal(got[0, :, :, :5], want[0, :, :, :5]) and torch.equal(got[0, :, :, 6:], want[0, :, :, 6:])
     seen = got[0, sees][..., 5].float()
     assert seen.isnan().all() if bad != bad else (seen == bad).all()
+
+
+@gpu
+@pytest.mark.parametrize(('contexts', 'rows', 'HQ', 'HK', 'D', 'page_size', 'dtype'), [([0, 0, 0], [513, 1, 300], 4, 2, 64, 16, BF), ([5, 0, 130], [513, 1, 300], 4, 2, 64, 16, BF), ([0], [900], 2, 1, 128, 64, HF),
+                                                                                      ([0], [700], 2, 1, 80, 10, HF), ([3], [260], 2, 2, 256, 32, BF), ([10, 20, 30, 0], [0, 0, 3, 0], 4, 2, 64, 16, BF)])
+def test_whole_prompts(contexts, rows, HQ, HK, D, page_size, dtype):
+    """Rows just appended that see each other only, or little besides."""
+    Step(contexts, rows, page_size, HQ, HK, D, dtype, packed=True).check()
+
+
+@gpu
+@pytest.mark.parametrize('page_size', [4096, 4095])
+def test_pages_longer_than_the_sequences(page_size):
+    Step([3000, 1, 4094], [3, 3, 3], page_size, 4, 2, 64, BF).check()
+
+
+@gpu
+@pytest.mark.parametrize('rows', [2, 40])
+def test_tensors_that_share_memory(rows):
+    """Keys and values as halves of a head's row or as one tensor; sequences that read the same pages; one sequence's queries, length, pages and mask for all."""
+    both = torch.randn(12, 16, 2, 128, generator=torch.Generator().manual_seed(0)).to(BF).to(DEV)
+    step = Step([60, 60], [rows] * 2, 16, 4, 2, 64, BF)
+    step.t = torch.arange(12, dtype=torch.int32).expand(2, 12)
+    for step.k_cache, step.v_cache in ((both[..., :64], both[..., 64:]), (both[..., :64], both[..., :64])):
+        step.q = step.q[:1].expand(2, rows, 4, 64)
+        step.mask = None
+        want = step.check()
+        step.mask = torch.ones(rows, rows, dtype=torch.bool).tril()
+        context, t = torch.tensor([60], dtype=torch.int32, device=DEV).expand(2), torch.arange(12, dtype=torch.int32, device=DEV)[None].expand(2, 12)
+        assert torch.equal(_attn().paged_attn(step.q, step.k_cache, step.v_cache, t, context, tree_mask=step.mask.to(DEV).expand(2, rows, rows)), want)
+        step.mask = torch.ones(1, rows, dtype=torch.bool).expand(rows, rows)
+        step.check()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [BF, HF])
+@pytest.mark.parametrize('rows', [4, 40])
+def test_scales_of_any_sign(rows, dtype):
+    step = Step([100, 7], [rows] * 2, 16, 4, 2, 128, dtype)
+    for scale in (0.0, 4.0, -0.5, -3.0):
+        step.check(scale=scale)
